@@ -49,6 +49,8 @@ typedef enum sb_status_code {
 #define SB_ELEMENT_TYPE_FLOAT_32 ((0x21u << 24) | 32u)
 #define SB_ELEMENT_TYPE_BFLOAT_16 ((0x31u << 24) | 16u)
 #define SB_ELEMENT_TYPE_INT_32 ((0x11u << 24) | 32u)
+/* Buffers of the decoding operators only: no program has 8-bit tensors. */
+#define SB_ELEMENT_TYPE_INT_8 ((0x11u << 24) | 8u)
 
 /* Arithmetic used for dot_general contractions of f32 tensors.  Other ops
  * compute in the graph's types (f32; bf16 tensors as bf16, rounding every op's
@@ -149,6 +151,9 @@ SB_API sb_status* sb_session_call(sb_session* session, const char* qualified_nam
 SB_API sb_status* sb_buffer_allocate_copy(sb_session* session, size_t rank, const uint64_t* shape,
                                           uint32_t element_type, const void* host_data,
                                           size_t byte_length, sb_buffer** out_buffer);
+/* A buffer of zeros (a key/value cache before its first token). */
+SB_API sb_status* sb_buffer_allocate_zero(sb_session* session, size_t rank, const uint64_t* shape,
+                                          uint32_t element_type, sb_buffer** out_buffer);
 /* Wraps caller-owned device memory without copying; the caller keeps it alive.
  * The pointer must be 16-byte aligned (vector loads and TMA read it directly). */
 SB_API sb_status* sb_buffer_wrap_device(sb_session* session, size_t rank, const uint64_t* shape,
@@ -207,6 +212,86 @@ SB_API void sb_adamw_options_initialize(sb_adamw_options* options);
 SB_API sb_status* sb_optimizer_adamw_step(sb_session* session, size_t leaf_count, sb_buffer* const* params,
                                           sb_buffer* const* grads, sb_buffer* const* m, sb_buffer* const* v,
                                           const sb_adamw_options* options, float* out_global_norm);
+
+/* --- decoding operators ------------------------------------------------------ *
+ * A generation loop over a key/value cache: write the new tokens' keys and
+ * values, attend over the cache, select the continuations of a beam search and
+ * rearrange the caches to follow it.  No counterpart in the reference, whose
+ * sample.shf reruns the whole window per token.  Each call is one kernel on
+ * the session stream (sb_beam_reorder: one per 48 states), returns once it is
+ * enqueued, allocates nothing and uses no workspace, so a call may be captured
+ * into a CUDA graph of the session stream.  Results do not depend on timing.
+ * Buffers are row-major, of this session or wrapped memory of its device.
+ * Index buffers are i32; their values are read on the device and values out of
+ * range have the meaning stated, never a fault.  Unless stated otherwise a
+ * written buffer must not overlap another argument. */
+
+/* A cache [slots, heads, capacity, head size]: f32, bf16 or int8; the head
+ * size is a multiple of 16 up to 256.  An int8 cache has one f32 scale per row
+ * (k_scale, v_scale [slots, heads, capacity]; NULL for f32 and bf16 caches) and
+ * stands for code * scale, where a row x was written as
+ *   scale = max|x| / 127 rounded to f32,
+ *   code  = x / scale rounded to the nearest integer, ties to even, exactly
+ * (all zero when the scale is 0).  A NaN is written as 0, an infinity as the
+ * largest finite f32 of its sign. */
+typedef struct sb_kv_cache {
+  sb_buffer *k, *v, *k_scale, *v_scale;
+} sb_kv_cache;
+
+/* Row (n, t, h) of k, v [slots, tokens, heads, head size] (f32 or bf16) is
+ * written to position positions[n] + t of slot n, rounded to nearest in a bf16
+ * cache.  A slot with a negative position is idle: nothing is written.  Nor is
+ * anything at positions beyond the capacity. */
+SB_API sb_status* sb_kv_cache_write(sb_session* session, const sb_kv_cache* cache, sb_buffer* positions,
+                                    sb_buffer* k, sb_buffer* v);
+
+/* The values at positions starts[n] + i (starts NULL: i) to row (n, h, i) of
+ * k_out, v_out [slots, heads, rows, head size] (f32 or bf16).  Rows whose
+ * position is outside the cache, and rows i >= counts[n] (counts NULL: none),
+ * are left as they were. */
+SB_API sb_status* sb_kv_cache_read(sb_session* session, const sb_kv_cache* cache, sb_buffer* starts,
+                                   sb_buffer* counts, sb_buffer* k_out, sb_buffer* v_out);
+
+/* out = softmax(scale q k^T) v for up to 64 tokens per slot whose keys and
+ * values stand at positions positions[n] + t of the cache (sb_kv_cache_write
+ * puts them there).  Token t attends to the positions before positions[n], to
+ * itself, and to its ancestors among the tokens: with parents NULL all earlier
+ * ones (a chain), else those on the path parents[n][t], parents[n][parents[n]
+ * [t]], .. (a tree of drafted tokens); a parent outside [0, t) ends the path.
+ * q, out [slots, tokens, query heads, head size], f32 or bf16; query head h
+ * reads cache head h / (query heads / heads).  Positions beyond the capacity
+ * hold nothing; a slot with a negative position is idle.  A token without keys
+ * gets zeros.  What stands at positions that a token does not attend to does
+ * not matter, NaN included.  Scores, softmax and sums are f32. */
+SB_API sb_status* sb_kv_cache_attention(sb_session* session, const sb_kv_cache* cache, sb_buffer* positions,
+                                        sb_buffer* parents, sb_buffer* q, float scale, sb_buffer* out);
+
+/* Beam search: of the beams x vocabulary continuations of each group, with
+ *   value(w, v) = scores[w] + (logits[w, v] - log sum_u exp logits[w, u])
+ * in f64, the `beams` largest in descending order: out_scores (f32),
+ * out_parents (w) and out_tokens (v), all [groups, beams], beams <= 16.
+ * logits [groups * beams, vocabulary], f32 or bf16.  Within a beam the logits
+ * order the candidates, the lower token first among equals; between beams of
+ * equal value the lower beam comes first.  A NaN logit counts as -inf; a beam
+ * whose score or sum is not finite has value -inf throughout (its tokens in
+ * ascending order): before the first step, scores of 0, -inf, .. keep beams
+ * that hold the same prefix from giving the same continuation.  With eos >= 0,
+ * finished[w] != 0 marks a beam that continues with eos alone, at its own
+ * score, and out_finished tells whether the parent was finished or the token
+ * is eos; with eos < 0 both are NULL.  out_scores may be scores and
+ * out_finished may be finished. */
+SB_API sb_status* sb_beam_select(sb_session* session, sb_buffer* logits, sb_buffer* scores, sb_buffer* finished,
+                                 int64_t eos, sb_buffer* out_scores, sb_buffer* out_parents, sb_buffer* out_tokens,
+                                 sb_buffer* out_finished);
+
+/* In place, for every state [groups * beams, ..] (f32, bf16, i32 or int8): row
+ * g * beams + j takes the former content of row g * beams + parents[g][j].  A
+ * parent outside [0, beams) leaves its row alone.  With time_axes[i] >= 1 only
+ * the first lengths[source row] entries along that dimension are taken over
+ * (lengths [groups * beams], NULL: all) and the rest of the row stays; -1
+ * takes whole rows over whatever lengths says. */
+SB_API sb_status* sb_beam_reorder(sb_session* session, size_t state_count, sb_buffer* const* states,
+                                  const int32_t* time_axes, sb_buffer* parents, sb_buffer* lengths);
 
 /* --- allocation-free GEMM --------------------------------------------------- *
  * No counterpart in the reference.  For callers that must not allocate device

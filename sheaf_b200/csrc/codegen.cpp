@@ -22,6 +22,7 @@ const char* ctype_of(DType t) {
     case DType::I32: return "int";
     case DType::I64: return "long long";
     case DType::I1: return "bool";
+    case DType::I8: return "signed char";
   }
   return "float";
 }

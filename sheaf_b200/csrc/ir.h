@@ -10,14 +10,15 @@
 
 namespace sb {
 
-enum class DType : uint8_t { F32, BF16, F64, I32, I64, I1 };
+// I8 is the type of a quantised cache's buffers (never parsed from a program).
+enum class DType : uint8_t { F32, BF16, F64, I32, I64, I1, I8 };
 
 inline int dtype_bytes(DType t) {
   switch (t) {
     case DType::F32: case DType::I32: return 4;
     case DType::BF16: return 2;
     case DType::F64: case DType::I64: return 8;
-    case DType::I1: return 1;
+    case DType::I1: case DType::I8: return 1;
   }
   return 4;
 }

@@ -1,0 +1,384 @@
+// Beam search: the selection of the W best continuations of each group of W
+// beams (beam_select) and the rearrangement of per-beam state to follow it
+// (beam_reorder).
+//
+//   cand(w, v) = score_w + (z_wv - lse_w),  lse_w = log sum_v exp z_wv
+//   selected: the W largest of the W x V candidates, by (value, then lowest
+//   w V + v).
+//
+// Reading the logits once bounds the selection.  A cluster of C CTAs carries a
+// group; each warp streams pieces of one beam's row and keeps in its lanes the
+// W best of what it has seen as 64-bit keys (order-preserving image of the
+// logit above the complemented index: unique, so equal logits order by index
+// and every step has one answer).  A piece is filtered by the larger of the
+// list's last key and the W-th best of the 32 lanes' own best keys, which
+// leaves little more than W values to insert.  After a cluster barrier CTA r
+// joins the lists of beams r, r + C, ..; after a second one CTA 0 orders the
+// W x W survivors.  Lists cross CTAs through distributed shared memory, so
+// there is no workspace, no atomic and no second launch.
+//
+// Within a beam the order is the logits' own.  Between beams it needs lse: the
+// sums run in f64, since an f32 sum is off by about 1e-7 of a candidate's
+// value and would decide near ties by its rounding.
+#include <cuda_bf16.h>
+
+#include <cmath>
+
+#include "kernels.h"
+#include "pdl.h"
+#include "tc_common.h"
+
+namespace sb {
+namespace {
+
+constexpr int kSelWarps = 16, kSelThreads = kSelWarps * 32;
+constexpr int EPC = 32;              // values per lane and piece
+constexpr int kPiece = EPC * 32;     // values per warp and piece
+constexpr int W_MAX = (int)kBeamMax;
+using u64 = unsigned long long;
+
+struct SelectParams {
+  const void* logits;
+  const float* scores;
+  const int* finished;
+  float* out_scores;
+  int *out_parents, *out_tokens, *out_finished;
+  int64_t V, total;  // total: values of the whole logits buffer
+  int W, eos;
+};
+
+// Order-preserving image of an f32 that is not NaN.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ u64 shfl64(u64 x, int src) { return __shfl_sync(0xffffffffu, x, src); }
+
+// A warp's list: lane j < W holds the j-th largest key, 0 where there is none
+// (every real key is above 0).
+__device__ __forceinline__ void insert(u64& list, u64 key, int lane, int W) {
+  const int rank = __popc(__ballot_sync(0xffffffffu, lane < W && list > key));
+  const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
+  if (lane < W && lane >= rank) list = lane == rank ? key : up;
+}
+
+// Values i .. i + 3 (f32) or i .. i + 7 (bf16) of the row that starts at
+// element `base` of the buffer, as a 16-byte load: `at` is the element of the
+// buffer that the load starts at (a multiple of the load's width).  Elements
+// outside the row are -inf.  The buffer's last elements are loaded one by one
+// where the 16 bytes would pass its end.
+template <bool BF>
+__device__ __forceinline__ void load_piece(const void* buf, int64_t at, int64_t base, int64_t V, int64_t total, float* x) {
+  constexpr int N = BF ? 8 : 4;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = -INFINITY;
+  if (at >= base + V) return;
+  if (at + N <= total) {
+    const uint4 r = *(const uint4*)((const uint8_t*)buf + at * (BF ? 2 : 4));
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (BF) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        x[i] = __uint_as_float(w[i]);
+      }
+    }
+  } else {
+    for (int i = 0; i < N; ++i)
+      if (at + i < total)
+        x[i] = BF ? __bfloat162float(((const __nv_bfloat16*)buf)[at + i]) : ((const float*)buf)[at + i];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (at + i < base || at + i >= base + V || x[i] != x[i]) x[i] = -INFINITY;  // NaN counts as -inf
+}
+
+// Sum of exp(x - m) kept with the maximum it refers to.
+__device__ __forceinline__ void join(double& m, double& s, double m2, double s2) {
+  const double mx = fmax(m, m2);
+  if (mx == -INFINITY) return;
+  s = s * exp(m - mx) + s2 * exp(m2 - mx);
+  m = mx;
+}
+
+struct SelectShared {
+  u64 list[kSelWarps][W_MAX];
+  double m[kSelWarps], s[kSelWarps];
+  // rank 0: the candidates of every beam
+  double cand[W_MAX][W_MAX];
+  int token[W_MAX][W_MAX];
+  int done[W_MAX];
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t remote(const T* p, uint32_t rank) { return tc::cluster_addr(p, rank); }
+__device__ __forceinline__ u64 ld_remote64(uint32_t a) {
+  u64 x;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(a));
+  return x;
+}
+__device__ __forceinline__ void st_remote64(uint32_t a, u64 x) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(x) : "memory");
+}
+__device__ __forceinline__ void st_remote32(uint32_t a, uint32_t x) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
+}
+
+template <bool BF>
+__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
+  pdl_prologue();
+  __shared__ SelectShared sh;
+  constexpr int N = BF ? 8 : 4;
+  const uint32_t crank = tc::cluster_rank();
+  uint32_t C;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int W = p.W;
+  const int64_t g = blockIdx.x / C;
+  // warps of the cluster per beam; warp `gid` streams every `per`-th piece of its beam
+  const int warps = (int)C * kSelWarps, per = warps / W;
+  const int gid = (int)crank * kSelWarps + warp, beam = gid / per, sub = gid % per;
+  u64 list = 0;
+  double m = -INFINITY, sum = 0.;
+  const bool over = p.eos >= 0 && beam < W && p.finished[g * W + beam];
+  if (beam < W && !over) {
+    const int64_t base = (g * W + beam) * p.V;
+    const int64_t first = base - base % N;  // 16-byte boundary at or before the row
+    const int64_t pieces = (base + p.V - first + kPiece - 1) / kPiece;
+    for (int64_t c = sub; c < pieces; c += per) {
+      const int64_t at0 = first + c * kPiece + lane * N;
+      float x[EPC];
+#pragma unroll
+      for (int i = 0; i < EPC / N; ++i) load_piece<BF>(p.logits, at0 + i * 32 * N, base, p.V, p.total, x + i * N);
+      float mx = x[0];
+#pragma unroll
+      for (int i = 1; i < EPC; ++i) mx = fmaxf(mx, x[i]);
+      // lane's best key: its largest value at the lowest index
+      int64_t bi = 0;
+#pragma unroll
+      for (int i = EPC - 1; i >= 0; --i)
+        if (x[i] == mx) bi = at0 + (i / N) * 32 * N + i % N - base;
+      const bool none = bi < 0 || bi >= p.V;
+      const u64 best = none ? 0 : (u64)ordered(mx) << 32 | (uint32_t)~(uint32_t)bi;
+      float wm = mx;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+      double acc = 0.;
+      if (wm != -INFINITY) {
+#pragma unroll 4
+        for (int i = 0; i < EPC; ++i) acc += exp((double)x[i] - (double)wm);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+      join(m, sum, (double)wm, acc);
+      // the W-th best of the lanes' best keys
+      int ahead = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) ahead += shfl64(best, i) > best;
+      const uint32_t at = __ballot_sync(0xffffffffu, ahead == W - 1);
+      u64 bar = shfl64(list, W - 1);
+      if (at) {
+        const u64 b2 = shfl64(best, __ffs(at) - 1);
+        if (b2 > bar) bar = b2 - 1;  // itself passes
+      }
+#pragma unroll
+      for (int i = 0; i < EPC; ++i) {
+        const int64_t idx = at0 + (i / N) * 32 * N + i % N - base;
+        const u64 key = idx < 0 || idx >= p.V ? 0 : (u64)ordered(x[i]) << 32 | (uint32_t)~(uint32_t)idx;
+        uint32_t hit = __ballot_sync(0xffffffffu, key > bar);
+        while (hit) {
+          const int src = __ffs(hit) - 1;
+          hit &= hit - 1;
+          insert(list, shfl64(key, src), lane, W);
+        }
+      }
+    }
+  }
+  if (lane < W_MAX) sh.list[warp][lane] = lane < W ? list : 0;
+  if (lane == 0) sh.m[warp] = m, sh.s[warp] = sum;
+  tc::cluster_sync();
+
+  // CTA r joins beams r, r + C, ..: one warp each
+  for (int b = (int)crank + (int)C * warp; b < W; b += (int)C * kSelWarps) {
+    u64 best = 0;
+    double bm = -INFINITY, bs = 0.;
+    for (int k = 0; k < per; ++k) {
+      const int id = b * per + k, r = id / kSelWarps, w = id % kSelWarps;
+      const u64 mine = lane < W ? ld_remote64(remote(&sh.list[w][lane], r)) : 0;
+      for (int j = 0; j < W; ++j) {  // sorted: stop at the first that does not get in
+        const u64 key = shfl64(mine, j);
+        if (key <= shfl64(best, W - 1)) break;
+        insert(best, key, lane, W);
+      }
+      join(bm, bs, __longlong_as_double((long long)ld_remote64(remote(&sh.m[w], r))),
+           __longlong_as_double((long long)ld_remote64(remote(&sh.s[w], r))));
+    }
+    const float score = p.scores[g * W + b];
+    const bool fin = p.eos >= 0 && p.finished[g * W + b];
+    const double lse = bm + log(bs);
+    const int have = (int)min((int64_t)W, p.V);
+    double value = -INFINITY;
+    int token = lane;
+    if (isfinite(score) && fin) {
+      // the end token alone, then the others from the lowest
+      value = lane == 0 ? (double)score : -INFINITY;
+      token = lane == 0 ? p.eos : lane - 1 + (lane - 1 >= p.eos);
+    } else if (isfinite(score) && isfinite(lse)) {
+      token = (int)~(uint32_t)best;
+      value = (double)score + ((double)unordered((uint32_t)(best >> 32)) - lse);
+    }
+    if (lane < W) {
+      if (lane >= have) value = -INFINITY, token = -1;  // no such candidate
+      st_remote64(remote(&sh.cand[b][lane], 0), (u64)__double_as_longlong(value));
+      st_remote32(remote(&sh.token[b][lane], 0), (uint32_t)token);
+      if (lane == 0) st_remote32(remote(&sh.done[b], 0), fin ? 1u : 0u);
+    }
+  }
+  tc::cluster_sync();
+  if (crank != 0) return;
+  // rank of each survivor among all
+  for (int i = tid; i < W * W; i += kSelThreads) {
+    const int b = i / W, j = i % W, tok = sh.token[b][j];
+    if (tok < 0) continue;
+    const double v = sh.cand[b][j];
+    int rank = 0;
+    for (int k = 0; k < W * W; ++k) {  // among equals the lower beam, and a beam's own order
+      const double v2 = sh.cand[k / W][k % W];
+      rank += sh.token[k / W][k % W] >= 0 && (v2 > v || (v2 == v && k < i));
+    }
+    if (rank < W) {
+      const int64_t o = g * W + rank;
+      p.out_scores[o] = (float)v;
+      p.out_parents[o] = b;
+      p.out_tokens[o] = tok;
+      if (p.eos >= 0) p.out_finished[o] = sh.done[b] || tok == p.eos;
+    }
+  }
+}
+
+struct ReorderParams {
+  struct State {
+    uint8_t* p;
+    int64_t row_bytes, T, inner;
+    int64_t units;      // pieces of `unit` bytes per row
+    int64_t first;      // first block of the state
+    int unit;
+  };
+  static constexpr int kStates = 48;
+  State s[kStates];
+  int count;
+  const int *parents, *lengths;
+  int W;
+};
+
+constexpr int kReThreads = 256;
+
+template <typename U, int W>
+__device__ __forceinline__ void reorder_piece(const ReorderParams::State& s, int64_t g, int64_t u, const int* src,
+                                              const int64_t* live, int w) {
+  if (u >= s.units) return;
+  const int64_t t = s.T ? (u * (int64_t)sizeof(U) / s.inner) % s.T : -1;  // -1: whole rows
+  uint8_t* row0 = s.p + g * w * s.row_bytes + u * (int64_t)sizeof(U);
+  U v[W];
+  // every read comes before the first write: this thread alone touches these bytes of the group's rows
+#pragma unroll
+  for (int j = 0; j < W; ++j)
+    if (j < w && src[j] != j && (t < 0 || t < live[j])) v[j] = *(const U*)(row0 + src[j] * s.row_bytes);
+#pragma unroll
+  for (int j = 0; j < W; ++j)
+    if (j < w && src[j] != j && (t < 0 || t < live[j])) *(U*)(row0 + j * s.row_bytes) = v[j];
+}
+
+template <int W>
+__global__ void __launch_bounds__(kReThreads) reorder_kernel(const __grid_constant__ ReorderParams p) {
+  pdl_prologue();
+  __shared__ int src[W];
+  __shared__ int64_t live[W];  // entries to take over
+  int lo = 0, hi = p.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if ((int64_t)blockIdx.x >= p.s[mid].first) lo = mid;
+    else hi = mid - 1;
+  }
+  const ReorderParams::State& s = p.s[lo];
+  const int64_t per_group = (s.units + kReThreads - 1) / kReThreads;
+  const int64_t b = (int64_t)blockIdx.x - s.first, g = b / per_group, u = (b % per_group) * kReThreads + threadIdx.x;
+  if (threadIdx.x < W) {
+    const int j = threadIdx.x;
+    int q = j < p.W ? p.parents[g * p.W + j] : j;
+    if (q < 0 || q >= p.W) q = j;
+    src[j] = q;
+    live[j] = p.lengths && j < p.W ? (int64_t)p.lengths[g * p.W + q] : s.T;
+  }
+  __syncthreads();
+  switch (s.unit) {
+    case 16: reorder_piece<uint4, W>(s, g, u, src, live, p.W); break;
+    case 8: reorder_piece<uint2, W>(s, g, u, src, live, p.W); break;
+    case 4: reorder_piece<uint32_t, W>(s, g, u, src, live, p.W); break;
+    case 2: reorder_piece<uint16_t, W>(s, g, u, src, live, p.W); break;
+    default: reorder_piece<uint8_t, W>(s, g, u, src, live, p.W); break;
+  }
+}
+
+}  // namespace
+
+cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
+  if (a.G == 0) return cudaSuccess;
+  SelectParams p = {a.logits, a.scores, a.finished, a.out_scores, a.out_parents, a.out_tokens, a.out_finished,
+                    a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos};
+  // a warp for every two pieces of the group's logits, until every SM has a CTA
+  const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);
+  int C = 1;
+  while (C < 8 && a.G * C < 296 && pieces > C * kSelWarps) C *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.G * C));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  pdl_attribute(&at[0]);
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)C;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  launch_counter().fetch_add(1, std::memory_order_relaxed);
+  return a.bf16 ? cudaLaunchKernelEx(&cfg, select_kernel<true>, p) : cudaLaunchKernelEx(&cfg, select_kernel<false>, p);
+}
+
+cudaError_t beam_reorder(const BeamState* states, int64_t count, const int* parents, const int* lengths, int64_t G,
+                         int64_t W, cudaStream_t stream) {
+  for (int64_t at = 0; at < count;) {
+    ReorderParams p;
+    p.count = 0;
+    p.parents = parents;
+    p.lengths = lengths;
+    p.W = (int)W;
+    int64_t blocks = 0;
+    for (; at < count && p.count < ReorderParams::kStates; ++at) {
+      const BeamState& s = states[at];
+      if (s.row_bytes == 0) continue;
+      int unit = 16;
+      while (s.inner % unit) unit /= 2;
+      const int64_t units = s.row_bytes / unit, more = G * ((units + kReThreads - 1) / kReThreads);
+      if (more > INT32_MAX) return cudaErrorInvalidValue;
+      if (blocks + more > INT32_MAX) break;
+      p.s[p.count++] = {(uint8_t*)s.p, s.row_bytes, s.T, s.inner, units, blocks, unit};
+      blocks += more;
+    }
+    if (p.count == 0) continue;
+    const dim3 grid((unsigned)blocks), block(kReThreads);
+    cudaError_t e = W <= 2   ? launch_pdl(reorder_kernel<2>, grid, block, 0, stream, p)
+                    : W <= 4 ? launch_pdl(reorder_kernel<4>, grid, block, 0, stream, p)
+                    : W <= 8 ? launch_pdl(reorder_kernel<8>, grid, block, 0, stream, p)
+                             : launch_pdl(reorder_kernel<16>, grid, block, 0, stream, p);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace sb

@@ -238,4 +238,69 @@ struct AdamwScalars {
 cudaError_t adamw_step(const OptLeaf* leaves, const OptChunk* chunks, int n_chunks, float* partials,
                        float* norm_out, const AdamwScalars& a, cudaStream_t stream);
 
+// Decoding operators (kernels/kv_cache.cu, cache_attention.cu, beam.cu).  None
+// of them uses a workspace.  A cache is [N, H, T, D], D a multiple of 16 up to
+// kKvMaxDim; an int8 cache holds codes and one f32 scale per row [N, H, T].
+enum class KvType : int { F32, BF16, I8 };
+constexpr int64_t kKvMaxDim = 256;
+struct KvCacheView {
+  void *k = nullptr, *v = nullptr;
+  float *k_scale = nullptr, *v_scale = nullptr;  // int8 only
+  KvType type = KvType::F32;
+  int64_t N = 0, H = 0, T = 0, D = 0;
+};
+// Rows k, v [N, S, H, D] (f32 or bf16) to positions positions[n] + s.  Nothing
+// is written for a slot with a negative position, or at positions >= T.
+cudaError_t kv_cache_write(const KvCacheView& c, const int* positions, const void* k, const void* v, bool in_bf16,
+                           int64_t S, cudaStream_t stream);
+// The values at positions starts[n] + i (starts null: i), i < min(S,
+// counts[n]), to k_out, v_out [N, H, S, D] (f32 or bf16).  Rows of positions
+// outside [0, T) and rows i >= counts[n] are left as they were.
+cudaError_t kv_cache_read(const KvCacheView& c, const int* starts, const int* counts, void* k_out, void* v_out,
+                          bool out_bf16, int64_t S, cudaStream_t stream);
+
+// Attention of S tokens per slot over the cache: token s of slot n, whose key
+// and value stand at position positions[n] + s, attends to the positions
+// before positions[n], to itself and to its ancestors among the S tokens
+// (parents null: all earlier ones; else parents [N, S], a value outside [0, s)
+// meaning none).  Positions outside [0, T) hold nothing; a slot with a negative
+// position has no keys.  A token without keys gets zeros.
+constexpr int64_t kKvMaxTokens = 64;
+struct CacheAttnArgs {
+  KvCacheView cache;
+  const int* positions = nullptr;
+  const int* parents = nullptr;
+  const void* q = nullptr;  // [N, S, Hq, D], f32 or bf16; head h reads cache head h / (Hq / H)
+  void* out = nullptr;      // as q
+  bool bf16 = false;
+  int64_t S = 0, Hq = 0;
+  float scale = 1.f;  // multiplier of q.k before the softmax
+};
+cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
+
+// Beam search: the W best continuations of each group of W beams over a
+// vocabulary of V (see sb_beam_select).
+constexpr int64_t kBeamMax = 16;
+struct BeamSelectArgs {
+  const void* logits = nullptr;  // [G * W, V], f32 or bf16
+  bool bf16 = false;
+  const float* scores = nullptr;   // [G, W]
+  const int* finished = nullptr;   // [G, W], with eos >= 0
+  float* out_scores = nullptr;
+  int *out_parents = nullptr, *out_tokens = nullptr, *out_finished = nullptr;
+  int64_t G = 0, W = 0, V = 0, eos = -1;
+};
+cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream);
+
+// In place: row g * W + j of every state becomes row g * W + parents[g, j]
+// (the row's old content); a parent outside [0, W) leaves its row alone.  A
+// state's row is [outer, T, inner bytes]; only the first lengths[source row]
+// of the T entries are copied (lengths null: all; T 0: whole rows always).
+struct BeamState {
+  void* p = nullptr;
+  int64_t row_bytes = 0, T = 0, inner = 0;  // inner: bytes of one entry
+};
+cudaError_t beam_reorder(const BeamState* states, int64_t count, const int* parents, const int* lengths, int64_t G,
+                         int64_t W, cudaStream_t stream);
+
 }  // namespace sb

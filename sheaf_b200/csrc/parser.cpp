@@ -22,6 +22,7 @@ const char* dtype_name(DType t) {
     case DType::I32: return "i32";
     case DType::I64: return "i64";
     case DType::I1: return "i1";
+    case DType::I8: return "i8";
   }
   return "?";
 }

@@ -59,6 +59,7 @@ bool etype_to_dtype(uint32_t et, DType* out) {
     case SB_ELEMENT_TYPE_FLOAT_32: *out = DType::F32; return true;
     case SB_ELEMENT_TYPE_BFLOAT_16: *out = DType::BF16; return true;
     case SB_ELEMENT_TYPE_INT_32: *out = DType::I32; return true;
+    case SB_ELEMENT_TYPE_INT_8: *out = DType::I8; return true;
   }
   return false;
 }
@@ -68,6 +69,7 @@ uint32_t dtype_to_etype(DType t) {
     case DType::F32: return SB_ELEMENT_TYPE_FLOAT_32;
     case DType::BF16: return SB_ELEMENT_TYPE_BFLOAT_16;
     case DType::I32: return SB_ELEMENT_TYPE_INT_32;
+    case DType::I8: return SB_ELEMENT_TYPE_INT_8;
     default: return 0;
   }
 }
@@ -122,6 +124,7 @@ struct sb_buffer {
   size_t bytes = 0;
   bool owned = false;
   sb::Type type;
+  int wrapped_on = -1;                // CUDA device of wrapped memory, -1 when the driver does not know it
   std::shared_ptr<sb::OutSlot> slot;  // output of a graph replay: memory owned by the slot
 };
 
@@ -1591,6 +1594,34 @@ sb_status* sb_buffer_allocate_copy(sb_session* s, size_t rank, const uint64_t* s
   return nullptr;
 }
 
+sb_status* sb_buffer_allocate_zero(sb_session* s, size_t rank, const uint64_t* shape, uint32_t et, sb_buffer** out) {
+  if (!s || !out || (rank && !shape)) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL argument");
+  Type t;
+  if (!etype_to_dtype(et, &t.dtype)) return make_status(SB_STATUS_INVALID_ARGUMENT, "unsupported element type");
+  // the byte length must fit: checked on the non-zero extents
+  uint64_t bytes = (uint64_t)dtype_bytes(t.dtype);
+  for (size_t i = 0; i < rank; ++i) {
+    if (shape[i] > (uint64_t)INT64_MAX || (shape[i] && bytes > (uint64_t)INT64_MAX / shape[i]))
+      return make_status(SB_STATUS_INVALID_ARGUMENT, "shape is too large");
+    if (shape[i]) bytes *= shape[i];
+    t.shape.push_back((int64_t)shape[i]);
+  }
+  std::lock_guard<std::mutex> g(s->mu);
+  SB_CUDA(cudaSetDevice(s->dev->ordinal));
+  sb_status* st = nullptr;
+  sb_buffer* b = new_device_buffer(s->dev, t, &st);
+  if (!b) return st;
+  if (b->bytes) {
+    cudaError_t e = cudaMemsetAsync(b->ptr, 0, b->bytes, s->dev->stream);
+    if (e != cudaSuccess) {
+      sb_buffer_release(b);
+      return cuda_status(e, "cudaMemsetAsync");
+    }
+  }
+  *out = b;
+  return nullptr;
+}
+
 sb_status* sb_buffer_wrap_device(sb_session* s, size_t rank, const uint64_t* shape, uint32_t et, void* dptr,
                                  size_t bytes, sb_buffer** out) {
   if (!s || !out || (rank && !shape)) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL argument");
@@ -1606,6 +1637,12 @@ sb_status* sb_buffer_wrap_device(sb_session* s, size_t rank, const uint64_t* sha
   b->bytes = bytes;
   b->ptr = dptr;
   b->owned = false;
+  cudaPointerAttributes at;
+  if (bytes && cudaPointerGetAttributes(&at, dptr) == cudaSuccess) {
+    if (at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) b->wrapped_on = at.device;
+  } else {
+    cudaGetLastError();
+  }
   *out = b;
   return nullptr;
 }
@@ -1691,6 +1728,272 @@ sb_status* sb_optimizer_adamw_step(sb_session* s, size_t n, sb_buffer* const* pa
   if (e != cudaSuccess) return cuda_status(e, "sb_optimizer_adamw_step");
   if (out_global_norm) return wait_stream(s, s->opts.world_size > 1 ? deadline_ms(s) : 0);
   return nullptr;
+}
+
+// --- decoding operators ------------------------------------------------------
+
+namespace {
+
+// Checks of one buffer argument: present, of this session (or wrapped memory
+// of its device), of one of `types` (a bit per DType) and of `shape`.
+sb_status* op_buffer(const sb_session* s, const sb_buffer* b, const char* what, uint32_t types,
+                     const std::vector<int64_t>& shape) {
+  auto bad = [&](const std::string& why) {
+    return make_status(SB_STATUS_INVALID_ARGUMENT, std::string(what) + ": " + why);
+  };
+  if (!b) return bad("NULL buffer");
+  if (b->dev ? b->dev.get() != s->dev.get() : (b->bytes && b->wrapped_on != s->dev->ordinal))
+    return bad(b->dev ? "buffer of another session" : "wrapped memory is not on the session's device");
+  if (!(types >> (int)b->type.dtype & 1u)) return bad(std::string("element type ") + dtype_name(b->type.dtype));
+  if (b->type.shape != shape) {
+    Type want = b->type;
+    want.shape = shape;
+    return bad("got " + b->type.str() + ", expected " + want.str());
+  }
+  return nullptr;
+}
+
+constexpr uint32_t bit(DType t) { return 1u << (int)t; }
+constexpr uint32_t kFloats = bit(DType::F32) | bit(DType::BF16);
+
+bool overlap(const sb_buffer* a, const sb_buffer* b) {
+  if (!a || !b || !a->bytes || !b->bytes) return false;
+  const uintptr_t x = (uintptr_t)a->ptr, y = (uintptr_t)b->ptr;
+  return x < y + b->bytes && y < x + a->bytes;
+}
+
+// The buffers in `written` must not overlap one another or any in `read`.
+sb_status* op_aliases(std::initializer_list<const sb_buffer*> written, std::initializer_list<const sb_buffer*> read) {
+  for (auto a = written.begin(); a != written.end(); ++a) {
+    for (auto b = a + 1; b != written.end(); ++b)
+      if (overlap(*a, *b)) return make_status(SB_STATUS_INVALID_ARGUMENT, "two written buffers overlap");
+    for (auto b : read)
+      if (overlap(*a, b)) return make_status(SB_STATUS_INVALID_ARGUMENT, "a written buffer overlaps one that is read");
+  }
+  return nullptr;
+}
+
+#define SB_OP(expr)                  \
+  do {                               \
+    if (sb_status* st_ = (expr)) return st_; \
+  } while (0)
+
+sb_status* op_cache(const sb_session* s, const sb_kv_cache* c, KvCacheView* out) {
+  if (!c) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL cache");
+  if (!c->k) return make_status(SB_STATUS_INVALID_ARGUMENT, "cache keys: NULL buffer");
+  const std::vector<int64_t> shape = c->k->type.shape;
+  if (shape.size() != 4)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "cache keys: got " + c->k->type.str() +
+                                                       ", expected [slots, heads, capacity, head size]");
+  const DType dt = c->k->type.dtype;
+  SB_OP(op_buffer(s, c->k, "cache keys", kFloats | bit(DType::I8), shape));
+  SB_OP(op_buffer(s, c->v, "cache values", bit(dt), shape));
+  if (shape[3] < 16 || shape[3] > kKvMaxDim || shape[3] % 16)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "head size must be a multiple of 16 from 16 to 256, got " +
+                                                       std::to_string(shape[3]));
+  for (int i = 0; i < 3; ++i)
+    if (shape[i] > INT32_MAX) return make_status(SB_STATUS_INVALID_ARGUMENT, "cache dimension is too large");
+  if (dt == DType::I8) {
+    const std::vector<int64_t> rows(shape.begin(), shape.begin() + 3);
+    SB_OP(op_buffer(s, c->k_scale, "key scales", bit(DType::F32), rows));
+    SB_OP(op_buffer(s, c->v_scale, "value scales", bit(DType::F32), rows));
+  } else if (c->k_scale || c->v_scale) {
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "only an int8 cache has scales");
+  }
+  out->k = c->k->ptr;
+  out->v = c->v->ptr;
+  out->k_scale = c->k_scale ? (float*)c->k_scale->ptr : nullptr;
+  out->v_scale = c->v_scale ? (float*)c->v_scale->ptr : nullptr;
+  out->type = dt == DType::F32 ? KvType::F32 : dt == DType::BF16 ? KvType::BF16 : KvType::I8;
+  out->N = shape[0];
+  out->H = shape[1];
+  out->T = shape[2];
+  out->D = shape[3];
+  return nullptr;
+}
+
+sb_status* op_rank4(const sb_buffer* b, const char* what) {
+  if (!b) return make_status(SB_STATUS_INVALID_ARGUMENT, std::string(what) + ": NULL buffer");
+  if (b->type.shape.size() != 4)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, std::string(what) + ": got " + b->type.str() + ", expected rank 4");
+  return nullptr;
+}
+
+const int* ints(const sb_buffer* b) { return b ? (const int*)b->ptr : nullptr; }
+
+}  // namespace
+
+sb_status* sb_kv_cache_write(sb_session* s, const sb_kv_cache* cache, sb_buffer* positions, sb_buffer* k,
+                             sb_buffer* v) {
+  if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
+  KvCacheView c;
+  SB_OP(op_cache(s, cache, &c));
+  SB_OP(op_rank4(k, "keys"));
+  const int64_t S = k->type.shape[1];
+  SB_OP(op_buffer(s, k, "keys", kFloats, {c.N, S, c.H, c.D}));
+  SB_OP(op_buffer(s, v, "values", bit(k->type.dtype), {c.N, S, c.H, c.D}));
+  SB_OP(op_buffer(s, positions, "positions", bit(DType::I32), {c.N}));
+  SB_OP(op_aliases({cache->k, cache->v, cache->k_scale, cache->v_scale}, {k, v, positions}));
+  std::lock_guard<std::mutex> g(s->mu);
+  SB_CUDA(cudaSetDevice(s->dev->ordinal));
+  if (!k->bytes || !c.T) return nullptr;
+  cudaError_t e = kv_cache_write(c, ints(positions), k->ptr, v->ptr, k->type.dtype == DType::BF16, S, s->dev->stream);
+  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_write");
+}
+
+sb_status* sb_kv_cache_read(sb_session* s, const sb_kv_cache* cache, sb_buffer* starts, sb_buffer* counts,
+                            sb_buffer* k_out, sb_buffer* v_out) {
+  if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
+  KvCacheView c;
+  SB_OP(op_cache(s, cache, &c));
+  SB_OP(op_rank4(k_out, "keys out"));
+  const int64_t S = k_out->type.shape[2];
+  SB_OP(op_buffer(s, k_out, "keys out", kFloats, {c.N, c.H, S, c.D}));
+  SB_OP(op_buffer(s, v_out, "values out", bit(k_out->type.dtype), {c.N, c.H, S, c.D}));
+  if (starts) SB_OP(op_buffer(s, starts, "starts", bit(DType::I32), {c.N}));
+  if (counts) SB_OP(op_buffer(s, counts, "counts", bit(DType::I32), {c.N}));
+  SB_OP(op_aliases({k_out, v_out}, {cache->k, cache->v, cache->k_scale, cache->v_scale, starts, counts}));
+  std::lock_guard<std::mutex> g(s->mu);
+  SB_CUDA(cudaSetDevice(s->dev->ordinal));
+  if (!k_out->bytes || !c.T) return nullptr;
+  cudaError_t e = kv_cache_read(c, ints(starts), ints(counts), k_out->ptr, v_out->ptr,
+                                k_out->type.dtype == DType::BF16, S, s->dev->stream);
+  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_read");
+}
+
+sb_status* sb_kv_cache_attention(sb_session* s, const sb_kv_cache* cache, sb_buffer* positions, sb_buffer* parents,
+                                 sb_buffer* q, float scale, sb_buffer* out) {
+  if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
+  KvCacheView c;
+  SB_OP(op_cache(s, cache, &c));
+  SB_OP(op_rank4(q, "queries"));
+  const int64_t S = q->type.shape[1], Hq = q->type.shape[2];
+  SB_OP(op_buffer(s, q, "queries", kFloats, {c.N, S, Hq, c.D}));
+  SB_OP(op_buffer(s, out, "output", bit(q->type.dtype), {c.N, S, Hq, c.D}));
+  SB_OP(op_buffer(s, positions, "positions", bit(DType::I32), {c.N}));
+  if (parents) SB_OP(op_buffer(s, parents, "parents", bit(DType::I32), {c.N, S}));
+  if (c.H ? Hq % c.H != 0 : Hq != 0)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "query heads (" + std::to_string(Hq) +
+                                                       ") must be a multiple of the cache's heads (" +
+                                                       std::to_string(c.H) + ")");
+  if (S > kKvMaxTokens)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "at most " + std::to_string(kKvMaxTokens) +
+                                                       " tokens per slot, got " + std::to_string(S));
+  if (!std::isfinite(scale)) return make_status(SB_STATUS_INVALID_ARGUMENT, "scale is not finite");
+  SB_OP(op_aliases({out}, {cache->k, cache->v, cache->k_scale, cache->v_scale, positions, parents, q}));
+  std::lock_guard<std::mutex> g(s->mu);
+  SB_CUDA(cudaSetDevice(s->dev->ordinal));
+  if (!out->bytes) return nullptr;
+  if (!c.T) {  // a cache without positions: no keys
+    SB_CUDA(cudaMemsetAsync(out->ptr, 0, out->bytes, s->dev->stream));
+    return nullptr;
+  }
+  CacheAttnArgs a;
+  a.cache = c;
+  a.positions = ints(positions);
+  a.parents = ints(parents);
+  a.q = q->ptr;
+  a.out = out->ptr;
+  a.bf16 = q->type.dtype == DType::BF16;
+  a.S = S;
+  a.Hq = Hq;
+  a.scale = scale;
+  cudaError_t e = cache_attention(a, s->dev->stream);
+  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_attention");
+}
+
+sb_status* sb_beam_select(sb_session* s, sb_buffer* logits, sb_buffer* scores, sb_buffer* finished, int64_t eos,
+                          sb_buffer* out_scores, sb_buffer* out_parents, sb_buffer* out_tokens,
+                          sb_buffer* out_finished) {
+  if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
+  if (!scores || !logits) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL buffer");
+  if (scores->type.shape.size() != 2 || logits->type.shape.size() != 2)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "scores and logits have two dimensions, got " +
+                                                       scores->type.str() + " and " + logits->type.str());
+  BeamSelectArgs a;
+  a.G = scores->type.shape[0];
+  a.W = scores->type.shape[1];
+  a.V = logits->type.shape[1];
+  if (a.W < 1 || a.W > kBeamMax)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "1 to " + std::to_string(kBeamMax) + " beams, got " +
+                                                       std::to_string(a.W));
+  if (a.G > INT32_MAX / 8 || a.V > INT32_MAX) return make_status(SB_STATUS_INVALID_ARGUMENT, "dimension is too large");
+  const std::vector<int64_t> gw = {a.G, a.W};
+  SB_OP(op_buffer(s, logits, "logits", kFloats, {a.G * a.W, a.V}));
+  SB_OP(op_buffer(s, scores, "scores", bit(DType::F32), gw));
+  SB_OP(op_buffer(s, out_scores, "scores out", bit(DType::F32), gw));
+  SB_OP(op_buffer(s, out_parents, "parents out", bit(DType::I32), gw));
+  SB_OP(op_buffer(s, out_tokens, "tokens out", bit(DType::I32), gw));
+  if (eos >= 0) {
+    if (eos >= a.V) return make_status(SB_STATUS_INVALID_ARGUMENT, "the end token is outside the vocabulary");
+    SB_OP(op_buffer(s, finished, "finished", bit(DType::I32), gw));
+    SB_OP(op_buffer(s, out_finished, "finished out", bit(DType::I32), gw));
+  } else if (finished || out_finished) {
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "finished beams need an end token");
+  }
+  if (a.V * a.W < a.W) return make_status(SB_STATUS_INVALID_ARGUMENT, "empty vocabulary");
+  // a group's scores and flags are read before its results are written: those two may be updated in place
+  SB_OP(op_aliases({out_scores, out_parents, out_tokens, out_finished}, {logits}));
+  SB_OP(op_aliases({out_parents, out_tokens, out_finished}, {scores}));
+  SB_OP(op_aliases({out_scores, out_parents, out_tokens}, {finished}));
+  if ((overlap(out_scores, scores) && out_scores->ptr != scores->ptr) ||
+      (overlap(out_finished, finished) && out_finished->ptr != finished->ptr))
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "a written buffer overlaps one that is read");
+  std::lock_guard<std::mutex> g(s->mu);
+  SB_CUDA(cudaSetDevice(s->dev->ordinal));
+  a.logits = logits->ptr;
+  a.bf16 = logits->type.dtype == DType::BF16;
+  a.scores = (const float*)scores->ptr;
+  a.finished = ints(finished);
+  a.out_scores = (float*)out_scores->ptr;
+  a.out_parents = (int*)out_parents->ptr;
+  a.out_tokens = (int*)out_tokens->ptr;
+  a.out_finished = out_finished ? (int*)out_finished->ptr : nullptr;
+  a.eos = eos < 0 ? -1 : eos;
+  cudaError_t e = beam_select(a, s->dev->stream);
+  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_beam_select");
+}
+
+sb_status* sb_beam_reorder(sb_session* s, size_t count, sb_buffer* const* states, const int32_t* time_axes,
+                           sb_buffer* parents, sb_buffer* lengths) {
+  if (!s || (count && (!states || !time_axes))) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL argument");
+  if (!parents || parents->type.shape.size() != 2)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "parents has two dimensions: groups and beams");
+  const int64_t G = parents->type.shape[0], W = parents->type.shape[1];
+  SB_OP(op_buffer(s, parents, "parents", bit(DType::I32), {G, W}));
+  if (W < 1 || W > kBeamMax)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "1 to " + std::to_string(kBeamMax) + " beams, got " +
+                                                       std::to_string(W));
+  if (G > INT32_MAX) return make_status(SB_STATUS_INVALID_ARGUMENT, "dimension is too large");
+  if (lengths) SB_OP(op_buffer(s, lengths, "lengths", bit(DType::I32), {G * W}));
+  std::vector<BeamState> st(count);
+  for (size_t i = 0; i < count; ++i) {
+    const std::string what = "state " + std::to_string(i);
+    if (!states[i]) return make_status(SB_STATUS_INVALID_ARGUMENT, what + ": NULL buffer");
+    const std::vector<int64_t>& shape = states[i]->type.shape;
+    if (shape.empty() || shape[0] != G * W)
+      return make_status(SB_STATUS_INVALID_ARGUMENT, what + ": got " + states[i]->type.str() +
+                                                         ", expected one row per beam (" + std::to_string(G * W) + ")");
+    SB_OP(op_buffer(s, states[i], what.c_str(), kFloats | bit(DType::I32) | bit(DType::I8), shape));
+    const int32_t axis = time_axes[i];
+    if (axis < -1 || axis == 0 || axis >= (int64_t)shape.size())
+      return make_status(SB_STATUS_INVALID_ARGUMENT, what + ": no time axis " + std::to_string(axis));
+    st[i].p = states[i]->ptr;
+    st[i].row_bytes = G * W ? (int64_t)states[i]->bytes / (G * W) : 0;
+    st[i].inner = dtype_bytes(states[i]->type.dtype);
+    st[i].T = axis < 0 ? 0 : shape[axis];
+    for (size_t d = axis < 0 ? 1 : axis + 1; d < shape.size(); ++d) st[i].inner *= shape[d];
+    if (overlap(states[i], parents) || overlap(states[i], lengths))
+      return make_status(SB_STATUS_INVALID_ARGUMENT, what + " overlaps parents or lengths");
+    for (size_t j = 0; j < i; ++j)
+      if (overlap(states[i], states[j]))
+        return make_status(SB_STATUS_INVALID_ARGUMENT, what + " overlaps state " + std::to_string(j));
+  }
+  std::lock_guard<std::mutex> g(s->mu);
+  SB_CUDA(cudaSetDevice(s->dev->ordinal));
+  if (W == 1) return nullptr;  // nothing can move
+  cudaError_t e = beam_reorder(st.data(), (int64_t)count, ints(parents), ints(lengths), G, W, s->dev->stream);
+  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_beam_reorder");
 }
 
 sb_status* sb_buffer_d2h(sb_session* s, sb_buffer* b, void* host, size_t bytes, int64_t timeout_ms) {

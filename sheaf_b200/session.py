@@ -13,6 +13,7 @@ sheaf/src/interpreter/value.rs:69-93); integer index tensors travel as f32
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from typing import List, Optional, Sequence
 
@@ -24,11 +25,14 @@ LIB_PATH = os.path.join(_HERE, "libsheafb200.so")
 ELEMENT_TYPE_FLOAT_32 = (0x21 << 24) | 32
 ELEMENT_TYPE_BFLOAT_16 = (0x31 << 24) | 16
 ELEMENT_TYPE_INT_32 = (0x11 << 24) | 32
+ELEMENT_TYPE_INT_8 = (0x11 << 24) | 8
 
 PRECISIONS = {"fp32": 0, "tf32": 1, "bf16": 2}
 REDUCE = {None: 0, "none": 0, "sum": 1, "mean": 2}
 
-_NP_OF_ETYPE = {ELEMENT_TYPE_FLOAT_32: np.float32, ELEMENT_TYPE_INT_32: np.int32}
+_NP_OF_ETYPE = {ELEMENT_TYPE_FLOAT_32: np.float32, ELEMENT_TYPE_INT_32: np.int32, ELEMENT_TYPE_INT_8: np.int8}
+_ETYPE_OF_NAME = {"f32": ELEMENT_TYPE_FLOAT_32, "bf16": ELEMENT_TYPE_BFLOAT_16, "i32": ELEMENT_TYPE_INT_32,
+                  "int8": ELEMENT_TYPE_INT_8}
 _ETYPE_OF_NP = {np.dtype(np.float32): ELEMENT_TYPE_FLOAT_32, np.dtype(np.int32): ELEMENT_TYPE_INT_32}
 
 
@@ -49,6 +53,10 @@ class _AdamwOptions(ctypes.Structure):
     _fields_ = [("learning_rate", ctypes.c_float), ("beta1", ctypes.c_float), ("beta2", ctypes.c_float),
                 ("epsilon", ctypes.c_float), ("weight_decay", ctypes.c_float), ("max_grad_norm", ctypes.c_float),
                 ("step", ctypes.c_int64)]
+
+
+class _KvCache(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")]
 
 
 class _Stats(ctypes.Structure):
@@ -78,6 +86,8 @@ SIGNATURES = {
                              ctypes.POINTER(ctypes.c_size_t)]),
     "sb_buffer_allocate_copy": (_P, [_P, ctypes.c_size_t, ctypes.POINTER(ctypes.c_uint64), ctypes.c_uint32,
                                      _P, ctypes.c_size_t, ctypes.POINTER(_P)]),
+    "sb_buffer_allocate_zero": (_P, [_P, ctypes.c_size_t, ctypes.POINTER(ctypes.c_uint64), ctypes.c_uint32,
+                                     ctypes.POINTER(_P)]),
     "sb_buffer_wrap_device": (_P, [_P, ctypes.c_size_t, ctypes.POINTER(ctypes.c_uint64), ctypes.c_uint32,
                                    _P, ctypes.c_size_t, ctypes.POINTER(_P)]),
     "sb_buffer_d2h": (_P, [_P, _P, _P, ctypes.c_size_t, ctypes.c_int64]),
@@ -95,6 +105,11 @@ SIGNATURES = {
     "sb_adamw_options_initialize": (None, [ctypes.POINTER(_AdamwOptions)]),
     "sb_optimizer_adamw_step": (_P, [_P, ctypes.c_size_t, ctypes.POINTER(_P), ctypes.POINTER(_P), ctypes.POINTER(_P),
                                      ctypes.POINTER(_P), ctypes.POINTER(_AdamwOptions), ctypes.POINTER(ctypes.c_float)]),
+    "sb_kv_cache_write": (_P, [_P, ctypes.POINTER(_KvCache), _P, _P, _P]),
+    "sb_kv_cache_read": (_P, [_P, ctypes.POINTER(_KvCache), _P, _P, _P, _P]),
+    "sb_kv_cache_attention": (_P, [_P, ctypes.POINTER(_KvCache), _P, _P, _P, ctypes.c_float, _P]),
+    "sb_beam_select": (_P, [_P, _P, _P, _P, ctypes.c_int64, _P, _P, _P, _P]),
+    "sb_beam_reorder": (_P, [_P, ctypes.c_size_t, ctypes.POINTER(_P), ctypes.POINTER(ctypes.c_int32), _P, _P]),
     "sb_gemm_f32_splitk_noalloc": (ctypes.c_int, [_P, _P, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P]),
     "sb_module_inspect": (_P, [ctypes.c_char_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_char_p, ctypes.c_size_t]),
     "sb_module_kernel_source": (_P, [ctypes.c_char_p, ctypes.c_size_t, ctypes.c_char_p, ctypes.c_char_p,
@@ -250,6 +265,32 @@ class DeviceBuffer:
             self.release()
         except Exception:
             pass
+
+
+class KVCache:
+    """A key/value cache: device buffers k, v [slots, heads, capacity, head size]
+    (f32, bf16 or int8) and, for int8, the row scales [slots, heads, capacity].
+    `B200Session.kv_cache` allocates one; this constructor groups buffers that
+    exist (the calls check them)."""
+
+    def __init__(self, k: DeviceBuffer, v: DeviceBuffer, k_scale: Optional[DeviceBuffer] = None,
+                 v_scale: Optional[DeviceBuffer] = None):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    def _c(self) -> _KvCache:
+        return _KvCache(_handle(self.k), _handle(self.v), _handle(self.k_scale), _handle(self.v_scale))
+
+    def buffers(self) -> List[DeviceBuffer]:
+        """The cache's buffers, each with its time axis at 2 (for `beam_reorder`)."""
+        return [b for b in (self.k, self.v, self.k_scale, self.v_scale) if b is not None]
+
+    def release(self):
+        for b in self.buffers():
+            b.release()
+
+
+def _handle(b: Optional[DeviceBuffer]):
+    return None if b is None else b.handle
 
 
 FLAG_NO_ATTENTION_FUSION = 2  # SB_SESSION_FLAG_NO_ATTENTION_FUSION
@@ -414,12 +455,19 @@ class B200Session:
         if not t.is_cuda or not t.is_contiguous():
             raise B200Error(3, "wrap_torch needs a contiguous CUDA tensor")
         et = {torch.float32: ELEMENT_TYPE_FLOAT_32, torch.int32: ELEMENT_TYPE_INT_32,
-              torch.bfloat16: ELEMENT_TYPE_BFLOAT_16}[t.dtype]
+              torch.bfloat16: ELEMENT_TYPE_BFLOAT_16, torch.int8: ELEMENT_TYPE_INT_8}[t.dtype]
         shape = (ctypes.c_uint64 * max(t.dim(), 1))(*t.shape)
         h = ctypes.c_void_p()
         _check(library().sb_buffer_wrap_device(self._h, t.dim(), shape, et, ctypes.c_void_p(t.data_ptr()),
                                                t.numel() * t.element_size(), ctypes.byref(h)))
         return DeviceBuffer(self, h, keepalive=t)
+
+    def zeros(self, shape: Sequence[int], dtype: str = "f32") -> DeviceBuffer:
+        """A device buffer of zeros; dtype "f32", "bf16", "i32" or "int8"."""
+        dims = (ctypes.c_uint64 * max(len(shape), 1))(*shape)
+        h = ctypes.c_void_p()
+        _check(library().sb_buffer_allocate_zero(self._h, len(shape), dims, _ETYPE_OF_NAME[dtype], ctypes.byref(h)))
+        return DeviceBuffer(self, h)
 
     # calls -------------------------------------------------------------------
     def call_device(self, name: str, args: Sequence, reduce: Optional[Sequence] = None) -> List[DeviceBuffer]:
@@ -460,6 +508,62 @@ class B200Session:
         _check(library().sb_optimizer_adamw_step(self._h, n, arr(params), arr(grads), arr(m), arr(v), ctypes.byref(o),
                                                  ctypes.byref(norm) if return_norm else None))
         return (t + 1, norm.value) if return_norm else t + 1
+
+    # decoding ----------------------------------------------------------------
+    # Each call enqueues its work on the session stream and returns.  Buffers of
+    # other CUDA users (`wrap_torch`) are ordered against that stream by the
+    # caller (`cuda_stream`).
+    def kv_cache(self, slots: int, heads: int, capacity: int, head_dim: int, dtype: str = "f32") -> KVCache:
+        """An empty key/value cache; dtype "f32", "bf16" or "int8" (codes and one
+        f32 scale per row)."""
+        if dtype not in ("f32", "bf16", "int8"):
+            raise B200Error(3, f"a cache is f32, bf16 or int8, not {dtype}")
+        shape = (slots, heads, capacity, head_dim)
+        k, v = (self.zeros(shape, dtype) for _ in range(2))
+        if dtype != "int8":
+            return KVCache(k, v)
+        return KVCache(k, v, *(self.zeros(shape[:3]) for _ in range(2)))
+
+    def kv_cache_write(self, cache: KVCache, positions: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer):
+        """Puts rows k, v [slots, tokens, heads, head size] at positions
+        positions[n] + t of the cache (sb_kv_cache_write)."""
+        _check(library().sb_kv_cache_write(self._h, cache._c(), _handle(positions), _handle(k), _handle(v)))
+
+    def kv_cache_read(self, cache: KVCache, k_out: DeviceBuffer, v_out: DeviceBuffer,
+                      starts: Optional[DeviceBuffer] = None, counts: Optional[DeviceBuffer] = None):
+        """The values at positions starts[n] + i, i < counts[n], to rows i of
+        k_out, v_out [slots, heads, rows, head size] (sb_kv_cache_read)."""
+        _check(library().sb_kv_cache_read(self._h, cache._c(), _handle(starts), _handle(counts), _handle(k_out),
+                                          _handle(v_out)))
+
+    def kv_cache_attention(self, cache: KVCache, positions: DeviceBuffer, q: DeviceBuffer, out: DeviceBuffer,
+                           parents: Optional[DeviceBuffer] = None, scale: Optional[float] = None):
+        """out = softmax(scale q k^T) v of the tokens at positions[n] + t over the
+        cache; they form a chain, or the tree that `parents` [slots, tokens] gives
+        (sb_kv_cache_attention).  scale defaults to 1 / sqrt(head size)."""
+        if scale is None:
+            scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape and q.shape[-1] else 1.0
+        _check(library().sb_kv_cache_attention(self._h, cache._c(), _handle(positions), _handle(parents), _handle(q),
+                                               scale, _handle(out)))
+
+    def beam_select(self, logits: DeviceBuffer, scores: DeviceBuffer, out_scores: DeviceBuffer,
+                    out_parents: DeviceBuffer, out_tokens: DeviceBuffer, finished: Optional[DeviceBuffer] = None,
+                    out_finished: Optional[DeviceBuffer] = None, eos: int = -1):
+        """The best continuations of each group of beams (sb_beam_select)."""
+        _check(library().sb_beam_select(self._h, _handle(logits), _handle(scores), _handle(finished), eos,
+                                        _handle(out_scores), _handle(out_parents), _handle(out_tokens),
+                                        _handle(out_finished)))
+
+    def beam_reorder(self, states: Sequence[DeviceBuffer], parents: DeviceBuffer, time_axes: Sequence[int],
+                     lengths: Optional[DeviceBuffer] = None):
+        """Rearranges per-beam state in place to follow the selected beams
+        (sb_beam_reorder): one time axis per state, -1 for whole rows."""
+        n = len(states)
+        if len(time_axes) != n:
+            raise B200Error(3, "states and time_axes must have the same length")
+        arr = (ctypes.c_void_p * max(n, 1))(*[_handle(b) for b in states])
+        axes = (ctypes.c_int32 * max(n, 1))(*time_axes)
+        _check(library().sb_beam_reorder(self._h, n, arr, axes, _handle(parents), _handle(lengths)))
 
     def call(self, name: str, args: Sequence) -> List[np.ndarray]:
         outs = self.call_device(name, args)

@@ -1,0 +1,613 @@
+"""The decoding operators (key/value cache write, read and attention; beam
+selection and reordering) against the 64-bit restatement in
+oracle/decode_ref.py, through the C ABI."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+from oracle import decode_ref as R
+from sheaf_b200 import session as S
+
+U32 = 2.0 ** -24   # half a step of f32, relative
+UBF = 2.0 ** -8    # half a step of bf16, relative
+KINDS = ("f32", "bf16", "int8")
+
+
+# ------------------------------------------------------------------ host (no GPU)
+
+def test_oracle_codes_round_ties_to_even_and_keep_the_largest():
+    x = np.float32([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, 126.5, -127.0]])
+    q, s = R.quantise(x)
+    assert s[0] == 1.0 and q.tolist() == [[127, 0, 2, 2, 0, -2, 126, -127]]
+    q, s = R.quantise(np.zeros((1, 4), np.float32))
+    assert s[0] == 0 and not q.any()
+
+
+def test_oracle_ancestors_of_a_tree_and_a_chain():
+    seen = R.ancestors([-1, 0, 0, 1, 9, -7], 6)
+    assert [np.flatnonzero(r).tolist() for r in seen] == [[0], [0, 1], [0, 2], [0, 1, 3], [4], [5]]
+    assert (R.ancestors(None, 5) == np.tril(np.ones((5, 5), bool))).all()
+
+
+def test_oracle_beam_first_step_and_finished_beams():
+    logits = np.log(np.float64([[0.5, 0.3, 0.2]] * 2))
+    s, p, t, f = R.beam_select(logits, np.float32([[0, -np.inf]]))
+    assert p.tolist() == [[0, 0]] and t.tolist() == [[0, 1]]
+    s, p, t, f = R.beam_select(logits, np.float32([[-1, -0.1]]), np.int32([[0, 1]]), 2)
+    assert p.tolist() == [[1, 0]] and t.tolist() == [[2, 0]] and f.tolist() == [[1, 0]]
+
+
+def test_oracle_reorder_reads_the_old_rows():
+    x = np.arange(8, dtype=np.float32).reshape(4, 2)
+    got = R.reorder(x, np.int32([[1, 0], [1, 5]]), 1, np.int32([1, 2, 0, 1]))
+    assert got.tolist() == [[2, 3], [0, 3], [6, 5], [6, 7]]
+
+
+def test_null_arguments_are_refused_on_the_host(lib):
+    cache = S._KvCache()
+    calls = [lib.sb_kv_cache_write(None, cache, None, None, None),
+             lib.sb_kv_cache_read(None, cache, None, None, None, None),
+             lib.sb_kv_cache_attention(None, cache, None, None, None, 1.0, None),
+             lib.sb_beam_select(None, None, None, None, -1, None, None, None, None),
+             lib.sb_beam_reorder(None, 0, None, None, None, None),
+             lib.sb_buffer_allocate_zero(None, 0, None, S.ELEMENT_TYPE_INT_8, None)]
+    for st in calls:
+        assert st and lib.sb_status_code_of(st) == 3
+        lib.sb_status_free(st)
+
+
+def test_python_checks_before_the_library():
+    s = object.__new__(S.B200Session)
+    with pytest.raises(S.B200Error):
+        s.kv_cache(1, 1, 8, 16, dtype="int4")
+    with pytest.raises(S.B200Error):
+        s.beam_reorder([None], None, [1, 2])
+
+
+# ------------------------------------------------------------------ device
+
+@pytest.fixture(scope="module")
+def sess(lib):
+    s = S.B200Session(device=0, precision="fp32")
+    yield s
+    s.close()
+
+
+def put(sess, a, kind=None):
+    """Device copy of a host array; bf16 arrays hold bf16 values as f32."""
+    a = np.ascontiguousarray(a)
+    if kind == "bf16":
+        return sess.buffer(a, bf16=True)
+    if a.dtype == np.int8:
+        import torch
+        b = sess.wrap_torch(torch.from_numpy(a).cuda())
+        torch.cuda.synchronize()
+        return b
+    return sess.buffer(a)
+
+
+def rand(rng, shape, kind="f32"):
+    x = rng.standard_normal(shape).astype(np.float32)
+    return R.bf16_round(x) if kind == "bf16" else x
+
+
+def make_cache(sess, rng, shape, kind, fill=None):
+    """A filled device cache, its arrays (values or codes) and its scales."""
+    arrays, scales = [], []
+    for _ in range(2):
+        if kind == "int8":
+            arrays.append(rng.integers(-127, 128, shape).astype(np.int8))
+            scales.append((rng.random(shape[:3]) * 0.02 + 0.005).astype(np.float32))
+        else:
+            arrays.append(rand(rng, shape, kind) if fill is None else np.full(shape, fill, np.float32))
+    bufs = [put(sess, a, kind) for a in arrays] + [put(sess, s) for s in scales]
+    return S.KVCache(*bufs), arrays, scales
+
+
+def values(arrays, scales):
+    if not scales:
+        return [a.astype(np.float64) for a in arrays]
+    return [a.astype(np.float64) * s.astype(np.float64)[..., None] for a, s in zip(arrays, scales)]
+
+
+WRITE_SHAPES = [  # slots, tokens, heads, capacity, head size
+    (1, 1, 1, 1, 16), (1, 1, 6, 16, 64), (3, 5, 2, 9, 48), (2, 7, 3, 12, 80), (5, 2, 1, 4, 256), (2, 33, 4, 40, 128),
+    (4, 3, 5, 8, 32)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", WRITE_SHAPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+def test_write_then_read(sess, shape, kind, src):
+    N, n_tok, H, T, D = shape
+    rng = np.random.default_rng([*shape, KINDS.index(kind), len(src)])
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    pos = rng.integers(0, max(1, T - n_tok + 1), N).astype(np.int32)
+    if N > 1:
+        pos[0] = -1 if N > 2 else T - 1          # idle, or running over the capacity
+        pos[-1] = 2 ** 31 - 1 if N > 3 else T - 1
+    x = [rand(rng, (N, n_tok, H, D), src) for _ in range(2)]
+    sess.kv_cache_write(cache, put(sess, pos), put(sess, x[0], src), put(sess, x[1], src))
+    want = [a.copy() for a in arrays]
+    wscale = [s.copy() for s in scales]
+    for i in range(2):
+        R.write(want[i], wscale[i] if kind == "int8" else kind, pos, x[i])
+    got = cache.buffers()
+    for i in range(2):
+        assert np.array_equal(got[i].to_host(), want[i])
+        if kind == "int8":
+            assert np.array_equal(got[2 + i].to_host(), wscale[i])
+    # read back: a window that starts before and ends after the cache, ragged counts
+    rows = T + 3
+    starts = rng.integers(-2, T + 1, N).astype(np.int32)
+    counts = rng.integers(-1, rows + 2, N).astype(np.int32)
+    for out in ("f32", "bf16"):
+        before = [rand(rng, (N, H, rows, D), out) for _ in range(2)]
+        outs = [put(sess, b, out) for b in before]
+        sess.kv_cache_read(cache, outs[0], outs[1], starts=put(sess, starts), counts=put(sess, counts))
+        for i in range(2):
+            ref = before[i].copy()
+            val = want[i] if kind != "int8" else want[i].astype(np.float32) * wscale[i][..., None]
+            for n in range(N):
+                for r in range(min(rows, max(0, int(counts[n])))):
+                    t = int(starts[n]) + r
+                    if 0 <= t < T:
+                        ref[n, :, r] = R.bf16_round(val[n, :, t]) if out == "bf16" else val[n, :, t]
+            assert np.array_equal(outs[i].to_host(), ref)
+    # the whole cache, no starts and counts
+    outs = [sess.zeros((N, H, T, D)) for _ in range(2)]
+    sess.kv_cache_read(cache, outs[0], outs[1])
+    for i in range(2):
+        val = want[i] if kind != "int8" else want[i].astype(np.float32) * wscale[i][..., None]
+        assert np.array_equal(outs[i].to_host(), val)
+
+
+@pytest.mark.gpu
+def test_write_codes_of_hard_rows(sess):
+    """Ties, zeros, subnormal rows, NaN and infinities: codes and scales are the
+    definition's, exactly."""
+    rng = np.random.default_rng(5)
+    D, rows = 64, []
+    rows.append(np.zeros(D))
+    rows.append(np.r_[127.0, np.arange(63) - 31.5])                     # ties at scale 1
+    rows.append(np.r_[127.0, np.arange(63) - 31.5] * 2.0 ** -130)      # the same with a subnormal scale
+    rows.append(np.full(D, 2.0 ** -149))                               # the scale rounds to 0
+    rows.append(np.r_[190 * 2.0 ** -149, np.full(63, 2.0 ** -149)])     # scale one step, code clamped
+    rows.append(np.r_[np.nan, np.inf, -np.inf, rng.standard_normal(61)])
+    rows.append(np.r_[3.4028234e38, rng.standard_normal(63) * 1e37])
+    s = np.float32(0.1237)
+    k = np.arange(63) - 31
+    rows.append(np.r_[np.float32(127 * s), (k + 0.5) * s])               # next to ties of a scale that is not a power of 2
+    x = np.float32(rows + [np.float32(rng.standard_normal(D) * 10.0 ** e) for e in range(-40, 39)])
+    x = x.reshape(1, len(x), 1, D)
+    cache = sess.kv_cache(1, 1, x.shape[1], D, "int8")
+    zero = put(sess, np.int32([0]))
+    sess.kv_cache_write(cache, zero, put(sess, x), put(sess, -x))
+    for b, sc, y in ((cache.k, cache.k_scale, x), (cache.v, cache.v_scale, -x)):
+        q, s = R.quantise(y[0, :, 0])
+        assert np.array_equal(sc.to_host()[0, 0], s)
+        assert np.array_equal(b.to_host()[0, 0], q)
+
+
+def attention_bound(dots, vmax, live, D, out, kind):
+    """How far an f32 evaluation may be from the 64-bit result, per element.
+    A score is D products added in f32 with q pre-scaled: at most (D + 4) half
+    steps of sum |q k| scale, in units of log2 e less than 2 of it; a relative
+    error of e in every probability moves the output by at most 2 e max|v|;
+    exp2 and the running rescalings add a few half steps per term and the sums
+    at most one per addition (`live` of them)."""
+    e = 2 * (D + 4) * U32 * dots + (live + 64) * U32
+    b = 2 * e * vmax
+    if kind == "bf16":
+        b = b + UBF * np.abs(out).max(-1)
+    return b[..., None]
+
+
+ATT_CASES = [  # slots, tokens, q heads, heads, capacity, head size, positions
+    (1, 1, 1, 1, 1, 16, [0]),
+    (1, 1, 6, 6, 256, 64, [200]),
+    (4, 1, 4, 4, 70, 64, [-1, 0, 69, 70]),            # idle, first token, last place, full
+    (3, 1, 8, 2, 133, 128, [1, 64, 132]),
+    (2, 1, 6, 2, 40, 80, [7, 39]),
+    (2, 1, 2, 2, 37, 256, [36, 2 ** 31 - 1]),
+    (2, 1, 5, 1, 90, 32, [17, 88]),
+    (2, 5, 3, 3, 50, 48, [0, 44]),
+    (3, 7, 4, 2, 60, 64, [3, 56, -5]),                # the tokens run over the capacity; idle
+    (1, 64, 2, 2, 300, 64, [200]),
+    (2, 63, 8, 4, 130, 128, [0, 66]),
+    (1, 64, 16, 2, 200, 128, [130]),
+    (2, 16, 4, 4, 1100, 64, [1000, 513]),
+    (1, 33, 8, 1, 777, 64, [700]),
+    (1, 9, 4, 2, 70, 256, [50]),
+    (2, 12, 2, 1, 33, 16, [20, 30]),
+]
+
+
+def tree_of(rng, N, n_tok):
+    p = np.zeros((N, n_tok), np.int32)
+    for n in range(N):
+        for s in range(n_tok):
+            p[n, s] = rng.integers(max(-1, s - 6), s) if s else -1
+    if n_tok > 4:  # values outside [0, t) end the path
+        p[0, 3], p[-1, 4] = 3, -9
+        p[0, n_tok - 1] = 2 ** 31 - 1
+    return p
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", ATT_CASES, ids=lambda c: "x".join(map(str, c[:6])))
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("tree", [False, True])
+def test_attention(sess, case, kind, src, tree):
+    N, n_tok, Hq, H, T, D, pos = case
+    if tree and n_tok == 1:
+        pytest.skip("one token has no tree")
+    rng = np.random.default_rng(n_tok * 1000 + T + D)
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    q = rand(rng, (N, n_tok, Hq, D), src)
+    parents = tree_of(rng, N, n_tok) if tree else None
+    scale = 1 / math.sqrt(D) if not tree else 0.3
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, scale, parents)
+    out = put(sess, np.full(q.shape, 7.0, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out,
+                            parents=None if parents is None else put(sess, parents), scale=None if not tree else scale)
+    got = out.to_host()
+    assert (np.abs(got - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
+    assert not got[live == 0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D", [(1, 1, 64), (1, 4, 128), (6, 2, 64), (40, 2, 64), (40, 4, 128)])
+def test_attention_ignores_what_it_does_not_attend_to(sess, kind, src, n_tok, G, D):
+    """NaN and infinities behind the last token, and in drafted tokens that are
+    no ancestors, change nothing; a NaN in an ancestor reaches its descendants."""
+    rng = np.random.default_rng(n_tok + G)
+    N, H, T, pos = 2, 2, 210, [150, 33]
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    q = rand(rng, (N, n_tok, G * H, D), src)
+    parents = np.full((N, n_tok), -1, np.int32)
+    if n_tok > 5:
+        parents[:, 5] = 2
+    run = lambda: _attend(sess, arrays, scales, kind, pos, q, src, parents)
+    clean = run()
+    bad = [np.nan, np.inf, -np.inf]
+    for n in range(N):
+        for t in range(pos[n] + n_tok, T):
+            for i in range(2):
+                if scales:
+                    scales[i][n, :, t] = bad[t % 3]
+                else:
+                    arrays[i][n, :, t] = bad[t % 3]
+    assert np.array_equal(run(), clean)
+    if n_tok > 5:
+        for n in range(N):
+            for i in range(2):
+                if scales:
+                    scales[i][n, :, pos[n] + 2] = np.nan
+                else:
+                    arrays[i][n, :, pos[n] + 2] = np.nan
+        got = run()
+        others = [s for s in range(n_tok) if s not in (2, 5)]
+        assert np.isnan(got[:, [2, 5]]).all()
+        # a kernel may treat tokens next to bad values in another order of operations: the probabilities' rounding
+        # and the output's, each at most half a step of the output's type on either side, times the largest value
+        vmax = max(np.abs(values(arrays, scales)[1][n, :, :pos[n] + 2]).max() for n in range(N))
+        step = UBF if src == "bf16" else 2.0 ** -17
+        assert (np.abs(got[:, others] - clean[:, others]) <= 4 * step * vmax).all()
+
+
+def _attend(sess, arrays, scales, kind, pos, q, src, parents):
+    cache = S.KVCache(*([put(sess, a, kind) for a in arrays] + [put(sess, s) for s in scales]))
+    out = put(sess, np.zeros(q.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out, parents=put(sess, parents))
+    return out.to_host()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+def test_attention_over_a_cache_beyond_32_bit_offsets(sess, kind, src):
+    """2^31 values and more per buffer: the last slot's rows are found."""
+    import torch
+    N, H, T, D = 3, 1, 6_000_000, 128
+    free = torch.cuda.mem_get_info()[0]
+    if free < 16 << 30:
+        pytest.skip("not enough memory")
+    rng = np.random.default_rng(11)
+    cache = sess.kv_cache(N, H, T, D, kind)
+    pos = np.int32([5, T - 2, T - 1])
+    n_tok = 2
+    x = [rand(rng, (N, n_tok, H, D)) for _ in range(2)]
+    sess.kv_cache_write(cache, put(sess, pos), put(sess, x[0]), put(sess, x[1]))
+    outs = [sess.zeros((N, H, n_tok, D)) for _ in range(2)]
+    sess.kv_cache_read(cache, outs[0], outs[1], starts=put(sess, pos))
+    vals = [o.to_host().astype(np.float64) for o in outs]
+    for i in range(2):
+        q, s = R.quantise(x[i])
+        want = q.astype(np.float32) * s[..., None] if kind == "int8" else R.bf16_round(x[i])
+        for n in range(N):
+            for t in range(n_tok):
+                if pos[n] + t < T:
+                    assert np.array_equal(vals[i][n, :, t].astype(np.float32), want[n, t])
+    # every other key is zero: its score is 0, its value 0
+    qv = rand(rng, (N, n_tok, 1, D), src) * 4
+    qv = R.bf16_round(qv)
+    out = put(sess, np.zeros(qv.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, pos), put(sess, qv, src), out, scale=0.25)
+    got = out.to_host()
+    for n in range(N):
+        for s in range(n_tok):
+            e = [(np.exp(0.25 * float(vals[0][n, 0, j] @ qv[n, s, 0])), vals[1][n, 0, j]) for j in range(s + 1)
+                 if pos[n] + j < T]
+            total = min(int(pos[n]), T) + sum(a for a, _ in e)
+            ref = sum(a * b for a, b in e) / total
+            # sums of 6e6 equal terms: each lane adds a fraction of them in order
+            tol = (2 * 132 * U32 * 100 + T / 256 * U32) * np.abs(ref).max() + (UBF * np.abs(ref).max() if src == "bf16" else 0)
+            assert np.abs(got[n, s, 0] - ref).max() <= tol + 1e-12
+    cache.release()
+
+
+SELECT_CASES = [  # groups, beams, vocabulary
+    (1, 1, 1), (1, 1, 2), (1, 4, 65), (3, 5, 7), (2, 16, 3), (2, 16, 16), (4, 8, 1000), (1, 16, 50257), (2, 3, 4097),
+    (70, 2, 129), (1, 7, 131071), (5, 8, 50304)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G,W,V", SELECT_CASES)
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("ends", [False, True])
+def test_beam_select(sess, G, W, V, kind, ends):
+    rng = np.random.default_rng(G + 10 * W + V)
+    logits = (rng.standard_normal((G * W, V)) * 3).astype(np.float32)
+    if kind == "bf16":
+        logits = R.bf16_round(logits)  # many equal logits
+    scores = -np.sort(rng.random((G, W)) * 9).astype(np.float32)
+    eos = V // 2 if ends else -1
+    fin = (rng.random((G, W)) < 0.4).astype(np.int32)
+    check_select(sess, logits, scores, fin, eos, kind)
+
+
+def check_select(sess, logits, scores, fin, eos, kind="f32"):
+    ref = R.beam_select(logits, scores, fin, eos)
+    sc, fi = put(sess, scores), put(sess, fin)
+    par, tok = sess.zeros(scores.shape, "i32"), sess.zeros(scores.shape, "i32")
+    # scores and flags in place, as a search loop keeps them
+    if eos >= 0:
+        sess.beam_select(put(sess, logits, kind), sc, sc, par, tok, finished=fi, out_finished=fi, eos=eos)
+        assert np.array_equal(fi.to_host(), ref[3])
+    else:
+        sess.beam_select(put(sess, logits, kind), sc, sc, par, tok)
+    assert np.array_equal(par.to_host(), ref[1])
+    assert np.array_equal(tok.to_host(), ref[2])
+    # the value is formed in f64 and rounded once
+    got = sc.to_host().astype(np.float64)
+    same = got == ref[0]
+    with np.errstate(invalid="ignore"):
+        assert (same | (np.abs(got - ref[0]) <= U32 * np.abs(ref[0]) * 1.001 + 1e-13)).all()
+
+
+@pytest.mark.gpu
+def test_beam_select_ties_masks_and_bad_values(sess):
+    rng = np.random.default_rng(2)
+    W, V = 6, 3000
+    zero = np.zeros((1, W), np.int32)
+    # every logit equal: the lowest tokens of the best beam, and of equal beams in turn
+    check_select(sess, np.zeros((W, V), np.float32), np.float32([[-1] * W]), zero, -1)
+    check_select(sess, np.zeros((W, V), np.float32), np.float32([[0] + [-np.inf] * (W - 1)]), zero, 7)
+    # identical beams (same prefix): exact ties between beams
+    row = rng.standard_normal((1, V)).astype(np.float32)
+    check_select(sess, np.repeat(row, W, 0), np.float32([[-2] * W]), zero, -1)
+    # all but a few tokens masked, a whole beam masked, NaN, the lowest finite value, infinities
+    x = np.full((W, V), -np.inf, np.float32)
+    x[0, [5, 2999]] = [1.0, 1.0]
+    x[1, 17] = -3e38
+    x[2] = np.finfo(np.float32).min
+    x[3] = np.nan
+    x[4, 3] = np.inf
+    check_select(sess, x, np.float32([[-1, -2, -3, -4, -5, -6]]), zero, -1)
+    check_select(sess, x, np.float32([[-np.inf, np.nan, -3, -4, -5, np.inf]]), zero, 2)
+    # every beam finished
+    check_select(sess, rng.standard_normal((W, V)).astype(np.float32), -np.float32([[1, 5, 2, 2, 9, 0]]), zero + 1, 0)
+    # values that differ beyond 32 bits only: the sums decide between beams
+    base = rng.standard_normal(V).astype(np.float32)
+    x = np.stack([base] * W)
+    x[1:, -1] += np.float32([1e-3, 2e-3, 3e-3, 4e-3, 5e-3])
+    check_select(sess, x, np.float32([[-40] * W]), zero, -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("G,W", [(1, 1), (1, 2), (3, 3), (2, 8), (1, 16), (5, 11)])
+def test_beam_reorder(sess, G, W):
+    rng = np.random.default_rng(W)
+    N = G * W
+    T = 19
+    states = [(rand(rng, (N, 3, T, 16)), 2, None), (rand(rng, (N, 2, T, 48), "bf16"), 2, "bf16"),
+              (rng.integers(-127, 128, (N, 2, T, 16)).astype(np.int8), 2, None), (rand(rng, (N, 3, T)), 2, None),
+              (rng.integers(0, 99, (N, T)).astype(np.int32), 1, None), (rand(rng, (N, 5), "bf16"), -1, "bf16"),
+              (rng.integers(-9, 9, (N, 7)).astype(np.int8), 1, None), (rand(rng, (N,)), -1, None),
+              (rand(rng, (N, T, 3, 2)), 1, None), (rand(rng, (N, 2, 0, 4)), 2, None)]
+    states += [(rng.integers(0, 9, (N, 2)).astype(np.int32), -1, None) for _ in range(50)]  # two launches
+    parents = rng.integers(0, W, (G, W)).astype(np.int32)
+    if W > 2:
+        parents[0, 1], parents[-1, 2] = W, -1  # out of range: the row stays
+    lengths = rng.integers(-1, T + 3, N).astype(np.int32)
+    for lens in (None, lengths):
+        bufs = [put(sess, a, k) for a, _, k in states]
+        sess.beam_reorder(bufs, put(sess, parents), [ax for _, ax, _ in states],
+                          lengths=None if lens is None else put(sess, lens))
+        for b, (a, ax, _) in zip(bufs, states):
+            assert np.array_equal(b.to_host(), R.reorder(a, parents, ax, lens)), (a.shape, ax)
+
+
+@pytest.mark.gpu
+def test_refusals_launch_nothing(sess, lib):
+    other = S.B200Session(device=0, precision="fp32")
+    z = sess.zeros
+    c8, c32 = sess.kv_cache(2, 2, 8, 32, "int8"), sess.kv_cache(2, 2, 8, 32)
+    pos = z((2,), "i32")
+    kv = [z((2, 1, 2, 32)) for _ in range(2)]
+    q, out = z((2, 1, 4, 32)), z((2, 1, 4, 32))
+    n0 = lib.sb_kernel_launch_count()
+
+    def refused(f, *a, **k):
+        with pytest.raises(S.B200Error) as e:
+            f(*a, **k)
+        assert e.value.code == 3
+
+    w = lambda c, p=pos, k=kv[0], v=kv[1]: sess.kv_cache_write(c, p, k, v)
+    refused(w, S.KVCache(c8.k, c8.v))                                   # int8 without scales
+    refused(w, S.KVCache(c32.k, c32.v, c8.k_scale, c8.v_scale))         # f32 with scales
+    refused(w, S.KVCache(c32.k, c8.v, c8.k_scale, c8.v_scale))          # types differ
+    refused(w, S.KVCache(c32.k, c32.k))                                 # one buffer for both
+    refused(w, S.KVCache(c8.k, c8.v, c8.k_scale, z((2, 2, 9))))         # scale shape
+    refused(w, S.KVCache(None, c32.v))
+    for d in (8, 24, 272):
+        refused(w, sess.kv_cache(2, 2, 8, d), k=z((2, 1, 2, d)), v=z((2, 1, 2, d)))
+    refused(w, c32, p=z((3,), "i32"))
+    refused(w, c32, p=z((2,)))                                          # positions are i32
+    refused(w, c32, p=other.zeros((2,), "i32"))                         # another session's buffer
+    refused(w, c32, k=z((2, 1, 2, 16)))
+    refused(w, c32, k=z((2, 1, 32)))
+    refused(w, c32, k=z((2, 1, 2, 32), "bf16"))                         # k and v differ
+    refused(w, c32, k=None)
+    refused(sess.kv_cache_read, c32, z((2, 2, 4, 32)), z((2, 2, 5, 32)))
+    refused(sess.kv_cache_read, c32, z((2, 2, 4, 32), "i32"), z((2, 2, 4, 32), "i32"))
+    refused(sess.kv_cache_read, c32, c32.k, z((2, 2, 8, 32)))           # out of the cache into itself
+    refused(sess.kv_cache_read, c32, z((2, 2, 4, 32)), z((2, 2, 4, 32)), starts=z((1,), "i32"))
+    a = sess.kv_cache_attention
+    refused(a, c32, pos, q, q)
+    refused(a, c32, pos, z((2, 1, 3, 32)), z((2, 1, 3, 32)))            # 3 query heads on 2
+    refused(a, c32, pos, z((2, 65, 2, 32)), z((2, 65, 2, 32)))          # more than 64 tokens
+    refused(a, c32, pos, q, z((2, 1, 4, 32), "bf16"))
+    refused(a, c32, pos, q, out, parents=z((2, 2), "i32"))
+    refused(a, c32, pos, q, out, scale=float("nan"))
+    refused(a, c32, None, q, out)
+    lg, sc, i1, i2, i3 = z((4, 9)), z((2, 2)), z((2, 2), "i32"), z((2, 2), "i32"), z((2, 2), "i32")
+    b = sess.beam_select
+    refused(b, lg, z((2, 3)), z((2, 3)), i1, i2)
+    refused(b, z((34, 9)), z((2, 17)), z((2, 17)), z((2, 17), "i32"), z((2, 17), "i32"))
+    refused(b, z((4, 0)), sc, sc, i1, i2)
+    refused(b, lg, sc, sc, i1, i1)
+    refused(b, lg, sc, sc, i1, i2, eos=3)                               # an end token needs the flags
+    refused(b, lg, sc, sc, i1, i2, finished=i3, out_finished=i3, eos=9)
+    refused(b, lg, sc, sc, i1, i2, finished=i3, out_finished=i3)
+    refused(b, lg, sc, sc, i1, i2, finished=i1, out_finished=i3, eos=1)
+    refused(b, z((4, 9), "i32"), sc, sc, i1, i2)
+    par = z((2, 2), "i32")
+    r = sess.beam_reorder
+    refused(r, [z((3, 4))], par, [1])
+    refused(r, [z((4, 4))], par, [2])
+    refused(r, [z((4, 4))], par, [0])
+    refused(r, [z((4, 4))], z((4,), "i32"), [1])
+    refused(r, [lg, lg], par, [1, 1])
+    refused(r, [z((4, 4))], par, [1], lengths=z((2,), "i32"))
+    refused(r, [None], par, [1])
+    lens = z((4,), "i32")
+    refused(r, [lens], par, [-1], lengths=lens)
+    assert lib.sb_kernel_launch_count() == n0
+    # empty calls do nothing and succeed
+    e = sess.kv_cache(0, 2, 8, 32)
+    sess.kv_cache_write(e, z((0,), "i32"), z((0, 1, 2, 32)), z((0, 1, 2, 32)))
+    sess.kv_cache_attention(e, z((0,), "i32"), z((0, 1, 2, 32)), z((0, 1, 2, 32)))
+    e = sess.kv_cache(2, 2, 0, 32, "int8")
+    w(e)
+    o = put(sess, np.ones((2, 1, 4, 32), np.float32))
+    sess.kv_cache_attention(e, pos, q, o)
+    assert not o.to_host().any()
+    b(z((0, 9)), z((0, 2)), z((0, 2)), z((0, 2), "i32"), z((0, 2), "i32"))
+    r([], par, [])
+    r([z((0, 4))], z((0, 2), "i32"), [1])
+    assert lib.sb_kernel_launch_count() == n0
+    other.close()
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_the_run(sess):
+    """The same call gives the same bits, alone, between other calls and from
+    two sessions at once."""
+    rng = np.random.default_rng(8)
+    other = S.B200Session(device=0, precision="fp32")
+    got = []
+    for s in (sess, other):
+        cache, arrays, scales = make_cache(s, np.random.default_rng(1), (3, 4, 900, 64), "int8")
+        q = put(s, rand(np.random.default_rng(2), (3, 20, 8, 64)))
+        pos = put(s, np.int32([850, 3, 400]))
+        lg = put(s, rand(np.random.default_rng(3), (12, 5000)))
+        sc = put(s, -np.abs(rand(np.random.default_rng(4), (3, 4))))
+        got.append((s, cache, q, pos, lg, sc))
+    outs = []
+    for _ in range(3):
+        for s, cache, q, pos, lg, sc in got:
+            o, osc, op, ot = s.zeros((3, 20, 8, 64)), s.zeros((3, 4)), s.zeros((3, 4), "i32"), s.zeros((3, 4), "i32")
+            s.kv_cache_attention(cache, pos, q, o)
+            s.beam_select(lg, sc, osc, op, ot)
+            outs.append((o, osc, op, ot))
+    first = [b.to_host() for b in outs[0]]
+    for o in outs[1:]:
+        for a, b in zip(first, o):
+            assert np.array_equal(a, b.to_host())
+    other.close()
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed(sess):
+    """A write, attention, selection and reorder captured on the session stream
+    and replayed on new inputs equal the calls made one by one."""
+    import torch
+    G, W, H, T, D, V = 2, 3, 2, 50, 64, 300
+    N = G * W
+    rng = np.random.default_rng(3)
+    dev = torch.device("cuda:0")
+    t = {"k": torch.zeros(N, 2, H, D, device=dev), "v": torch.zeros(N, 2, H, D, device=dev),
+         "q": torch.zeros(N, 2, 2 * H, D, device=dev), "out": torch.zeros(N, 2, 2 * H, D, device=dev),
+         "pos": torch.zeros(N, dtype=torch.int32, device=dev), "lg": torch.zeros(N, V, device=dev),
+         "sc": torch.zeros(G, W, device=dev), "par": torch.zeros(G, W, dtype=torch.int32, device=dev),
+         "tok": torch.zeros(G, W, dtype=torch.int32, device=dev)}
+    b = {k: sess.wrap_torch(x) for k, x in t.items()}
+    cache = sess.kv_cache(N, H, T, D, "int8")
+
+    def step():
+        sess.kv_cache_write(cache, b["pos"], b["k"], b["v"])
+        sess.kv_cache_attention(cache, b["pos"], b["q"], b["out"])
+        sess.beam_select(b["lg"], b["sc"], b["sc"], b["par"], b["tok"])
+        sess.beam_reorder(cache.buffers(), b["par"], [2] * 4)
+
+    def feed(seed):
+        r = np.random.default_rng(seed)
+        for k in ("k", "v", "q", "lg", "sc"):
+            t[k].copy_(torch.from_numpy(rand(r, tuple(t[k].shape))))
+        t["pos"].copy_(torch.from_numpy(r.integers(0, T - 2, N).astype(np.int32)))
+        torch.cuda.synchronize()
+
+    def results():
+        sess.synchronize()
+        return [t[k].cpu().numpy() for k in ("out", "sc", "par", "tok")] + [x.to_host() for x in cache.buffers()]
+
+
+    want = []
+    for seed in range(3):
+        feed(seed)
+        step()
+        want.append(results())
+    cache.release()
+    cache = sess.kv_cache(N, H, T, D, "int8")
+    sess.synchronize()
+    stream = torch.cuda.ExternalStream(sess.cuda_stream, device=dev)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        step()
+    for seed in range(3):
+        feed(seed)
+        with torch.cuda.stream(stream):
+            g.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(results(), want[seed]):
+            assert np.array_equal(a, c)
+    del g
