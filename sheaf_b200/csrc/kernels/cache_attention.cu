@@ -396,6 +396,7 @@ cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream) {
+  if (cache_attention_tc_takes(a)) return cache_attention_tc(a, stream);
   switch (a.cache.type) {
     case KvType::F32: return by_dim<float>(a, stream);
     case KvType::BF16: return by_dim<__nv_bfloat16>(a, stream);

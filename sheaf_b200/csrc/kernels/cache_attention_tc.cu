@@ -1,0 +1,768 @@
+// Attention of a chain or tree of drafted tokens over a bf16 or int8 cache on
+// the tcgen05 tensor cores.  Same definition as cache_attention.cu; used where
+// many query rows (tokens x query heads that share a cache head) read the same
+// keys, so that the products and not the loads bound the CUDA cores.
+//
+// A cluster of C CTAs carries up to 256 rows of one (slot, cache head); the
+// key tiles are split over its CTAs.  A CTA runs two softmax streams of four
+// warps, each with its own S tile and O accumulator in TMEM:
+//   more than 128 rows: stream a takes rows 128 a .., both read every tile;
+//   otherwise:          stream a takes the tiles of parity a, both with the
+//                       same rows (their results are joined at the end); with
+//                       at most 64 rows stream 1 uses the upper half of the
+//                       TMEM lanes, so the two use different SM quarters.
+// While one stream turns S into P the tensor cores work for the other.  Warp
+// roles: 8 softmax, 4 loading, 1 issuing the MMAs.
+//
+//   S = Q K^T   bf16 operands.  f32 queries are split exactly into three bf16
+//               parts (8 mantissa bits each) whose products accumulate into
+//               the same f32 S, so S has f32 accuracy; cache values are bf16
+//               or int8 codes, which bf16 holds exactly.
+//   P           exp2(S - m) times the value row's int8 scale, written back over
+//               S in TMEM as bf16 (bf16 output: one rounding, as large as the
+//               output's own) or as three bf16 parts (f32 output: f32 accuracy;
+//               two parts would leave 2^-16 of each probability).
+//   O += P V    the maximum m a row refers to moves only when it would grow by
+//               more than 2^8, so O is rescaled in the first tiles and then
+//               hardly ever; exact since P, O and the sum l share m.
+//
+// bf16 tiles arrive by TMA, int8 tiles through registers (codes to bf16 on the
+// way to swizzled shared memory).  Rows of V behind the last token are zeroed
+// (0 x NaN would reach every row); a value of a drafted token that is not
+// finite is taken out of the tile and added to the rows that attend to it when
+// the outputs are joined.
+//
+// Every mbarrier wait is bounded.  TMEM is freed before the cluster barrier: a
+// CTA that holds TMEM never waits for another CTA.
+#include <cuda_bf16.h>
+
+#include <cmath>
+
+#include "kernels.h"
+#include "pdl.h"
+#include "tc_common.h"
+
+namespace sb {
+namespace {
+
+using namespace tc;
+
+constexpr int kSoftWarps = 8, kLoadWarps = 4, kWarps = kSoftWarps + kLoadWarps + 1, kThreads = kWarps * 32;
+constexpr int kLoadThreads = kLoadWarps * 32;
+constexpr int NS = 2;   // K and V tiles in flight
+constexpr int NSC = 4;  // rows of scales in flight (see the loader)
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;  // a row's maximum moves when it would grow by more than this (log2)
+
+struct Params {
+  const void *k, *v;
+  const float *ks, *vs;
+  const int *positions, *parents;
+  const void* q;
+  void* out;
+  int q_bf16;
+  int H, G, S, D, pairs;  // pairs: blocks of MAXR rows
+  int64_t T;
+  float scale2;
+};
+
+// D (TMEM) (+)= A (TMEM, bf16 pairs: lane = row, column = two k) * B.
+__device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
+  tmem_ld16_async(taddr, r);
+  tmem_ld16_async(taddr + 16, r + 16);
+}
+__device__ __forceinline__ void reg_fence32(uint32_t* r) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// (lo, hi) f32 to packed bf16, rounded to nearest even
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// 16 codes to 16 bf16 values.  A code's low 7 bits and its sign bit, each put
+// under the exponent of 128 (bf16 steps of 1 from 128 to 256), differ by the
+// code: (128 + low) - (128 or 256) = code, exactly.
+__device__ __forceinline__ void codes_to_bf16(const uint4& c, uint4* out) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t t = __byte_perm(w[i / 2], 0, i & 1 ? 0x4342 : 0x4140);
+    const uint32_t a = (t & 0x007f007fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
+    __nv_bfloat162 x = __hsub2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+    o[i] = *(uint32_t*)&x;
+  }
+  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// 16-byte unit u (of 8 per 128-byte row and 64-value chunk) of row r in a
+// 128-byte-swizzled tile of `rows` rows.
+__device__ __forceinline__ uint32_t unit_at(int rows, int r, int unit) {
+  return (uint32_t)((unit >> 3) * rows * 128 + r * 128 + (((unit & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void loaders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kLoadThreads) : "memory"); }
+
+template <int DP, int BN, int QP>
+struct Cfg {
+  static constexpr int MAXR = QP == 3 && DP == 128 ? 128 : 256;  // query rows of a CTA
+  static constexpr int QTILE = 128 * DP * 2;                     // one part of 128 rows
+  static constexpr int Q_BYTES = (MAXR / 128) * QP * QTILE;
+  static constexpr int TILE = BN * DP * 2;
+  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NS * TILE, END = V_OFF + NS * TILE;
+  static constexpr int LDO = DP + 4;  // padded row of the joined outputs, f32
+  static constexpr int JOIN = 256 * LDO * 4;
+  static constexpr int SMEM = END > JOIN ? END : JOIN;
+  static constexpr uint32_t COLS = 512;
+  // S (P's first two parts in place), O, P's third part; two streams each
+  static constexpr uint32_t S_COL = 0, O_COL = 2 * BN, T_COL = O_COL + 2 * DP;
+  static_assert(2 * BN + 2 * DP + (QP == 3 ? BN : 0) <= 512, "TMEM columns");
+};
+
+struct Shared {
+  uint64_t k_full[NS], k_free[NS], v_full[NS], v_free[NS], sc_full[NSC], s_bar[2], p_bar[2], o_bar[2], raw;
+  uint32_t tslot;
+  volatile int abort_flag;
+  int bad;  // a drafted value that is not finite was taken out of a tile
+  unsigned long long mask[kKvMaxTokens];
+  int jump[kKvMaxTokens];
+  float m[256], l[256];
+};
+
+// see cache_attention.cu
+__device__ void tree_masks(const int* parents, int S, int lane, unsigned long long* mask, int* jump) {
+  for (int s = lane; s < S; s += 32) {
+    const int q = parents ? parents[s] : s - 1;
+    jump[s] = q >= 0 && q < s ? q : -1;
+    mask[s] = 1ull << s;
+  }
+  __syncwarp();
+  for (int d = 1; d < S; d *= 2) {
+    unsigned long long m[2];
+    int j[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = lane + 32 * i;
+      if (s < S) {
+        const int t = jump[s];
+        m[i] = mask[s] | (t >= 0 ? mask[t] : 0ull);
+        j[i] = t >= 0 ? jump[t] : -1;
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = lane + 32 * i;
+      if (s < S) mask[s] = m[i], jump[s] = j[i];
+    }
+    __syncwarp();
+  }
+}
+
+// I8: int8 cache, else bf16.  QP: parts of a query (1: bf16, 3: f32).
+template <int DP, int BN, int QP, bool I8>
+__global__ void __launch_bounds__(kThreads, 1)
+    cache_attn_tc(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const Params p,
+                  int* err) {
+  using F = Cfg<DP, BN, QP>;
+  pdl_prologue();
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ Shared sh;
+  __shared__ __align__(16) float sc_k[I8 ? NSC : 1][I8 ? BN : 4], sc_v[I8 ? NSC : 1][I8 ? BN : 4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  uint32_t C;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
+  const int64_t item = blockIdx.x / C;
+  const int pair = (int)(item % p.pairs);
+  const int64_t nh = item / p.pairs, n = nh / p.H;
+  const int h = (int)(nh % p.H);
+  const int64_t pos = p.positions[n];
+  const int64_t pre = pos < 0 ? 0 : min(pos, p.T), end = pos < 0 ? 0 : min(pos + p.S, p.T);
+  const int r0 = pair * F::MAXR, rows = min(F::MAXR, p.S * p.G - r0);
+  const bool split = rows > 128;                 // streams by rows, else by tiles
+  const int up = !split && rows <= 64 ? 64 : 0;  // stream 1's first TMEM lane
+  // this CTA's tiles [first, first + nt)
+  const int tiles = (int)((end + BN - 1) / BN);
+  const int first = (int)((int64_t)tiles * rank / C), nt = (int)((int64_t)tiles * (rank + 1) / C) - first;
+  const bool aligned = !(smem_u32(smem) & 1023u);
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&sh.k_full[i], I8 ? kLoadWarps : 1);
+      mbar_init(&sh.v_full[i], I8 ? kLoadWarps : 1);
+      mbar_init(&sh.k_free[i], 1);
+      mbar_init(&sh.v_free[i], 1);
+    }
+    for (int i = 0; i < NSC; ++i) mbar_init(&sh.sc_full[i], kLoadWarps);
+    for (int a = 0; a < 2; ++a) {
+      const int mine = split ? min(128, rows - 128 * a) : rows;
+      mbar_init(&sh.s_bar[a], 1);
+      mbar_init(&sh.p_bar[a], (uint32_t)((mine + 31) / 32));
+      mbar_init(&sh.o_bar[a], 1);
+    }
+    mbar_init(&sh.raw, 1);
+    sh.abort_flag = aligned ? 0 : 1;
+    sh.bad = 0;
+    if (!aligned) atomicExch(err, 50);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async();
+  }
+  if (warp == 0) tmem_alloc(&sh.tslot, F::COLS);
+  if (warp == 1) tree_masks(p.parents ? p.parents + n * p.S : nullptr, p.S, lane, sh.mask, sh.jump);
+  // queries into swizzled K-major tiles: tile (row block, part) of 128 rows;
+  // one block of rows repeated at lane `up` when stream 1 uses those lanes
+  if (nt > 0 && aligned) {
+    constexpr int UNITS = DP / 8;
+    const int blocks = split ? 2 : 1;
+    for (int i = tid; i < blocks * 128 * UNITS; i += kThreads) {
+      const int u = i % UNITS, r = (i / UNITS) % 128, b = i / (UNITS * 128);
+      const int local = split ? b * 128 + r : (up && r >= 64 ? r - 64 : r);
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      if (local < rows && u * 8 < p.D) {
+        const int row = r0 + local;
+        const int64_t at = ((n * p.S + row / p.G) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + u * 8;
+        if (QP == 1) {
+          *(uint4*)x = *(const uint4*)((const __nv_bfloat16*)p.q + at);
+        } else {
+          const float4* s = (const float4*)((const float*)p.q + at);
+          const float4 a = s[0], c = s[1];
+          x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
+        }
+      }
+      uint8_t* dst = smem + b * QP * F::QTILE + unit_at(128, r, u);
+      if (QP == 1) {
+        *(uint4*)dst = *(const uint4*)x;
+      } else {
+        // x = part 0 + part 1 + part 2, each a bf16 rounding of what is left
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= p.scale2;
+#pragma unroll
+        for (int part = 0; part < QP; ++part) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+            x[2 * j] -= bf_lo(w[j]);
+            x[2 * j + 1] -= bf_hi(w[j]);
+          }
+          *(uint4*)(dst + part * F::QTILE) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+    fence_proxy_async();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tslot;
+  volatile int* abort_flag = &sh.abort_flag;
+  // tiles of stream a, and the i-th of them (relative to `first`)
+  auto count = [&](int a) { return split ? nt : (nt - a + 1) / 2; };
+  auto tile = [&](int a, int i) { return split ? i : 2 * i + a; };
+
+  if (warp < kSoftWarps) {
+    // ------------------------------------------------------------ softmax
+    const int a = warp >> 2, quad = warp & 3;
+    const int lo_lane = split ? 0 : a * up;  // the stream's first TMEM lane
+    const int mine = split ? min(128, rows - 128 * a) : rows;
+    const int q0 = quad * 32 - lo_lane;  // first row of this warp within the stream
+    if (q0 >= 0 && q0 < mine) {
+      const int local = q0 + lane;  // row within the stream
+      const int row = r0 + (split ? 128 * a : 0) + min(local, mine - 1);
+      const unsigned long long seen = sh.mask[row / p.G];
+      const uint32_t tl = (uint32_t)(quad * 32) << 16;
+      const uint32_t tS = tmem + tl + F::S_COL + (uint32_t)(a * BN), tO = tmem + tl + F::O_COL + (uint32_t)(a * DP);
+      const uint32_t tT = tmem + tl + F::T_COL + (uint32_t)(a * BN / 2);
+      const float f0 = QP == 1 ? p.scale2 : 1.f;
+      float m = -INFINITY, l = 0.f;
+      const int cnt = count(a);
+      bool ok = true;
+      for (int i = 0; i < cnt && ok; ++i) {
+        const int t = tile(a, i);
+        const int64_t t0 = (int64_t)(first + t) * BN;
+        if (I8) ok = mbar_wait(&sh.sc_full[t % NSC], (uint32_t)(t / NSC) & 1u, abort_flag, err, 51);
+        ok = ok && mbar_wait(&sh.s_bar[a], (uint32_t)i & 1u, abort_flag, err, 52);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        fence_after();
+        const float* fk = I8 ? sc_k[t % NSC] : nullptr;
+        const float* fv = I8 ? sc_v[t % NSC] : nullptr;
+        // columns this row sees: bit c of vis
+        uint32_t vis[BN / 32];
+        const bool masked = t0 + BN > pre;
+        if (masked) {
+          const int64_t off = pos - t0;  // column of drafted token 0
+#pragma unroll
+          for (int w = 0; w < BN / 32; ++w) {
+            const int64_t c0 = w * 32;
+            uint32_t bits = pre - t0 >= c0 + 32 ? ~0u : pre - t0 <= c0 ? 0u : (1u << (pre - t0 - c0)) - 1u;
+            const int64_t sh_r = c0 - off;  // drafted token at the word's first column
+            uint32_t d = 0;
+            if (sh_r >= 0) d = sh_r < 64 ? (uint32_t)(seen >> sh_r) : 0u;
+            else if (sh_r > -32) d = (uint32_t)(seen << -sh_r);
+            const uint32_t fit = end - t0 >= c0 + 32 ? ~0u : end - t0 <= c0 ? 0u : (1u << (end - t0 - c0)) - 1u;
+            vis[w] = (bits | (pos < p.T ? d : 0u)) & fit;
+          }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t r[32];
+          tmem_ld32_async(tS + (uint32_t)c, r);
+          tmem_wait_ld();
+          reg_fence32(r);
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 f = I8 ? *(const float4*)(fk + c + j) : make_float4(f0, f0, f0, f0);
+            const float g[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float x = __uint_as_float(r[j + k]) * g[k];
+              if (masked && !(vis[c / 32] >> (j + k) & 1u)) x = -INFINITY;
+              mx = fmaxf(mx, x);
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, mx > m + kLazy || (m == -INFINITY && mx > m))) {
+          const float mn = fmaxf(m, mx);
+          const float f = mn == -INFINITY ? 0.f : ex2(m - mn);
+          if (i > 0) {
+            ok = mbar_wait(&sh.o_bar[a], (uint32_t)(i - 1) & 1u, abort_flag, err, 53);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+#pragma unroll
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t r[32];
+              tmem_ld32_async(tO + (uint32_t)c, r);
+              tmem_wait_ld();
+              reg_fence32(r);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
+              tmem_st16u(tO + (uint32_t)c, r);
+              tmem_st16u(tO + (uint32_t)c + 16, r + 16);
+            }
+            tmem_wait_st();
+          }
+          l *= f;
+          m = mn;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t r[32];
+          tmem_ld32_async(tS + (uint32_t)c, r);
+          tmem_wait_ld();
+          reg_fence32(r);
+          float x[32], s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 f = I8 ? *(const float4*)(fk + c + j) : make_float4(f0, f0, f0, f0);
+            const float4 e = I8 ? *(const float4*)(fv + c + j) : make_float4(1.f, 1.f, 1.f, 1.f);
+            const float g[4] = {f.x, f.y, f.z, f.w}, w[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bool see = !masked || (vis[c / 32] >> (j + k) & 1u);
+              float y = ex2(fmaf(__uint_as_float(r[j + k]), g[k], -base));
+              if (!see) y = 0.f;
+              s4[k] += y;
+              x[j + k] = I8 && see ? y * w[k] : y;
+            }
+          }
+          l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+#pragma unroll
+          for (int part = 0; part < QP; ++part) {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              w[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+              if (part + 1 < QP) {
+                x[2 * j] -= bf_lo(w[j]);
+                x[2 * j + 1] -= bf_hi(w[j]);
+              }
+            }
+            tmem_st16u(part < 2 ? tS + (uint32_t)(c + 16 * part) : tT + (uint32_t)(c / 2), w);
+          }
+        }
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_bar[a]);
+      }
+      const int at = (split ? 128 * a : a * 128) + local;
+      if (local < mine) sh.m[at] = m, sh.l[at] = l;
+    }
+  } else if (warp < kSoftWarps + kLoadWarps) {
+    // ------------------------------------------------------------ loading
+    const int lt = tid - kSoftWarps * 32, lw = warp - kSoftWarps;
+    auto slot_free = [&](uint64_t* bars, int t, int code) {
+      return t < NS || mbar_wait(&bars[t % NS], (uint32_t)(t / NS - 1) & 1u, abort_flag, err, code);
+    };
+    if constexpr (I8) {
+      constexpr int UNITS = DP / 16;                        // 16-code pieces of a row
+      constexpr int PER = BN * UNITS / kLoadThreads;        // per thread and tile
+      uint4 rk[PER], rv[PER];
+      float nk = 0.f, nv = 0.f;
+      auto fetch = [&](const void* base, int t, uint4* r) {
+        const int64_t t0 = (int64_t)(first + t) * BN;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const int i = j * kLoadThreads + lt, row = i / UNITS, u = i % UNITS;
+          r[j] = make_uint4(0, 0, 0, 0);
+          if (t < nt && t0 + row < end && u * 16 < p.D)
+            r[j] = *(const uint4*)((const int8_t*)base + (nh * p.T + t0 + row) * p.D + u * 16);
+        }
+      };
+      auto fetch_scales = [&](int t) {
+        const int64_t at = (int64_t)(first + t) * BN + lt;
+        nk = nv = 0.f;
+        if (lt < BN && t < nt && at < end) nk = p.ks[nh * p.T + at], nv = p.vs[nh * p.T + at];
+      };
+      auto put = [&](uint8_t* dst, const uint4* r) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const int i = j * kLoadThreads + lt, row = i / UNITS, u = i % UNITS;
+          uint4 o[2];
+          codes_to_bf16(r[j], o);
+          *(uint4*)(dst + unit_at(BN, row, 2 * u)) = o[0];
+          *(uint4*)(dst + unit_at(BN, row, 2 * u + 1)) = o[1];
+        }
+      };
+      fetch(p.k, 0, rk);
+      fetch(p.v, 0, rv);
+      fetch_scales(0);
+      for (int t = 0; t < nt; ++t) {
+        if (!__all_sync(0xffffffffu, slot_free(sh.k_free, t, 54))) break;
+        put(smem + F::K_OFF + (t % NS) * F::TILE, rk);
+        // The slot of these scales was last used by tile t - NSC.  Its softmax
+        // is over: V of tile t - 1 went into a slot that PV of tile t - 1 - NS
+        // had left, and V of tile t - 2 into that of tile t - 2 - NS = t - NSC.
+        if (lt < BN) {
+          sc_k[t % NSC][lt] = QP == 1 ? nk * p.scale2 : nk;
+          sc_v[t % NSC][lt] = nv;
+        }
+        fetch(p.k, t + 1, rk);
+        fetch_scales(t + 1);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh.k_full[t % NS]);
+          mbar_arrive(&sh.sc_full[t % NSC]);
+        }
+        if (!__all_sync(0xffffffffu, slot_free(sh.v_free, t, 55))) break;
+        put(smem + F::V_OFF + (t % NS) * F::TILE, rv);
+        fetch(p.v, t + 1, rv);
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.v_full[t % NS]);
+      }
+    } else {
+      // Every loading thread passes every mended tile's barrier, whatever was
+      // aborted (an aborted wait returns at once), so none is left waiting.
+      int mended = 0, sent_k = 0, sent_v = 0, sent_raw = 0;
+      for (int t = 0; t < nt; ++t) {
+        const int64_t t0 = (int64_t)(first + t) * BN;
+        const int s = t % NS;
+        uint8_t *dk = smem + F::K_OFF + s * F::TILE, *dv = smem + F::V_OFF + s * F::TILE;
+        const bool mend = t0 + BN > pre;  // drafted tokens or the end of the sequence
+        bool ok = true;
+        if (lt == 0) {
+          ok = slot_free(sh.k_free, t, 54);
+          if (ok) {
+            mbar_expect_tx(&sh.k_full[s], F::TILE);
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c)
+              tma_load_3d(dk + c * BN * 128, &mK, &sh.k_full[s], c * 64, (int)t0, (int)nh);
+            sent_k = t + 1;
+            ok = slot_free(sh.v_free, t, 55);
+          }
+          if (ok) {
+            uint64_t* bar = mend ? &sh.raw : &sh.v_full[s];
+            mbar_expect_tx(bar, F::TILE);
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c) tma_load_3d(dv + c * BN * 128, &mV, bar, c * 64, (int)t0, (int)nh);
+            if (mend) ++sent_raw;
+            else sent_v = t + 1;
+          }
+        }
+        if (mend) {
+          ok = mbar_wait(&sh.raw, (uint32_t)mended & 1u, abort_flag, err, 56) && ok;
+          ++mended;
+          for (int i = lt; i < BN * (DP / 8); i += kLoadThreads) {
+            const int row = i / (DP / 8);
+            uint4* x = (uint4*)(dv + unit_at(BN, row, i % (DP / 8)));
+            if (t0 + row >= end) {
+              *x = make_uint4(0, 0, 0, 0);
+            } else if (t0 + row >= pre) {
+              uint32_t w[4] = {x->x, x->y, x->z, x->w};
+              bool bad = false;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, bad = true;
+                if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, bad = true;
+              }
+              if (bad) {
+                *x = make_uint4(w[0], w[1], w[2], w[3]);
+                sh.bad = 1;
+              }
+            }
+          }
+          fence_proxy_async();
+          loaders_sync();
+          if (lt == 0) mbar_arrive(&sh.v_full[s]);
+        }
+      }
+      // After an abort: no copy of this CTA may still be in flight when it
+      // leaves.  The MMA warp may not have waited for the last ones.
+      if (lt == 0 && *abort_flag) {
+        const unsigned long long t1 = now_ns() + kTimeoutNs;
+        for (int s = max(0, sent_k - NS); s < sent_k; ++s)
+          while (!mbar_try_wait(&sh.k_full[s % NS], (uint32_t)(s / NS) & 1u) && now_ns() < t1) {}
+        for (int s = max(0, sent_v - NS); s < sent_v; ++s)
+          while (!mbar_try_wait(&sh.v_full[s % NS], (uint32_t)(s / NS) & 1u) && now_ns() < t1) {}
+        while (sent_raw && !mbar_try_wait(&sh.raw, (uint32_t)(sent_raw - 1) & 1u) && now_ns() < t1) {}
+      }
+    }
+    (void)lw;
+  } else if (lane == 0) {
+    // ------------------------------------------------------------ MMA issue
+    const uint32_t id_s = idesc_bf16(128, BN, 0, 0), id_o = idesc_bf16(128, DP, 0, 1);
+    const uint32_t sq = smem_u32(smem), sk = sq + F::K_OFF, sv = sq + F::V_OFF;
+    auto issue_s = [&](int a, int t) {
+      if (!mbar_wait(&sh.k_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 57)) return false;
+      fence_after();
+      const uint32_t d = tmem + F::S_COL + (uint32_t)(a * BN);
+      const uint32_t q = sq + (split ? (uint32_t)(a * QP * F::QTILE) : 0u), k = sk + (uint32_t)((t % NS) * F::TILE);
+#pragma unroll
+      for (int part = 0; part < QP; ++part)
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+          mma_bf16(d, smem_desc(q + (uint32_t)(part * F::QTILE + (kk / 4) * 128 * 128 + (kk % 4) * 32), 16, 1024, 2),
+                   smem_desc(k + (uint32_t)((kk / 4) * BN * 128 + (kk % 4) * 32), 16, 1024, 2), id_s,
+                   part + kk > 0 ? 1u : 0u);
+      mma_commit(&sh.s_bar[a]);
+      if (!split || a == 1) mma_commit(&sh.k_free[t % NS]);
+      return true;
+    };
+    bool ok = true;
+    for (int a = 0; a < 2 && ok; ++a)
+      if (count(a) > 0) ok = issue_s(a, tile(a, 0));
+    for (int i = 0; i < count(0) && ok; ++i) {
+      for (int a = 0; a < 2 && ok; ++a) {
+        if (i >= count(a)) continue;
+        const int t = tile(a, i);
+        ok = mbar_wait(&sh.p_bar[a], (uint32_t)i & 1u, abort_flag, err, 58) &&
+             mbar_wait(&sh.v_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 59);
+        if (!ok) break;
+        fence_after();
+        const uint32_t d = tmem + F::O_COL + (uint32_t)(a * DP), pa = tmem + F::S_COL + (uint32_t)(a * BN);
+        const uint32_t v = sv + (uint32_t)((t % NS) * F::TILE);
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk) {
+          const uint64_t bd = smem_desc(v + (uint32_t)(kk * 2048), BN * 128, 1024, 2);
+          const uint32_t pc = pa + (uint32_t)((kk / 2) * 32 + (kk % 2) * 8);
+          mma_bf16_ts(d, pc, bd, id_o, i + kk > 0 ? 1u : 0u);
+          if (QP == 3) {
+            mma_bf16_ts(d, pc + 16, bd, id_o, 1u);
+            mma_bf16_ts(d, tmem + F::T_COL + (uint32_t)(a * BN / 2 + kk * 8), bd, id_o, 1u);
+          }
+        }
+        mma_commit(&sh.o_bar[a]);
+        if (!split || a == 1) mma_commit(&sh.v_free[t % NS]);
+        if (i + 1 < count(a)) ok = issue_s(a, tile(a, i + 1));
+      }
+    }
+    // the accumulators are final, and no MMA reads shared memory, once these pass
+    for (int a = 0; a < 2 && ok; ++a)
+      if (count(a) > 0) ok = mbar_wait(&sh.o_bar[a], (uint32_t)(count(a) - 1) & 1u, abort_flag, err, 60);
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const bool failed = sh.abort_flag != 0;
+
+  // outputs of the two streams to shared memory: row a * 128 + local
+  float* so = (float*)smem;
+  if (warp < kSoftWarps && !failed) {
+    const int a = warp >> 2, quad = warp & 3;
+    const int mine = split ? min(128, rows - 128 * a) : rows, q0 = quad * 32 - (split ? 0 : a * up);
+    if (q0 >= 0 && q0 < mine) {
+      const int local = q0 + lane;
+      const uint32_t tO = tmem + ((uint32_t)(quad * 32) << 16) + F::O_COL + (uint32_t)(a * DP);
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t r[32];
+        tmem_ld32_async(tO + (uint32_t)c, r);
+        tmem_wait_ld();
+        reg_fence32(r);
+        if (local < mine)
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *(uint4*)(so + (a * 128 + local) * F::LDO + c + j) =
+                count(a) > 0 ? make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    fence_after();
+    tmem_dealloc(tmem, F::COLS);
+  }
+  __syncthreads();
+  cluster_sync();
+  if (!failed) {
+    // rank c joins rows c, c + C, ..: one warp a row, lane j < np holds the weight of part j
+    const int np = split ? (int)C : 2 * (int)C;
+    int bad = 0;
+    if (!I8)
+      for (uint32_t c = 0; c < C; ++c) {
+        int x;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(cluster_addr(&sh.bad, c)));
+        bad |= x;
+      }
+    for (int i = (int)rank + (int)C * warp; i < rows; i += (int)C * kWarps) {
+      float pm = -INFINITY, pl = 0.f;
+      // part j: CTA j (split), or CTA j / 2, stream j % 2
+      const int at_j = split ? i : (lane & 1) * 128 + i;
+      if (lane < np) {
+        const uint32_t c = (uint32_t)(split ? lane : lane / 2);
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm) : "r"(cluster_addr(&sh.m[at_j], c)));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pl) : "r"(cluster_addr(&sh.l[at_j], c)));
+      }
+      float mx = pm;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float wgt = lane < np ? ex2(pm - (mx == -INFINITY ? 0.f : mx)) : 0.f;
+      float l = pl * wgt;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const int row = r0 + i, t = row / p.G;
+      const unsigned long long fit = end - pos >= 64 ? ~0ull : end > pos ? (1ull << (end - pos)) - 1 : 0ull;
+      const unsigned long long drafted = pos >= 0 ? sh.mask[t] & fit : 0ull;
+      const bool any = pre > 0 || drafted;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j = 0; j < np; ++j) {
+        const float w = __shfl_sync(0xffffffffu, wgt, j);
+        if (lane < DP / 4) {
+          const uint32_t c = (uint32_t)(split ? j : j / 2);
+          const int at = split ? i : (j & 1) * 128 + i;
+          float4 x;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                       : "r"(cluster_addr(so + at * F::LDO + lane * 4, c)));
+          if (w != 0.f) {  // a part without keys has no meaning for its row
+            acc.x = fmaf(x.x, w, acc.x);
+            acc.y = fmaf(x.y, w, acc.y);
+            acc.z = fmaf(x.z, w, acc.z);
+            acc.w = fmaf(x.w, w, acc.w);
+          }
+        }
+      }
+      if (lane * 4 < p.D) {
+        float y[4] = {acc.x / l, acc.y / l, acc.z / l, acc.w / l};
+        if (bad)
+          for (int j = 0; j < p.S; ++j)
+            if (drafted >> j & 1ull)
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                const float v = __bfloat162float(((const __nv_bfloat16*)p.v)[(nh * p.T + pos + j) * p.D + lane * 4 + d]);
+                if (!isfinite(v)) y[d] += v;
+              }
+        if (!any) y[0] = y[1] = y[2] = y[3] = 0.f;
+        const int64_t at = ((n * p.S + t) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + lane * 4;
+        if (QP == 1) *(uint2*)((__nv_bfloat16*)p.out + at) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        else *(float4*)((float*)p.out + at) = make_float4(y[0], y[1], y[2], y[3]);
+      }
+    }
+  }
+  cluster_sync();
+}
+
+template <int DP, int BN, int QP, bool I8>
+cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
+  using F = Cfg<DP, BN, QP>;
+  const KvCacheView& c = a.cache;
+  const int G = (int)(a.Hq / c.H), rows = (int)a.S * G, pairs = (rows + F::MAXR - 1) / F::MAXR;
+  Params p = {c.k, c.v, c.k_scale, c.v_scale, a.positions, a.parents, a.q, a.out, a.bf16 ? 1 : 0, (int)c.H, G, (int)a.S,
+              (int)c.D, pairs, c.T, a.scale * kLog2e};
+  CUtensorMap mk{}, mv{};
+  if (!I8) {
+    const uint64_t dims[3] = {(uint64_t)c.D, (uint64_t)c.T, (uint64_t)(c.N * c.H)};
+    const uint64_t strides[2] = {(uint64_t)c.D * 2, (uint64_t)(c.T * c.D) * 2};
+    if (!tc_make_map_bf16(&mk, c.k, 3, dims, strides, BN) || !tc_make_map_bf16(&mv, c.v, 3, dims, strides, BN))
+      return cudaErrorNotSupported;
+  }
+  int* err = tc_error_word();
+  if (!err) return cudaErrorMemoryAllocation;
+  const int64_t items = c.N * c.H * pairs;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  // one CTA fits an SM: split until the CTAs fill the SMs once, or a CTA has two tiles
+  int C = 1;
+  while (C < 8 && items * (C + 1) <= sms && c.T / (C + 1) >= 2 * BN) ++C;
+  if (items * C > INT32_MAX) return cudaErrorInvalidValue;
+  auto kern = cache_attn_tc<DP, BN, QP, I8>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * C));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = F::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  pdl_attribute(&at[0]);
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)C;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  launch_counter().fetch_add(1, std::memory_order_relaxed);
+  return cudaLaunchKernelEx(&cfg, kern, mk, mv, p, err);
+}
+
+}  // namespace
+
+bool cache_attention_tc_takes(const CacheAttnArgs& a) {
+  return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 && a.S * (a.Hq / a.cache.H) > 8;
+}
+
+cudaError_t cache_attention_tc(const CacheAttnArgs& a, cudaStream_t stream) {
+  const bool i8 = a.cache.type == KvType::I8;
+  if (a.cache.D <= 64) {
+    if (a.bf16) return i8 ? launch<64, 128, 1, true>(a, stream) : launch<64, 128, 1, false>(a, stream);
+    return i8 ? launch<64, 128, 3, true>(a, stream) : launch<64, 128, 3, false>(a, stream);
+  }
+  if (a.bf16) return i8 ? launch<128, 128, 1, true>(a, stream) : launch<128, 128, 1, false>(a, stream);
+  return i8 ? launch<128, 64, 3, true>(a, stream) : launch<128, 64, 3, false>(a, stream);
+}
+
+}  // namespace sb

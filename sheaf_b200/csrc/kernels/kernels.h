@@ -171,6 +171,8 @@ cudaError_t gemm_tcgen05_group(const GemmArgs* g, int n, int cfg, cudaStream_t s
 // memory window misaligned (9), or the row scatter-add found inconsistent
 // segment offsets (41..43).  Reads a device word (synchronizing).
 int gemm_tcgen05_error();
+// That device word, allocated on the first call.
+int* tc_error_word();
 
 // Fused attention, head dim 64 (kernels/attention.cu).  Views are [B,H,T,64]
 // with unit stride on the last dim; strides in elements.
@@ -277,6 +279,12 @@ struct CacheAttnArgs {
   float scale = 1.f;  // multiplier of q.k before the softmax
 };
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
+// The tensor-core kernel (kernels/cache_attention_tc.cu) and the calls it is
+// for: bf16 or int8 caches of head size 64 to 128 with more than 8 query rows
+// per cache head.  cache_attention calls it; it reports failed waits through
+// the tensor-core error word (codes 50..60).
+bool cache_attention_tc_takes(const CacheAttnArgs& a);
+cudaError_t cache_attention_tc(const CacheAttnArgs& a, cudaStream_t stream);
 
 // Beam search: the W best continuations of each group of W beams over a
 // vocabulary of V (see sb_beam_select).

@@ -1304,6 +1304,7 @@ sb_status* sb_session_create(const sb_session_options* o, sb_session** out) {
   s->dev->ordinal = o->device_ordinal;
   SB_CUDA(cudaSetDevice(o->device_ordinal));
   SB_CUDA(cudaStreamCreateWithFlags(&s->dev->stream, cudaStreamNonBlocking));
+  tc_error_word();  // allocated here, so that no later call allocates it inside a stream capture
   if (o->world_size > 1 && (o->flags & SB_SESSION_FLAG_OVERLAP_ALLREDUCE)) {
     SB_CUDA(cudaStreamCreateWithFlags(&s->dev->comm_stream, cudaStreamNonBlocking));
     SB_CUDA(cudaEventCreateWithFlags(&s->dev->ready, cudaEventDisableTiming));
@@ -1898,6 +1899,7 @@ sb_status* sb_kv_cache_attention(sb_session* s, const sb_kv_cache* cache, sb_buf
   a.S = S;
   a.Hq = Hq;
   a.scale = scale;
+  if (cache_attention_tc_takes(a)) s->used_tc = true;
   cudaError_t e = cache_attention(a, s->dev->stream);
   return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_attention");
 }

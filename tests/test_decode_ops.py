@@ -198,11 +198,14 @@ def attention_bound(dots, vmax, live, D, out, kind):
     steps of sum |q k| scale, in units of log2 e less than 2 of it; a relative
     error of e in every probability moves the output by at most 2 e max|v|;
     exp2 and the running rescalings add a few half steps per term and the sums
-    at most one per addition (`live` of them)."""
+    at most one per addition (`live` of them).  A bf16 evaluation may also round
+    each probability (times its value row's scale) to bf16 before the second
+    product: each term p v moves by at most half a bf16 step of itself, so the
+    output by at most UBF sum p |v| <= UBF max|v|; and it rounds the output."""
     e = 2 * (D + 4) * U32 * dots + (live + 64) * U32
     b = 2 * e * vmax
     if kind == "bf16":
-        b = b + UBF * np.abs(out).max(-1)
+        b = b + UBF * vmax + UBF * np.abs(out).max(-1)
     return b[..., None]
 
 
