@@ -12,7 +12,8 @@
 //                       at most 64 rows stream 1 uses the upper half of the
 //                       TMEM lanes, so the two use different SM quarters.
 // While one stream turns S into P the tensor cores work for the other.  Warp
-// roles: 8 softmax, 4 loading, 1 issuing the MMAs.
+// roles: 8 softmax, 4 loading, 2 issuing the MMAs (one thread needs about 80
+// cycles per tcgen05.mma, more than the 64 that one takes), 2 helpers.
 //
 //   S = Q K^T   bf16 operands.  f32 queries are split exactly into three bf16
 //               parts (8 mantissa bits each) whose products accumulate into
@@ -37,6 +38,7 @@
 #include <cuda_bf16.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "kernels.h"
 #include "pdl.h"
@@ -47,7 +49,18 @@ namespace {
 
 using namespace tc;
 
-constexpr int kSoftWarps = 8, kLoadWarps = 4, kWarps = kSoftWarps + kLoadWarps + 1, kThreads = kWarps * 32;
+// warps 0-7 softmax, 8-11 loading, 12 and 13 MMA issue (one per stream), 14, 15
+// and the softmax warps stage the queries
+constexpr int kSoftWarps = 8, kLoadWarps = 4, kMmaWarp = 12, kWarps = 16, kThreads = kWarps * 32;
+constexpr int kStageWarps = kWarps - kLoadWarps - 2;
+// Registers per thread of the four warpgroups: 2 softmax, loading, the rest.
+// They add up to the launch's 4 x 128.
+constexpr int kRegsSoft = 168, kRegsLoad = 104, kRegsRest = 72, kRegsLaunch = 128;
+static_assert(2 * kRegsSoft + kRegsLoad + kRegsRest == 4 * kRegsLaunch, "register shares");
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int NS = 2;   // K and V tiles in flight
 constexpr int NSC = 4;  // rows of scales in flight (see the loader)
@@ -77,8 +90,14 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
 }
 
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t* r) {
-  tmem_ld16_async(taddr, r);
-  tmem_ld16_async(taddr + 16, r + 16);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
 }
 __device__ __forceinline__ void reg_fence32(uint32_t* r) {
 #pragma unroll
@@ -91,6 +110,31 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// Two f32 at once (sm_100 packed arithmetic).
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*(uint64_t*)&d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*(uint64_t*)&d) : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*(uint64_t*)&d)
+      : "l"(*(uint64_t*)&a), "l"(*(uint64_t*)&b), "l"(*(uint64_t*)&c));
+  return d;
 }
 
 // (lo, hi) f32 to packed bf16, rounded to nearest even
@@ -144,13 +188,14 @@ struct Cfg {
 };
 
 struct Shared {
-  uint64_t k_full[NS], k_free[NS], v_full[NS], v_free[NS], sc_full[NSC], s_bar[2], p_bar[2], o_bar[2], raw;
+  uint64_t k_full[NS], k_free[NS], v_full[NS], v_free[NS], sc_full[NSC], s_bar[2], p_bar[2], o_bar[2], raw, q_bar;
   uint32_t tslot;
   volatile int abort_flag;
   int bad;  // a drafted value that is not finite was taken out of a tile
   unsigned long long mask[kKvMaxTokens];
   int jump[kKvMaxTokens];
   float m[256], l[256];
+  float wgt[256 * 2];  // rows of a rank x parts: at most 256 / C x C, or 128 / C x 2 C
 };
 
 // see cache_attention.cu
@@ -215,8 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < NS; ++i) {
       mbar_init(&sh.k_full[i], I8 ? kLoadWarps : 1);
       mbar_init(&sh.v_full[i], I8 ? kLoadWarps : 1);
-      mbar_init(&sh.k_free[i], 1);
-      mbar_init(&sh.v_free[i], 1);
+      mbar_init(&sh.k_free[i], split ? 2 : 1);  // the streams that read the tile
+      mbar_init(&sh.v_free[i], split ? 2 : 1);
     }
     for (int i = 0; i < NSC; ++i) mbar_init(&sh.sc_full[i], kLoadWarps);
     for (int a = 0; a < 2; ++a) {
@@ -226,6 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.o_bar[a], 1);
     }
     mbar_init(&sh.raw, 1);
+    mbar_init(&sh.q_bar, kStageWarps);
     sh.abort_flag = aligned ? 0 : 1;
     sh.bad = 0;
     if (!aligned) atomicExch(err, 50);
@@ -233,51 +279,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_proxy_async();
   }
   if (warp == 0) tmem_alloc(&sh.tslot, F::COLS);
-  if (warp == 1) tree_masks(p.parents ? p.parents + n * p.S : nullptr, p.S, lane, sh.mask, sh.jump);
-  // queries into swizzled K-major tiles: tile (row block, part) of 128 rows;
-  // one block of rows repeated at lane `up` when stream 1 uses those lanes
-  if (nt > 0 && aligned) {
-    constexpr int UNITS = DP / 8;
-    const int blocks = split ? 2 : 1;
-    for (int i = tid; i < blocks * 128 * UNITS; i += kThreads) {
-      const int u = i % UNITS, r = (i / UNITS) % 128, b = i / (UNITS * 128);
-      const int local = split ? b * 128 + r : (up && r >= 64 ? r - 64 : r);
-      float x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
-      if (local < rows && u * 8 < p.D) {
-        const int row = r0 + local;
-        const int64_t at = ((n * p.S + row / p.G) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + u * 8;
-        if (QP == 1) {
-          *(uint4*)x = *(const uint4*)((const __nv_bfloat16*)p.q + at);
-        } else {
-          const float4* s = (const float4*)((const float*)p.q + at);
-          const float4 a = s[0], c = s[1];
-          x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = c.x, x[5] = c.y, x[6] = c.z, x[7] = c.w;
-        }
-      }
-      uint8_t* dst = smem + b * QP * F::QTILE + unit_at(128, r, u);
-      if (QP == 1) {
-        *(uint4*)dst = *(const uint4*)x;
-      } else {
-        // x = part 0 + part 1 + part 2, each a bf16 rounding of what is left
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= p.scale2;
-#pragma unroll
-        for (int part = 0; part < QP; ++part) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
-            x[2 * j] -= bf_lo(w[j]);
-            x[2 * j + 1] -= bf_hi(w[j]);
-          }
-          *(uint4*)(dst + part * F::QTILE) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-    }
-    fence_proxy_async();
-  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -287,8 +288,72 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto count = [&](int a) { return split ? nt : (nt - a + 1) / 2; };
   auto tile = [&](int a, int i) { return split ? i : 2 * i + a; };
 
+  // Queries into swizzled K-major tiles: tile (row block, part) of 128 rows; one
+  // block of rows repeated at lane `up` when stream 1 uses those lanes.
+  // `w` of kStageWarps warps.  A negative scale of bf16 queries goes into their
+  // signs, so that the softmax can take maxima before it scales.
+  auto stage_q = [&](int w) {
+    // a thread keeps its 8-value column `u` and walks the rows
+    constexpr int UNITS = DP / 8, RSTEP = kStageWarps * 32 / UNITS, LOADS = QP == 1 ? 1 : 2, BATCH = QP == 1 ? 8 : 4;
+    static_assert(kStageWarps * 32 % UNITS == 0, "whole rows per step");
+    const int u = (w * 32 + lane) % UNITS, total = nt > 0 && aligned ? (split ? 256 : 128) : 0;
+    const int64_t q0 = (n * p.S * p.H + h) * p.G * p.D + u * 8;
+    const int64_t token = (int64_t)p.H * p.G * p.D;
+#pragma unroll 1
+    for (int k0 = (w * 32 + lane) / UNITS; k0 < total; k0 += BATCH * RSTEP) {
+      uint4 raw[BATCH][LOADS];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int i = k0 + k * RSTEP, local = up ? i & 63 : i;
+#pragma unroll
+        for (int c = 0; c < LOADS; ++c) raw[k][c] = make_uint4(0, 0, 0, 0);
+        if (i < total && local < rows && u * 8 < p.D) {
+          const int row = r0 + local, s = row / p.G, g = row - s * p.G;
+          const int64_t at = q0 + s * token + g * p.D;
+#pragma unroll
+          for (int c = 0; c < LOADS; ++c)
+            raw[k][c] = *(const uint4*)((const uint8_t*)p.q + (at + 4 * c) * (QP == 1 ? 2 : 4));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int i = k0 + k * RSTEP;
+        if (i >= total) continue;
+        uint8_t* dst = smem + (i >> 7) * QP * F::QTILE + unit_at(128, i & 127, u);
+        if (QP == 1) {
+          const uint32_t flip = p.scale2 < 0.f ? 0x80008000u : 0u;
+          const uint4 x = raw[k][0];
+          *(uint4*)dst = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+        } else {
+          // x = part 0 + part 1 + part 2, each a bf16 rounding of what is left
+          float x[8];
+          *(uint4*)x = raw[k][0];
+          *(uint4*)(x + 4) = raw[k][LOADS - 1];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] *= p.scale2;
+#pragma unroll
+          for (int part = 0; part < QP; ++part) {
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              y[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+              x[2 * j] -= bf_lo(y[j]);
+              x[2 * j + 1] -= bf_hi(y[j]);
+            }
+            *(uint4*)(dst + part * F::QTILE) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+      }
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.q_bar);
+  };
+
   if (warp < kSoftWarps) {
     // ------------------------------------------------------------ softmax
+    regs_inc<kRegsSoft>();
+    stage_q(warp);
     const int a = warp >> 2, quad = warp & 3;
     const int lo_lane = split ? 0 : a * up;  // the stream's first TMEM lane
     const int mine = split ? min(128, rows - 128 * a) : rows;
@@ -296,67 +361,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (q0 >= 0 && q0 < mine) {
       const int local = q0 + lane;  // row within the stream
       const int row = r0 + (split ? 128 * a : 0) + min(local, mine - 1);
-      const unsigned long long seen = sh.mask[row / p.G];
       const uint32_t tl = (uint32_t)(quad * 32) << 16;
       const uint32_t tS = tmem + tl + F::S_COL + (uint32_t)(a * BN), tO = tmem + tl + F::O_COL + (uint32_t)(a * DP);
       const uint32_t tT = tmem + tl + F::T_COL + (uint32_t)(a * BN / 2);
-      const float f0 = QP == 1 ? p.scale2 : 1.f;
-      float m = -INFINITY, l = 0.f;
+      const float f0 = fabsf(p.scale2);  // bf16 queries over a bf16 cache: scaled here
+      float m = -INFINITY;
+      float2 l2 = make_float2(0.f, 0.f);
       const int cnt = count(a);
-      bool ok = true;
-      for (int i = 0; i < cnt && ok; ++i) {
+      // the drafted tokens' masks and every warp's part of the queries are there
+      bool ok = mbar_wait(&sh.q_bar, 0, abort_flag, err, 61);
+      const unsigned long long seen = sh.mask[row / p.G];
+      for (int i = 0; i < cnt; ++i) {
         const int t = tile(a, i);
         const int64_t t0 = (int64_t)(first + t) * BN;
-        if (I8) ok = mbar_wait(&sh.sc_full[t % NSC], (uint32_t)(t / NSC) & 1u, abort_flag, err, 51);
+        if (I8) ok = ok && mbar_wait(&sh.sc_full[t % NSC], (uint32_t)(t / NSC) & 1u, abort_flag, err, 51);
         ok = ok && mbar_wait(&sh.s_bar[a], (uint32_t)i & 1u, abort_flag, err, 52);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
         const float* fk = I8 ? sc_k[t % NSC] : nullptr;
         const float* fv = I8 ? sc_v[t % NSC] : nullptr;
-        // columns this row sees: bit c of vis
-        uint32_t vis[BN / 32];
-        const bool masked = t0 + BN > pre;
-        if (masked) {
-          const int64_t off = pos - t0;  // column of drafted token 0
-#pragma unroll
-          for (int w = 0; w < BN / 32; ++w) {
-            const int64_t c0 = w * 32;
-            uint32_t bits = pre - t0 >= c0 + 32 ? ~0u : pre - t0 <= c0 ? 0u : (1u << (pre - t0 - c0)) - 1u;
-            const int64_t sh_r = c0 - off;  // drafted token at the word's first column
-            uint32_t d = 0;
-            if (sh_r >= 0) d = sh_r < 64 ? (uint32_t)(seen >> sh_r) : 0u;
-            else if (sh_r > -32) d = (uint32_t)(seen << -sh_r);
-            const uint32_t fit = end - t0 >= c0 + 32 ? ~0u : end - t0 <= c0 ? 0u : (1u << (end - t0 - c0)) - 1u;
-            vis[w] = (bits | (pos < p.T ? d : 0u)) & fit;
-          }
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t r[32];
-          tmem_ld32_async(tS + (uint32_t)c, r);
-          tmem_wait_ld();
-          reg_fence32(r);
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 f = I8 ? *(const float4*)(fk + c + j) : make_float4(f0, f0, f0, f0);
-            const float g[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float x = __uint_as_float(r[j + k]) * g[k];
-              if (masked && !(vis[c / 32] >> (j + k) & 1u)) x = -INFINITY;
-              mx = fmaxf(mx, x);
-            }
-          }
-        }
-        if (__any_sync(0xffffffffu, mx > m + kLazy || (m == -INFINITY && mx > m))) {
-          const float mn = fmaxf(m, mx);
-          const float f = mn == -INFINITY ? 0.f : ex2(m - mn);
+        // the row's maximum moves to mn: O and l are rescaled
+        auto rescale = [&](float mx) {
+          const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 0.f : ex2(m - mn);
           if (i > 0) {
-            ok = mbar_wait(&sh.o_bar[a], (uint32_t)(i - 1) & 1u, abort_flag, err, 53);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_bar[a], (uint32_t)(i - 1) & 1u, abort_flag, err, 53));
+            if (!ok) return;
             fence_after();
 #pragma unroll
             for (int c = 0; c < DP; c += 32) {
@@ -371,73 +401,191 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_wait_st();
           }
-          l *= f;
+          l2.x *= f;
+          l2.y *= f;
           m = mn;
-        }
-        const float base = m == -INFINITY ? 0.f : m;
+        };
+        auto moves = [&](float mx) { return __any_sync(0xffffffffu, mx > m + kLazy); };
+        // P of the tile from S; `vis`: the columns the row sees
+        auto softmax = [&](auto mask_tag, const uint32_t* vis) {
+          constexpr bool MASK = decltype(mask_tag)::value;
+          if constexpr (QP == 1) {
+            // One pass with the maximum as it stands: P is kept in registers
+            // until the tile's own maximum is known.  If that moved too far
+            // (always in the first tile) the pass runs again.
+            for (;;) {
+              const float base = m == -INFINITY ? 0.f : m;
+              const float2 nb = make_float2(-base, -base);
+              float mx = -INFINITY;
+              float2 s2 = make_float2(0.f, 0.f);
+              uint32_t w[BN / 2];
+              uint32_t r[2][32];
+              tmem_ld32_async(tS, r[0]);
 #pragma unroll
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t r[32];
-          tmem_ld32_async(tS + (uint32_t)c, r);
-          tmem_wait_ld();
-          reg_fence32(r);
-          float x[32], s4[4] = {0.f, 0.f, 0.f, 0.f};
+              for (int c = 0; c < BN; c += 32) {
+                uint32_t* x = r[(c / 32) & 1];
+                tmem_wait_ld();
+                reg_fence32(x);
+                if (c + 32 < BN) tmem_ld32_async(tS + (uint32_t)(c + 32), r[(c / 32 + 1) & 1]);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 f = I8 ? *(const float4*)(fk + c + j) : make_float4(f0, f0, f0, f0);
-            const float4 e = I8 ? *(const float4*)(fv + c + j) : make_float4(1.f, 1.f, 1.f, 1.f);
-            const float g[4] = {f.x, f.y, f.z, f.w}, w[4] = {e.x, e.y, e.z, e.w};
+                for (int j = 0; j < 32; j += 4) {
+                  float4 f = make_float4(f0, f0, f0, f0), e = f;
+                  if (I8) f = *(const float4*)(fk + c + j), e = *(const float4*)(fv + c + j);
+                  const float2 g[2] = {make_float2(f.x, f.y), make_float2(f.z, f.w)};
+                  const float2 h2[2] = {make_float2(e.x, e.y), make_float2(e.z, e.w)};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const bool see = !masked || (vis[c / 32] >> (j + k) & 1u);
-              float y = ex2(fmaf(__uint_as_float(r[j + k]), g[k], -base));
-              if (!see) y = 0.f;
-              s4[k] += y;
-              x[j + k] = I8 && see ? y * w[k] : y;
+                  for (int k = 0; k < 2; ++k) {
+                    float2 s = make_float2(__uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1]));
+                    const bool v0 = !MASK || (vis[c / 32] >> (j + 2 * k) & 1u);
+                    const bool v1 = !MASK || (vis[c / 32] >> (j + 2 * k + 1) & 1u);
+                    if (I8) s = mul2(s, g[k]);
+                    if (MASK) s.x = v0 ? s.x : -INFINITY, s.y = v1 ? s.y : -INFINITY;
+                    mx = fmaxf(mx, fmaxf(s.x, s.y));
+                    s = I8 ? add2(s, nb) : fma2(s, g[k], nb);
+                    float2 y = make_float2(ex2(s.x), ex2(s.y));
+                    if (MASK && !I8) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;  // f0 may be 0
+                    s2 = add2(s2, y);
+                    if (I8) {
+                      y = mul2(y, h2[k]);
+                      if (MASK) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;
+                    }
+                    w[(c + j) / 2 + k] = pack_bf16(y.x, y.y);
+                  }
+                }
+              }
+              if (!I8 && mx != -INFINITY) mx *= f0;
+              if (moves(mx)) {
+                rescale(mx);
+                if (!ok) return;
+                continue;
+              }
+              l2 = add2(l2, s2);
+#pragma unroll
+              for (int c = 0; c < BN / 32; ++c) tmem_st16u(tS + (uint32_t)(32 * c), w + 16 * c);
+              return;
             }
-          }
-          l += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+          } else {
+            float mx = -INFINITY;
 #pragma unroll
-          for (int part = 0; part < QP; ++part) {
-            uint32_t w[16];
+            for (int c = 0; c < BN; c += 32) {
+              uint32_t r[32];
+              tmem_ld32_async(tS + (uint32_t)c, r);
+              tmem_wait_ld();
+              reg_fence32(r);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              w[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
-              if (part + 1 < QP) {
-                x[2 * j] -= bf_lo(w[j]);
-                x[2 * j + 1] -= bf_hi(w[j]);
+              for (int j = 0; j < 32; j += 4) {
+                float4 f = make_float4(1.f, 1.f, 1.f, 1.f);
+                if (I8) f = *(const float4*)(fk + c + j);
+                const float g[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  float s = __uint_as_float(r[j + k]);
+                  if (I8) s *= g[k];
+                  if (MASK && !(vis[c / 32] >> (j + k) & 1u)) s = -INFINITY;
+                  mx = fmaxf(mx, s);
+                }
               }
             }
-            tmem_st16u(part < 2 ? tS + (uint32_t)(c + 16 * part) : tT + (uint32_t)(c / 2), w);
+            if (moves(mx)) {
+              rescale(mx);
+              if (!ok) return;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) {
+              uint32_t r[32];
+              tmem_ld32_async(tS + (uint32_t)c, r);
+              tmem_wait_ld();
+              reg_fence32(r);
+#pragma unroll
+              for (int half = 0; half < 32; half += 16) {
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  float4 f = make_float4(1.f, 1.f, 1.f, 1.f), e = f;
+                  if (I8) f = *(const float4*)(fk + c + half + j), e = *(const float4*)(fv + c + half + j);
+                  const float g[4] = {f.x, f.y, f.z, f.w}, h4[4] = {e.x, e.y, e.z, e.w};
+                  float y[4];
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const bool see = !MASK || (vis[c / 32] >> (half + j + k) & 1u);
+                    const float s = __uint_as_float(r[half + j + k]);
+                    y[k] = ex2(I8 ? fmaf(s, g[k], -base) : s - base);
+                    if (MASK) y[k] = see ? y[k] : 0.f;
+                    x[j + k] = y[k];
+                    if (I8 && see) x[j + k] *= h4[k];
+                  }
+                  l2 = add2(l2, add2(make_float2(y[0], y[1]), make_float2(y[2], y[3])));
+                }
+#pragma unroll
+                for (int part = 0; part < QP; ++part) {
+                  uint32_t w[8];
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) {
+                    w[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+                    if (part + 1 < QP) x[2 * j] -= bf_lo(w[j]), x[2 * j + 1] -= bf_hi(w[j]);
+                  }
+                  tmem_st8u((part < 2 ? tS + (uint32_t)(c + 16 * part) : tT + (uint32_t)(c / 2)) + half / 2, w);
+                }
+              }
+            }
           }
+        };
+        if (t0 + BN > pre) {
+          uint32_t vis[BN / 32];
+          const int64_t off = pos - t0;  // column of drafted token 0
+#pragma unroll
+          for (int w = 0; w < BN / 32; ++w) {
+            const int64_t c0 = w * 32;
+            const uint32_t before = pre - t0 >= c0 + 32 ? ~0u : pre - t0 <= c0 ? 0u : (1u << (pre - t0 - c0)) - 1u;
+            const int64_t j0 = c0 - off;  // drafted token at the word's first column
+            uint32_t d = 0;
+            if (j0 >= 0) d = j0 < 64 ? (uint32_t)(seen >> j0) : 0u;
+            else if (j0 > -32) d = (uint32_t)(seen << -j0);
+            const uint32_t fit = end - t0 >= c0 + 32 ? ~0u : end - t0 <= c0 ? 0u : (1u << (end - t0 - c0)) - 1u;
+            vis[w] = (before | (pos < p.T ? d : 0u)) & fit;
+          }
+          softmax(std::true_type{}, vis);
+        } else {
+          softmax(std::false_type{}, nullptr);
         }
+        if (!ok) break;
         tmem_wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_bar[a]);
       }
+      const float l = l2.x + l2.y;
       const int at = (split ? 128 * a : a * 128) + local;
       if (local < mine) sh.m[at] = m, sh.l[at] = l;
     }
+    __syncwarp();
+    regs_dec<kRegsLaunch>();
   } else if (warp < kSoftWarps + kLoadWarps) {
     // ------------------------------------------------------------ loading
-    const int lt = tid - kSoftWarps * 32, lw = warp - kSoftWarps;
+    regs_dec<kRegsLoad>();
+    const int lt = tid - kSoftWarps * 32;
     auto slot_free = [&](uint64_t* bars, int t, int code) {
       return t < NS || mbar_wait(&bars[t % NS], (uint32_t)(t / NS - 1) & 1u, abort_flag, err, code);
     };
     if constexpr (I8) {
-      constexpr int UNITS = DP / 16;                        // 16-code pieces of a row
-      constexpr int PER = BN * UNITS / kLoadThreads;        // per thread and tile
+      constexpr int UNITS = DP / 16;                  // 16-code pieces of a row
+      constexpr int PER = BN * UNITS / kLoadThreads;  // per thread and tile
+      constexpr int RSTEP = kLoadThreads / UNITS;     // rows between a thread's pieces (a multiple of 8)
+      static_assert(RSTEP % 8 == 0, "a thread's pieces share a swizzle phase");
+      const int u = lt % UNITS, row0 = lt / UNITS;
+      const bool has = u * 16 < p.D;
+      const int64_t at0 = (nh * p.T + (int64_t)first * BN + row0) * p.D + u * 16;
+      const uint32_t put0 = unit_at(BN, row0, 2 * u), put1 = unit_at(BN, row0, 2 * u + 1);
       uint4 rk[PER], rv[PER];
       float nk = 0.f, nv = 0.f;
       auto fetch = [&](const void* base, int t, uint4* r) {
-        const int64_t t0 = (int64_t)(first + t) * BN;
+        const int8_t* src = (const int8_t*)base + at0 + (int64_t)t * BN * p.D;
+        const int left = t < nt ? (int)min((int64_t)BN, end - (int64_t)(first + t) * BN) : 0;  // rows of the tile
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          const int i = j * kLoadThreads + lt, row = i / UNITS, u = i % UNITS;
           r[j] = make_uint4(0, 0, 0, 0);
-          if (t < nt && t0 + row < end && u * 16 < p.D)
-            r[j] = *(const uint4*)((const int8_t*)base + (nh * p.T + t0 + row) * p.D + u * 16);
+          if (has && row0 + j * RSTEP < left) r[j] = *(const uint4*)(src + (int64_t)(j * RSTEP) * p.D);
         }
       };
       auto fetch_scales = [&](int t) {
@@ -448,11 +596,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto put = [&](uint8_t* dst, const uint4* r) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          const int i = j * kLoadThreads + lt, row = i / UNITS, u = i % UNITS;
           uint4 o[2];
           codes_to_bf16(r[j], o);
-          *(uint4*)(dst + unit_at(BN, row, 2 * u)) = o[0];
-          *(uint4*)(dst + unit_at(BN, row, 2 * u + 1)) = o[1];
+          *(uint4*)(dst + put0 + j * RSTEP * 128) = o[0];
+          *(uint4*)(dst + put1 + j * RSTEP * 128) = o[1];
         }
       };
       fetch(p.k, 0, rk);
@@ -465,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // is over: V of tile t - 1 went into a slot that PV of tile t - 1 - NS
         // had left, and V of tile t - 2 into that of tile t - 2 - NS = t - NSC.
         if (lt < BN) {
-          sc_k[t % NSC][lt] = QP == 1 ? nk * p.scale2 : nk;
+          sc_k[t % NSC][lt] = QP == 1 ? nk * fabsf(p.scale2) : nk;
           sc_v[t % NSC][lt] = nv;
         }
         fetch(p.k, t + 1, rk);
@@ -550,62 +697,72 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (sent_raw && !mbar_try_wait(&sh.raw, (uint32_t)(sent_raw - 1) & 1u) && now_ns() < t1) {}
       }
     }
-    (void)lw;
-  } else if (lane == 0) {
-    // ------------------------------------------------------------ MMA issue
-    const uint32_t id_s = idesc_bf16(128, BN, 0, 0), id_o = idesc_bf16(128, DP, 0, 1);
-    const uint32_t sq = smem_u32(smem), sk = sq + F::K_OFF, sv = sq + F::V_OFF;
-    auto issue_s = [&](int a, int t) {
-      if (!mbar_wait(&sh.k_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 57)) return false;
-      fence_after();
-      const uint32_t d = tmem + F::S_COL + (uint32_t)(a * BN);
-      const uint32_t q = sq + (split ? (uint32_t)(a * QP * F::QTILE) : 0u), k = sk + (uint32_t)((t % NS) * F::TILE);
+  } else {
+    regs_dec<kRegsRest>();
+    const int a = warp - kMmaWarp;
+    if (a > 1) {
+      if (a == 2) tree_masks(p.parents ? p.parents + n * p.S : nullptr, p.S, lane, sh.mask, sh.jump);
+      stage_q(warp - kLoadWarps - 2);
+    } else if (lane == 0) {
+      // ---------------------------------------------------------- MMA issue of stream a
+      const uint32_t id_s = idesc_bf16(128, BN, 0, 0), id_o = idesc_bf16(128, DP, 0, 1);
+      const uint32_t sq = smem_u32(smem) + (split ? (uint32_t)(a * QP * F::QTILE) : 0u);
+      const uint32_t sk = smem_u32(smem) + F::K_OFF, sv = smem_u32(smem) + F::V_OFF;
+      const uint32_t ts = tmem + F::S_COL + (uint32_t)(a * BN), to = tmem + F::O_COL + (uint32_t)(a * DP);
+      const uint32_t tt = tmem + F::T_COL + (uint32_t)(a * BN / 2);
+      const int cnt = count(a);
+      bool ok = mbar_wait(&sh.q_bar, 0, abort_flag, err, 62);
+      // S of tile i, then O of it: tcgen05 MMAs of one thread run in issue
+      // order, so S of tile i + 1 overwrites P of tile i after O has read it
+      for (int i = 0; i <= cnt && ok; ++i) {
+        if (i > 0) {
+          const int t = tile(a, i - 1);
+          ok = mbar_wait(&sh.p_bar[a], (uint32_t)(i - 1) & 1u, abort_flag, err, 58) &&
+               mbar_wait(&sh.v_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 59);
+          if (!ok) break;
+          fence_after();
+          const uint64_t bd = smem_desc(sv + (uint32_t)((t % NS) * F::TILE), BN * 128, 1024, 2);
 #pragma unroll
-      for (int part = 0; part < QP; ++part)
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
-          mma_bf16(d, smem_desc(q + (uint32_t)(part * F::QTILE + (kk / 4) * 128 * 128 + (kk % 4) * 32), 16, 1024, 2),
-                   smem_desc(k + (uint32_t)((kk / 4) * BN * 128 + (kk % 4) * 32), 16, 1024, 2), id_s,
-                   part + kk > 0 ? 1u : 0u);
-      mma_commit(&sh.s_bar[a]);
-      if (!split || a == 1) mma_commit(&sh.k_free[t % NS]);
-      return true;
-    };
-    bool ok = true;
-    for (int a = 0; a < 2 && ok; ++a)
-      if (count(a) > 0) ok = issue_s(a, tile(a, 0));
-    for (int i = 0; i < count(0) && ok; ++i) {
-      for (int a = 0; a < 2 && ok; ++a) {
-        if (i >= count(a)) continue;
-        const int t = tile(a, i);
-        ok = mbar_wait(&sh.p_bar[a], (uint32_t)i & 1u, abort_flag, err, 58) &&
-             mbar_wait(&sh.v_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 59);
-        if (!ok) break;
-        fence_after();
-        const uint32_t d = tmem + F::O_COL + (uint32_t)(a * DP), pa = tmem + F::S_COL + (uint32_t)(a * BN);
-        const uint32_t v = sv + (uint32_t)((t % NS) * F::TILE);
-#pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
-          const uint64_t bd = smem_desc(v + (uint32_t)(kk * 2048), BN * 128, 1024, 2);
-          const uint32_t pc = pa + (uint32_t)((kk / 2) * 32 + (kk % 2) * 8);
-          mma_bf16_ts(d, pc, bd, id_o, i + kk > 0 ? 1u : 0u);
-          if (QP == 3) {
-            mma_bf16_ts(d, pc + 16, bd, id_o, 1u);
-            mma_bf16_ts(d, tmem + F::T_COL + (uint32_t)(a * BN / 2 + kk * 8), bd, id_o, 1u);
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            const uint32_t pc = ts + (uint32_t)((kk / 2) * 32 + (kk % 2) * 8);
+            mma_bf16_ts(to, pc, bd + kk * (2048 >> 4), id_o, i > 1 || kk > 0 ? 1u : 0u);
+            if (QP == 3) {
+              mma_bf16_ts(to, pc + 16, bd + kk * (2048 >> 4), id_o, 1u);
+              mma_bf16_ts(to, tt + (uint32_t)(kk * 8), bd + kk * (2048 >> 4), id_o, 1u);
+            }
           }
+          mma_commit(&sh.o_bar[a]);
+          mma_commit(&sh.v_free[t % NS]);
         }
-        mma_commit(&sh.o_bar[a]);
-        if (!split || a == 1) mma_commit(&sh.v_free[t % NS]);
-        if (i + 1 < count(a)) ok = issue_s(a, tile(a, i + 1));
+        if (i < cnt) {
+          const int t = tile(a, i);
+          ok = mbar_wait(&sh.k_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 57);
+          if (!ok) break;
+          fence_after();
+          const uint64_t qd = smem_desc(sq, 16, 1024, 2);
+          const uint64_t kd = smem_desc(sk + (uint32_t)((t % NS) * F::TILE), 16, 1024, 2);
+#pragma unroll
+          for (int part = QP - 1; part >= 0; --part)  // the accumulator truncates: small products first
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; ++kk)
+              mma_bf16(ts, qd + ((part * F::QTILE + (kk / 4) * 128 * 128 + (kk % 4) * 32) >> 4),
+                       kd + (((kk / 4) * BN * 128 + (kk % 4) * 32) >> 4), id_s, part < QP - 1 || kk > 0 ? 1u : 0u);
+          mma_commit(&sh.s_bar[a]);
+          mma_commit(&sh.k_free[t % NS]);
+        }
       }
+      // the accumulator is final, and no MMA of the stream reads shared memory, once this passes
+      if (ok && cnt > 0) mbar_wait(&sh.o_bar[a], (uint32_t)(cnt - 1) & 1u, abort_flag, err, 60);
     }
-    // the accumulators are final, and no MMA reads shared memory, once these pass
-    for (int a = 0; a < 2 && ok; ++a)
-      if (count(a) > 0) ok = mbar_wait(&sh.o_bar[a], (uint32_t)(count(a) - 1) & 1u, abort_flag, err, 60);
   }
+  // Registers go back to the launch's share: the loading and MMA warpgroups take
+  // theirs only once every softmax warp has had and returned its own (before
+  // that, a warpgroup that is done early could take what a softmax warp still
+  // waits for, and neither would go on).
   __syncwarp();
   fence_before();
   __syncthreads();
+  if (warp >= kSoftWarps) regs_inc<kRegsLaunch>();
   fence_after();
   const bool failed = sh.abort_flag != 0;
 
@@ -640,8 +797,37 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   cluster_sync();
   if (!failed) {
-    // rank c joins rows c, c + C, ..: one warp a row, lane j < np holds the weight of part j
-    const int np = split ? (int)C : 2 * (int)C;
+    // Rank c joins rows c, c + C, ..  First a thread per row turns the parts'
+    // maxima and sums into weights (part j: CTA j when split, else CTA j / 2,
+    // stream j % 2), then the outputs are summed with every load of a thread's
+    // values under way at once.
+    const int np = split ? (int)C : 2 * (int)C, mine = rows > (int)rank ? (rows - (int)rank + (int)C - 1) / (int)C : 0;
+    float* wgt = sh.wgt;
+    for (int k = tid; k < mine; k += kThreads) {
+      const int i = k * (int)C + (int)rank;
+      float pm[16], pl[16], mx = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        pm[j] = -INFINITY, pl[j] = 0.f;
+        if (j < np) {
+          const uint32_t c = (uint32_t)(split ? j : j / 2);
+          const int at = split ? i : (j & 1) * 128 + i;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm[j]) : "r"(cluster_addr(&sh.m[at], c)));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pl[j]) : "r"(cluster_addr(&sh.l[at], c)));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, pm[j]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        pm[j] = ex2(pm[j] - base);
+        l = fmaf(pl[j], pm[j], l);
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (j < np) wgt[k * np + j] = pm[j] / l;
+    }
     int bad = 0;
     if (!I8)
       for (uint32_t c = 0; c < C; ++c) {
@@ -649,56 +835,50 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(cluster_addr(&sh.bad, c)));
         bad |= x;
       }
-    for (int i = (int)rank + (int)C * warp; i < rows; i += (int)C * kWarps) {
-      float pm = -INFINITY, pl = 0.f;
-      // part j: CTA j (split), or CTA j / 2, stream j % 2
-      const int at_j = split ? i : (lane & 1) * 128 + i;
-      if (lane < np) {
-        const uint32_t c = (uint32_t)(split ? lane : lane / 2);
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm) : "r"(cluster_addr(&sh.m[at_j], c)));
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pl) : "r"(cluster_addr(&sh.l[at_j], c)));
-      }
-      float mx = pm;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float wgt = lane < np ? ex2(pm - (mx == -INFINITY ? 0.f : mx)) : 0.f;
-      float l = pl * wgt;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      const int row = r0 + i, t = row / p.G;
-      const unsigned long long fit = end - pos >= 64 ? ~0ull : end > pos ? (1ull << (end - pos)) - 1 : 0ull;
-      const unsigned long long drafted = pos >= 0 ? sh.mask[t] & fit : 0ull;
-      const bool any = pre > 0 || drafted;
+    __syncthreads();
+    constexpr int LPR = DP / 4;
+    const int gl = tid % LPR;
+    for (int k = tid / LPR; k < mine; k += kThreads / LPR) {
+      const int i = k * (int)C + (int)rank;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int j = 0; j < np; ++j) {
-        const float w = __shfl_sync(0xffffffffu, wgt, j);
-        if (lane < DP / 4) {
-          const uint32_t c = (uint32_t)(split ? j : j / 2);
-          const int at = split ? i : (j & 1) * 128 + i;
-          float4 x;
-          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                       : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                       : "r"(cluster_addr(so + at * F::LDO + lane * 4, c)));
-          if (w != 0.f) {  // a part without keys has no meaning for its row
-            acc.x = fmaf(x.x, w, acc.x);
-            acc.y = fmaf(x.y, w, acc.y);
-            acc.z = fmaf(x.z, w, acc.z);
-            acc.w = fmaf(x.w, w, acc.w);
+      for (int j0 = 0; j0 < np; j0 += 8) {
+        float4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j0 + j < np) {
+            const uint32_t c = (uint32_t)(split ? j0 + j : (j0 + j) / 2);
+            const int at = split ? i : (j & 1) * 128 + i;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(x[j].x), "=f"(x[j].y), "=f"(x[j].z), "=f"(x[j].w)
+                         : "r"(cluster_addr(so + at * F::LDO + gl * 4, c)));
           }
-        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j0 + j < np) {
+            const float w = wgt[k * np + j0 + j];
+            if (w != 0.f) {  // a part without keys has no meaning for its row
+              acc.x = fmaf(x[j].x, w, acc.x);
+              acc.y = fmaf(x[j].y, w, acc.y);
+              acc.z = fmaf(x[j].z, w, acc.z);
+              acc.w = fmaf(x[j].w, w, acc.w);
+            }
+          }
       }
-      if (lane * 4 < p.D) {
-        float y[4] = {acc.x / l, acc.y / l, acc.z / l, acc.w / l};
+      if (gl * 4 < p.D) {
+        const int row = r0 + i, t = row / p.G;
+        const unsigned long long fit = end - pos >= 64 ? ~0ull : end > pos ? (1ull << (end - pos)) - 1 : 0ull;
+        const unsigned long long drafted = pos >= 0 ? sh.mask[t] & fit : 0ull;
+        float y[4] = {acc.x, acc.y, acc.z, acc.w};
         if (bad)
           for (int j = 0; j < p.S; ++j)
             if (drafted >> j & 1ull)
 #pragma unroll
               for (int d = 0; d < 4; ++d) {
-                const float v = __bfloat162float(((const __nv_bfloat16*)p.v)[(nh * p.T + pos + j) * p.D + lane * 4 + d]);
+                const float v = __bfloat162float(((const __nv_bfloat16*)p.v)[(nh * p.T + pos + j) * p.D + gl * 4 + d]);
                 if (!isfinite(v)) y[d] += v;
               }
-        if (!any) y[0] = y[1] = y[2] = y[3] = 0.f;
-        const int64_t at = ((n * p.S + t) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + lane * 4;
+        if (pre <= 0 && !drafted) y[0] = y[1] = y[2] = y[3] = 0.f;
+        const int64_t at = ((n * p.S + t) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + gl * 4;
         if (QP == 1) *(uint2*)((__nv_bfloat16*)p.out + at) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
         else *(float4*)((float*)p.out + at) = make_float4(y[0], y[1], y[2], y[3]);
       }

@@ -267,6 +267,30 @@ def test_attention(sess, case, kind, src, tree):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 40.0])
+@pytest.mark.parametrize("n_tok,G,D", [(1, 2, 64), (20, 2, 64), (40, 4, 128)])
+def test_attention_scales(sess, kind, src, scale, n_tok, G, D):
+    """Scales of 0, negative, and large enough that maxima move by far more than
+    an exponent range between tiles."""
+    rng = np.random.default_rng(n_tok)
+    N, H, T, pos = 1, 2, 700, [600]
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    if not scales:  # growing keys: later tiles hold larger scores
+        for a in arrays:
+            a *= np.linspace(0.1, 1, T, dtype=np.float32)[:, None]
+            a[...] = R.bf16_round(a)
+        cache = S.KVCache(*[put(sess, a, kind) for a in arrays])
+    q = rand(rng, (N, n_tok, G * H, D), src)
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, scale)
+    out = put(sess, np.zeros(q.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out, scale=scale)
+    assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
 @pytest.mark.parametrize("n_tok,G,D", [(1, 1, 64), (1, 4, 128), (6, 2, 64), (40, 2, 64), (40, 4, 128)])
 def test_attention_ignores_what_it_does_not_attend_to(sess, kind, src, n_tok, G, D):
     """NaN and infinities behind the last token, and in drafted tokens that are
