@@ -20,32 +20,15 @@
 // its slice of the outputs from all C shared memories in rank order.  So the
 // split needs no workspace in memory and no atomics: results do not depend on
 // timing, and graphs that run at the same time share nothing.
-#include <cuda_bf16.h>
-
-#include <cmath>
-
-#include "kernels.h"
-#include "pdl.h"
-#include "tc_common.h"
+#include "cache_attn.h"
 
 namespace sb {
 namespace {
 
+using namespace cattn;
+
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int EPL = 8;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Params {
-  const void *k, *v;
-  const float *ks, *vs;
-  const int *positions, *parents;
-  const void* q;
-  void* out;
-  int bf16;  // q and out
-  int H, G, S, D, chunks;  // chunks of R rows
-  int64_t T;
-  float scale2;  // scale * log2(e)
-};
 
 template <typename T>
 struct Raw;  // 8 values as loaded
@@ -92,74 +75,29 @@ __device__ __forceinline__ void zero_raw(Raw<CT>& r) {
   r = Raw<CT>{};
 }
 
-// Which of the S drafted tokens token s attends to: bit j of mask[s].  The
-// parents' chains are closed by pointer doubling in shared memory (log2 S
-// rounds).  One warp.
-__device__ void tree_masks(const int* parents, int S, int lane, unsigned long long* mask, int* jump) {
-  for (int s = lane; s < S; s += 32) {
-    const int q = parents ? parents[s] : s - 1;
-    jump[s] = q >= 0 && q < s ? q : -1;
-    mask[s] = 1ull << s;
-  }
-  __syncwarp();
-  for (int d = 1; d < S; d *= 2) {
-    unsigned long long m[2];
-    int j[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int s = lane + 32 * i;
-      if (s < S) {
-        const int t = jump[s];
-        m[i] = mask[s] | (t >= 0 ? mask[t] : 0ull);
-        j[i] = t >= 0 ? jump[t] : -1;
-      }
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int s = lane + 32 * i;
-      if (s < S) mask[s] = m[i], jump[s] = j[i];
-    }
-    __syncwarp();
-  }
-}
-
 template <typename CT, int LPK, int R, int U>
 __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
   pdl_prologue();
   constexpr int KPW = 32 / LPK;   // rows of the cache a warp loads at once
   constexpr int DP = LPK * EPL;   // head size, padded
   constexpr int TK = KPW * U;
-  extern __shared__ float sm[];
-  float* s_o = sm;                              // [kWarps][R][DP]; the CTA's sum replaces warp 0's
-  float* s_m = sm + kWarps * R * DP;            // [kWarps][R]
-  float* s_l = s_m + kWarps * R;
+  extern __shared__ __align__(16) float sm[];  // [kWarps + 1][R][DP]
   __shared__ unsigned long long s_mask[kKvMaxTokens];
   __shared__ int s_jump[kKvMaxTokens];
-  __shared__ float c_m[R], c_l[R];
-
-  const uint32_t rank = tc::cluster_rank();
-  uint32_t C;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
+  __shared__ float s_m[kWarps * R], s_l[kWarps * R], s_ml[2 * R];
+  const Place w = find_place(p);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gl = lane % LPK, grp = lane / LPK;
-  const int64_t item = blockIdx.x / C;
-  const int chunk = (int)(item % p.chunks);
-  const int64_t nh = item / p.chunks, n = nh / p.H;
-  const int h = (int)(nh % p.H);
-  const int64_t pos = p.positions[n];
-  // keys: [0, pre) before the drafted tokens, [pos, end) drafted
-  const int64_t pre = pos < 0 ? 0 : min(pos, p.T), end = pos < 0 ? 0 : min(pos + p.S, p.T);
-  if (warp == 0) tree_masks(p.parents ? p.parents + n * p.S : nullptr, p.S, lane, s_mask, s_jump);
+  if (warp == 0) tree_masks(p.parents ? p.parents + w.n * p.S : nullptr, p.S, lane, s_mask, s_jump);
   __syncthreads();
 
-  const int rows = p.S * p.G, r0 = chunk * R;
+  const int r0 = w.chunk * R, rows = min(R, p.S * p.G - r0);
   float q[R][EPL], o[R][EPL], m[R], l[R];
   int tok[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int row = min(r0 + r, rows - 1);
+    const int row = r0 + min(r, rows - 1);
     tok[r] = row / p.G;
-    const int64_t at = ((n * p.S + tok[r]) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + gl * EPL;
+    const int64_t at = row_at(p, w, row) + gl * EPL;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) q[r][i] = o[r][i] = 0.f;
     if (gl * EPL < p.D) {
@@ -180,9 +118,9 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
   }
 
   // this CTA's positions
-  const int64_t per = (end + C - 1) / C, lo = min((int64_t)rank * per, end), hi = min(lo + per, end);
-  const CT* kb = (const CT*)p.k + nh * p.T * p.D + gl * EPL;
-  const CT* vb = (const CT*)p.v + nh * p.T * p.D + gl * EPL;
+  const int64_t per = (w.end + w.C - 1) / w.C, lo = min((int64_t)w.rank * per, w.end), hi = min(lo + per, w.end);
+  const CT* kb = (const CT*)p.k + w.nh * p.T * p.D + gl * EPL;
+  const CT* vb = (const CT*)p.v + w.nh * p.T * p.D + gl * EPL;
   const bool live_lane = gl * EPL < p.D;
   for (int64_t t0 = lo + warp * TK; t0 < hi; t0 += kWarps * TK) {
     Raw<CT> kr[U], vr[U];
@@ -199,8 +137,8 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
           load_raw(vb + t * p.D, vr[u]);
         }
         if constexpr (sizeof(CT) == 1) {
-          ksc[u] = p.ks[nh * p.T + t];
-          vsc[u] = p.vs[nh * p.T + t];
+          ksc[u] = p.ks[w.nh * p.T + t];
+          vsc[u] = p.vs[w.nh * p.T + t];
         }
       }
     }
@@ -220,14 +158,16 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
         s[u][r] = a;
       }
     }
+    const bool masked = t0 + TK > w.pre || t0 + TK > hi;
+    if (masked) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t t = t0 + u * KPW + grp;
+      for (int u = 0; u < U; ++u) {
+        const int64_t t = t0 + u * KPW + grp;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        bool see = t < hi;
-        if (t >= pre && t < hi) see = (s_mask[tok[r]] >> (t - pos)) & 1ull;
-        if (!see) s[u][r] = -INFINITY;
+        for (int r = 0; r < R; ++r) {
+          const bool see = t < hi && (t < w.pre || (s_mask[tok[r]] >> (t - w.pos) & 1ull));
+          if (!see) s[u][r] = -INFINITY;
+        }
       }
     }
 #pragma unroll
@@ -253,12 +193,12 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
       widen(vr[u], x);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        float w = s[u][r];
-        if constexpr (sizeof(CT) == 1) w *= vsc[u];
-        // a masked position holds anything, NaN included: it adds nothing
-        if (s[u][r] != 0.f) {
+        float y = s[u][r];
+        if constexpr (sizeof(CT) == 1) y *= vsc[u];
+        // a masked position may hold anything, NaN included: it adds nothing
+        if (!masked || s[u][r] != 0.f) {
 #pragma unroll
-          for (int i = 0; i < EPL; ++i) o[r][i] = fmaf(w, x[i], o[r][i]);
+          for (int i = 0; i < EPL; ++i) o[r][i] = fmaf(y, x[i], o[r][i]);
         }
       }
     }
@@ -268,111 +208,34 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
 #pragma unroll
-    for (int w = LPK; w < 32; w *= 2) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m[r], w), l2 = __shfl_xor_sync(0xffffffffu, l[r], w);
+    for (int x = LPK; x < 32; x *= 2) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m[r], x), l2 = __shfl_xor_sync(0xffffffffu, l[r], x);
       const float mx = fmaxf(m[r], m2), base = mx == -INFINITY ? 0.f : mx;
       const float a = exp2f(m[r] - base), b = exp2f(m2 - base);
       l[r] = l[r] * a + l2 * b;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) o[r][i] = o[r][i] * a + __shfl_xor_sync(0xffffffffu, o[r][i], w) * b;
+      for (int i = 0; i < EPL; ++i) o[r][i] = o[r][i] * a + __shfl_xor_sync(0xffffffffu, o[r][i], x) * b;
       m[r] = mx;
     }
     if (grp == 0) {
 #pragma unroll
-      for (int i = 0; i < EPL; ++i) s_o[(warp * R + r) * DP + gl * EPL + i] = o[r][i];
+      for (int i = 0; i < EPL; ++i) sm[(warp * R + r) * DP + gl * EPL + i] = o[r][i];
       if (gl == 0) s_m[warp * R + r] = m[r], s_l[warp * R + r] = l[r];
     }
   }
-  __syncthreads();
-  // join the warps
-  for (int i = tid; i < R * DP; i += kThreads) {
-    const int r = i / DP;
-    float mx = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, s_m[w * R + r]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float a = 0.f, b = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2f(s_m[w * R + r] - base);
-      a += s_o[w * R * DP + i] * f;
-      b += s_l[w * R + r] * f;
-    }
-    s_o[i] = a;
-    if (i % DP == 0) c_m[r] = mx, c_l[r] = b;
-  }
-  tc::cluster_sync();
-  // join the cluster: rank c of C finishes outputs i = c (mod C) in steps of a CTA
-  for (int i = (int)rank * kThreads + tid; i < R * DP; i += (int)C * kThreads) {
-    const int r = i / DP, d = i % DP;
-    float mx = -INFINITY;
-    for (uint32_t c = 0; c < C; ++c) {
-      float x;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::cluster_addr(&c_m[r], c)));
-      mx = fmaxf(mx, x);
-    }
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float a = 0.f, b = 0.f;
-    for (uint32_t c = 0; c < C; ++c) {
-      float xm, xl, xo;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(xm) : "r"(tc::cluster_addr(&c_m[r], c)));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(xl) : "r"(tc::cluster_addr(&c_l[r], c)));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(xo) : "r"(tc::cluster_addr(&s_o[i], c)));
-      const float f = exp2f(xm - base);
-      a += xo * f;
-      b += xl * f;
-    }
-    const int row = r0 + r;
-    if (row < rows && d < p.D) {
-      const int t = row / p.G;
-      // keys the token sees: the positions before, and its drafted ones that fit the cache
-      const unsigned long long fit = end - pos >= 64 ? ~0ull : end > pos ? (1ull << (end - pos)) - 1 : 0ull;
-      const bool any = pos >= 0 && (pre > 0 || (s_mask[t] & fit));
-      const float y = any ? a / b : 0.f;
-      const int64_t at = ((n * p.S + t) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + d;
-      if (p.bf16) ((__nv_bfloat16*)p.out)[at] = __float2bfloat16_rn(y);
-      else ((float*)p.out)[at] = y;
-    }
-  }
-  tc::cluster_sync();  // no CTA leaves while another may read its shared memory
+  join_and_store<kWarps, R, DP>(p, w, r0, rows, sm, s_m, s_l, sm + kWarps * R * DP, s_ml, s_mask,
+                                [](unsigned long long, int, float*) {});
 }
 
 template <typename CT, int LPK, int R, int U>
 cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
-  const KvCacheView& c = a.cache;
-  const int G = (int)(a.Hq / c.H), rows = (int)a.S * G, chunks = (rows + R - 1) / R;
-  Params p = {c.k, c.v, c.k_scale, c.v_scale, a.positions, a.parents, a.q, a.out, a.bf16 ? 1 : 0, (int)c.H, G, (int)a.S,
-              (int)c.D, chunks, c.T, a.scale * kLog2e};
-  const int64_t items = c.N * c.H * chunks;
-  static const int sms = [] {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
-  }();
+  const Params p = make_params(a, R);
+  const int64_t items = a.cache.N * a.cache.H * p.chunks;
   // split until every SM has two CTAs or a CTA has fewer than 64 positions
   int C = 1;
-  while (C < 8 && items * C < 2 * sms && c.T / (2 * C) >= 32) C *= 2;
-  if (items * C > INT32_MAX) return cudaErrorInvalidValue;
-  const size_t smem = (size_t)(kWarps * R * (LPK * EPL + 2)) * sizeof(float);
-  auto kern = cache_attn_kernel<CT, LPK, R, U>;
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(items * C));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[2];
-  pdl_attribute(&at[0]);
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = (unsigned)C;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  launch_counter().fetch_add(1, std::memory_order_relaxed);
-  return cudaLaunchKernelEx(&cfg, kern, p);
+  while (C < kMaxCluster && items * C < 2 * sm_count() && a.cache.T / (2 * C) >= 32) C *= 2;
+  const size_t smem = (size_t)((kWarps + 1) * R * LPK * EPL) * sizeof(float);
+  return launch_cluster(cache_attn_kernel<CT, LPK, R, U>, items * C, C, kThreads, smem, stream, p);
 }
 
 template <typename CT, int LPK>
@@ -396,6 +259,7 @@ cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream) {
+  if (cache_attention_mma_takes(a)) return cache_attention_mma(a, stream);
   if (cache_attention_tc_takes(a)) return cache_attention_tc(a, stream);
   switch (a.cache.type) {
     case KvType::F32: return by_dim<float>(a, stream);

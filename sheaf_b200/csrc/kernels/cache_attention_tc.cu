@@ -35,18 +35,14 @@
 //
 // Every mbarrier wait is bounded.  TMEM is freed before the cluster barrier: a
 // CTA that holds TMEM never waits for another CTA.
-#include <cuda_bf16.h>
-
-#include <cmath>
 #include <type_traits>
 
-#include "kernels.h"
-#include "pdl.h"
-#include "tc_common.h"
+#include "cache_attn.h"
 
 namespace sb {
 namespace {
 
+using namespace cattn;
 using namespace tc;
 
 // warps 0-7 softmax, 8-11 loading, 12 and 13 MMA issue (one per stream), 14, 15
@@ -64,20 +60,7 @@ __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.a
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int NS = 2;   // K and V tiles in flight
 constexpr int NSC = 4;  // rows of scales in flight (see the loader)
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;  // a row's maximum moves when it would grow by more than this (log2)
-
-struct Params {
-  const void *k, *v;
-  const float *ks, *vs;
-  const int *positions, *parents;
-  const void* q;
-  void* out;
-  int q_bf16;
-  int H, G, S, D, pairs;  // pairs: blocks of MAXR rows
-  int64_t T;
-  float scale2;
-};
 
 // D (TMEM) (+)= A (TMEM, bf16 pairs: lane = row, column = two k) * B.
 __device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bd, uint32_t idesc, uint32_t acc) {
@@ -198,36 +181,6 @@ struct Shared {
   float wgt[256 * 2];  // rows of a rank x parts: at most 256 / C x C, or 128 / C x 2 C
 };
 
-// see cache_attention.cu
-__device__ void tree_masks(const int* parents, int S, int lane, unsigned long long* mask, int* jump) {
-  for (int s = lane; s < S; s += 32) {
-    const int q = parents ? parents[s] : s - 1;
-    jump[s] = q >= 0 && q < s ? q : -1;
-    mask[s] = 1ull << s;
-  }
-  __syncwarp();
-  for (int d = 1; d < S; d *= 2) {
-    unsigned long long m[2];
-    int j[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int s = lane + 32 * i;
-      if (s < S) {
-        const int t = jump[s];
-        m[i] = mask[s] | (t >= 0 ? mask[t] : 0ull);
-        j[i] = t >= 0 ? jump[t] : -1;
-      }
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int s = lane + 32 * i;
-      if (s < S) mask[s] = m[i], jump[s] = j[i];
-    }
-    __syncwarp();
-  }
-}
-
 // I8: int8 cache, else bf16.  QP: parts of a query (1: bf16, 3: f32).
 template <int DP, int BN, int QP, bool I8>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -239,16 +192,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ Shared sh;
   __shared__ __align__(16) float sc_k[I8 ? NSC : 1][I8 ? BN : 4], sc_v[I8 ? NSC : 1][I8 ? BN : 4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = cluster_rank();
-  uint32_t C;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(C));
-  const int64_t item = blockIdx.x / C;
-  const int pair = (int)(item % p.pairs);
-  const int64_t nh = item / p.pairs, n = nh / p.H;
-  const int h = (int)(nh % p.H);
-  const int64_t pos = p.positions[n];
-  const int64_t pre = pos < 0 ? 0 : min(pos, p.T), end = pos < 0 ? 0 : min(pos + p.S, p.T);
-  const int r0 = pair * F::MAXR, rows = min(F::MAXR, p.S * p.G - r0);
+  const Place w = find_place(p);
+  const uint32_t rank = w.rank, C = w.C;
+  const int64_t n = w.n, nh = w.nh, pos = w.pos, pre = w.pre, end = w.end;
+  const int h = w.h, r0 = w.chunk * F::MAXR, rows = min(F::MAXR, p.S * p.G - r0);
   const bool split = rows > 128;                 // streams by rows, else by tiles
   const int up = !split && rows <= 64 ? 64 : 0;  // stream 1's first TMEM lane
   // this CTA's tiles [first, first + nt)
@@ -290,17 +237,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // Queries into swizzled K-major tiles: tile (row block, part) of 128 rows; one
   // block of rows repeated at lane `up` when stream 1 uses those lanes.
-  // `w` of kStageWarps warps.  A negative scale of bf16 queries goes into their
+  // Warp `sw` of kStageWarps.  A negative scale of bf16 queries goes into their
   // signs, so that the softmax can take maxima before it scales.
-  auto stage_q = [&](int w) {
+  auto stage_q = [&](int sw) {
     // a thread keeps its 8-value column `u` and walks the rows
     constexpr int UNITS = DP / 8, RSTEP = kStageWarps * 32 / UNITS, LOADS = QP == 1 ? 1 : 2, BATCH = QP == 1 ? 8 : 4;
     static_assert(kStageWarps * 32 % UNITS == 0, "whole rows per step");
-    const int u = (w * 32 + lane) % UNITS, total = nt > 0 && aligned ? (split ? 256 : 128) : 0;
+    const int u = (sw * 32 + lane) % UNITS, total = nt > 0 && aligned ? (split ? 256 : 128) : 0;
     const int64_t q0 = (n * p.S * p.H + h) * p.G * p.D + u * 8;
     const int64_t token = (int64_t)p.H * p.G * p.D;
 #pragma unroll 1
-    for (int k0 = (w * 32 + lane) / UNITS; k0 < total; k0 += BATCH * RSTEP) {
+    for (int k0 = (sw * 32 + lane) / UNITS; k0 < total; k0 += BATCH * RSTEP) {
       uint4 raw[BATCH][LOADS];
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
@@ -535,15 +482,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t vis[BN / 32];
           const int64_t off = pos - t0;  // column of drafted token 0
 #pragma unroll
-          for (int w = 0; w < BN / 32; ++w) {
-            const int64_t c0 = w * 32;
+          for (int vw = 0; vw < BN / 32; ++vw) {
+            const int64_t c0 = vw * 32;
             const uint32_t before = pre - t0 >= c0 + 32 ? ~0u : pre - t0 <= c0 ? 0u : (1u << (pre - t0 - c0)) - 1u;
             const int64_t j0 = c0 - off;  // drafted token at the word's first column
             uint32_t d = 0;
             if (j0 >= 0) d = j0 < 64 ? (uint32_t)(seen >> j0) : 0u;
             else if (j0 > -32) d = (uint32_t)(seen << -j0);
             const uint32_t fit = end - t0 >= c0 + 32 ? ~0u : end - t0 <= c0 ? 0u : (1u << (end - t0 - c0)) - 1u;
-            vis[w] = (before | (pos < p.T ? d : 0u)) & fit;
+            vis[vw] = (before | (pos < p.T ? d : 0u)) & fit;
           }
           softmax(std::true_type{}, vis);
         } else {
@@ -865,9 +812,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
       }
       if (gl * 4 < p.D) {
-        const int row = r0 + i, t = row / p.G;
-        const unsigned long long fit = end - pos >= 64 ? ~0ull : end > pos ? (1ull << (end - pos)) - 1 : 0ull;
-        const unsigned long long drafted = pos >= 0 ? sh.mask[t] & fit : 0ull;
+        const int row = r0 + i;
+        const unsigned long long drafted = drafted_seen(w, sh.mask[row / p.G]);
         float y[4] = {acc.x, acc.y, acc.z, acc.w};
         if (bad)
           for (int j = 0; j < p.S; ++j)
@@ -878,9 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!isfinite(v)) y[d] += v;
               }
         if (pre <= 0 && !drafted) y[0] = y[1] = y[2] = y[3] = 0.f;
-        const int64_t at = ((n * p.S + t) * p.H * p.G + (int64_t)h * p.G + row % p.G) * p.D + gl * 4;
-        if (QP == 1) *(uint2*)((__nv_bfloat16*)p.out + at) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-        else *(float4*)((float*)p.out + at) = make_float4(y[0], y[1], y[2], y[3]);
+        store4(p, row_at(p, w, row) + gl * 4, make_float4(y[0], y[1], y[2], y[3]));
       }
     }
   }
@@ -891,9 +835,7 @@ template <int DP, int BN, int QP, bool I8>
 cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   using F = Cfg<DP, BN, QP>;
   const KvCacheView& c = a.cache;
-  const int G = (int)(a.Hq / c.H), rows = (int)a.S * G, pairs = (rows + F::MAXR - 1) / F::MAXR;
-  Params p = {c.k, c.v, c.k_scale, c.v_scale, a.positions, a.parents, a.q, a.out, a.bf16 ? 1 : 0, (int)c.H, G, (int)a.S,
-              (int)c.D, pairs, c.T, a.scale * kLog2e};
+  const Params p = make_params(a, F::MAXR);
   CUtensorMap mk{}, mv{};
   if (!I8) {
     const uint64_t dims[3] = {(uint64_t)c.D, (uint64_t)c.T, (uint64_t)(c.N * c.H)};
@@ -903,36 +845,17 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   }
   int* err = tc_error_word();
   if (!err) return cudaErrorMemoryAllocation;
-  const int64_t items = c.N * c.H * pairs;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t items = c.N * c.H * p.chunks;
   // one CTA fits an SM: split until the CTAs fill the SMs once, or a CTA has two tiles
   int C = 1;
-  while (C < 8 && items * (C + 1) <= sms && c.T / (C + 1) >= 2 * BN) ++C;
-  if (items * C > INT32_MAX) return cudaErrorInvalidValue;
-  auto kern = cache_attn_tc<DP, BN, QP, I8>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(items * C));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = F::SMEM;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[2];
-  pdl_attribute(&at[0]);
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = (unsigned)C;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  launch_counter().fetch_add(1, std::memory_order_relaxed);
-  return cudaLaunchKernelEx(&cfg, kern, mk, mv, p, err);
+  while (C < kMaxCluster && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 2 * BN) ++C;
+  return launch_cluster(cache_attn_tc<DP, BN, QP, I8>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);
 }
 
 }  // namespace
 
 bool cache_attention_tc_takes(const CacheAttnArgs& a) {
-  return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 && a.S * (a.Hq / a.cache.H) > 8;
+  return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 && a.S * (a.Hq / a.cache.H) > (a.bf16 ? 16 : 4);
 }
 
 cudaError_t cache_attention_tc(const CacheAttnArgs& a, cudaStream_t stream) {

@@ -1,0 +1,242 @@
+// Parts shared by the kernels of attention over a key/value cache
+// (cache_attention.cu, cache_attention_mma.cu, cache_attention_tc.cu).
+// Included by .cu files only.
+#pragma once
+#include <cuda_bf16.h>
+
+#include <cmath>
+
+#include "kernels.h"
+#include "pdl.h"
+#include "tc_common.h"
+
+namespace sb {
+namespace cattn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+  const void *k, *v;
+  const float *ks, *vs;
+  const int *positions, *parents;
+  const void* q;
+  void* out;
+  int bf16;             // q and out
+  int H, G, S, D;       // cache heads, query heads per cache head, tokens, head size
+  int chunks;           // blocks of query rows (token x query head) per (slot, cache head)
+  int64_t T;
+  float scale2;         // scale * log2(e)
+};
+
+inline Params make_params(const CacheAttnArgs& a, int chunk_rows) {
+  const KvCacheView& c = a.cache;
+  const int G = (int)(a.Hq / c.H), rows = (int)a.S * G;
+  return {c.k, c.v, c.k_scale, c.v_scale, a.positions, a.parents, a.q, a.out, a.bf16 ? 1 : 0, (int)c.H, G, (int)a.S,
+          (int)c.D, (rows + chunk_rows - 1) / chunk_rows, c.T, a.scale * kLog2e};
+}
+
+inline int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n;
+}
+
+template <typename... K, typename... A>
+cudaError_t launch_cluster(void (*kern)(K...), int64_t blocks, int cluster, int threads, size_t smem,
+                           cudaStream_t stream, A&&... args) {
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  pdl_attribute(&at[0]);
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  launch_counter().fetch_add(1, std::memory_order_relaxed);
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t c;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(c));
+  return c;
+}
+
+// Where a CTA stands: the (slot, cache head) and block of rows of its cluster,
+// and the keys there: positions [0, pre) before the drafted tokens, and the
+// drafted ones at [pos, end).
+struct Place {
+  uint32_t rank, C;
+  int chunk, h;
+  int64_t nh, n, pos, pre, end;
+};
+__device__ __forceinline__ Place find_place(const Params& p) {
+  Place w;
+  w.rank = tc::cluster_rank();
+  w.C = cluster_size();
+  const unsigned item = blockIdx.x / w.C;
+  w.chunk = (int)(item % (unsigned)p.chunks);
+  const unsigned nh = item / (unsigned)p.chunks;
+  w.nh = nh;
+  w.n = nh / (unsigned)p.H;
+  w.h = (int)(nh % (unsigned)p.H);
+  w.pos = p.positions[w.n];
+  w.pre = w.pos < 0 ? 0 : min(w.pos, p.T);
+  w.end = w.pos < 0 ? 0 : min(w.pos + p.S, p.T);
+  return w;
+}
+
+// Element offset of row `row` (token row / G, query head h G + row % G) in q and out.
+__device__ __forceinline__ int64_t row_at(const Params& p, const Place& w, int row) {
+  const int s = row / p.G, g = row - s * p.G;
+  return (((w.n * p.S + s) * p.H + w.h) * p.G + g) * p.D;
+}
+
+// Which of the S drafted tokens token s attends to: bit j of mask[s].  The
+// parents' chains are closed by pointer doubling in shared memory (log2 S
+// rounds).  One warp.
+__device__ __forceinline__ void tree_masks(const int* parents, int S, int lane, unsigned long long* mask, int* jump) {
+  for (int s = lane; s < S; s += 32) {
+    const int q = parents ? parents[s] : s - 1;
+    jump[s] = q >= 0 && q < s ? q : -1;
+    mask[s] = 1ull << s;
+  }
+  __syncwarp();
+  for (int d = 1; d < S; d *= 2) {
+    unsigned long long m[2];
+    int j[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = lane + 32 * i;
+      if (s < S) {
+        const int t = jump[s];
+        m[i] = mask[s] | (t >= 0 ? mask[t] : 0ull);
+        j[i] = t >= 0 ? jump[t] : -1;
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int s = lane + 32 * i;
+      if (s < S) mask[s] = m[i], jump[s] = j[i];
+    }
+    __syncwarp();
+  }
+}
+
+// The drafted tokens that a token with mask `mask` sees and that fit the cache.
+__device__ __forceinline__ unsigned long long drafted_seen(const Place& w, unsigned long long mask) {
+  const int64_t fit = w.end - w.pos;
+  return w.pos < 0 || fit <= 0 ? 0ull : fit >= 64 ? mask : mask & ((1ull << fit) - 1);
+}
+
+__device__ __forceinline__ float ld_remote(const float* p, uint32_t rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::cluster_addr(p, rank)));
+  return x;
+}
+__device__ __forceinline__ float4 ld_remote4(const float* p, uint32_t rank) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+               : "r"(tc::cluster_addr(p, rank)));
+  return x;
+}
+
+__device__ __forceinline__ void store4(const Params& p, int64_t at, float4 y) {
+  if (p.bf16) {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(y.x, y.y), __floats2bfloat162_rn(y.z, y.w)};
+    *(uint2*)((__nv_bfloat16*)p.out + at) = *(uint2*)h;
+  } else {
+    *(float4*)((float*)p.out + at) = y;
+  }
+}
+
+constexpr int kMaxCluster = 8;
+
+// The partial results of up to R rows, joined and written: first the NW warps'
+// of a CTA, then the CTAs' of the cluster (rank c finishes every C-th piece of
+// 4 values).  part_o [NW][R][DP], part_m, part_l [NW][R] in shared memory (m:
+// base-2 maximum, l: sum); every thread of the CTA calls, before which the
+// parts were written.  cta_o [R][DP] and cta_ml [2 R] are shared too.  fix(row,
+// d, y) may amend the finished values; a row without keys gets zeros.
+template <int NW, int R, int DP, typename Fix>
+__device__ __forceinline__ void join_and_store(const Params& p, const Place& w, int r0, int rows,
+                                               const float* part_o, const float* part_m, const float* part_l,
+                                               float* cta_o, float* cta_ml, const unsigned long long* mask, Fix fix) {
+  constexpr int V = DP / 4;
+  const int tid = threadIdx.x;
+  __syncthreads();
+  for (int i = tid; i < rows * V; i += NW * 32) {
+    const int r = i / V, d = (i % V) * 4;
+    float m[NW], mx = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < NW; ++j) mx = fmaxf(mx, m[j] = part_m[j * R + r]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < NW; ++j) {
+      const float f = exp2f(m[j] - base);
+      const float4 x = *(const float4*)(part_o + (j * R + r) * DP + d);
+      a.x = fmaf(x.x, f, a.x);
+      a.y = fmaf(x.y, f, a.y);
+      a.z = fmaf(x.z, f, a.z);
+      a.w = fmaf(x.w, f, a.w);
+      l = fmaf(part_l[j * R + r], f, l);
+    }
+    *(float4*)(cta_o + r * DP + d) = a;
+    if (d == 0) cta_ml[r] = mx, cta_ml[R + r] = l;
+  }
+  if (w.C > 1) tc::cluster_sync();
+  else __syncthreads();
+  for (int i = (int)w.rank * NW * 32 + tid; i < rows * V; i += (int)w.C * NW * 32) {
+    const int r = i / V, d = (i % V) * 4;
+    float m[kMaxCluster], l[kMaxCluster];
+    float4 x[kMaxCluster];
+#pragma unroll
+    for (uint32_t c = 0; c < kMaxCluster; ++c) {
+      m[c] = -INFINITY, l[c] = 0.f, x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (c < w.C) {
+        m[c] = ld_remote(&cta_ml[r], c);
+        l[c] = ld_remote(&cta_ml[R + r], c);
+        x[c] = ld_remote4(cta_o + r * DP + d, c);
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) mx = fmaxf(mx, m[c]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      const float f = exp2f(m[c] - base);
+      a.x = fmaf(x[c].x, f, a.x);
+      a.y = fmaf(x[c].y, f, a.y);
+      a.z = fmaf(x[c].z, f, a.z);
+      a.w = fmaf(x[c].w, f, a.w);
+      sum = fmaf(l[c], f, sum);
+    }
+    if (d < p.D) {
+      const int row = r0 + r;
+      const unsigned long long seen = drafted_seen(w, mask[row / p.G]);
+      float y[4] = {a.x / sum, a.y / sum, a.z / sum, a.w / sum};
+      fix(seen, d, y);
+      if (w.pre <= 0 && !seen) y[0] = y[1] = y[2] = y[3] = 0.f;
+      store4(p, row_at(p, w, row) + d, make_float4(y[0], y[1], y[2], y[3]));
+    }
+  }
+  if (w.C > 1) tc::cluster_sync();  // no CTA leaves while another may read its shared memory
+}
+
+}  // namespace cattn
+}  // namespace sb

@@ -279,10 +279,14 @@ struct CacheAttnArgs {
   float scale = 1.f;  // multiplier of q.k before the softmax
 };
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
-// The tensor-core kernel (kernels/cache_attention_tc.cu) and the calls it is
-// for: bf16 or int8 caches of head size 64 to 128 with more than 8 query rows
-// per cache head.  cache_attention calls it; it reports failed waits through
-// the tensor-core error word (codes 50..60).
+// The kernels for bf16 and int8 caches of head size 64 to 128 and the calls
+// they take (cache_attention dispatches): up to 16 bf16 or 4 f32 query rows
+// (tokens x query heads per cache head) multiply with warp instructions
+// (kernels/cache_attention_mma.cu), more rows with tcgen05
+// (kernels/cache_attention_tc.cu, which reports failed waits through the
+// tensor-core error word, codes 50..62).
+bool cache_attention_mma_takes(const CacheAttnArgs& a);
+cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream);
 bool cache_attention_tc_takes(const CacheAttnArgs& a);
 cudaError_t cache_attention_tc(const CacheAttnArgs& a, cudaStream_t stream);
 
