@@ -4,15 +4,19 @@
 //
 // Reading the cache once bounds it; on the CUDA cores the products (2 FMA per
 // value and row) pass that from 2 to 4 rows on.  Here a warp multiplies with
-// m16n8k16 bf16 instructions straight from the registers it loads into: no
-// shared memory, no barrier in the loop.  (A tcgen05 tile has 128 rows, of
-// which up to 16 would be used, and needs every tile staged and converted in
-// shared memory; cache_attention_tc.cu takes over where its rows fill.)
+// m16n8k16 bf16 instructions.  (A tcgen05 tile has 128 rows, of which up to 16
+// would be used, and needs every tile converted and swizzled in shared memory;
+// cache_attention_tc.cu takes over where its rows fill.)
+//
+// Each warp streams its steps of keys through its own ring of stages in shared
+// memory, filled by TMA (one lane issues 2 to 4 copies a step; loads into
+// registers kept too few bytes under way, and asynchronous copies per lane cost
+// too many instructions).  There is no barrier between warps in the loop.
 //
 //   S = Q K^T  A = Q (16 rows), B = K: lane (g, c) = (lane / 4, lane % 4) holds
 //              key g's values.  The head dimension may be summed in any order,
-//              so a lane takes consecutive values (one 16-byte load: 8 bf16 or
-//              16 codes) and Q is laid out to match.
+//              so a lane takes consecutive values (one 16-byte piece: 8 bf16
+//              or 16 codes) and Q is laid out to match.
 //   O += P V   A = P: the accumulators of S are its operand layout already.  B
 //              pairs two keys of one column: lane (g, c) loads consecutive
 //              columns of keys 2c, 2c + 1, 2c + 8, 2c + 9 and pairs them by
@@ -61,18 +65,13 @@ __device__ __forceinline__ uint32_t codes(uint32_t t) {
   return *(uint32_t*)&x;
 }
 
-__device__ __forceinline__ uint4 load16(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
+// Four bytes to shared memory, asynchronously; zero where `in` is false.
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ uint2 load8(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Takes values that are not finite out of a word of two bf16.
 __device__ __forceinline__ uint32_t finite_only(uint32_t w, bool& bad) {
@@ -87,20 +86,46 @@ template <int DP, bool I8, bool Q32>
 struct MmaCfg {
   static constexpr int RMAX = Q32 ? 4 : 16, NR = Q32 ? 1 : 2;  // rows of the CTA, of a lane
   static constexpr int KB = I8 ? 32 : 16;                      // keys per step
-  static constexpr int EK = I8 ? 16 : 8;                       // values of a lane's K load
-  static constexpr int KL = DP / (4 * EK);                     // K loads per key
-  static constexpr int EV = I8 ? DP / 8 : 8;                   // values of a lane's V load
-  static constexpr int VL = DP / (8 * EV);                     // V loads per key
-  static constexpr int SMEM = (kWarps + 1) * RMAX * DP * 4;
+  static constexpr int EK = I8 ? 16 : 8;                       // values of a lane's 16-byte piece of K
+  static constexpr int KL = DP / (4 * EK);                     // such pieces per key
+  static constexpr int EV = I8 ? DP / 8 : 8;                   // values of a lane's piece of V
+  static constexpr int VL = DP / (8 * EV);                     // such pieces per key
+  static constexpr int RB = DP * (I8 ? 1 : 2) < 128 ? 64 : 128;  // bytes of a row in a TMA box
+  static constexpr int BOXES = DP * (I8 ? 1 : 2) / RB, BOX = KB * RB;
+  // a warp's stage: K boxes, V boxes; its scales stand behind all stages
+  static constexpr int STAGE = 2 * BOXES * BOX, STAGES = 3;
+  static constexpr int SC_OFF = kWarps * STAGES * STAGE, END = SC_OFF + (I8 ? kWarps * STAGES * KB * 8 : 0);
+  static constexpr int JOIN = (kWarps + 1) * RMAX * DP * 4;
+  static constexpr int SMEM = END > JOIN ? END : JOIN;
 };
 
+// The keys of a block of 8 in the order in which the fragments' columns take
+// them, so that the 16-byte pieces that a quarter of a warp reads together lie
+// in different banks of the swizzled boxes, for K (two keys, four pieces each)
+// and V (four keys, two pieces each).
+template <int RB>
+__device__ __forceinline__ int key_of(int x) {
+  if (RB == 128) return x & 1 ? (x - 1) ^ 5 : x;  // 0 5 2 7 4 1 6 3
+  const int e = ((x >> 1) & 1) | ((x >> 1) & 2) << 1;
+  return x & 1 ? e ^ 3 : e;  // 0 3 1 2 4 7 5 6
+}
+// Byte of piece u (16 bytes) of row `key` in a box, as TMA swizzles it.
+template <int RB>
+__device__ __forceinline__ int piece_at(int key, int u) {
+  return key * RB + ((RB == 128 ? u ^ (key & 7) : u ^ (key >> 1 & 3)) << 4);
+}
+
 template <int DP, bool I8, bool Q32>
-__global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
+__global__ void __launch_bounds__(kThreads)
+    cache_attn_mma(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const Params p,
+                   int* err) {
   using F = MmaCfg<DP, I8, Q32>;
   constexpr int KB = F::KB, NB = KB / 8, KG = KB / 16, EK = F::EK, KL = F::KL, VL = F::VL, NR = F::NR, RMAX = F::RMAX;
-  constexpr int ES = I8 ? 1 : 2;  // bytes per value
+  constexpr int RB = F::RB, BOX = F::BOX, STAGES = F::STAGES;
   pdl_prologue();
-  extern __shared__ __align__(16) float sm[];
+  extern __shared__ __align__(1024) float sm[];  // the warps' stages, later their partial outputs
+  __shared__ uint64_t s_full[kWarps][F::STAGES];
+  __shared__ volatile int s_abort;
   __shared__ unsigned long long s_mask[kKvMaxTokens];
   __shared__ int s_jump[kKvMaxTokens];
   __shared__ float s_m[kWarps * RMAX], s_l[kWarps * RMAX], s_ml[2 * RMAX];
@@ -112,67 +137,46 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
   const int64_t per = ((w.end + w.C - 1) / w.C + KB - 1) / KB * KB;
   const int64_t lo = min((int64_t)w.rank * per, w.end), hi = min(lo + per, w.end);
 
-  const uint8_t* kb = (const uint8_t*)p.k + w.nh * p.T * p.D * ES;
-  const uint8_t* vb = (const uint8_t*)p.v + w.nh * p.T * p.D * ES;
   const float *ksb = I8 ? p.ks + w.nh * p.T : nullptr, *vsb = I8 ? p.vs + w.nh * p.T : nullptr;
-  const int64_t rs = (int64_t)p.D * ES;
-  uint4 kr[NB][KL];
-  uint4 vr[KG][4][VL];
-  float ks[NB][2], vs[NB][2];
-  auto load_k = [&](int64_t t0) {
+  uint8_t* const ring = (uint8_t*)sm + warp * STAGES * F::STAGE;
+  float* const scales = (float*)((uint8_t*)sm + F::SC_OFF) + warp * STAGES * KB * 2;
+  uint64_t* const full = s_full[warp];
+  if (tid == 0) {
+    for (int i = 0; i < kWarps * STAGES; ++i) tc::mbar_init(&s_full[0][i], 1);
+    s_bad = 0;
+    s_abort = tc::smem_u32(sm) & 1023u ? 1 : 0;
+    if (s_abort) atomicExch(err, 63);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_proxy_async();
+  }
+  __syncthreads();
+  // One step's keys into stage `st` of this warp: boxes by TMA (rows behind the
+  // cache's capacity arrive as zeros), scales by asynchronous copies.
+  auto fetch = [&](int64_t t, int st) {
+    if (lane == 0 && !s_abort) {
+      tc::mbar_expect_tx(&full[st], F::STAGE);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int64_t t = t0 + b * 8 + g;
-#pragma unroll
-      for (int i = 0; i < KL; ++i) {
-        const int d = i * 4 * EK + c * EK;
-        kr[b][i] = make_uint4(0, 0, 0, 0);
-        if (t < hi && d < p.D) kr[b][i] = load16(kb + t * rs + d * ES);
-      }
-      if (I8) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int64_t t2 = t0 + b * 8 + 2 * c + i;
-          ks[b][i] = t2 < hi ? ksb[t2] : 0.f;
-        }
+      for (int i = 0; i < F::BOXES; ++i) {
+        uint8_t* dst = ring + st * F::STAGE + i * BOX;
+        tc::tma_load_3d(dst, &mK, &full[st], i * (RB / (I8 ? 1 : 2)), (int)t, (int)w.nh);
+        tc::tma_load_3d(dst + F::BOXES * BOX, &mV, &full[st], i * (RB / (I8 ? 1 : 2)), (int)t, (int)w.nh);
       }
     }
-  };
-  auto load_v = [&](int64_t t0) {
-#pragma unroll
-    for (int k = 0; k < KG; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t t = t0 + k * 16 + 2 * c + (i & 1) + (i >> 1) * 8;
-#pragma unroll
-        for (int j = 0; j < VL; ++j) {
-          const int d = j * 8 * F::EV + g * F::EV;
-          vr[k][i][j] = make_uint4(0, 0, 0, 0);
-          if (t < hi && d < p.D) {
-            if (F::EV * ES == 8) {
-              const uint2 x = load8(vb + t * rs + d * ES);
-              vr[k][i][j].x = x.x, vr[k][i][j].y = x.y;
-            } else {
-              vr[k][i][j] = load16(vb + t * rs + d * ES);
-            }
-          }
-        }
-      }
-    if (I8) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int64_t t = t0 + b * 8 + 2 * c + i;
-          vs[b][i] = t < hi ? vsb[t] : 0.f;
-        }
+    if (I8) {  // KB = 32: a scale of each kind per lane
+      const bool in = t + lane < w.end;
+      const uint32_t at = tc::smem_u32(scales + st * KB * 2 + lane);
+      copy4(at, in ? ksb + t + lane : ksb, in);
+      copy4(at + KB * 4, in ? vsb + t + lane : vsb, in);
     }
   };
   int64_t t0 = lo + warp * KB;
-  load_k(t0);
-  load_v(t0);
+  constexpr int STRIDE = kWarps * KB;
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) {
+    if (t0 + i * STRIDE < hi) fetch(t0 + i * STRIDE, i);
+    copies_commit();
+  }
   if (warp == 0) tree_masks(p.parents ? p.parents + w.n * p.S : nullptr, p.S, lane, s_mask, s_jump);
-  if (tid == 0) s_bad = 0;
 
   // Q: k-step s takes values d .. d + 3 of the lane's EK
   uint32_t q[DP / 16][4];
@@ -183,7 +187,8 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
       const int row = g & 3;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < rows && d < p.D) x = *(const float4*)((const float*)p.q + row_at(p, w, r0 + row) + d);
-      const float y[4] = {x.x * p.scale2, x.y * p.scale2, x.z * p.scale2, x.w * p.scale2};
+      // the pairs of an int8 word: bytes 0 and 2, bytes 1 and 3
+      const float y[4] = {x.x * p.scale2, (I8 ? x.z : x.y) * p.scale2, (I8 ? x.y : x.z) * p.scale2, x.w * p.scale2};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint32_t a = pack_bf16(y[2 * i], y[2 * i + 1]);
@@ -198,8 +203,8 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
         const int row = g + 8 * r;
         uint2 x = make_uint2(0, 0);
         if (row < rows && d < p.D) x = *(const uint2*)((const __nv_bfloat16*)p.q + row_at(p, w, r0 + row) + d);
-        q[s][r] = x.x;
-        q[s][2 + r] = x.y;
+        q[s][r] = I8 ? __byte_perm(x.x, x.y, 0x5410) : x.x;  // see above
+        q[s][2 + r] = I8 ? __byte_perm(x.x, x.y, 0x7632) : x.y;
       }
     }
   }
@@ -214,27 +219,39 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
 #pragma unroll
   for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.f;
 
-  for (; t0 < hi; t0 += kWarps * KB) {
+  const int kg = key_of<RB>(g), kc[2] = {key_of<RB>(2 * c), key_of<RB>(2 * c + 1)};
+  int st = 0;
+  uint32_t phase = 0;
+  for (; t0 < hi; t0 += STRIDE) {
+    copies_wait<STAGES - 1>();
+    if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[st], phase, &s_abort, err, 64))) break;
+    const uint8_t *const stage = ring + st * F::STAGE, *const stage_v = stage + F::BOXES * BOX;
+    const float* const sc = scales + st * KB * 2;
     float s[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
+    for (int i = 0; i < KL; ++i) {
+      uint4 x[NB];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const uint4& x = kr[b][k / (EK / 4)];
-        const uint32_t word[4] = {x.x, x.y, x.z, x.w};
-        if (I8) {
-          const uint32_t y = word[k % 4];
-          mma16816(s[b], q[k], codes(__byte_perm(y, 0, 0x4140)), codes(__byte_perm(y, 0, 0x4342)));
-        } else {
-          mma16816(s[b], q[k], word[(k % 2) * 2], word[(k % 2) * 2 + 1]);
+      for (int b = 0; b < NB; ++b)
+        x[b] = *(const uint4*)(stage + (i * 4 * 16 / RB) * BOX + piece_at<RB>(b * 8 + kg, (i * 4) % (RB / 16) + c));
+#pragma unroll
+      for (int k = 0; k < EK / 4; ++k)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint32_t word[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
+          const uint32_t* a = q[i * (EK / 4) + k];
+          if (I8) mma16816(s[b], a, codes(word[k]), codes(word[k] >> 8));
+          else mma16816(s[b], a, word[(k % 2) * 2], word[(k % 2) * 2 + 1]);
         }
-      }
+    }
     // scores of the lane's NR rows and two keys per block, in units of log2
     float x[NB][NR][2];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      float2 f = make_float2(1.f, 1.f);
+      if (I8) f = make_float2(sc[b * 8 + kc[0]], sc[b * 8 + kc[1]]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (Q32) {
@@ -246,40 +263,22 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
         }
         if (I8)
 #pragma unroll
-          for (int r = 0; r < NR; ++r) x[b][r][i] *= ks[b][i];
+          for (int r = 0; r < NR; ++r) x[b][r][i] *= i ? f.y : f.x;
       }
-    const int64_t tn = t0 + kWarps * KB;
-    load_k(tn);  // under way during the softmax and the second product
+    }
     const bool masked = t0 + KB > w.pre || t0 + KB > hi;
     if (masked) {
-      bool bad = false;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int64_t t = t0 + b * 8 + 2 * c + i;
+          const int64_t t = t0 + b * 8 + kc[i];
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
             const bool see = t < hi && (t < w.pre || (seen[r] >> (t - w.pos) & 1ull));
             if (!see) x[b][r][i] = -INFINITY;
           }
         }
-      if (!I8) {
-#pragma unroll
-        for (int k = 0; k < KG; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t t = t0 + k * 16 + 2 * c + (i & 1) + (i >> 1) * 8;
-            if (t >= w.pre)
-#pragma unroll
-              for (int j = 0; j < VL; ++j) {
-                uint4& y = vr[k][i][j];
-                y = make_uint4(finite_only(y.x, bad), finite_only(y.y, bad), finite_only(y.z, bad),
-                               finite_only(y.w, bad));
-              }
-          }
-        if (bad) s_bad = 1;
-      }
     }
     float mx[NR];
     bool move = false;
@@ -311,12 +310,14 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const float base = m[r] == -INFINITY ? 0.f : m[r];
+        float2 f = make_float2(1.f, 1.f);
+        if (I8) f = make_float2(sc[KB + b * 8 + kc[0]], sc[KB + b * 8 + kc[1]]);
         float y[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float e = tc::ex2(x[b][r][i] - base);
           l[r] += e;
-          y[i] = I8 ? (masked && x[b][r][i] == -INFINITY ? 0.f : e * vs[b][i]) : e;
+          y[i] = I8 ? (masked && x[b][r][i] == -INFINITY ? 0.f : e * (i ? f.y : f.x)) : e;
         }
         uint32_t* dst = &a[b / 2][(b & 1) * 2];
         const uint32_t h1 = pack_bf16(y[0], y[1]);
@@ -335,16 +336,30 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
       for (int j = 0; j < VL; ++j) {
         uint32_t word[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          word[i][0] = vr[k][i][j].x, word[i][1] = vr[k][i][j].y, word[i][2] = vr[k][i][j].z, word[i][3] = vr[k][i][j].w;
+        for (int i = 0; i < 4; ++i) {
+          const int key = k * 16 + kc[i & 1] + (i >> 1) * 8;
+          if (F::EV * (I8 ? 1 : 2) == 8) {
+            const uint2 x2 = *(const uint2*)(stage_v + piece_at<RB>(key, g >> 1) + (g & 1) * 8);
+            word[i][0] = x2.x, word[i][1] = x2.y;
+          } else {
+            const uint4 x4 = *(const uint4*)(stage_v + j * BOX + piece_at<RB>(key, g));
+            word[i][0] = x4.x, word[i][1] = x4.y, word[i][2] = x4.z, word[i][3] = x4.w;
+          }
+          if (!I8 && masked && t0 + key >= w.pre) {
+            bool bad = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) word[i][e] = finite_only(word[i][e], bad);
+            if (bad && t0 + key < w.end) s_bad = 1;
+          }
+        }
 #pragma unroll
         for (int e = 0; e < F::EV; ++e) {
           uint32_t b[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (I8) {
-              const int by = e % 4;
-              b[i] = codes(__byte_perm(word[2 * i][e / 4], word[2 * i + 1][e / 4], by * 0x11 | (by + 4) * 0x1100));
+            if (I8) {  // bytes e of the two keys to bytes 0 and 2
+              const uint32_t y = __byte_perm(word[2 * i][e / 4], word[2 * i + 1][e / 4], e & 2 ? 0x7632 : 0x5410);
+              b[i] = codes(e & 1 ? y >> 8 : y);
             } else {
               b[i] = __byte_perm(word[2 * i][e / 2], word[2 * i + 1][e / 2], e & 1 ? 0x7632 : 0x5410);
             }
@@ -352,8 +367,20 @@ __global__ void __launch_bounds__(kThreads) cache_attn_mma(const Params p) {
           mma16816(o[j * F::EV + e], a[k], b[0], b[1]);
         }
       }
-    load_v(tn);
+    __syncwarp();  // the stage has been read
+    if (t0 + STAGES * STRIDE < hi) fetch(t0 + STAGES * STRIDE, st);
+    copies_commit();
+    if (++st == STAGES) st = 0, phase ^= 1u;
   }
+  copies_wait<0>();
+  if (s_abort && lane == 0 && t0 < hi) {  // the boxes of the steps that were not taken may still be on their way
+    const unsigned long long give_up = tc::now_ns() + tc::kTimeoutNs;
+    for (int i = 0; i < STAGES && t0 < hi; ++i, t0 += STRIDE) {
+      while (!tc::mbar_try_wait(&full[st], phase) && tc::now_ns() < give_up) {}
+      if (++st == STAGES) st = 0, phase ^= 1u;
+    }
+  }
+  __syncthreads();  // every warp has read its last stage: the memory takes the partial outputs
 
   // the warp's parts: row, and columns 2c, 2c + 1 of block (j, e) = value (2c) EV + e of load j
 #pragma unroll
@@ -402,11 +429,18 @@ template <int DP, bool I8, bool Q32>
 cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   using F = MmaCfg<DP, I8, Q32>;
   const Params p = make_params(a, F::RMAX);
-  const int64_t items = a.cache.N * a.cache.H * p.chunks;
+  const KvCacheView& c = a.cache;
+  CUtensorMap mk, mv;
+  if (!tc_make_map_rows(&mk, c.k, I8, c.D, c.T, c.N * c.H, F::RB, F::KB) ||
+      !tc_make_map_rows(&mv, c.v, I8, c.D, c.T, c.N * c.H, F::RB, F::KB))
+    return cudaErrorNotSupported;
+  int* err = tc_error_word();
+  if (!err) return cudaErrorMemoryAllocation;
+  const int64_t items = c.N * c.H * p.chunks;
   // split until the SMs hold their CTAs twice over, or a warp would have one step
   int C = 1;
-  while (C < kMaxCluster && items * C < 3 * sm_count() && a.cache.T / (2 * C) >= kWarps * F::KB) C *= 2;
-  return launch_cluster(cache_attn_mma<DP, I8, Q32>, items * C, C, kThreads, F::SMEM, stream, p);
+  while (C < kMaxCluster && items * C < 3 * sm_count() && c.T / (2 * C) >= kWarps * F::KB) C *= 2;
+  return launch_cluster(cache_attn_mma<DP, I8, Q32>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);
 }
 
 }  // namespace

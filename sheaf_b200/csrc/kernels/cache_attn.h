@@ -45,7 +45,7 @@ template <typename... K, typename... A>
 cudaError_t launch_cluster(void (*kern)(K...), int64_t blocks, int cluster, int threads, size_t smem,
                            cudaStream_t stream, A&&... args) {
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  if (smem > 48 * 1024) {
+  if (smem > 40 * 1024) {  // with the static part it may pass the default 48 KB
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }

@@ -284,7 +284,7 @@ cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
 // (tokens x query heads per cache head) multiply with warp instructions
 // (kernels/cache_attention_mma.cu), more rows with tcgen05
 // (kernels/cache_attention_tc.cu, which reports failed waits through the
-// tensor-core error word, codes 50..62).
+// tensor-core error word, codes 50..64).
 bool cache_attention_mma_takes(const CacheAttnArgs& a);
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream);
 bool cache_attention_tc_takes(const CacheAttnArgs& a);

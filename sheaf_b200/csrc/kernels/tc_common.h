@@ -22,6 +22,11 @@ bool tc_make_map(CUtensorMap* m, const float* base, int rank, const uint64_t* di
 bool tc_make_map_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
                       const uint64_t* strides_bytes, uint32_t box_rows);
 
+// [outer, rows, cols] with `cols` contiguous, of bf16 or bytes: boxes of 64 or
+// 128 bytes by box_rows rows, swizzled over their width.
+bool tc_make_map_rows(CUtensorMap* m, const void* base, bool bytes, uint64_t cols, uint64_t rows, uint64_t outer,
+                      uint32_t box_bytes, uint32_t box_rows);
+
 // Device word that every tcgen05 kernel sets when a bounded wait expires.
 int* tc_error_word();
 

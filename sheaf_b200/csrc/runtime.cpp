@@ -1899,7 +1899,7 @@ sb_status* sb_kv_cache_attention(sb_session* s, const sb_kv_cache* cache, sb_buf
   a.S = S;
   a.Hq = Hq;
   a.scale = scale;
-  if (cache_attention_tc_takes(a)) s->used_tc = true;
+  if (cache_attention_tc_takes(a) || cache_attention_mma_takes(a)) s->used_tc = true;
   cudaError_t e = cache_attention(a, s->dev->stream);
   return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_attention");
 }
