@@ -22,14 +22,16 @@
 //              columns of keys 2c, 2c + 1, 2c + 8, 2c + 9 and pairs them by
 //              byte permutation; the columns' order is undone at the end.
 //
-// f32 queries: a value is the sum of three bf16 parts, exactly.  With at most
-// four rows the parts fill the 16 rows of A (0-3 first, 8-11 second, 4-7 third
-// part), so f32 accuracy costs no more instructions; S is the sum over a
+// f32 queries: a value is the sum of three bf16 (f16) parts, exactly.  With at
+// most four rows the parts fill the 16 rows of A (0-3 first, 8-11 second, 4-7
+// third part), so f32 accuracy costs no more instructions; S is the sum over a
 // lane's two rows and its partner's.  P is split the same way, and the parts'
 // products accumulate apart.
 //
-// int8 codes become bf16 exactly (see codes below); key scales multiply S,
-// value scales P.
+// int8 codes become f16 exactly (see codes below), and Q and P are f16 there
+// too; key scales multiply S, value scales P.
+#include <cuda_fp16.h>
+
 #include "cache_attn.h"
 
 namespace sb {
@@ -37,33 +39,57 @@ namespace {
 
 using namespace cattn;
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr float kLazy = 8.f;  // a row's maximum moves when it would grow by more than this (log2)
 
+// D += A B, 16 x 8 x 16, of bf16 or f16 values.
+template <bool F16>
 __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+// Two f32 rounded to packed bf16 or f16, and what the rounding left of them.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+template <bool F16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (F16) return __half22float2(*(const __half2*)&w);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t take2(float& lo, float& hi) {
+  const uint32_t w = pack2<F16>(lo, hi);
+  const float2 f = unpack2<F16>(w);
+  lo -= f.x;
+  hi -= f.y;
+  return w;
+}
 
-// Two codes, in bytes 0 and 2 of t (bytes 1 and 3: anything), to two bf16
-// values.  A code's low 7 bits and its sign bit, each put under the exponent of
-// 128 (bf16 steps of 1 from 128 to 256), differ by the code:
-// (128 + low) - (128 or 256) = code, exactly.
+// Codes c in bytes 0 and 2 of t (bytes 1 and 3: anything) to two f16 values.
+// 0x6400 + (c + 128) is 1024 + c + 128 as f16 (steps of 1 there): c exactly,
+// after a subtraction.  (bf16 has no steps of 1 beyond 8 bits and would need
+// twice the instructions, which bound the int8 kernel.)
 __device__ __forceinline__ uint32_t codes(uint32_t t) {
-  const uint32_t a = (t & 0x007f007fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
-  __nv_bfloat162 x = __hsub2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+  const uint32_t a = (t & 0x00ff00ffu) ^ 0x64806480u;
+  __half2 x = __hsub2(*(const __half2*)&a, __half2half2(__ushort_as_half(0x6480)));
   return *(uint32_t*)&x;
 }
+// (c + 128) 2^-24, a subnormal f16, in one instruction: for the first product,
+// where sum q (c + 128) - 128 sum q costs one or two of 24 bits.
+__device__ __forceinline__ uint32_t codes_plus_128(uint32_t t) { return (t & 0x00ff00ffu) ^ 0x00800080u; }
 
 // Four bytes to shared memory, asynchronously; zero where `in` is false.
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool in) {
@@ -82,7 +108,7 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w, bool& bad) {
 
 // DP: head size padded to 64 or 128.  Q32: f32 queries, at most 4 rows; else
 // bf16 queries, at most 16.
-template <int DP, bool I8, bool Q32>
+template <int DP, bool I8, bool Q32, int NW>
 struct MmaCfg {
   static constexpr int RMAX = Q32 ? 4 : 16, NR = Q32 ? 1 : 2;  // rows of the CTA, of a lane
   static constexpr int KB = I8 ? 32 : 16;                      // keys per step
@@ -94,8 +120,9 @@ struct MmaCfg {
   static constexpr int BOXES = DP * (I8 ? 1 : 2) / RB, BOX = KB * RB;
   // a warp's stage: K boxes, V boxes; its scales stand behind all stages
   static constexpr int STAGE = 2 * BOXES * BOX, STAGES = 3;
-  static constexpr int SC_OFF = kWarps * STAGES * STAGE, END = SC_OFF + (I8 ? kWarps * STAGES * KB * 8 : 0);
-  static constexpr int JOIN = (kWarps + 1) * RMAX * DP * 4;
+  static constexpr int SC_OFF = NW * STAGES * STAGE, END = SC_OFF + (I8 ? NW * STAGES * KB * 8 : 0);
+  static constexpr int THREADS = NW * 32;
+  static constexpr int JOIN = (NW + 1) * RMAX * DP * 4;
   static constexpr int SMEM = END > JOIN ? END : JOIN;
 };
 
@@ -115,20 +142,21 @@ __device__ __forceinline__ int piece_at(int key, int u) {
   return key * RB + ((RB == 128 ? u ^ (key & 7) : u ^ (key >> 1 & 3)) << 4);
 }
 
-template <int DP, bool I8, bool Q32>
-__global__ void __launch_bounds__(kThreads)
+template <int DP, bool I8, bool Q32, int NW>
+__global__ void __launch_bounds__(NW * 32)
     cache_attn_mma(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const Params p,
                    int* err) {
-  using F = MmaCfg<DP, I8, Q32>;
+  using F = MmaCfg<DP, I8, Q32, NW>;
+  constexpr bool F16 = I8;  // operands: f16 for int8 caches, bf16 for bf16 ones
   constexpr int KB = F::KB, NB = KB / 8, KG = KB / 16, EK = F::EK, KL = F::KL, VL = F::VL, NR = F::NR, RMAX = F::RMAX;
   constexpr int RB = F::RB, BOX = F::BOX, STAGES = F::STAGES;
   pdl_prologue();
   extern __shared__ __align__(1024) float sm[];  // the warps' stages, later their partial outputs
-  __shared__ uint64_t s_full[kWarps][F::STAGES];
+  __shared__ uint64_t s_full[NW][F::STAGES];
   __shared__ volatile int s_abort;
   __shared__ unsigned long long s_mask[kKvMaxTokens];
   __shared__ int s_jump[kKvMaxTokens];
-  __shared__ float s_m[kWarps * RMAX], s_l[kWarps * RMAX], s_ml[2 * RMAX];
+  __shared__ float s_m[NW * RMAX], s_l[NW * RMAX], s_ml[2 * RMAX];
   __shared__ int s_bad;
   const Place w = find_place(p);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -142,7 +170,7 @@ __global__ void __launch_bounds__(kThreads)
   float* const scales = (float*)((uint8_t*)sm + F::SC_OFF) + warp * STAGES * KB * 2;
   uint64_t* const full = s_full[warp];
   if (tid == 0) {
-    for (int i = 0; i < kWarps * STAGES; ++i) tc::mbar_init(&s_full[0][i], 1);
+    for (int i = 0; i < NW * STAGES; ++i) tc::mbar_init(&s_full[0][i], 1);
     s_bad = 0;
     s_abort = tc::smem_u32(sm) & 1023u ? 1 : 0;
     if (s_abort) atomicExch(err, 63);
@@ -170,7 +198,7 @@ __global__ void __launch_bounds__(kThreads)
     }
   };
   int64_t t0 = lo + warp * KB;
-  constexpr int STRIDE = kWarps * KB;
+  constexpr int STRIDE = NW * KB;
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) {
     if (t0 + i * STRIDE < hi) fetch(t0 + i * STRIDE, i);
@@ -178,34 +206,75 @@ __global__ void __launch_bounds__(kThreads)
   }
   if (warp == 0) tree_masks(p.parents ? p.parents + w.n * p.S : nullptr, p.S, lane, s_mask, s_jump);
 
-  // Q: k-step s takes values d .. d + 3 of the lane's EK
+  // Q: k-step s takes values d .. d + 3 of the lane's EK, as the pairs of an
+  // int8 word (bytes 0 and 2, bytes 1 and 3) or of consecutive bf16 values.
+  // For f16 a row is scaled by a power of two to a largest value in [2^14,
+  // 2^15), which keeps what is 2^-38 of it; S is multiplied back by `fs`.
   uint32_t q[DP / 16][4];
+  float fs[NR], sum_q[NR];
 #pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const int d = (s / (EK / 4)) * 4 * EK + c * EK + (s % (EK / 4)) * 4;
-    if (Q32) {
-      const int row = g & 3;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < rows && d < p.D) x = *(const float4*)((const float*)p.q + row_at(p, w, r0 + row) + d);
-      // the pairs of an int8 word: bytes 0 and 2, bytes 1 and 3
-      const float y[4] = {x.x * p.scale2, (I8 ? x.z : x.y) * p.scale2, (I8 ? x.y : x.z) * p.scale2, x.w * p.scale2};
+  for (int r = 0; r < NR; ++r) {
+    const int row = Q32 ? g & 3 : g + 8 * r;
+    const bool in = row < rows;
+    const int64_t at = in ? row_at(p, w, r0 + row) : 0;
+    float y[DP / 16][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t a = pack_bf16(y[2 * i], y[2 * i + 1]);
-        const float e0 = y[2 * i] - bf_lo(a), e1 = y[2 * i + 1] - bf_hi(a);
-        const uint32_t b = pack_bf16(e0, e1), l3 = pack_bf16(e0 - bf_lo(b), e1 - bf_hi(b));
-        q[s][2 * i] = g < 4 ? a : l3;
-        q[s][2 * i + 1] = g < 4 ? b : 0u;
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = (s / (EK / 4)) * 4 * EK + c * EK + (s % (EK / 4)) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[s][i] = 0.f;
+      if (in && d < p.D) {
+        if (Q32) {
+          *(float4*)y[s] = *(const float4*)((const float*)p.q + at + d);
+        } else {
+          const uint2 x = *(const uint2*)((const __nv_bfloat16*)p.q + at + d);
+          const float2 a = unpack2<false>(x.x), b = unpack2<false>(x.y);
+          y[s][0] = a.x, y[s][1] = a.y, y[s][2] = b.x, y[s][3] = b.y;
+        }
       }
-    } else {
+    }
+    float up = 1.f;
+    fs[r] = p.scale2;
+    sum_q[r] = 0.f;
+    if (F16) {
+      float big = 0.f;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int row = g + 8 * r;
-        uint2 x = make_uint2(0, 0);
-        if (row < rows && d < p.D) x = *(const uint2*)((const __nv_bfloat16*)p.q + row_at(p, w, r0 + row) + d);
-        q[s][r] = I8 ? __byte_perm(x.x, x.y, 0x5410) : x.x;  // see above
-        q[s][2 + r] = I8 ? __byte_perm(x.x, x.y, 0x7632) : x.y;
+      for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(y[s][i]));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // 2^(14 - e) for a largest value of exponent e, within f32's normal range
+      const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
+      up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+      fs[r] = p.scale2 * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      float2 a = make_float2(y[s][0] * up, y[s][I8 ? 2 : 1] * up), b = make_float2(y[s][I8 ? 1 : 2] * up, y[s][3] * up);
+      if (Q32) {
+        const uint32_t a1 = take2<F16>(a.x, a.y), b1 = take2<F16>(b.x, b.y);
+        const uint32_t a2 = take2<F16>(a.x, a.y), b2 = take2<F16>(b.x, b.y);
+        const uint32_t a3 = pack2<F16>(a.x, a.y), b3 = pack2<F16>(b.x, b.y);
+        q[s][0] = g < 4 ? a1 : a3;
+        q[s][1] = g < 4 ? a2 : 0u;
+        q[s][2] = g < 4 ? b1 : b3;
+        q[s][3] = g < 4 ? b2 : 0u;
+      } else {
+        q[s][r] = pack2<F16>(a.x, a.y);
+        q[s][2 + r] = pack2<F16>(b.x, b.y);
+        if (F16) {
+          const float2 a1 = unpack2<F16>(q[s][r]), b1 = unpack2<F16>(q[s][2 + r]);
+          sum_q[r] += (a1.x + a1.y) + (b1.x + b1.y);
+        }
       }
+    }
+    if (F16 && !Q32) {
+      sum_q[r] += __shfl_xor_sync(0xffffffffu, sum_q[r], 1);
+      sum_q[r] += __shfl_xor_sync(0xffffffffu, sum_q[r], 2);
+      // acc = 2^-24 sum q (c + 128):  S = acc 2^24 fs - 128 fs sum q
+      sum_q[r] *= 128.f * fs[r];
+      fs[r] *= 16777216.f;
     }
   }
   __syncthreads();
@@ -220,8 +289,9 @@ __global__ void __launch_bounds__(kThreads)
   for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.f;
 
   const int kg = key_of<RB>(g), kc[2] = {key_of<RB>(2 * c), key_of<RB>(2 * c + 1)};
-  int st = 0;
+  int st = 0, vref = -100;
   uint32_t phase = 0;
+  float vdown = 0.f;
   for (; t0 < hi; t0 += STRIDE) {
     copies_wait<STAGES - 1>();
     if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[st], phase, &s_abort, err, 64))) break;
@@ -242,8 +312,9 @@ __global__ void __launch_bounds__(kThreads)
         for (int b = 0; b < NB; ++b) {
           const uint32_t word[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
           const uint32_t* a = q[i * (EK / 4) + k];
-          if (I8) mma16816(s[b], a, codes(word[k]), codes(word[k] >> 8));
-          else mma16816(s[b], a, word[(k % 2) * 2], word[(k % 2) * 2 + 1]);
+          if (I8 && Q32) mma16816<F16>(s[b], a, codes(word[k]), codes(word[k] >> 8));
+          else if (I8) mma16816<F16>(s[b], a, codes_plus_128(word[k]), codes_plus_128(word[k] >> 8));
+          else mma16816<F16>(s[b], a, word[(k % 2) * 2], word[(k % 2) * 2 + 1]);
         }
     }
     // scores of the lane's NR rows and two keys per block, in units of log2
@@ -256,10 +327,11 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = 0; i < 2; ++i) {
         if (Q32) {
           const float y = s[b][i] + s[b][2 + i];
-          x[b][0][i] = y + __shfl_xor_sync(0xffffffffu, y, 16);
+          x[b][0][i] = (y + __shfl_xor_sync(0xffffffffu, y, 16)) * fs[0];
         } else {
 #pragma unroll
-          for (int r = 0; r < NR; ++r) x[b][r][i] = s[b][2 * r + i] * p.scale2;
+          for (int r = 0; r < NR; ++r)
+            x[b][r][i] = I8 ? fmaf(s[b][2 * r + i], fs[r], -sum_q[r]) : s[b][2 * r + i] * fs[r];
         }
         if (I8)
 #pragma unroll
@@ -304,6 +376,22 @@ __global__ void __launch_bounds__(kThreads)
         }
       }
     }
+    if (I8) {
+      // P times the value scales goes into f16 relative to 2^vref, above the
+      // largest scale so far: at most 2^(8 + 6), with steps of 2^-30 below 1
+      const float mine = fabsf(sc[KB + lane]);
+      const int e = mine < INFINITY ? (int)(__float_as_uint(mine) >> 23) - 126 : -125;
+      const int top = max(__reduce_max_sync(0xffffffffu, e), -100);
+      if (top > vref) {
+        const float f = tc::ex2((float)(vref - top));
+#pragma unroll
+        for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[j][i] *= f;
+        vref = top;
+        vdown = __uint_as_float((uint32_t)(127 + 6 - vref) << 23);
+      }
+    }
     uint32_t a[KG][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -311,7 +399,7 @@ __global__ void __launch_bounds__(kThreads)
       for (int r = 0; r < NR; ++r) {
         const float base = m[r] == -INFINITY ? 0.f : m[r];
         float2 f = make_float2(1.f, 1.f);
-        if (I8) f = make_float2(sc[KB + b * 8 + kc[0]], sc[KB + b * 8 + kc[1]]);
+        if (I8) f = make_float2(sc[KB + b * 8 + kc[0]] * vdown, sc[KB + b * 8 + kc[1]] * vdown);
         float y[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -320,14 +408,12 @@ __global__ void __launch_bounds__(kThreads)
           y[i] = I8 ? (masked && x[b][r][i] == -INFINITY ? 0.f : e * (i ? f.y : f.x)) : e;
         }
         uint32_t* dst = &a[b / 2][(b & 1) * 2];
-        const uint32_t h1 = pack_bf16(y[0], y[1]);
         if (Q32) {
-          const float e0 = y[0] - bf_lo(h1), e1 = y[1] - bf_hi(h1);
-          const uint32_t h2 = pack_bf16(e0, e1), h3 = pack_bf16(e0 - bf_lo(h2), e1 - bf_hi(h2));
+          const uint32_t h1 = take2<F16>(y[0], y[1]), h2 = take2<F16>(y[0], y[1]), h3 = pack2<F16>(y[0], y[1]);
           dst[0] = g < 4 ? h1 : h3;
           dst[1] = g < 4 ? h2 : 0u;
         } else {
-          dst[r] = h1;
+          dst[r] = pack2<F16>(y[0], y[1]);
         }
       }
 #pragma unroll
@@ -364,7 +450,7 @@ __global__ void __launch_bounds__(kThreads)
               b[i] = __byte_perm(word[2 * i][e / 2], word[2 * i + 1][e / 2], e & 1 ? 0x7632 : 0x5410);
             }
           }
-          mma16816(o[j * F::EV + e], a[k], b[0], b[1]);
+          mma16816<F16>(o[j * F::EV + e], a[k], b[0], b[1]);
         }
       }
     __syncwarp();  // the stage has been read
@@ -383,6 +469,7 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();  // every warp has read its last stage: the memory takes the partial outputs
 
   // the warp's parts: row, and columns 2c, 2c + 1 of block (j, e) = value (2c) EV + e of load j
+  const float vup = __uint_as_float((uint32_t)(127 - 6 + vref) << 23);
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -398,6 +485,7 @@ __global__ void __launch_bounds__(kThreads)
           y += o[j][2 + i];
           y += __shfl_xor_sync(0xffffffffu, y, 16);
         }
+        if (I8) y *= vup;
         const int d = (j / F::EV) * 8 * F::EV + (2 * c + i) * F::EV + j % F::EV;
         if (!Q32 || g < 4) sm[(warp * RMAX + row) * DP + d] = y;
       }
@@ -413,8 +501,8 @@ __global__ void __launch_bounds__(kThreads)
       bad |= y;
     }
   }
-  join_and_store<kWarps, RMAX, DP>(
-      p, w, r0, rows, sm, s_m, s_l, sm + kWarps * RMAX * DP, s_ml, s_mask, [&](unsigned long long see, int d, float* y) {
+  join_and_store<NW, RMAX, DP>(
+      p, w, r0, rows, sm, s_m, s_l, sm + NW * RMAX * DP, s_ml, s_mask, [&](unsigned long long see, int d, float* y) {
         if (!bad) return;
         for (int j = 0; j < p.S; ++j)
           if (see >> j & 1ull)
@@ -425,9 +513,9 @@ __global__ void __launch_bounds__(kThreads)
       });
 }
 
-template <int DP, bool I8, bool Q32>
-cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
-  using F = MmaCfg<DP, I8, Q32>;
+template <int DP, bool I8, bool Q32, int NW>
+cudaError_t launch(const CacheAttnArgs& a, int C, cudaStream_t stream) {
+  using F = MmaCfg<DP, I8, Q32, NW>;
   const Params p = make_params(a, F::RMAX);
   const KvCacheView& c = a.cache;
   CUtensorMap mk, mv;
@@ -436,11 +524,21 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
     return cudaErrorNotSupported;
   int* err = tc_error_word();
   if (!err) return cudaErrorMemoryAllocation;
-  const int64_t items = c.N * c.H * p.chunks;
-  // split until the SMs hold their CTAs twice over, or a warp would have one step
+  return launch_cluster(cache_attn_mma<DP, I8, Q32, NW>, c.N * c.H * p.chunks * C, C, F::THREADS, F::SMEM, stream, mk,
+                        mv, p, err);
+}
+
+template <int DP, bool I8, bool Q32>
+cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
+  const int64_t rmax = Q32 ? 4 : 16, rows = a.S * (a.Hq / a.cache.H);
+  const int64_t items = a.cache.N * a.cache.H * ((rows + rmax - 1) / rmax);
+  // Many items: CTAs of two warps, of which an SM holds enough for one wave.
+  // Few: four warps, split until the SMs hold their CTAs or a warp would have
+  // one step.
+  if (items >= 3 * sm_count()) return launch<DP, I8, Q32, 2>(a, 1, stream);
   int C = 1;
-  while (C < kMaxCluster && items * C < 3 * sm_count() && c.T / (2 * C) >= kWarps * F::KB) C *= 2;
-  return launch_cluster(cache_attn_mma<DP, I8, Q32>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);
+  while (C < kMaxCluster && items * C < 3 * sm_count() && a.cache.T / (2 * C) >= 4 * (I8 ? 32 : 16)) C *= 2;
+  return launch<DP, I8, Q32, 4>(a, C, stream);
 }
 
 }  // namespace
@@ -453,11 +551,11 @@ bool cache_attention_mma_takes(const CacheAttnArgs& a) {
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream) {
   const bool i8 = a.cache.type == KvType::I8;
   if (a.cache.D <= 64) {
-    if (a.bf16) return i8 ? launch<64, true, false>(a, stream) : launch<64, false, false>(a, stream);
-    return i8 ? launch<64, true, true>(a, stream) : launch<64, false, true>(a, stream);
+    if (a.bf16) return i8 ? by_items<64, true, false>(a, stream) : by_items<64, false, false>(a, stream);
+    return i8 ? by_items<64, true, true>(a, stream) : by_items<64, false, true>(a, stream);
   }
-  if (a.bf16) return i8 ? launch<128, true, false>(a, stream) : launch<128, false, false>(a, stream);
-  return i8 ? launch<128, true, true>(a, stream) : launch<128, false, true>(a, stream);
+  if (a.bf16) return i8 ? by_items<128, true, false>(a, stream) : by_items<128, false, false>(a, stream);
+  return i8 ? by_items<128, true, true>(a, stream) : by_items<128, false, true>(a, stream);
 }
 
 }  // namespace sb
