@@ -221,7 +221,8 @@ SB_API sb_status* sb_optimizer_adamw_step(sb_session* session, size_t leaf_count
  * the session stream (sb_beam_reorder: one per 48 states), returns once it is
  * enqueued, allocates nothing and uses no workspace, so a call may be captured
  * into a CUDA graph of the session stream.  Results do not depend on timing.
- * Buffers are row-major, of this session or wrapped memory of its device.
+ * Buffers are row-major, of this session or wrapped memory of its device;
+ * wrapped f32 caches, keys and values are 32-byte aligned.
  * Index buffers are i32; their values are read on the device and values out of
  * range have the meaning stated, never a fault.  Unless stated otherwise a
  * written buffer must not overlap another argument. */
@@ -268,8 +269,9 @@ SB_API sb_status* sb_kv_cache_attention(sb_session* session, const sb_kv_cache* 
 
 /* Beam search: of the beams x vocabulary continuations of each group, with
  *   value(w, v) = scores[w] + (logits[w, v] - log sum_u exp logits[w, u])
- * in f64, the `beams` largest in descending order: out_scores (f32),
- * out_parents (w) and out_tokens (v), all [groups, beams], beams <= 16.
+ * the `beams` largest in descending order: out_scores (f32), out_parents (w)
+ * and out_tokens (v), all [groups, beams], beams <= 16.  The order is that of
+ * f64 sums; the scores are within 4e-6 of them before their own rounding.
  * logits [groups * beams, vocabulary], f32 or bf16.  Within a beam the logits
  * order the candidates, the lower token first among equals; between beams of
  * equal value the lower beam comes first.  A NaN logit counts as -inf; a beam

@@ -10,16 +10,18 @@
 // group; each warp streams pieces of one beam's row and keeps in its lanes the
 // W best of what it has seen as 64-bit keys (order-preserving image of the
 // logit above the complemented index: unique, so equal logits order by index
-// and every step has one answer).  A piece is filtered by the larger of the
-// list's last key and the W-th best of the 32 lanes' own best keys, which
-// leaves little more than W values to insert.  After a cluster barrier CTA r
-// joins the lists of beams r, r + C, ..; after a second one CTA 0 orders the
-// W x W survivors.  Lists cross CTAs through distributed shared memory, so
-// there is no workspace, no atomic and no second launch.
+// and every step has one answer).  Few values of a piece pass the list's last
+// key; where many do (the first piece) they are first filtered by the W-th best
+// of the 32 lanes' own best keys.  After a cluster barrier CTA r joins the lists
+// of beams r, r + C, .. and sends them to every CTA; after a second one each CTA
+// orders the W x W survivors.  Lists cross CTAs through distributed shared
+// memory, so there is no workspace, no atomic and no second launch.
 //
-// Within a beam the order is the logits' own.  Between beams it needs lse: the
-// sums run in f64, since an f32 sum is off by about 1e-7 of a candidate's
-// value and would decide near ties by its rounding.
+// Within a beam the order is the logits' own.  Between beams it needs lse.  The
+// first round sums f32 exponentials, off by less than kFastError; if two
+// neighbours of the result from different beams are closer than twice that (or
+// tie), the group's sums are taken again in f64, whose exponentials would
+// otherwise bound the kernel.  So the order is that of f64 sums in every case.
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -32,10 +34,18 @@ namespace sb {
 namespace {
 
 constexpr int kSelWarps = 16, kSelThreads = kSelWarps * 32;
+// Bound on the error of an lse from f32 exponentials of V <= 2^31 values.  A
+// term 2^-t has a relative error of at most 2^-22 (ex2) + 2^-23.4 t (its
+// argument, two roundings), and terms with t > 32 + log2 of the sum of the
+// others' number are below it; the mean t of the sum's weight is at most
+// log2(V) < 32; 32 terms are added in a tree of depth 5 in f32, the rest in f64:
+// 2^-22 + 32 * 2^-23.4 + 5 * 2^-24 < 4e-6.
+constexpr double kFastError = 4e-6;
 constexpr int EPC = 32;              // values per lane and piece
 constexpr int kPiece = EPC * 32;     // values per warp and piece
 constexpr int W_MAX = (int)kBeamMax;
 using u64 = unsigned long long;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct SelectParams {
   const void* logits;
@@ -65,68 +75,77 @@ __device__ __forceinline__ void insert(u64& list, u64 key, int lane, int W) {
   if (lane < W && lane >= rank) list = lane == rank ? key : up;
 }
 
-// Values i .. i + 3 (f32) or i .. i + 7 (bf16) of the row that starts at
-// element `base` of the buffer, as a 16-byte load: `at` is the element of the
-// buffer that the load starts at (a multiple of the load's width).  Elements
-// outside the row are -inf.  The buffer's last elements are loaded one by one
-// where the 16 bytes would pass its end.
+// The N = 4 (f32) or 8 (bf16) values of a 16-byte load.
 template <bool BF>
-__device__ __forceinline__ void load_piece(const void* buf, int64_t at, int64_t base, int64_t V, int64_t total, float* x) {
-  constexpr int N = BF ? 8 : 4;
+__device__ __forceinline__ void load_vec(const void* buf, int64_t at, float* x) {
+  const uint4 r = *(const uint4*)((const uint8_t*)buf + at * (BF ? 2 : 4));
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = -INFINITY;
-  if (at >= base + V) return;
-  if (at + N <= total) {
-    const uint4 r = *(const uint4*)((const uint8_t*)buf + at * (BF ? 2 : 4));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (BF) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        x[i] = __uint_as_float(w[i]);
-      }
+  for (int i = 0; i < 4; ++i) {
+    if (BF) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      x[i] = __uint_as_float(w[i]);
     }
-  } else {
-    for (int i = 0; i < N; ++i)
-      if (at + i < total)
-        x[i] = BF ? __bfloat162float(((const __nv_bfloat16*)buf)[at + i]) : ((const float*)buf)[at + i];
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (at + i < base || at + i >= base + V || x[i] != x[i]) x[i] = -INFINITY;  // NaN counts as -inf
 }
 
-// Sum of exp(x - m) kept with the maximum it refers to.
-__device__ __forceinline__ void join(double& m, double& s, double m2, double s2) {
-  const double mx = fmax(m, m2);
-  if (mx == -INFINITY) return;
-  s = s * exp(m - mx) + s2 * exp(m2 - mx);
-  m = mx;
+// Values at .. at + N - 1 of the logits buffer (at: a multiple of N) where they
+// belong to the row [base, base + V), -inf elsewhere and for NaN.  `inside`: all
+// of them do.  The buffer's last values are loaded one by one where the 16
+// bytes would pass its end.
+template <bool BF>
+__device__ __forceinline__ void load_piece(const void* buf, bool inside, int64_t at, int64_t base, int64_t V,
+                                           int64_t total, float* x) {
+  constexpr int N = BF ? 8 : 4;
+  if (inside) {
+    load_vec<BF>(buf, at, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = -INFINITY;
+    if (at < base + V && at + N <= total) {
+      load_vec<BF>(buf, at, x);
+    } else if (at < base + V) {
+      for (int i = 0; i < N; ++i)
+        if (at + i < total)
+          x[i] = BF ? __bfloat162float(((const __nv_bfloat16*)buf)[at + i]) : ((const float*)buf)[at + i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (at + i < base || at + i >= base + V) x[i] = -INFINITY;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = fmaxf(x[i], -INFINITY);  // the number of the two
 }
 
 struct SelectShared {
   u64 list[kSelWarps][W_MAX];
-  double m[kSelWarps], s[kSelWarps];
-  // rank 0: the candidates of every beam
+  double s[kSelWarps];
+  float m[kSelWarps];
+  // the candidates of every beam, best first (each CTA has them all)
   double cand[W_MAX][W_MAX];
   int token[W_MAX][W_MAX];
   int done[W_MAX];
+  double best[W_MAX + 1];  // the first W + 1 of them, and their beams
+  int beam[W_MAX + 1], pick[W_MAX];
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t remote(const T* p, uint32_t rank) { return tc::cluster_addr(p, rank); }
-__device__ __forceinline__ u64 ld_remote64(uint32_t a) {
+__device__ __forceinline__ u64 ld_remote64(const void* p, uint32_t rank) {
   u64 x;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(a));
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(tc::cluster_addr(p, rank)));
   return x;
 }
-__device__ __forceinline__ void st_remote64(uint32_t a, u64 x) {
-  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(x) : "memory");
+__device__ __forceinline__ float ld_remote_f(const float* p, uint32_t rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(tc::cluster_addr(p, rank)));
+  return x;
 }
-__device__ __forceinline__ void st_remote32(uint32_t a, uint32_t x) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
+__device__ __forceinline__ void st_remote64(const void* p, uint32_t rank, u64 x) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(tc::cluster_addr(p, rank)), "l"(x) : "memory");
+}
+__device__ __forceinline__ void st_remote32(const void* p, uint32_t rank, uint32_t x) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(p, rank)), "r"(x) : "memory");
 }
 
 template <bool BF>
@@ -143,121 +162,206 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
   // warps of the cluster per beam; warp `gid` streams every `per`-th piece of its beam
   const int warps = (int)C * kSelWarps, per = warps / W;
   const int gid = (int)crank * kSelWarps + warp, beam = gid / per, sub = gid % per;
+  const bool mine = beam < W && !(p.eos >= 0 && p.finished[g * W + beam]);
+  const int64_t base = (g * W + (mine ? beam : 0)) * p.V;
+  const int64_t first = base - base % N;  // 16-byte boundary at or before the row
+  const int64_t pieces = (base + p.V - first + kPiece - 1) / kPiece;
   u64 list = 0;
-  double m = -INFINITY, sum = 0.;
-  const bool over = p.eos >= 0 && beam < W && p.finished[g * W + beam];
-  if (beam < W && !over) {
-    const int64_t base = (g * W + beam) * p.V;
-    const int64_t first = base - base % N;  // 16-byte boundary at or before the row
-    const int64_t pieces = (base + p.V - first + kPiece - 1) / kPiece;
-    for (int64_t c = sub; c < pieces; c += per) {
-      const int64_t at0 = first + c * kPiece + lane * N;
-      float x[EPC];
+  float m = -INFINITY;
+
+  for (int round = 0;; ++round) {
+    double sum = 0.;
+    if (mine && round == 0) {
+      for (int64_t c = sub; c < pieces; c += per) {
+        const int64_t at0 = first + c * kPiece + lane * N;
+        const bool inside = first + c * kPiece >= base && first + (c + 1) * kPiece <= base + p.V;
+        float x[EPC];
 #pragma unroll
-      for (int i = 0; i < EPC / N; ++i) load_piece<BF>(p.logits, at0 + i * 32 * N, base, p.V, p.total, x + i * N);
-      float mx = x[0];
+        for (int i = 0; i < EPC / N; ++i)
+          load_piece<BF>(p.logits, inside, at0 + i * 32 * N, base, p.V, p.total, x + i * N);
+        float mx = x[0];
 #pragma unroll
-      for (int i = 1; i < EPC; ++i) mx = fmaxf(mx, x[i]);
-      // lane's best key: its largest value at the lowest index
-      int64_t bi = 0;
+        for (int i = 1; i < EPC; ++i) mx = fmaxf(mx, x[i]);
+        float wm = mx;
 #pragma unroll
-      for (int i = EPC - 1; i >= 0; --i)
-        if (x[i] == mx) bi = at0 + (i / N) * 32 * N + i % N - base;
-      const bool none = bi < 0 || bi >= p.V;
-      const u64 best = none ? 0 : (u64)ordered(mx) << 32 | (uint32_t)~(uint32_t)bi;
-      float wm = mx;
+        for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+        const float mn = fmaxf(m, wm);
+        if (mn != -INFINITY) {
+          if (mn > m) sum *= (double)exp2f((m - mn) * kLog2e);
+          m = mn;
+          float e[EPC];
 #pragma unroll
-      for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-      double acc = 0.;
-      if (wm != -INFINITY) {
-#pragma unroll 4
-        for (int i = 0; i < EPC; ++i) acc += exp((double)x[i] - (double)wm);
+          for (int i = 0; i < EPC; ++i) e[i] = tc::ex2((x[i] - m) * kLog2e);
+#pragma unroll
+          for (int w = EPC / 2; w; w >>= 1)
+#pragma unroll
+            for (int i = 0; i < w; ++i) e[i] += e[i + w];
+          sum += (double)e[0];  // per lane
+        }
+        // values that pass the list's last key; -inf passes too while the list is not full
+        u64 bar = shfl64(list, W - 1);
+        const float barf = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+        if (!__any_sync(0xffffffffu, mx >= barf)) continue;
+        int hits = 0;
+#pragma unroll
+        for (int i = 0; i < EPC; ++i) hits += x[i] >= barf;
+        if (__reduce_add_sync(0xffffffffu, hits) > 2 * W) {
+          int64_t bi = -1;  // the lane's best key: its largest value at the lowest index
+#pragma unroll
+          for (int i = EPC - 1; i >= 0; --i)
+            if (x[i] == mx) bi = at0 + (i / N) * 32 * N + i % N - base;
+          const u64 best = bi < 0 || bi >= p.V ? 0 : (u64)ordered(mx) << 32 | (uint32_t)~(uint32_t)bi;
+          int ahead = 0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ahead += shfl64(best, i) > best;
+          const uint32_t at = __ballot_sync(0xffffffffu, ahead == W - 1);
+          if (at) {
+            const u64 b2 = shfl64(best, __ffs(at) - 1);
+            if (b2 > bar) bar = b2 - 1;  // itself passes
+          }
+        }
+        const float pass = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < EPC; ++i) {
+          if (!__any_sync(0xffffffffu, x[i] >= pass)) continue;
+          const int64_t idx = at0 + (i / N) * 32 * N + i % N - base;
+          const u64 key = idx < 0 || idx >= p.V ? 0 : (u64)ordered(x[i]) << 32 | (uint32_t)~(uint32_t)idx;
+          uint32_t hit = __ballot_sync(0xffffffffu, key > bar);
+          while (hit) {
+            const int src = __ffs(hit) - 1;
+            hit &= hit - 1;
+            insert(list, shfl64(key, src), lane, W);
+          }
+        }
       }
+      if (lane < W_MAX) sh.list[warp][lane] = lane < W ? list : 0;
+    } else if (mine) {  // again, in f64; m is the warp's maximum
+      for (int64_t c = sub; c < pieces; c += per) {
+        const int64_t at0 = first + c * kPiece + lane * N;
+#pragma unroll 1
+        for (int i = 0; i < EPC / N; ++i) {
+          float x[N];
+          load_piece<BF>(p.logits, false, at0 + i * 32 * N, base, p.V, p.total, x);
+          if (m != -INFINITY)
 #pragma unroll
-      for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-      join(m, sum, (double)wm, acc);
-      // the W-th best of the lanes' best keys
-      int ahead = 0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) ahead += shfl64(best, i) > best;
-      const uint32_t at = __ballot_sync(0xffffffffu, ahead == W - 1);
-      u64 bar = shfl64(list, W - 1);
-      if (at) {
-        const u64 b2 = shfl64(best, __ffs(at) - 1);
-        if (b2 > bar) bar = b2 - 1;  // itself passes
+            for (int k = 0; k < N; ++k) sum += exp((double)x[k] - (double)m);
+        }
       }
+    } else if (round == 0 && lane < W_MAX) {
+      sh.list[warp][lane] = 0;
+    }
 #pragma unroll
-      for (int i = 0; i < EPC; ++i) {
-        const int64_t idx = at0 + (i / N) * 32 * N + i % N - base;
-        const u64 key = idx < 0 || idx >= p.V ? 0 : (u64)ordered(x[i]) << 32 | (uint32_t)~(uint32_t)idx;
-        uint32_t hit = __ballot_sync(0xffffffffu, key > bar);
-        while (hit) {
-          const int src = __ffs(hit) - 1;
-          hit &= hit - 1;
-          insert(list, shfl64(key, src), lane, W);
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sh.m[warp] = m, sh.s[warp] = sum;
+    tc::cluster_sync();
+
+    // CTA r joins beams r, r + C, ..: one warp each
+    for (int b = (int)crank + (int)C * warp; b < W; b += (int)C * kSelWarps) {
+      u64 best = 0;
+      float pm = -INFINITY;  // lane k (and k + 32, ..): the parts of the sum
+      double ps = 0.;
+      for (int k0 = 0; k0 < per; k0 += 8) {
+        u64 part[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int id = b * per + k0 + k;
+          part[k] = k0 + k < per && lane < W ? ld_remote64(&sh.list[id % kSelWarps][lane], id / kSelWarps) : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (k0 + k == 0) {
+            best = part[k];
+            continue;
+          }
+          for (int j = 0; j < W; ++j) {  // sorted: stop at the first that does not get in
+            const u64 key = shfl64(part[k], j);
+            if (key <= shfl64(best, W - 1)) break;
+            insert(best, key, lane, W);
+          }
+        }
+      }
+      for (int k = lane; k < per; k += 32) {
+        const int id = b * per + k;
+        const float m2 = ld_remote_f(&sh.m[id % kSelWarps], id / kSelWarps);
+        const double s2 = __longlong_as_double((long long)ld_remote64(&sh.s[id % kSelWarps], id / kSelWarps));
+        const float mx = fmaxf(pm, m2);
+        if (mx != -INFINITY) {
+          ps = ps * exp((double)pm - (double)mx) + s2 * exp((double)m2 - (double)mx);
+          pm = mx;
+        }
+      }
+      float top = pm;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      ps = pm == -INFINITY ? 0. : ps * exp((double)pm - (double)top);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
+      const float score = p.scores[g * W + b];
+      const bool fin = p.eos >= 0 && p.finished[g * W + b];
+      const double lse = (double)top + log(ps);
+      const int have = (int)min((int64_t)W, p.V);
+      double value = -INFINITY;
+      int token = lane;
+      if (isfinite(score) && fin) {
+        // the end token alone, then the others from the lowest
+        value = lane == 0 ? (double)score : -INFINITY;
+        token = lane == 0 ? p.eos : lane - 1 + (lane - 1 >= p.eos);
+      } else if (isfinite(score) && isfinite(lse)) {
+        token = (int)~(uint32_t)best;
+        value = (double)score + ((double)unordered((uint32_t)(best >> 32)) - lse);
+      }
+      if (lane < W) {
+        if (lane >= have) value = -INFINITY, token = -1;  // no such candidate
+        for (uint32_t c = 0; c < C; ++c) {
+          st_remote64(&sh.cand[b][lane], c, (u64)__double_as_longlong(value));
+          st_remote32(&sh.token[b][lane], c, (uint32_t)token);
+          if (lane == 0) st_remote32(&sh.done[b], c, fin ? 1u : 0u);
         }
       }
     }
-  }
-  if (lane < W_MAX) sh.list[warp][lane] = lane < W ? list : 0;
-  if (lane == 0) sh.m[warp] = m, sh.s[warp] = sum;
-  tc::cluster_sync();
-
-  // CTA r joins beams r, r + C, ..: one warp each
-  for (int b = (int)crank + (int)C * warp; b < W; b += (int)C * kSelWarps) {
-    u64 best = 0;
-    double bm = -INFINITY, bs = 0.;
-    for (int k = 0; k < per; ++k) {
-      const int id = b * per + k, r = id / kSelWarps, w = id % kSelWarps;
-      const u64 mine = lane < W ? ld_remote64(remote(&sh.list[w][lane], r)) : 0;
-      for (int j = 0; j < W; ++j) {  // sorted: stop at the first that does not get in
-        const u64 key = shfl64(mine, j);
-        if (key <= shfl64(best, W - 1)) break;
-        insert(best, key, lane, W);
+    if (tid <= W) sh.beam[tid] = -1;
+    tc::cluster_sync();
+    // rank of each survivor: its place in its own list, and in every other by
+    // bisection (among equals the lower beam comes first)
+    for (int i = tid; i < W * W; i += kSelThreads) {
+      const int b = i / W, j = i % W, tok = sh.token[b][j];
+      if (tok < 0) continue;
+      const double v = sh.cand[b][j];
+      int rank = j;
+      for (int b2 = 0; b2 < W; ++b2) {
+        if (b2 == b) continue;
+        int n = 0;
+#pragma unroll
+        for (int step = W_MAX; step; step >>= 1)
+          if (n + step <= W && sh.token[b2][n + step - 1] >= 0 &&
+              (sh.cand[b2][n + step - 1] > v || (sh.cand[b2][n + step - 1] == v && b2 < b)))
+            n += step;
+        rank += n;
       }
-      join(bm, bs, __longlong_as_double((long long)ld_remote64(remote(&sh.m[w], r))),
-           __longlong_as_double((long long)ld_remote64(remote(&sh.s[w], r))));
+      if (rank <= W) sh.best[rank] = v, sh.beam[rank] = b;
+      if (rank < W) sh.pick[rank] = tok;
     }
-    const float score = p.scores[g * W + b];
-    const bool fin = p.eos >= 0 && p.finished[g * W + b];
-    const double lse = bm + log(bs);
-    const int have = (int)min((int64_t)W, p.V);
-    double value = -INFINITY;
-    int token = lane;
-    if (isfinite(score) && fin) {
-      // the end token alone, then the others from the lowest
-      value = lane == 0 ? (double)score : -INFINITY;
-      token = lane == 0 ? p.eos : lane - 1 + (lane - 1 >= p.eos);
-    } else if (isfinite(score) && isfinite(lse)) {
-      token = (int)~(uint32_t)best;
-      value = (double)score + ((double)unordered((uint32_t)(best >> 32)) - lse);
+    __syncthreads();
+    bool close = false;
+    if (round == 0 && tid < W) {
+      const int b1 = sh.beam[tid], b2 = sh.beam[tid + 1];
+      // finished beams' candidates and -inf are exact
+      close = b1 >= 0 && b2 >= 0 && b1 != b2 && sh.best[tid + 1] != -INFINITY &&
+              sh.best[tid] - sh.best[tid + 1] < 2 * kFastError + 1e-15 * fabs(sh.best[tid]);
     }
-    if (lane < W) {
-      if (lane >= have) value = -INFINITY, token = -1;  // no such candidate
-      st_remote64(remote(&sh.cand[b][lane], 0), (u64)__double_as_longlong(value));
-      st_remote32(remote(&sh.token[b][lane], 0), (uint32_t)token);
-      if (lane == 0) st_remote32(remote(&sh.done[b], 0), fin ? 1u : 0u);
+    if (__syncthreads_or(close)) {
+      tc::cluster_sync();  // every CTA has read the candidates before they are written again
+      continue;
     }
-  }
-  tc::cluster_sync();
-  if (crank != 0) return;
-  // rank of each survivor among all
-  for (int i = tid; i < W * W; i += kSelThreads) {
-    const int b = i / W, j = i % W, tok = sh.token[b][j];
-    if (tok < 0) continue;
-    const double v = sh.cand[b][j];
-    int rank = 0;
-    for (int k = 0; k < W * W; ++k) {  // among equals the lower beam, and a beam's own order
-      const double v2 = sh.cand[k / W][k % W];
-      rank += sh.token[k / W][k % W] >= 0 && (v2 > v || (v2 == v && k < i));
-    }
-    if (rank < W) {
-      const int64_t o = g * W + rank;
-      p.out_scores[o] = (float)v;
+    if (crank == 0 && tid < W) {
+      const int64_t o = g * W + tid;
+      const int b = sh.beam[tid], tok = sh.pick[tid];
+      p.out_scores[o] = (float)sh.best[tid];
       p.out_parents[o] = b;
       p.out_tokens[o] = tok;
       if (p.eos >= 0) p.out_finished[o] = sh.done[b] || tok == p.eos;
     }
+    return;
   }
 }
 
@@ -282,7 +386,12 @@ template <typename U, int W>
 __device__ __forceinline__ void reorder_piece(const ReorderParams::State& s, int64_t g, int64_t u, const int* src,
                                               const int64_t* live, int w) {
   if (u >= s.units) return;
-  const int64_t t = s.T ? (u * (int64_t)sizeof(U) / s.inner) % s.T : -1;  // -1: whole rows
+  // entry of the time axis; -1: whole rows
+  int64_t t = -1;
+  if (s.T) {
+    const int64_t at = u * (int64_t)sizeof(U);
+    t = s.row_bytes <= UINT32_MAX ? (uint32_t)at / (uint32_t)s.inner % (uint32_t)s.T : at / s.inner % s.T;
+  }
   uint8_t* row0 = s.p + g * w * s.row_bytes + u * (int64_t)sizeof(U);
   U v[W];
   // every read comes before the first write: this thread alone touches these bytes of the group's rows
@@ -331,10 +440,11 @@ cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
   if (a.G == 0) return cudaSuccess;
   SelectParams p = {a.logits, a.scores, a.finished, a.out_scores, a.out_parents, a.out_tokens, a.out_finished,
                     a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos};
-  // a warp for every two pieces of the group's logits, until every SM has a CTA
+  // split while the CTAs (one per SM) stay one wave and every warp has a piece
   const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);
-  int C = 1;
-  while (C < 8 && a.G * C < 296 && pieces > C * kSelWarps) C *= 2;
+  int dev = 0, sms = 148, C = 1;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  while (C < 8 && a.G * 2 * C <= sms && pieces > C * kSelWarps) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.G * C));
   cfg.blockDim = dim3(kSelThreads);

@@ -26,9 +26,10 @@ constexpr int EPL = 8;  // values per lane: one 16-byte load of bf16, two of f32
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float* x);
 template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* x) {
-  const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+__device__ __forceinline__ void load8<float>(const float* p, float* x) {  // p: 32-byte aligned
+  asm volatile("ld.global.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+               : "l"(p));
 }
 template <>
 __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float* x) {
@@ -53,9 +54,10 @@ __device__ __forceinline__ void load8<int8_t>(const int8_t* p, float* x) {
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* x);
 template <>
-__device__ __forceinline__ void store8<float>(float* p, const float* x) {
-  *(float4*)p = make_float4(x[0], x[1], x[2], x[3]);
-  *(float4*)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+__device__ __forceinline__ void store8<float>(float* p, const float* x) {  // p: 32-byte aligned
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+               "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
 }
 template <>
 __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const float* x) {
@@ -82,50 +84,62 @@ struct WriteParams {
   void* dst[2];        // the caches
   float* scale[2];
   const int* pos;
-  int64_t rows;  // N * S * H of one of the two
   int64_t T;
-  int S, H, D;
+  unsigned rows;    // S * H: a slot's rows of one of the two
+  unsigned blocks;  // per slot
+  int H, D;
 };
 
 // A group of LPR lanes carries one row: with 8 values a lane the row's largest
-// magnitude is a butterfly of log2(LPR) shuffles.
-template <typename TI, typename TC, int LPR>
+// magnitude is a butterfly of log2(LPR) shuffles.  A block takes RPT rows per
+// group of one slot's keys, then values; all their loads come first.
+template <typename TI, typename TC, int LPR, int RPT>
 __global__ void __launch_bounds__(kThreads) write_kernel(const WriteParams p) {
   pdl_prologue();
+  constexpr int GROUPS = kThreads / LPR;
   const int lane = threadIdx.x % LPR;
-  const int64_t r2 = (int64_t)blockIdx.x * (kThreads / LPR) + threadIdx.x / LPR;
-  const int which = r2 >= p.rows;
-  const int64_t r = r2 - (which ? p.rows : 0);
-  const int64_t h = r % p.H, ns = r / p.H, s = ns % p.S, n = ns / p.S;
-  const bool row = r < p.rows;
-  const int64_t first = row ? p.pos[n] : -1, t = first + s;
-  const bool in = first >= 0 && t < p.T && lane * EPL < p.D;
-  float x[EPL];
+  const unsigned n = blockIdx.x / p.blocks, r0 = blockIdx.x % p.blocks * (GROUPS * RPT) + threadIdx.x / LPR;
+  const int64_t first = p.pos[n];
+  float x[RPT][EPL];
+  int64_t at[RPT];
+  unsigned which[RPT];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) x[i] = 0.f;
-  if (in) load8((const TI*)p.src[which] + r * p.D + lane * EPL, x);
-  const int64_t at = (n * p.H + h) * p.T + t;
-  if constexpr (sizeof(TC) == 1) {
-    float m = 0.f;
+  for (int k = 0; k < RPT; ++k) {
+    unsigned r = r0 + k * GROUPS;
+    which[k] = r >= p.rows;
+    if (which[k]) r -= p.rows;
+    const unsigned s = r / p.H, h = r - s * p.H;
+    const int64_t t = first + s;
+    const bool in = r < p.rows && first >= 0 && t < p.T && lane * EPL < p.D;
+    at[k] = in ? ((int64_t)n * p.H + h) * p.T + t : -1;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -FLT_MAX), FLT_MAX);
-      m = fmaxf(m, fabsf(x[i]));
-    }
+    for (int i = 0; i < EPL; ++i) x[k][i] = 0.f;
+    if (in) load8((const TI*)(which[k] ? p.src[1] : p.src[0]) + ((int64_t)n * p.rows + r) * p.D + lane * EPL, x[k]);
+  }
 #pragma unroll
-    for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float sc = __fdiv_rn(m, 127.f);
-    if (in) {
-      uint32_t w[2] = {0, 0};
-      if (sc > 0.f) {
+  for (int k = 0; k < RPT; ++k) {
+    if constexpr (sizeof(TC) == 1) {
+      float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) w[i / 4] |= (uint32_t)(nearest_code(x[i], sc) & 255) << (8 * (i % 4));
+      for (int i = 0; i < EPL; ++i) {
+        x[k][i] = x[k][i] != x[k][i] ? 0.f : fminf(fmaxf(x[k][i], -FLT_MAX), FLT_MAX);
+        m = fmaxf(m, fabsf(x[k][i]));
       }
-      *(uint2*)((int8_t*)p.dst[which] + at * p.D + lane * EPL) = make_uint2(w[0], w[1]);
-      if (lane == 0) p.scale[which][at] = sc;
+#pragma unroll
+      for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float sc = __fdiv_rn(m, 127.f);
+      if (at[k] >= 0) {
+        uint32_t w[2] = {0, 0};
+        if (sc > 0.f) {
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) w[i / 4] |= (uint32_t)(nearest_code(x[k][i], sc) & 255) << (8 * (i % 4));
+        }
+        *(uint2*)((int8_t*)(which[k] ? p.dst[1] : p.dst[0]) + at[k] * p.D + lane * EPL) = make_uint2(w[0], w[1]);
+        if (lane == 0) (which[k] ? p.scale[1] : p.scale[0])[at[k]] = sc;
+      }
+    } else {
+      if (at[k] >= 0) store8((TC*)(which[k] ? p.dst[1] : p.dst[0]) + at[k] * p.D + lane * EPL, x[k]);
     }
-  } else {
-    if (in) store8((TC*)p.dst[which] + at * p.D + lane * EPL, x);
   }
 }
 
@@ -134,81 +148,115 @@ struct ReadParams {
   const float* scale[2];
   void* dst[2];  // [N, H, S, D]
   const int *starts, *counts;
-  int64_t units;  // 8-value pieces of one of the two outputs
   int64_t T, S;
+  unsigned blocks;  // per (slot, head) of one of the two
   int H, D;
 };
 
+constexpr int kReadUnits = 4;  // 8-value pieces per thread
+
+// For one (slot, head) both sides are contiguous: rows i of the output are rows
+// starts[n] + i of the cache, so a block copies a range of pieces and clips it to
+// the rows that exist and are counted.
 template <typename TC, typename TO>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
   pdl_prologue();
-  const int64_t u2 = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int which = u2 >= p.units;
-  const int64_t u = u2 - (which ? p.units : 0);
-  if (u >= p.units) return;
+  const unsigned b = blockIdx.x % p.blocks, item = blockIdx.x / p.blocks, which = item & 1, nh = item >> 1;
+  const unsigned n = nh / p.H;
+  const int64_t start = p.starts ? p.starts[n] : 0;
+  const int64_t lo = max((int64_t)0, -start);
+  int64_t hi = min(p.S, p.T - start);
+  if (p.counts) hi = min(hi, (int64_t)p.counts[n]);
   const int per = p.D / EPL;
-  const int64_t row = u / per, i = row % p.S, nh = row / p.S, n = nh / p.H;
-  const int64_t t = (p.starts ? (int64_t)p.starts[n] : 0) + i;
-  if (t < 0 || t >= p.T || (p.counts && i >= p.counts[n])) return;
-  const int64_t at = nh * p.T + t;
-  const int d = (int)(u % per) * EPL;
-  float x[EPL];
-  load8((const TC*)p.src[which] + at * p.D + d, x);
-  if constexpr (sizeof(TC) == 1) {
-    const float s = p.scale[which][at];
+  const int64_t u0 = (int64_t)b * (kThreads * kReadUnits) + threadIdx.x;
+  const TC* src = (const TC*)(which ? p.src[1] : p.src[0]) + ((int64_t)nh * p.T + start) * p.D;
+  TO* dst = (TO*)(which ? p.dst[1] : p.dst[0]) + (int64_t)nh * p.S * p.D;
+  float x[kReadUnits][EPL], s[kReadUnits];
+  bool in[kReadUnits];
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) x[j] *= s;
+  for (int k = 0; k < kReadUnits; ++k) {
+    const int64_t u = u0 + k * kThreads;
+    in[k] = u >= lo * per && u < hi * per;
+    s[k] = 1.f;
+    if (in[k]) {
+      load8(src + u * EPL, x[k]);
+      if constexpr (sizeof(TC) == 1) {
+        const int64_t row = u <= UINT32_MAX ? (int64_t)((uint32_t)u / (uint32_t)per) : u / per;
+        s[k] = (which ? p.scale[1] : p.scale[0])[(int64_t)nh * p.T + start + row];
+      }
+    }
   }
-  store8((TO*)p.dst[which] + row * p.D + d, x);
+#pragma unroll
+  for (int k = 0; k < kReadUnits; ++k) {
+    if (!in[k]) continue;
+    if constexpr (sizeof(TC) == 1) {
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) x[k][j] *= s[k];
+    }
+    store8(dst + (u0 + k * kThreads) * EPL, x[k]);
+  }
+}
+
+template <typename TI, typename TC, int LPR, int RPT>
+cudaError_t launch_write(WriteParams p, int64_t N, cudaStream_t stream) {
+  const int64_t per = kThreads / LPR * RPT;
+  const int64_t blocks = (2 * (int64_t)p.rows + per - 1) / per;
+  if (blocks * N > INT32_MAX) return cudaErrorInvalidValue;
+  p.blocks = (unsigned)blocks;
+  return launch_pdl(write_kernel<TI, TC, LPR, RPT>, dim3((unsigned)(blocks * N)), dim3(kThreads), 0, stream, p);
 }
 
 template <typename TI, typename TC, int LPR>
-cudaError_t launch_write(const WriteParams& p, cudaStream_t stream) {
-  const int64_t per = kThreads / LPR, blocks = (2 * p.rows + per - 1) / per;
-  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  return launch_pdl(write_kernel<TI, TC, LPR>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
+cudaError_t by_rows(const WriteParams& p, int64_t N, cudaStream_t stream) {
+  // several rows per group once there are blocks for every SM all the same
+  constexpr int64_t groups = kThreads / LPR;
+  if (2 * (int64_t)p.rows >= 4 * groups && N * 2 * p.rows / (4 * groups) >= 296)
+    return launch_write<TI, TC, LPR, 4>(p, N, stream);
+  return launch_write<TI, TC, LPR, 1>(p, N, stream);
 }
 
 template <typename TI, typename TC>
-cudaError_t write_rows(const WriteParams& p, cudaStream_t stream) {
-  if (p.D <= 16) return launch_write<TI, TC, 2>(p, stream);
-  if (p.D <= 32) return launch_write<TI, TC, 4>(p, stream);
-  if (p.D <= 64) return launch_write<TI, TC, 8>(p, stream);
-  if (p.D <= 128) return launch_write<TI, TC, 16>(p, stream);
-  return launch_write<TI, TC, 32>(p, stream);
+cudaError_t write_rows(const WriteParams& p, int64_t N, cudaStream_t stream) {
+  if (p.D <= 16) return by_rows<TI, TC, 2>(p, N, stream);
+  if (p.D <= 32) return by_rows<TI, TC, 4>(p, N, stream);
+  if (p.D <= 64) return by_rows<TI, TC, 8>(p, N, stream);
+  if (p.D <= 128) return by_rows<TI, TC, 16>(p, N, stream);
+  return by_rows<TI, TC, 32>(p, N, stream);
 }
 
 template <typename TC, typename TO>
-cudaError_t read_rows(const ReadParams& p, cudaStream_t stream) {
-  const int64_t blocks = (2 * p.units + kThreads - 1) / kThreads;
-  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-  return launch_pdl(read_kernel<TC, TO>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
+cudaError_t read_rows(ReadParams p, int64_t N, cudaStream_t stream) {
+  const int64_t units = p.S * (p.D / EPL), blocks = (units + kThreads * kReadUnits - 1) / (kThreads * kReadUnits);
+  if (blocks * 2 * N * p.H > INT32_MAX) return cudaErrorInvalidValue;
+  p.blocks = (unsigned)blocks;
+  return launch_pdl(read_kernel<TC, TO>, dim3((unsigned)(blocks * 2 * N * p.H)), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
 
 cudaError_t kv_cache_write(const KvCacheView& c, const int* positions, const void* k, const void* v, bool in_bf16,
                            int64_t S, cudaStream_t stream) {
-  WriteParams p = {{k, v}, {c.k, c.v}, {c.k_scale, c.v_scale}, positions, c.N * S * c.H, c.T, (int)S, (int)c.H,
-                   (int)c.D};
+  if (S * c.H > INT32_MAX) return cudaErrorInvalidValue;
+  const WriteParams p = {{k, v}, {c.k, c.v}, {c.k_scale, c.v_scale}, positions, c.T, (unsigned)(S * c.H), 0,
+                         (int)c.H, (int)c.D};
   using bf = __nv_bfloat16;
   switch (c.type) {
-    case KvType::F32: return in_bf16 ? write_rows<bf, float>(p, stream) : write_rows<float, float>(p, stream);
-    case KvType::BF16: return in_bf16 ? write_rows<bf, bf>(p, stream) : write_rows<float, bf>(p, stream);
-    case KvType::I8: return in_bf16 ? write_rows<bf, int8_t>(p, stream) : write_rows<float, int8_t>(p, stream);
+    case KvType::F32: return in_bf16 ? write_rows<bf, float>(p, c.N, stream) : write_rows<float, float>(p, c.N, stream);
+    case KvType::BF16: return in_bf16 ? write_rows<bf, bf>(p, c.N, stream) : write_rows<float, bf>(p, c.N, stream);
+    case KvType::I8: return in_bf16 ? write_rows<bf, int8_t>(p, c.N, stream) : write_rows<float, int8_t>(p, c.N, stream);
   }
   return cudaErrorInvalidValue;
 }
 
 cudaError_t kv_cache_read(const KvCacheView& c, const int* starts, const int* counts, void* k_out, void* v_out,
                           bool out_bf16, int64_t S, cudaStream_t stream) {
-  ReadParams p = {{c.k, c.v}, {c.k_scale, c.v_scale}, {k_out, v_out}, starts, counts, c.N * c.H * S * (c.D / EPL), c.T,
-                  S, (int)c.H, (int)c.D};
+  const ReadParams p = {{c.k, c.v}, {c.k_scale, c.v_scale}, {k_out, v_out}, starts, counts, c.T, S, 0, (int)c.H,
+                        (int)c.D};
   using bf = __nv_bfloat16;
   switch (c.type) {
-    case KvType::F32: return out_bf16 ? read_rows<float, bf>(p, stream) : read_rows<float, float>(p, stream);
-    case KvType::BF16: return out_bf16 ? read_rows<bf, bf>(p, stream) : read_rows<bf, float>(p, stream);
-    case KvType::I8: return out_bf16 ? read_rows<int8_t, bf>(p, stream) : read_rows<int8_t, float>(p, stream);
+    case KvType::F32: return out_bf16 ? read_rows<float, bf>(p, c.N, stream) : read_rows<float, float>(p, c.N, stream);
+    case KvType::BF16: return out_bf16 ? read_rows<bf, bf>(p, c.N, stream) : read_rows<bf, float>(p, c.N, stream);
+    case KvType::I8: return out_bf16 ? read_rows<int8_t, bf>(p, c.N, stream) : read_rows<int8_t, float>(p, c.N, stream);
   }
   return cudaErrorInvalidValue;
 }

@@ -1779,6 +1779,13 @@ sb_status* op_aliases(std::initializer_list<const sb_buffer*> written, std::init
     if (sb_status* st_ = (expr)) return st_; \
   } while (0)
 
+// Rows of f32 values are read and written 32 bytes at a time.
+sb_status* op_aligned(const sb_buffer* b, const char* what) {
+  if (b->type.dtype == DType::F32 && b->bytes && ((uintptr_t)b->ptr & 31))
+    return make_status(SB_STATUS_INVALID_ARGUMENT, std::string(what) + ": f32 rows must be 32-byte aligned");
+  return nullptr;
+}
+
 sb_status* op_cache(const sb_session* s, const sb_kv_cache* c, KvCacheView* out) {
   if (!c) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL cache");
   if (!c->k) return make_status(SB_STATUS_INVALID_ARGUMENT, "cache keys: NULL buffer");
@@ -1789,6 +1796,8 @@ sb_status* op_cache(const sb_session* s, const sb_kv_cache* c, KvCacheView* out)
   const DType dt = c->k->type.dtype;
   SB_OP(op_buffer(s, c->k, "cache keys", kFloats | bit(DType::I8), shape));
   SB_OP(op_buffer(s, c->v, "cache values", bit(dt), shape));
+  SB_OP(op_aligned(c->k, "cache keys"));
+  SB_OP(op_aligned(c->v, "cache values"));
   if (shape[3] < 16 || shape[3] > kKvMaxDim || shape[3] % 16)
     return make_status(SB_STATUS_INVALID_ARGUMENT, "head size must be a multiple of 16 from 16 to 256, got " +
                                                        std::to_string(shape[3]));
@@ -1833,6 +1842,8 @@ sb_status* sb_kv_cache_write(sb_session* s, const sb_kv_cache* cache, sb_buffer*
   const int64_t S = k->type.shape[1];
   SB_OP(op_buffer(s, k, "keys", kFloats, {c.N, S, c.H, c.D}));
   SB_OP(op_buffer(s, v, "values", bit(k->type.dtype), {c.N, S, c.H, c.D}));
+  SB_OP(op_aligned(k, "keys"));
+  SB_OP(op_aligned(v, "values"));
   SB_OP(op_buffer(s, positions, "positions", bit(DType::I32), {c.N}));
   SB_OP(op_aliases({cache->k, cache->v, cache->k_scale, cache->v_scale}, {k, v, positions}));
   std::lock_guard<std::mutex> g(s->mu);
@@ -1851,6 +1862,8 @@ sb_status* sb_kv_cache_read(sb_session* s, const sb_kv_cache* cache, sb_buffer* 
   const int64_t S = k_out->type.shape[2];
   SB_OP(op_buffer(s, k_out, "keys out", kFloats, {c.N, c.H, S, c.D}));
   SB_OP(op_buffer(s, v_out, "values out", bit(k_out->type.dtype), {c.N, c.H, S, c.D}));
+  SB_OP(op_aligned(k_out, "keys out"));
+  SB_OP(op_aligned(v_out, "values out"));
   if (starts) SB_OP(op_buffer(s, starts, "starts", bit(DType::I32), {c.N}));
   if (counts) SB_OP(op_buffer(s, counts, "counts", bit(DType::I32), {c.N}));
   SB_OP(op_aliases({k_out, v_out}, {cache->k, cache->v, cache->k_scale, cache->v_scale, starts, counts}));

@@ -413,11 +413,14 @@ def check_select(sess, logits, scores, fin, eos, kind="f32"):
         sess.beam_select(put(sess, logits, kind), sc, sc, par, tok)
     assert np.array_equal(par.to_host(), ref[1])
     assert np.array_equal(tok.to_host(), ref[2])
-    # the value is formed in f64 and rounded once
+    # The sums of f32 exponentials: a term 2^-t is off by 2^-22 (exp2) + 2^-23.4 t
+    # of itself (its argument's two roundings); t weighted by 2^-t averages at
+    # most log2(V) < 17 here; 32 terms are added in a tree of depth 5:
+    # 2^-22 + 17 * 2^-23.4 + 5 * 2^-24 < 2.1e-6, and the value is rounded once.
     got = sc.to_host().astype(np.float64)
     same = got == ref[0]
     with np.errstate(invalid="ignore"):
-        assert (same | (np.abs(got - ref[0]) <= U32 * np.abs(ref[0]) * 1.001 + 1e-13)).all()
+        assert (same | (np.abs(got - ref[0]) <= U32 * np.abs(ref[0]) + 2.1e-6)).all()
 
 
 @pytest.mark.gpu
@@ -475,6 +478,7 @@ def test_beam_reorder(sess, G, W):
 
 @pytest.mark.gpu
 def test_refusals_launch_nothing(sess, lib):
+    import torch
     other = S.B200Session(device=0, precision="fp32")
     z = sess.zeros
     c8, c32 = sess.kv_cache(2, 2, 8, 32, "int8"), sess.kv_cache(2, 2, 8, 32)
@@ -508,6 +512,8 @@ def test_refusals_launch_nothing(sess, lib):
     refused(sess.kv_cache_read, c32, z((2, 2, 4, 32), "i32"), z((2, 2, 4, 32), "i32"))
     refused(sess.kv_cache_read, c32, c32.k, z((2, 2, 8, 32)))           # out of the cache into itself
     refused(sess.kv_cache_read, c32, z((2, 2, 4, 32)), z((2, 2, 4, 32)), starts=z((1,), "i32"))
+    off = sess.wrap_torch(torch.zeros(2 * 2 * 8 * 32 + 4, device="cuda")[4:].view(2, 2, 8, 32))
+    refused(w, S.KVCache(off, c32.v))                                   # 16-byte aligned f32 rows
     a = sess.kv_cache_attention
     refused(a, c32, pos, q, q)
     refused(a, c32, pos, z((2, 1, 3, 32)), z((2, 1, 3, 32)))            # 3 query heads on 2
