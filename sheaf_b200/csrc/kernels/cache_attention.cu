@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
     }
   }
   join_and_store<kWarps, R, DP>(p, w, r0, rows, sm, s_m, s_l, sm + kWarps * R * DP, s_ml, s_mask,
-                                [](unsigned long long, int, float*) {});
+                                nullptr);
 }
 
 template <typename CT, int LPK, int R, int U>

@@ -106,12 +106,15 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w, bool& bad) {
   return w;
 }
 
-// DP: head size padded to 64 or 128.  Q32: f32 queries, at most 4 rows; else
-// bf16 queries, at most 16.
-template <int DP, bool I8, bool Q32, int NW>
+// DP: head size padded to 64 or 128.  MODE: bf16 queries of at most 16 rows
+// (kRows16) or 8 (kRows8: rows 8-15 of the second product hold what bf16 left of
+// P, so P has 16 bits), f32 queries of at most 4 rows (kF32).
+enum Mode { kRows16, kRows8, kF32 };
+template <int DP, bool I8, int MODE, int NW>
 struct MmaCfg {
-  static constexpr int RMAX = Q32 ? 4 : 16, NR = Q32 ? 1 : 2;  // rows of the CTA, of a lane
-  static constexpr int KB = I8 ? 32 : 16;                      // keys per step
+  static constexpr int RMAX = MODE == kF32 ? 4 : MODE == kRows8 ? 8 : 16;  // rows of the CTA
+  static constexpr int NR = MODE == kRows16 ? 2 : 1;                       // of a lane
+  static constexpr int KB = 4096 / (DP * (I8 ? 1 : 2));        // keys per step: 4 KB of K, 4 KB of V
   static constexpr int EK = I8 ? 16 : 8;                       // values of a lane's 16-byte piece of K
   static constexpr int KL = DP / (4 * EK);                     // such pieces per key
   static constexpr int EV = I8 ? DP / 8 : 8;                   // values of a lane's piece of V
@@ -142,15 +145,15 @@ __device__ __forceinline__ int piece_at(int key, int u) {
   return key * RB + ((RB == 128 ? u ^ (key & 7) : u ^ (key >> 1 & 3)) << 4);
 }
 
-template <int DP, bool I8, bool Q32, int NW>
+template <int DP, bool I8, int MODE, int NW>
 __global__ void __launch_bounds__(NW * 32)
     cache_attn_mma(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const Params p,
                    int* err) {
-  using F = MmaCfg<DP, I8, Q32, NW>;
+  using F = MmaCfg<DP, I8, MODE, NW>;
+  constexpr bool Q32 = MODE == kF32;
   constexpr bool F16 = I8;  // operands: f16 for int8 caches, bf16 for bf16 ones
   constexpr int KB = F::KB, NB = KB / 8, KG = KB / 16, EK = F::EK, KL = F::KL, VL = F::VL, NR = F::NR, RMAX = F::RMAX;
   constexpr int RB = F::RB, BOX = F::BOX, STAGES = F::STAGES;
-  pdl_prologue();
   extern __shared__ __align__(1024) float sm[];  // the warps' stages, later their partial outputs
   __shared__ uint64_t s_full[NW][F::STAGES];
   __shared__ volatile int s_abort;
@@ -158,8 +161,21 @@ __global__ void __launch_bounds__(NW * 32)
   __shared__ int s_jump[kKvMaxTokens];
   __shared__ float s_m[NW * RMAX], s_l[NW * RMAX], s_ml[2 * RMAX];
   __shared__ int s_bad;
-  const Place w = find_place(p);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  // nothing of the previous kernel is needed for this
+  if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mK) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mV) : "memory");
+    for (int i = 0; i < NW * STAGES; ++i) tc::mbar_init(&s_full[0][i], 1);
+    s_bad = 0;
+    s_abort = tc::smem_u32(sm) & 1023u ? 1 : 0;
+    if (s_abort) atomicExch(err, 63);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tc::fence_proxy_async();
+  }
+  __syncthreads();
+  pdl_prologue();
+  const Place w = find_place(p);
   const int r0 = w.chunk * RMAX, rows = min(RMAX, p.S * p.G - r0);
   // this CTA's keys, in whole steps of the warps' stride
   const int64_t per = ((w.end + w.C - 1) / w.C + KB - 1) / KB * KB;
@@ -169,34 +185,56 @@ __global__ void __launch_bounds__(NW * 32)
   uint8_t* const ring = (uint8_t*)sm + warp * STAGES * F::STAGE;
   float* const scales = (float*)((uint8_t*)sm + F::SC_OFF) + warp * STAGES * KB * 2;
   uint64_t* const full = s_full[warp];
-  if (tid == 0) {
-    for (int i = 0; i < NW * STAGES; ++i) tc::mbar_init(&s_full[0][i], 1);
-    s_bad = 0;
-    s_abort = tc::smem_u32(sm) & 1023u ? 1 : 0;
-    if (s_abort) atomicExch(err, 63);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    tc::fence_proxy_async();
-  }
-  __syncthreads();
   // One step's keys into stage `st` of this warp: boxes by TMA (rows behind the
   // cache's capacity arrive as zeros), scales by asynchronous copies.
   auto fetch = [&](int64_t t, int st) {
     if (lane == 0 && !s_abort) {
       tc::mbar_expect_tx(&full[st], F::STAGE);
+uint8_t* dst = ring + st * F::STAGE;
+      if (F::BOXES == 1 || p.D == DP) {
+        tc::tma_load_4d(dst, &mK, &full[st], 0, (int)t, 0, (int)w.nh);
+        tc::tma_load_4d(dst + F::BOXES * BOX, &mV, &full[st], 0, (int)t, 0, (int)w.nh);
+      } else {
 #pragma unroll
-      for (int i = 0; i < F::BOXES; ++i) {
-        uint8_t* dst = ring + st * F::STAGE + i * BOX;
-        tc::tma_load_3d(dst, &mK, &full[st], i * (RB / (I8 ? 1 : 2)), (int)t, (int)w.nh);
-        tc::tma_load_3d(dst + F::BOXES * BOX, &mV, &full[st], i * (RB / (I8 ? 1 : 2)), (int)t, (int)w.nh);
+        for (int i = 0; i < F::BOXES; ++i) {
+          tc::tma_load_4d(dst + i * BOX, &mK, &full[st], i * (RB / (I8 ? 1 : 2)), (int)t, 0, (int)w.nh);
+          tc::tma_load_4d(dst + (F::BOXES + i) * BOX, &mV, &full[st], i * (RB / (I8 ? 1 : 2)), (int)t, 0, (int)w.nh);
+        }
       }
     }
-    if (I8) {  // KB = 32: a scale of each kind per lane
-      const bool in = t + lane < w.end;
-      const uint32_t at = tc::smem_u32(scales + st * KB * 2 + lane);
-      copy4(at, in ? ksb + t + lane : ksb, in);
-      copy4(at + KB * 4, in ? vsb + t + lane : vsb, in);
+    if (I8) {
+#pragma unroll
+      for (int i = 0; i < KB / 32; ++i) {
+        const bool in = t + i * 32 + lane < w.end;
+        const uint32_t at = tc::smem_u32(scales + st * KB * 2 + i * 32 + lane);
+        copy4(at, in ? ksb + t + i * 32 + lane : ksb, in);
+        copy4(at + KB * 4, in ? vsb + t + i * 32 + lane : vsb, in);
+      }
     }
   };
+  // the queries' loads go out first, then the first steps' copies
+  float y[NR][DP / 16][4];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int row = Q32 ? g & 3 : g + 8 * r;
+    const bool in = row < rows;
+    const int64_t at = in ? row_at(p, w, r0 + row) : 0;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int d = (s / (EK / 4)) * 4 * EK + c * EK + (s % (EK / 4)) * 4;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in && d < p.D) {
+        if (Q32) {
+          x = *(const float4*)((const float*)p.q + at + d);
+        } else {
+          const uint2 z = *(const uint2*)((const __nv_bfloat16*)p.q + at + d);
+          const float2 a = unpack2<false>(z.x), b = unpack2<false>(z.y);
+          x = make_float4(a.x, a.y, b.x, b.y);
+        }
+      }
+      y[r][s][0] = x.x, y[r][s][1] = x.y, y[r][s][2] = x.z, y[r][s][3] = x.w;
+    }
+  }
   int64_t t0 = lo + warp * KB;
   constexpr int STRIDE = NW * KB;
 #pragma unroll
@@ -214,25 +252,6 @@ __global__ void __launch_bounds__(NW * 32)
   float fs[NR], sum_q[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    const int row = Q32 ? g & 3 : g + 8 * r;
-    const bool in = row < rows;
-    const int64_t at = in ? row_at(p, w, r0 + row) : 0;
-    float y[DP / 16][4];
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      const int d = (s / (EK / 4)) * 4 * EK + c * EK + (s % (EK / 4)) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[s][i] = 0.f;
-      if (in && d < p.D) {
-        if (Q32) {
-          *(float4*)y[s] = *(const float4*)((const float*)p.q + at + d);
-        } else {
-          const uint2 x = *(const uint2*)((const __nv_bfloat16*)p.q + at + d);
-          const float2 a = unpack2<false>(x.x), b = unpack2<false>(x.y);
-          y[s][0] = a.x, y[s][1] = a.y, y[s][2] = b.x, y[s][3] = b.y;
-        }
-      }
-    }
     float up = 1.f;
     fs[r] = p.scale2;
     sum_q[r] = 0.f;
@@ -241,7 +260,7 @@ __global__ void __launch_bounds__(NW * 32)
 #pragma unroll
       for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(y[s][i]));
+        for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(y[r][s][i]));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
       // 2^(14 - e) for a largest value of exponent e, within f32's normal range
@@ -251,7 +270,8 @@ __global__ void __launch_bounds__(NW * 32)
     }
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
-      float2 a = make_float2(y[s][0] * up, y[s][I8 ? 2 : 1] * up), b = make_float2(y[s][I8 ? 1 : 2] * up, y[s][3] * up);
+      float2 a = make_float2(y[r][s][0] * up, y[r][s][I8 ? 2 : 1] * up),
+             b = make_float2(y[r][s][I8 ? 1 : 2] * up, y[r][s][3] * up);
       if (Q32) {
         const uint32_t a1 = take2<F16>(a.x, a.y), b1 = take2<F16>(b.x, b.y);
         const uint32_t a2 = take2<F16>(a.x, a.y), b2 = take2<F16>(b.x, b.y);
@@ -263,6 +283,7 @@ __global__ void __launch_bounds__(NW * 32)
       } else {
         q[s][r] = pack2<F16>(a.x, a.y);
         q[s][2 + r] = pack2<F16>(b.x, b.y);
+        if (MODE == kRows8) q[s][1] = q[s][3] = 0u;
         if (F16) {
           const float2 a1 = unpack2<F16>(q[s][r]), b1 = unpack2<F16>(q[s][2 + r]);
           sum_q[r] += (a1.x + a1.y) + (b1.x + b1.y);
@@ -372,15 +393,19 @@ __global__ void __launch_bounds__(NW * 32)
 #pragma unroll
         for (int j = 0; j < DP / 8; ++j) {
           o[j][2 * r] *= f, o[j][2 * r + 1] *= f;
-          if (Q32) o[j][2] *= f, o[j][3] *= f;
+          if (MODE != kRows16) o[j][2] *= f, o[j][3] *= f;
         }
       }
     }
     if (I8) {
       // P times the value scales goes into f16 relative to 2^vref, above the
       // largest scale so far: at most 2^(8 + 6), with steps of 2^-30 below 1
-      const float mine = fabsf(sc[KB + lane]);
-      const int e = mine < INFINITY ? (int)(__float_as_uint(mine) >> 23) - 126 : -125;
+      int e = -125;
+#pragma unroll
+      for (int i = 0; i < KB / 32; ++i) {
+        const float mine = fabsf(sc[KB + i * 32 + lane]);
+        if (mine < INFINITY) e = max(e, (int)(__float_as_uint(mine) >> 23) - 126);
+      }
       const int top = max(__reduce_max_sync(0xffffffffu, e), -100);
       if (top > vref) {
         const float f = tc::ex2((float)(vref - top));
@@ -412,6 +437,9 @@ __global__ void __launch_bounds__(NW * 32)
           const uint32_t h1 = take2<F16>(y[0], y[1]), h2 = take2<F16>(y[0], y[1]), h3 = pack2<F16>(y[0], y[1]);
           dst[0] = g < 4 ? h1 : h3;
           dst[1] = g < 4 ? h2 : 0u;
+        } else if (MODE == kRows8) {
+          dst[0] = take2<F16>(y[0], y[1]);
+          dst[1] = pack2<F16>(y[0], y[1]);
         } else {
           dst[r] = pack2<F16>(y[0], y[1]);
         }
@@ -481,64 +509,42 @@ __global__ void __launch_bounds__(NW * 32)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float y = o[j][2 * r + i];
-        if (Q32) {
-          y += o[j][2 + i];
-          y += __shfl_xor_sync(0xffffffffu, y, 16);
-        }
+        if (MODE != kRows16) y += o[j][2 + i];
+        if (Q32) y += __shfl_xor_sync(0xffffffffu, y, 16);
         if (I8) y *= vup;
         const int d = (j / F::EV) * 8 * F::EV + (2 * c + i) * F::EV + j % F::EV;
         if (!Q32 || g < 4) sm[(warp * RMAX + row) * DP + d] = y;
       }
   }
-  int bad = 0;
-  if (!I8) {
-    // a drafted value that is not finite reaches the rows that see it: whichever CTA read it
-    __syncthreads();
-    if (w.C > 1) tc::cluster_sync();
-    for (uint32_t r = 0; r < w.C; ++r) {
-      int y;
-      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(y) : "r"(tc::cluster_addr(&s_bad, r)));
-      bad |= y;
-    }
-  }
-  join_and_store<NW, RMAX, DP>(
-      p, w, r0, rows, sm, s_m, s_l, sm + NW * RMAX * DP, s_ml, s_mask, [&](unsigned long long see, int d, float* y) {
-        if (!bad) return;
-        for (int j = 0; j < p.S; ++j)
-          if (see >> j & 1ull)
-            for (int i = 0; i < 4; ++i) {
-              const float v = __bfloat162float(((const __nv_bfloat16*)p.v)[(w.nh * p.T + w.pos + j) * p.D + d + i]);
-              if (!isfinite(v)) y[i] += v;
-            }
-      });
+  join_and_store<NW, RMAX, DP>(p, w, r0, rows, sm, s_m, s_l, sm + NW * RMAX * DP, s_ml, s_mask, I8 ? nullptr : &s_bad);
 }
 
-template <int DP, bool I8, bool Q32, int NW>
+template <int DP, bool I8, int MODE, int NW>
 cudaError_t launch(const CacheAttnArgs& a, int C, cudaStream_t stream) {
-  using F = MmaCfg<DP, I8, Q32, NW>;
+  using F = MmaCfg<DP, I8, MODE, NW>;
   const Params p = make_params(a, F::RMAX);
   const KvCacheView& c = a.cache;
   CUtensorMap mk, mv;
-  if (!tc_make_map_rows(&mk, c.k, I8, c.D, c.T, c.N * c.H, F::RB, F::KB) ||
-      !tc_make_map_rows(&mv, c.v, I8, c.D, c.T, c.N * c.H, F::RB, F::KB))
+  const uint32_t blocks = c.D == DP ? F::BOXES : 1;
+  if (!tc_make_map_rows(&mk, c.k, I8, c.D, c.T, c.N * c.H, F::RB, F::KB, blocks) ||
+      !tc_make_map_rows(&mv, c.v, I8, c.D, c.T, c.N * c.H, F::RB, F::KB, blocks))
     return cudaErrorNotSupported;
   int* err = tc_error_word();
   if (!err) return cudaErrorMemoryAllocation;
-  return launch_cluster(cache_attn_mma<DP, I8, Q32, NW>, c.N * c.H * p.chunks * C, C, F::THREADS, F::SMEM, stream, mk,
+  return launch_cluster(cache_attn_mma<DP, I8, MODE, NW>, c.N * c.H * p.chunks * C, C, F::THREADS, F::SMEM, stream, mk,
                         mv, p, err);
 }
 
-template <int DP, bool I8, bool Q32>
+template <int DP, bool I8, int MODE>
 cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
-  const int64_t rmax = Q32 ? 4 : 16, rows = a.S * (a.Hq / a.cache.H);
-  const int64_t items = a.cache.N * a.cache.H * ((rows + rmax - 1) / rmax);
+  const int64_t items = a.cache.N * a.cache.H;
   // Many items: CTAs of two warps, of which an SM holds enough for one wave.
   // Few: four warps, split until the SMs hold their CTAs or a warp would have
   // one step.
-  if (items >= 3 * sm_count()) return launch<DP, I8, Q32, 2>(a, 1, stream);
+  if (items >= 3 * sm_count()) return launch<DP, I8, MODE, 2>(a, 1, stream);
   int C = 1;
-  while (C < kMaxCluster && items * C < 3 * sm_count() && a.cache.T / (2 * C) >= 4 * (I8 ? 32 : 16)) C *= 2;
-  return launch<DP, I8, Q32, 4>(a, C, stream);
+  while (C < kMaxCluster && items * C < 3 * sm_count() && a.cache.T / (2 * C) >= 4 * MmaCfg<DP, I8, MODE, 4>::KB) C *= 2;
+  return launch<DP, I8, MODE, 4>(a, C, stream);
 }
 
 }  // namespace
@@ -549,13 +555,13 @@ bool cache_attention_mma_takes(const CacheAttnArgs& a) {
 }
 
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream) {
-  const bool i8 = a.cache.type == KvType::I8;
-  if (a.cache.D <= 64) {
-    if (a.bf16) return i8 ? by_items<64, true, false>(a, stream) : by_items<64, false, false>(a, stream);
-    return i8 ? by_items<64, true, true>(a, stream) : by_items<64, false, true>(a, stream);
-  }
-  if (a.bf16) return i8 ? by_items<128, true, false>(a, stream) : by_items<128, false, false>(a, stream);
-  return i8 ? by_items<128, true, true>(a, stream) : by_items<128, false, true>(a, stream);
+  const bool i8 = a.cache.type == KvType::I8, wide = a.cache.D > 64, few = a.S * (a.Hq / a.cache.H) <= 8;
+#define SB_BY_TYPE(MODE)                                                                            \
+  (wide ? i8 ? by_items<128, true, MODE>(a, stream) : by_items<128, false, MODE>(a, stream)          \
+   : i8 ? by_items<64, true, MODE>(a, stream)                                                        \
+        : by_items<64, false, MODE>(a, stream))
+  return !a.bf16 ? SB_BY_TYPE(kF32) : few ? SB_BY_TYPE(kRows8) : SB_BY_TYPE(kRows16);
+#undef SB_BY_TYPE
 }
 
 }  // namespace sb

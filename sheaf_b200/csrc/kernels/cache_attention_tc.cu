@@ -811,21 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
       }
-      if (gl * 4 < p.D) {
-        const int row = r0 + i;
-        const unsigned long long drafted = drafted_seen(w, sh.mask[row / p.G]);
-        float y[4] = {acc.x, acc.y, acc.z, acc.w};
-        if (bad)
-          for (int j = 0; j < p.S; ++j)
-            if (drafted >> j & 1ull)
-#pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                const float v = __bfloat162float(((const __nv_bfloat16*)p.v)[(nh * p.T + pos + j) * p.D + gl * 4 + d]);
-                if (!isfinite(v)) y[d] += v;
-              }
-        if (pre <= 0 && !drafted) y[0] = y[1] = y[2] = y[3] = 0.f;
-        store4(p, row_at(p, w, row) + gl * 4, make_float4(y[0], y[1], y[2], y[3]));
-      }
+      finish4(p, w, r0 + i, gl * 4, acc, 1.f, sh.mask, bad);
     }
   }
   cluster_sync();

@@ -163,79 +163,110 @@ __device__ __forceinline__ void store4(const Params& p, int64_t at, float4 y) {
 
 constexpr int kMaxCluster = 8;
 
+// The weights of N partial results with base-2 maxima m: f = 2^(m - max).
+template <int N>
+__device__ __forceinline__ float join_weights(const float* m, float* f) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < N; ++j) mx = fmaxf(mx, m[j]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] = exp2f(m[j] - base);
+  return mx;
+}
+__device__ __forceinline__ void add_scaled(float4& a, const float4& x, float f) {
+  a.x = fmaf(x.x, f, a.x);
+  a.y = fmaf(x.y, f, a.y);
+  a.z = fmaf(x.z, f, a.z);
+  a.w = fmaf(x.w, f, a.w);
+}
+
+// The finished values d .. d + 3 of row r0 + r: o / l, or zeros for a row
+// without keys.  `bad`: drafted bf16 values that are not finite were taken out
+// of the products; they go to the rows that see them.
+__device__ __forceinline__ void finish4(const Params& p, const Place& w, int row, int d, float4 o, float l,
+                                        const unsigned long long* mask, bool bad) {
+  if (d >= p.D) return;
+  const unsigned long long seen = drafted_seen(w, mask[row / p.G]);
+  float y[4] = {o.x / l, o.y / l, o.z / l, o.w / l};
+  if (bad)
+    for (int j = 0; j < p.S; ++j)
+      if (seen >> j & 1ull)
+        for (int i = 0; i < 4; ++i) {
+          const float v = __bfloat162float(((const __nv_bfloat16*)p.v)[(w.nh * p.T + w.pos + j) * p.D + d + i]);
+          if (!isfinite(v)) y[i] += v;
+        }
+  if (w.pre <= 0 && !seen) y[0] = y[1] = y[2] = y[3] = 0.f;
+  store4(p, row_at(p, w, row) + d, make_float4(y[0], y[1], y[2], y[3]));
+}
+
 // The partial results of up to R rows, joined and written: first the NW warps'
 // of a CTA, then the CTAs' of the cluster (rank c finishes every C-th piece of
 // 4 values).  part_o [NW][R][DP], part_m, part_l [NW][R] in shared memory (m:
-// base-2 maximum, l: sum); every thread of the CTA calls, before which the
-// parts were written.  cta_o [R][DP] and cta_ml [2 R] are shared too.  fix(row,
-// d, y) may amend the finished values; a row without keys gets zeros.
-template <int NW, int R, int DP, typename Fix>
+// base-2 maximum, l: sum); every thread of the CTA calls once it has written
+// its parts.  cta_o [R][DP] and cta_ml [2 R] are shared too; s_bad (may be
+// null): see finish4.
+template <int NW, int R, int DP>
 __device__ __forceinline__ void join_and_store(const Params& p, const Place& w, int r0, int rows,
                                                const float* part_o, const float* part_m, const float* part_l,
-                                               float* cta_o, float* cta_ml, const unsigned long long* mask, Fix fix) {
+                                               float* cta_o, float* cta_ml, const unsigned long long* mask,
+                                               const int* s_bad) {
   constexpr int V = DP / 4;
   const int tid = threadIdx.x;
   __syncthreads();
   for (int i = tid; i < rows * V; i += NW * 32) {
     const int r = i / V, d = (i % V) * 4;
-    float m[NW], mx = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int j = 0; j < NW; ++j) mx = fmaxf(mx, m[j] = part_m[j * R + r]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m[NW], f[NW], l = 0.f;
+    float4 x[NW], a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < NW; ++j) {
-      const float f = exp2f(m[j] - base);
-      const float4 x = *(const float4*)(part_o + (j * R + r) * DP + d);
-      a.x = fmaf(x.x, f, a.x);
-      a.y = fmaf(x.y, f, a.y);
-      a.z = fmaf(x.z, f, a.z);
-      a.w = fmaf(x.w, f, a.w);
-      l = fmaf(part_l[j * R + r], f, l);
+      m[j] = part_m[j * R + r];
+      x[j] = *(const float4*)(part_o + (j * R + r) * DP + d);
     }
-    *(float4*)(cta_o + r * DP + d) = a;
-    if (d == 0) cta_ml[r] = mx, cta_ml[R + r] = l;
+    const float mx = join_weights<NW>(m, f);
+#pragma unroll
+    for (int j = 0; j < NW; ++j) {
+      add_scaled(a, x[j], f[j]);
+      l = fmaf(part_l[j * R + r], f[j], l);
+    }
+    if (w.C == 1) {
+      finish4(p, w, r0 + r, d, a, l, mask, s_bad && *s_bad);
+    } else {
+      *(float4*)(cta_o + r * DP + d) = a;
+      if (d == 0) cta_ml[r] = mx, cta_ml[R + r] = l;
+    }
   }
-  if (w.C > 1) tc::cluster_sync();
-  else __syncthreads();
+  if (w.C == 1) return;
+  tc::cluster_sync();
+  int bad = 0;
+  if (s_bad)
+    for (uint32_t c = 0; c < w.C; ++c) {
+      int y;
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(y) : "r"(tc::cluster_addr(s_bad, c)));
+      bad |= y;
+    }
   for (int i = (int)w.rank * NW * 32 + tid; i < rows * V; i += (int)w.C * NW * 32) {
     const int r = i / V, d = (i % V) * 4;
-    float m[kMaxCluster], l[kMaxCluster];
-    float4 x[kMaxCluster];
+    float m[kMaxCluster], l[kMaxCluster], f[kMaxCluster], sum = 0.f;
+    float4 x[kMaxCluster], a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (uint32_t c = 0; c < kMaxCluster; ++c) {
-      m[c] = -INFINITY, l[c] = 0.f, x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+      m[c] = -INFINITY, l[c] = 0.f, x[c] = a;
       if (c < w.C) {
         m[c] = ld_remote(&cta_ml[r], c);
         l[c] = ld_remote(&cta_ml[R + r], c);
         x[c] = ld_remote4(cta_o + r * DP + d, c);
       }
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) mx = fmaxf(mx, m[c]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
+    join_weights<kMaxCluster>(m, f);
 #pragma unroll
     for (int c = 0; c < kMaxCluster; ++c) {
-      const float f = exp2f(m[c] - base);
-      a.x = fmaf(x[c].x, f, a.x);
-      a.y = fmaf(x[c].y, f, a.y);
-      a.z = fmaf(x[c].z, f, a.z);
-      a.w = fmaf(x[c].w, f, a.w);
-      sum = fmaf(l[c], f, sum);
+      add_scaled(a, x[c], f[c]);
+      sum = fmaf(l[c], f[c], sum);
     }
-    if (d < p.D) {
-      const int row = r0 + r;
-      const unsigned long long seen = drafted_seen(w, mask[row / p.G]);
-      float y[4] = {a.x / sum, a.y / sum, a.z / sum, a.w / sum};
-      fix(seen, d, y);
-      if (w.pre <= 0 && !seen) y[0] = y[1] = y[2] = y[3] = 0.f;
-      store4(p, row_at(p, w, row) + d, make_float4(y[0], y[1], y[2], y[3]));
-    }
+    finish4(p, w, r0 + r, d, a, sum, mask, bad);
   }
-  if (w.C > 1) tc::cluster_sync();  // no CTA leaves while another may read its shared memory
+  tc::cluster_sync();  // no CTA leaves while another may read its shared memory
 }
 
 }  // namespace cattn

@@ -909,13 +909,14 @@ bool tc_make_map_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t
 }
 
 bool tc_make_map_rows(CUtensorMap* m, const void* base, bool bytes, uint64_t cols, uint64_t rows, uint64_t outer,
-                      uint32_t box_bytes, uint32_t box_rows) {
+                      uint32_t box_bytes, uint32_t box_rows, uint32_t blocks) {
   auto enc = encode_fn();
-  if (!enc || (box_bytes != 64 && box_bytes != 128)) return false;
-  const uint64_t es = bytes ? 1 : 2;
-  const cuuint64_t d[3] = {cols, rows, outer}, st[2] = {cols * es, rows * cols * es};
-  const cuuint32_t box[3] = {(cuuint32_t)(box_bytes / es), box_rows, 1}, step[3] = {1, 1, 1};
-  return enc(m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)base, d, st, box,
+  const uint64_t es = bytes ? 1 : 2, width = box_bytes / es;
+  if (!enc || (box_bytes != 64 && box_bytes != 128) || !blocks || (blocks > 1 && cols != blocks * width)) return false;
+  const cuuint64_t d[4] = {blocks > 1 ? width : cols, rows, blocks, outer};
+  const cuuint64_t st[3] = {cols * es, blocks > 1 ? (cuuint64_t)box_bytes : cols * es, rows * cols * es};
+  const cuuint32_t box[4] = {(cuuint32_t)width, box_rows, blocks, 1}, step[4] = {1, 1, 1, 1};
+  return enc(m, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, d, st, box,
              step, CU_TENSOR_MAP_INTERLEAVE_NONE,
              box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

@@ -23,9 +23,12 @@ bool tc_make_map_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t
                       const uint64_t* strides_bytes, uint32_t box_rows);
 
 // [outer, rows, cols] with `cols` contiguous, of bf16 or bytes: boxes of 64 or
-// 128 bytes by box_rows rows, swizzled over their width.
+// 128 bytes by box_rows rows, swizzled over their width, as dims {width, rows,
+// column blocks, outer}.  With `blocks` > 1 a box holds that many column blocks
+// one after the other (cols must be whole blocks), else one, and cols need not
+// be whole blocks: then the map has one block of all columns.
 bool tc_make_map_rows(CUtensorMap* m, const void* base, bool bytes, uint64_t cols, uint64_t rows, uint64_t outer,
-                      uint32_t box_bytes, uint32_t box_rows);
+                      uint32_t box_bytes, uint32_t box_rows, uint32_t blocks);
 
 // Device word that every tcgen05 kernel sets when a bounded wait expires.
 int* tc_error_word();
