@@ -10,9 +10,11 @@
 // group; each warp streams pieces of one beam's row and keeps in its lanes the
 // W best of what it has seen as 64-bit keys (order-preserving image of the
 // logit above the complemented index: unique, so equal logits order by index
-// and every step has one answer).  Few values of a piece pass the list's last
-// key; where many do (the first piece) they are first filtered by the W-th best
-// of the 32 lanes' own best keys.  After a cluster barrier CTA r joins the lists
+// and every step has one answer).  The list starts as the W best of the lanes'
+// best keys in the first piece; after that few values pass the best W-th key
+// that any warp of the CTA has for the beam, and they are inserted one by one
+// (a lane offers its next value only if its second largest passes too).  After
+// a cluster barrier CTA r joins the lists
 // of beams r, r + C, .. and sends them to every CTA; after a second one each CTA
 // orders the W x W survivors.  Lists cross CTAs through distributed shared
 // memory, so there is no workspace, no atomic and no second launch.
@@ -38,10 +40,10 @@ constexpr int kSelWarps = 16, kSelThreads = kSelWarps * 32;
 // term 2^-t has a relative error of at most 2^-22 (ex2) + 2^-23.4 t (its
 // argument, two roundings), and terms with t > 32 + log2 of the sum of the
 // others' number are below it; the mean t of the sum's weight is at most
-// log2(V) < 32; 32 terms are added in a tree of depth 5 in f32, the rest in f64:
-// 2^-22 + 32 * 2^-23.4 + 5 * 2^-24 < 4e-6.
+// log2(V) < 32; 16 terms are added in f32 (at most 4 additions each), the rest
+// in f64: 2^-22 + 32 * 2^-23.4 + 4 * 2^-24 < 4e-6.
 constexpr double kFastError = 4e-6;
-constexpr int EPC = 32;              // values per lane and piece
+constexpr int EPC = 16;              // values per lane and piece
 constexpr int kPiece = EPC * 32;     // values per warp and piece
 constexpr int W_MAX = (int)kBeamMax;
 using u64 = unsigned long long;
@@ -121,6 +123,8 @@ __device__ __forceinline__ void load_piece(const void* buf, bool inside, int64_t
 
 struct SelectShared {
   u64 list[kSelWarps][W_MAX];
+  u64 sort[kSelWarps][32];  // a warp's first list
+  u64 bar[W_MAX];           // per beam: a key that W keys of the CTA reach
   double s[kSelWarps];
   float m[kSelWarps];
   // the candidates of every beam, best first (each CTA has them all)
@@ -149,7 +153,7 @@ __device__ __forceinline__ void st_remote32(const void* p, uint32_t rank, uint32
 }
 
 template <bool BF>
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectParams p) {
   pdl_prologue();
   __shared__ SelectShared sh;
   constexpr int N = BF ? 8 : 4;
@@ -168,6 +172,8 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
   const int64_t pieces = (base + p.V - first + kPiece - 1) / kPiece;
   u64 list = 0;
   float m = -INFINITY;
+  if (tid < W_MAX) sh.bar[tid] = 0;
+  __syncthreads();
 
   for (int round = 0;; ++round) {
     double sum = 0.;
@@ -179,9 +185,13 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
 #pragma unroll
         for (int i = 0; i < EPC / N; ++i)
           load_piece<BF>(p.logits, inside, at0 + i * 32 * N, base, p.V, p.total, x + i * N);
-        float mx = x[0];
+        // the lane's two largest values
+        float mx = x[0], m2 = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < EPC; ++i) mx = fmaxf(mx, x[i]);
+        for (int i = 1; i < EPC; ++i) {
+          m2 = fmaxf(m2, fminf(mx, x[i]));
+          mx = fmaxf(mx, x[i]);
+        }
         float wm = mx;
 #pragma unroll
         for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
@@ -189,50 +199,65 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
         if (mn != -INFINITY) {
           if (mn > m) sum *= (double)exp2f((m - mn) * kLog2e);
           m = mn;
-          float e[EPC];
+          float e[8];
 #pragma unroll
-          for (int i = 0; i < EPC; ++i) e[i] = tc::ex2((x[i] - m) * kLog2e);
+          for (int i = 0; i < EPC; ++i) {
+            const float y = tc::ex2((x[i] - m) * kLog2e);
+            e[i % 8] = i < 8 ? y : e[i % 8] + y;
+          }
 #pragma unroll
-          for (int w = EPC / 2; w; w >>= 1)
+          for (int w = 4; w; w >>= 1)
 #pragma unroll
             for (int i = 0; i < w; ++i) e[i] += e[i + w];
           sum += (double)e[0];  // per lane
         }
-        // values that pass the list's last key; -inf passes too while the list is not full
+        // The best that any warp of this CTA has W of for the beam bars the rest.
         u64 bar = shfl64(list, W - 1);
-        const float barf = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+        const u64 shared_bar = shfl64(*(volatile u64*)&sh.bar[beam], 0);
+        if (shared_bar > bar) bar = shared_bar;
+        float barf = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
         if (!__any_sync(0xffffffffu, mx >= barf)) continue;
-        int hits = 0;
+        // the lane's best key: its largest value at the lowest index; then the next ones
+        u64 last = ~0ull;
+        auto next = [&]() {
+          u64 best = 0;
 #pragma unroll
-        for (int i = 0; i < EPC; ++i) hits += x[i] >= barf;
-        if (__reduce_add_sync(0xffffffffu, hits) > 2 * W) {
-          int64_t bi = -1;  // the lane's best key: its largest value at the lowest index
-#pragma unroll
-          for (int i = EPC - 1; i >= 0; --i)
-            if (x[i] == mx) bi = at0 + (i / N) * 32 * N + i % N - base;
-          const u64 best = bi < 0 || bi >= p.V ? 0 : (u64)ordered(mx) << 32 | (uint32_t)~(uint32_t)bi;
+          for (int i = 0; i < EPC; ++i) {
+            const int64_t idx = at0 + (i / N) * 32 * N + i % N - base;
+            if (idx < 0 || idx >= p.V || x[i] < barf) continue;
+            const u64 key = (u64)ordered(x[i]) << 32 | (uint32_t)~(uint32_t)idx;
+            if (key < last && key > best) best = key;
+          }
+          last = best;
+          return best;
+        };
+        u64 key = 0;
+        if (mx >= barf) key = next();
+        if (!shfl64(list, 0)) {
+          // the first piece: the list starts as the W best of the lanes' best keys
+          u64* mine_keys = sh.sort[warp];
+          mine_keys[lane] = key;
+          __syncwarp();
           int ahead = 0;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) ahead += shfl64(best, i) > best;
-          const uint32_t at = __ballot_sync(0xffffffffu, ahead == W - 1);
-          if (at) {
-            const u64 b2 = shfl64(best, __ffs(at) - 1);
-            if (b2 > bar) bar = b2 - 1;  // itself passes
-          }
+          for (int i = 0; i < 32; ++i) ahead += mine_keys[i] > key || (mine_keys[i] == key && i < lane);
+          __syncwarp();
+          mine_keys[ahead] = key;
+          __syncwarp();
+          list = lane < W ? mine_keys[lane] : 0;
+          if (shfl64(list, W - 1) > bar) bar = shfl64(list, W - 1);
+          barf = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
+          if (ahead < W) key = m2 >= barf ? next() : 0;  // that one is in
         }
-        const float pass = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
-#pragma unroll
-        for (int i = 0; i < EPC; ++i) {
-          if (!__any_sync(0xffffffffu, x[i] >= pass)) continue;
-          const int64_t idx = at0 + (i / N) * 32 * N + i % N - base;
-          const u64 key = idx < 0 || idx >= p.V ? 0 : (u64)ordered(x[i]) << 32 | (uint32_t)~(uint32_t)idx;
-          uint32_t hit = __ballot_sync(0xffffffffu, key > bar);
-          while (hit) {
-            const int src = __ffs(hit) - 1;
-            hit &= hit - 1;
-            insert(list, shfl64(key, src), lane, W);
-          }
+        // keys that pass, one by one; a lane whose key went in offers its next
+        for (uint32_t hit; (hit = __ballot_sync(0xffffffffu, key > bar)) != 0;) {
+          const int src = __ffs(hit) - 1;
+          insert(list, shfl64(key, src), lane, W);
+          const u64 b2 = shfl64(list, W - 1);
+          if (b2 > bar) bar = b2, barf = unordered((uint32_t)(bar >> 32));
+          if (lane == src) key = m2 >= barf ? next() : 0;
         }
+        if (lane == 0 && bar > shared_bar) atomicMax(&sh.bar[beam], bar);
       }
       if (lane < W_MAX) sh.list[warp][lane] = lane < W ? list : 0;
     } else if (mine) {  // again, in f64; m is the warp's maximum
@@ -440,11 +465,11 @@ cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
   if (a.G == 0) return cudaSuccess;
   SelectParams p = {a.logits, a.scores, a.finished, a.out_scores, a.out_parents, a.out_tokens, a.out_finished,
                     a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos};
-  // split while the CTAs (one per SM) stay one wave and every warp has a piece
+  // split while the CTAs (two per SM) stay one wave and every warp has two pieces
   const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);
   int dev = 0, sms = 148, C = 1;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  while (C < 8 && a.G * 2 * C <= sms && pieces > C * kSelWarps) C *= 2;
+  while (C < 8 && a.G * 2 * C <= 2 * sms && pieces > 2 * C * kSelWarps) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.G * C));
   cfg.blockDim = dim3(kSelThreads);

@@ -41,15 +41,6 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
-template <>
-__device__ __forceinline__ void load8<int8_t>(const int8_t* p, float* x) {
-  const uint2 a = *(const uint2*)p;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] = (float)(int8_t)(a.x >> (8 * i));
-    x[4 + i] = (float)(int8_t)(a.y >> (8 * i));
-  }
-}
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* x);
@@ -67,9 +58,9 @@ __device__ __forceinline__ void store8<__nv_bfloat16>(__nv_bfloat16* p, const fl
   *(uint4*)p = *(uint4*)h;
 }
 
-// The integer nearest to x / s, ties to even, in exact arithmetic.  The f32
-// quotient is within one step of it; the remainder x - q s is exact in one
-// fma (a multiple of half an ulp of s, below 2^24 of them), so comparing it
+// The integer nearest to x / s, ties to even, in exact arithmetic, |x / s| <= 190.
+// The f32 quotient is within one step of it; the remainder x - q s is exact in
+// one fma (a multiple of half an ulp of s, below 2^24 of them), so comparing it
 // with s / 2 settles the last step.
 __device__ __forceinline__ int nearest_code(float x, float s) {
   float q = rintf(__fdiv_rn(x, s));
@@ -77,6 +68,32 @@ __device__ __forceinline__ int nearest_code(float x, float s) {
   if (r > s || (r == s && ((int)q & 1))) q += 1.f;
   if (r < -s || (r == -s && ((int)q & 1))) q -= 1.f;
   return (int)fminf(fmaxf(q, -127.f), 127.f);
+}
+
+// Codes of 8 values (finite, at most 127 (1 + 2^-24) s) as 8 bytes.  The common
+// way has no division: x (1 / s) is within 2^-15 of x / s, adding 1.5 2^23
+// rounds it to an integer q and leaves q in the sum's low byte, and where the
+// remainder is below s / 2 that q is the nearest.  Any other value of a lane
+// sends its 8 through nearest_code; so does a scale whose reciprocal or half
+// is not normal.
+__device__ __forceinline__ uint2 codes8(const float* x, float s) {
+  const float inv = __frcp_rn(s), half = 0.5f * s;
+  bool sure = s > 1e-36f && s < 1e36f;
+  uint32_t b[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const float y = fmaf(x[i], inv, 12582912.f);
+    b[i] = __float_as_uint(y);
+    sure = sure && fabsf(fmaf(-(y - 12582912.f), s, x[i])) < half;
+  }
+  if (!sure) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) b[i] = s > 0.f ? (uint32_t)nearest_code(x[i], s) : 0u;
+  }
+  uint2 w;
+  w.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  w.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+  return w;
 }
 
 struct WriteParams {
@@ -119,22 +136,25 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const WriteParams p) {
 #pragma unroll
   for (int k = 0; k < RPT; ++k) {
     if constexpr (sizeof(TC) == 1) {
-      float m = 0.f;
+      float m = 0.f, odd = 0.f;  // odd: NaN unless all values are finite
 #pragma unroll
       for (int i = 0; i < EPL; ++i) {
-        x[k][i] = x[k][i] != x[k][i] ? 0.f : fminf(fmaxf(x[k][i], -FLT_MAX), FLT_MAX);
+        odd = fmaf(x[k][i], 0.f, odd);
         m = fmaxf(m, fabsf(x[k][i]));
+      }
+      if (odd != 0.f) {
+        m = 0.f;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          x[k][i] = x[k][i] != x[k][i] ? 0.f : fminf(fmaxf(x[k][i], -FLT_MAX), FLT_MAX);
+          m = fmaxf(m, fabsf(x[k][i]));
+        }
       }
 #pragma unroll
       for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float sc = __fdiv_rn(m, 127.f);
       if (at[k] >= 0) {
-        uint32_t w[2] = {0, 0};
-        if (sc > 0.f) {
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) w[i / 4] |= (uint32_t)(nearest_code(x[k][i], sc) & 255) << (8 * (i % 4));
-        }
-        *(uint2*)((int8_t*)(which[k] ? p.dst[1] : p.dst[0]) + at[k] * p.D + lane * EPL) = make_uint2(w[0], w[1]);
+        *(uint2*)((int8_t*)(which[k] ? p.dst[1] : p.dst[0]) + at[k] * p.D + lane * EPL) = codes8(x[k], sc);
         if (lane == 0) (which[k] ? p.scale[1] : p.scale[0])[at[k]] = sc;
       }
     } else {
@@ -153,47 +173,72 @@ struct ReadParams {
   int H, D;
 };
 
-constexpr int kReadUnits = 4;  // 8-value pieces per thread
+constexpr int kReadUnits = 4;  // 16-byte pieces of the cache per thread
 
 // For one (slot, head) both sides are contiguous: rows i of the output are rows
 // starts[n] + i of the cache, so a block copies a range of pieces and clips it to
-// the rows that exist and are counted.
+// the rows that exist and are counted.  A thread's loads all come first: they
+// are what is under way while the block waits.
 template <typename TC, typename TO>
 __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
   pdl_prologue();
+  constexpr int PV = 16 / sizeof(TC);  // values of a piece
   const unsigned b = blockIdx.x % p.blocks, item = blockIdx.x / p.blocks, which = item & 1, nh = item >> 1;
   const unsigned n = nh / p.H;
   const int64_t start = p.starts ? p.starts[n] : 0;
   const int64_t lo = max((int64_t)0, -start);
   int64_t hi = min(p.S, p.T - start);
   if (p.counts) hi = min(hi, (int64_t)p.counts[n]);
-  const int per = p.D / EPL;
-  const int64_t u0 = (int64_t)b * (kThreads * kReadUnits) + threadIdx.x;
+  const int per = p.D / PV;
+  const int64_t u0 = (int64_t)b * (kThreads * kReadUnits) + threadIdx.x, u_lo = lo * per, u_hi = hi * per;
   const TC* src = (const TC*)(which ? p.src[1] : p.src[0]) + ((int64_t)nh * p.T + start) * p.D;
   TO* dst = (TO*)(which ? p.dst[1] : p.dst[0]) + (int64_t)nh * p.S * p.D;
-  float x[kReadUnits][EPL], s[kReadUnits];
-  bool in[kReadUnits];
+  const float* scale = sizeof(TC) == 1 ? (which ? p.scale[1] : p.scale[0]) + (int64_t)nh * p.T + start : nullptr;
+  uint4 raw[kReadUnits];
+  float s[kReadUnits];
 #pragma unroll
   for (int k = 0; k < kReadUnits; ++k) {
     const int64_t u = u0 + k * kThreads;
-    in[k] = u >= lo * per && u < hi * per;
     s[k] = 1.f;
-    if (in[k]) {
-      load8(src + u * EPL, x[k]);
-      if constexpr (sizeof(TC) == 1) {
-        const int64_t row = u <= UINT32_MAX ? (int64_t)((uint32_t)u / (uint32_t)per) : u / per;
-        s[k] = (which ? p.scale[1] : p.scale[0])[(int64_t)nh * p.T + start + row];
-      }
+    if (u >= u_lo && u < u_hi) {
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(raw[k].x), "=r"(raw[k].y), "=r"(raw[k].z), "=r"(raw[k].w)
+                   : "l"(src + u * PV));
+      if constexpr (sizeof(TC) == 1)
+        s[k] = scale[u <= UINT32_MAX ? (int64_t)((uint32_t)u / (uint32_t)per) : u / per];
     }
   }
 #pragma unroll
   for (int k = 0; k < kReadUnits; ++k) {
-    if (!in[k]) continue;
-    if constexpr (sizeof(TC) == 1) {
+    const int64_t u = u0 + k * kThreads;
+    if (u < u_lo || u >= u_hi) continue;
+    const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+    float x[PV];
 #pragma unroll
-      for (int j = 0; j < EPL; ++j) x[k][j] *= s[k];
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(TC) == 1) {
+        // byte c ^ 0x80 = c + 128 under 2^23, less 2^23 + 128: no conversion instruction
+        const uint32_t y = w[i] ^ 0x80808080u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[4 * i + j] = (__uint_as_float(__byte_perm(y, 0x4b000000u, 0x7440 + j)) - 8388736.f) * s[k];
+      } else if constexpr (sizeof(TC) == 2) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        x[i] = __uint_as_float(w[i]);
+      }
     }
-    store8(dst + (u0 + k * kThreads) * EPL, x[k]);
+    TO* to = dst + u * PV;
+    if constexpr (PV >= 8) {
+#pragma unroll
+      for (int i = 0; i < PV; i += 8) store8(to + i, x + i);
+    } else if constexpr (sizeof(TO) == 4) {
+      *(uint4*)to = raw[k];
+    } else {
+      __nv_bfloat162 h[2] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3])};
+      *(uint2*)to = *(uint2*)h;
+    }
   }
 }
 
@@ -226,7 +271,7 @@ cudaError_t write_rows(const WriteParams& p, int64_t N, cudaStream_t stream) {
 
 template <typename TC, typename TO>
 cudaError_t read_rows(ReadParams p, int64_t N, cudaStream_t stream) {
-  const int64_t units = p.S * (p.D / EPL), blocks = (units + kThreads * kReadUnits - 1) / (kThreads * kReadUnits);
+  const int64_t units = p.S * (p.D * (int64_t)sizeof(TC) / 16), blocks = (units + kThreads * kReadUnits - 1) / (kThreads * kReadUnits);
   if (blocks * 2 * N * p.H > INT32_MAX) return cudaErrorInvalidValue;
   p.blocks = (unsigned)blocks;
   return launch_pdl(read_kernel<TC, TO>, dim3((unsigned)(blocks * 2 * N * p.H)), dim3(kThreads), 0, stream, p);
