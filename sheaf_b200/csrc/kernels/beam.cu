@@ -6,18 +6,19 @@
 //   selected: the W largest of the W x V candidates, by (value, then lowest
 //   w V + v).
 //
-// Reading the logits once bounds the selection.  A cluster of C CTAs carries a
-// group; each warp streams pieces of one beam's row and keeps in its lanes the
-// W best of what it has seen as 64-bit keys (order-preserving image of the
-// logit above the complemented index: unique, so equal logits order by index
-// and every step has one answer).  The list starts as the W best of the lanes'
-// best keys in the first piece; after that few values pass the best W-th key
-// that any warp of the CTA has for the beam, and they are inserted one by one
-// (a lane offers its next value only if its second largest passes too).  After
-// a cluster barrier CTA r joins the lists
-// of beams r, r + C, .. and sends them to every CTA; after a second one each CTA
+// Reading the logits once bounds the selection, so the pass over them does as
+// little as it can: a cluster of C CTAs carries a group, each warp streams
+// pieces of one beam's row, and a lane keeps its largest value, that value's
+// lowest index and its sum of exponentials.  Lanes meet only at the end.  A
+// lane's best is a 64-bit key (order-preserving image of the logit above the
+// complemented index: unique, so equal logits order by index and every step
+// has one answer), and of a beam's W best values none can lie in a lane whose
+// best is not among the W best of all its lanes.  So each warp sends its W best
+// keys; after a cluster barrier CTA r finds the W best of beams r, r + C, ..,
+// reads the few values of those W lanes again (from L2) for others above the
+// W-th, and sends the result to every CTA; after a second barrier each CTA
 // orders the W x W survivors.  Lists cross CTAs through distributed shared
-// memory, so there is no workspace, no atomic and no second launch.
+// memory: no workspace, no atomics on memory and no second launch.
 //
 // Within a beam the order is the logits' own.  Between beams it needs lse.  The
 // first round sums f32 exponentials, off by less than kFastError; if two
@@ -40,10 +41,10 @@ constexpr int kSelWarps = 16, kSelThreads = kSelWarps * 32;
 // term 2^-t has a relative error of at most 2^-22 (ex2) + 2^-23.4 t (its
 // argument, two roundings), and terms with t > 32 + log2 of the sum of the
 // others' number are below it; the mean t of the sum's weight is at most
-// log2(V) < 32; 16 terms are added in f32 (at most 4 additions each), the rest
-// in f64: 2^-22 + 32 * 2^-23.4 + 4 * 2^-24 < 4e-6.
+// log2(V) < 32; 32 terms are added in f32 (at most 9 additions each), the rest
+// in f64: 2^-22 + 32 * 2^-23.4 + 9 * 2^-24 < 4e-6.
 constexpr double kFastError = 4e-6;
-constexpr int EPC = 16;              // values per lane and piece
+constexpr int EPC = 32;              // values per lane and piece
 constexpr int kPiece = EPC * 32;     // values per warp and piece
 constexpr int W_MAX = (int)kBeamMax;
 using u64 = unsigned long long;
@@ -69,14 +70,6 @@ __device__ __forceinline__ float unordered(uint32_t u) {
 }
 __device__ __forceinline__ u64 shfl64(u64 x, int src) { return __shfl_sync(0xffffffffu, x, src); }
 
-// A warp's list: lane j < W holds the j-th largest key, 0 where there is none
-// (every real key is above 0).
-__device__ __forceinline__ void insert(u64& list, u64 key, int lane, int W) {
-  const int rank = __popc(__ballot_sync(0xffffffffu, lane < W && list > key));
-  const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
-  if (lane < W && lane >= rank) list = lane == rank ? key : up;
-}
-
 // The N = 4 (f32) or 8 (bf16) values of a 16-byte load.
 template <bool BF>
 __device__ __forceinline__ void load_vec(const void* buf, int64_t at, float* x) {
@@ -94,8 +87,7 @@ __device__ __forceinline__ void load_vec(const void* buf, int64_t at, float* x) 
 }
 
 // Values at .. at + N - 1 of the logits buffer (at: a multiple of N) where they
-// belong to the row [base, base + V), -inf elsewhere and for NaN.  `inside`: all
-// of them do.  The buffer's last values are loaded one by one where the 16
+// belong to the row [base, base + V), -inf elsewhere.  `inside`: all of them do.  The buffer's last values are loaded one by one where the 16
 // bytes would pass its end.
 template <bool BF>
 __device__ __forceinline__ void load_piece(const void* buf, bool inside, int64_t at, int64_t base, int64_t V,
@@ -117,20 +109,25 @@ __device__ __forceinline__ void load_piece(const void* buf, bool inside, int64_t
     for (int i = 0; i < N; ++i)
       if (at + i < base || at + i >= base + V) x[i] = -INFINITY;
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = fmaxf(x[i], -INFINITY);  // the number of the two
 }
 
 struct SelectShared {
-  u64 list[kSelWarps][W_MAX];
-  u64 sort[kSelWarps][32];  // a warp's first list
-  u64 bar[W_MAX];           // per beam: a key that W keys of the CTA reach
+  u64 list[kSelWarps][W_MAX];  // a warp's best lanes' keys, in order
   double s[kSelWarps];
   float m[kSelWarps];
+  // the beams that this CTA joins: the keys of all their lists, the W best of
+  // them, and the other keys of those lanes that are above the W-th (a warp
+  // ranks its lanes' keys in its part of the pool before that)
+  u64 pool[kSelThreads];
+  u64 top[W_MAX][W_MAX];
+  u64 more[W_MAX][W_MAX * W_MAX];
+  int more_count[W_MAX];
+  double lse[W_MAX];
   // the candidates of every beam, best first (each CTA has them all)
-  double cand[W_MAX][W_MAX];
-  int token[W_MAX][W_MAX];
+  double cand[W_MAX][W_MAX + 1];  // padded: threads read down the columns
+  int token[W_MAX][W_MAX + 1];
   int done[W_MAX];
+  int rank[W_MAX * W_MAX];
   double best[W_MAX + 1];  // the first W + 1 of them, and their beams
   int beam[W_MAX + 1], pick[W_MAX];
 };
@@ -152,9 +149,33 @@ __device__ __forceinline__ void st_remote32(const void* p, uint32_t rank, uint32
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(tc::cluster_addr(p, rank)), "r"(x) : "memory");
 }
 
+// A beam's row in the logits: elements [base, base + V) of the buffer, streamed
+// in pieces from `first`, the 16-byte boundary at or before it.
+struct Row {
+  int64_t base, first, pieces;
+};
 template <bool BF>
-__global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectParams p) {
-  pdl_prologue();
+__device__ __forceinline__ Row row_of(const SelectParams& p, int64_t row) {
+  Row r;
+  r.base = row * p.V;
+  r.first = r.base & ~(int64_t)((BF ? 8 : 4) - 1);
+  r.pieces = (r.base + p.V - r.first + kPiece - 1) / kPiece;
+  return r;
+}
+template <bool BF>
+__device__ __forceinline__ void load_row(const SelectParams& p, const Row& r, int64_t c, int lane, float* x) {
+  constexpr int N = BF ? 8 : 4;
+  const bool inside = r.first + c * kPiece >= r.base && r.first + (c + 1) * kPiece <= r.base + p.V;
+#pragma unroll
+  for (int i = 0; i < EPC / N; ++i)
+    load_piece<BF>(p.logits, inside, r.first + c * kPiece + (i * 32 + lane) * N, r.base, p.V, p.total, x + i * N);
+}
+__device__ __forceinline__ u64 key_of(float x, int64_t idx) {
+  return (u64)ordered(x) << 32 | (uint32_t)~(uint32_t)idx;
+}
+
+template <bool BF>
+__global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectParams p) {
   __shared__ SelectShared sh;
   constexpr int N = BF ? 8 : 4;
   const uint32_t crank = tc::cluster_rank();
@@ -166,205 +187,242 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectPara
   // warps of the cluster per beam; warp `gid` streams every `per`-th piece of its beam
   const int warps = (int)C * kSelWarps, per = warps / W;
   const int gid = (int)crank * kSelWarps + warp, beam = gid / per, sub = gid % per;
+  const Row row = row_of<BF>(p, g * W + min(beam, W - 1));
+  // beams b = crank + q C that this CTA joins, and the keys of one's lists
+  const int joins = (int)crank < W ? (W - 1 - (int)crank) / (int)C + 1 : 0, keys = per * W;
+  pdl_prologue();
+  float x[EPC], y[EPC];
+  if (beam < W && sub < row.pieces) load_row<BF>(p, row, sub, lane, x);
   const bool mine = beam < W && !(p.eos >= 0 && p.finished[g * W + beam]);
-  const int64_t base = (g * W + (mine ? beam : 0)) * p.V;
-  const int64_t first = base - base % N;  // 16-byte boundary at or before the row
-  const int64_t pieces = (base + p.V - first + kPiece - 1) / kPiece;
-  u64 list = 0;
-  float m = -INFINITY;
-  if (tid < W_MAX) sh.bar[tid] = 0;
-  __syncthreads();
+  float wm = -INFINITY;  // the warp's maximum
 
   for (int round = 0;; ++round) {
     double sum = 0.;
-    if (mine && round == 0) {
-      for (int64_t c = sub; c < pieces; c += per) {
-        const int64_t at0 = first + c * kPiece + lane * N;
-        const bool inside = first + c * kPiece >= base && first + (c + 1) * kPiece <= base + p.V;
-        float x[EPC];
+    if (round == 0) {
+      float best = -INFINITY;  // the lane's
+      int at = -1;
+      if (mine) {
+        auto piece = [&](const float* x, int64_t c) {
+          float top = x[0];
 #pragma unroll
-        for (int i = 0; i < EPC / N; ++i)
-          load_piece<BF>(p.logits, inside, at0 + i * 32 * N, base, p.V, p.total, x + i * N);
-        // the lane's two largest values
-        float mx = x[0], m2 = -INFINITY;
+          for (int i = 1; i < EPC; ++i) top = fmaxf(top, x[i]);
+          if (top > best || at < 0) {
+            if (top > best) sum *= (double)tc::ex2((best - top) * kLog2e);
+            const int64_t at0 = row.first + c * kPiece + lane * N - row.base;
+            int found = -1;
+            if (top > -INFINITY) {
 #pragma unroll
-        for (int i = 1; i < EPC; ++i) {
-          m2 = fmaxf(m2, fminf(mx, x[i]));
-          mx = fmaxf(mx, x[i]);
-        }
-        float wm = mx;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-        const float mn = fmaxf(m, wm);
-        if (mn != -INFINITY) {
-          if (mn > m) sum *= (double)exp2f((m - mn) * kLog2e);
-          m = mn;
-          float e[8];
-#pragma unroll
-          for (int i = 0; i < EPC; ++i) {
-            const float y = tc::ex2((x[i] - m) * kLog2e);
-            e[i % 8] = i < 8 ? y : e[i % 8] + y;
+              for (int i = EPC - 1; i >= 0; --i)
+                if (x[i] == top) found = (i / N) * 32 * N + i % N;
+            } else {  // values outside the row are -inf too
+              for (int i = EPC - 1; i >= 0; --i) {
+                const int64_t idx = at0 + (i / N) * 32 * N + i % N;
+                if (idx >= 0 && idx < p.V) found = (i / N) * 32 * N + i % N;
+              }
+            }
+            if (found >= 0) best = top, at = (int)(at0 + found);
           }
+          const float base = best == -INFINITY ? 0.f : best;
+          auto sum_up = [&](bool clean) {
+            float e[4];
 #pragma unroll
-          for (int w = 4; w; w >>= 1)
-#pragma unroll
-            for (int i = 0; i < w; ++i) e[i] += e[i + w];
-          sum += (double)e[0];  // per lane
-        }
-        // The best that any warp of this CTA has W of for the beam bars the rest.
-        u64 bar = shfl64(list, W - 1);
-        const u64 shared_bar = shfl64(*(volatile u64*)&sh.bar[beam], 0);
-        if (shared_bar > bar) bar = shared_bar;
-        float barf = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
-        if (!__any_sync(0xffffffffu, mx >= barf)) continue;
-        // the lane's best key: its largest value at the lowest index; then the next ones
-        u64 last = ~0ull;
-        auto next = [&]() {
-          u64 best = 0;
-#pragma unroll
-          for (int i = 0; i < EPC; ++i) {
-            const int64_t idx = at0 + (i / N) * 32 * N + i % N - base;
-            if (idx < 0 || idx >= p.V || x[i] < barf) continue;
-            const u64 key = (u64)ordered(x[i]) << 32 | (uint32_t)~(uint32_t)idx;
-            if (key < last && key > best) best = key;
-          }
-          last = best;
-          return best;
+            for (int i = 0; i < EPC; ++i) {
+              const float v = tc::ex2(((clean ? fmaxf(x[i], -INFINITY) : x[i]) - base) * kLog2e);
+              e[i % 4] = i < 4 ? v : e[i % 4] + v;
+            }
+            return (e[0] + e[1]) + (e[2] + e[3]);
+          };
+          float s = sum_up(false);
+          if (s != s) s = sum_up(true);  // NaN counts as -inf (a sum that stays NaN has an infinity)
+          sum += (double)s;
         };
-        u64 key = 0;
-        if (mx >= barf) key = next();
-        if (!shfl64(list, 0)) {
-          // the first piece: the list starts as the W best of the lanes' best keys
-          u64* mine_keys = sh.sort[warp];
-          mine_keys[lane] = key;
-          __syncwarp();
-          int ahead = 0;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) ahead += mine_keys[i] > key || (mine_keys[i] == key && i < lane);
-          __syncwarp();
-          mine_keys[ahead] = key;
-          __syncwarp();
-          list = lane < W ? mine_keys[lane] : 0;
-          if (shfl64(list, W - 1) > bar) bar = shfl64(list, W - 1);
-          barf = bar ? unordered((uint32_t)(bar >> 32)) : -INFINITY;
-          if (ahead < W) key = m2 >= barf ? next() : 0;  // that one is in
+        for (int64_t c = sub; c < row.pieces; c += 2 * per) {  // the next piece is under way during one
+          if (c + per < row.pieces) load_row<BF>(p, row, c + per, lane, y);
+          piece(x, c);
+          if (c + per >= row.pieces) break;
+          if (c + 2 * per < row.pieces) load_row<BF>(p, row, c + 2 * per, lane, x);
+          piece(y, c + per);
         }
-        // keys that pass, one by one; a lane whose key went in offers its next
-        for (uint32_t hit; (hit = __ballot_sync(0xffffffffu, key > bar)) != 0;) {
-          const int src = __ffs(hit) - 1;
-          insert(list, shfl64(key, src), lane, W);
-          const u64 b2 = shfl64(list, W - 1);
-          if (b2 > bar) bar = b2, barf = unordered((uint32_t)(bar >> 32));
-          if (lane == src) key = m2 >= barf ? next() : 0;
-        }
-        if (lane == 0 && bar > shared_bar) atomicMax(&sh.bar[beam], bar);
       }
-      if (lane < W_MAX) sh.list[warp][lane] = lane < W ? list : 0;
-    } else if (mine) {  // again, in f64; m is the warp's maximum
-      for (int64_t c = sub; c < pieces; c += per) {
-        const int64_t at0 = first + c * kPiece + lane * N;
+      wm = best;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+      if (best != -INFINITY) sum *= (double)tc::ex2((best - wm) * kLog2e);
+      // the W best of the lanes' keys, in order
+      const u64 key = at < 0 ? 0 : key_of(best, at);
+      sh.pool[tid] = key;
+      __syncwarp();
+      int ahead = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const u64 k = sh.pool[warp * 32 + i];
+        ahead += k > key || (k == key && i < lane);
+      }
+      if (ahead < W) sh.list[warp][ahead] = key;
+    } else if (mine && wm != -INFINITY) {  // again, in f64
+#pragma unroll 1
+      for (int64_t c = sub; c < row.pieces; c += per) {
 #pragma unroll 1
         for (int i = 0; i < EPC / N; ++i) {
           float x[N];
-          load_piece<BF>(p.logits, false, at0 + i * 32 * N, base, p.V, p.total, x);
-          if (m != -INFINITY)
+          load_piece<BF>(p.logits, false, row.first + c * kPiece + (i * 32 + lane) * N, row.base, p.V, p.total, x);
 #pragma unroll
-            for (int k = 0; k < N; ++k) sum += exp((double)x[k] - (double)m);
+          for (int k = 0; k < N; ++k) sum += exp((double)fmaxf(x[k], -INFINITY) - (double)wm);
         }
       }
-    } else if (round == 0 && lane < W_MAX) {
-      sh.list[warp][lane] = 0;
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sh.m[warp] = m, sh.s[warp] = sum;
+    if (lane == 0) sh.m[warp] = wm, sh.s[warp] = sum;
     tc::cluster_sync();
 
-    // CTA r joins beams r, r + C, ..: one warp each
-    for (int b = (int)crank + (int)C * warp; b < W; b += (int)C * kSelWarps) {
-      u64 best = 0;
+    // CTA r joins beams r, r + C, ..
+    if (round == 0) {
+      if (tid < joins * keys) {
+        const int q = tid / keys, k = tid - q * keys, id = ((int)crank + q * (int)C) * per + k / W;
+        sh.pool[tid] = ld_remote64(&sh.list[id % kSelWarps][k % W], id / kSelWarps);
+      }
+      if (tid < W_MAX) sh.more_count[tid] = 0;
+      if (tid < W_MAX * W_MAX) (&sh.top[0][0])[tid] = 0;
+    }
+    for (int q = kSelWarps - 1 - warp; q < joins; q += kSelWarps) {  // the sums, by the last warps
+      const int b = (int)crank + q * (int)C;
       float pm = -INFINITY;  // lane k (and k + 32, ..): the parts of the sum
       double ps = 0.;
-      for (int k0 = 0; k0 < per; k0 += 8) {
-        u64 part[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int id = b * per + k0 + k;
-          part[k] = k0 + k < per && lane < W ? ld_remote64(&sh.list[id % kSelWarps][lane], id / kSelWarps) : 0;
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (k0 + k == 0) {
-            best = part[k];
-            continue;
-          }
-          for (int j = 0; j < W; ++j) {  // sorted: stop at the first that does not get in
-            const u64 key = shfl64(part[k], j);
-            if (key <= shfl64(best, W - 1)) break;
-            insert(best, key, lane, W);
-          }
-        }
-      }
       for (int k = lane; k < per; k += 32) {
         const int id = b * per + k;
         const float m2 = ld_remote_f(&sh.m[id % kSelWarps], id / kSelWarps);
         const double s2 = __longlong_as_double((long long)ld_remote64(&sh.s[id % kSelWarps], id / kSelWarps));
         const float mx = fmaxf(pm, m2);
         if (mx != -INFINITY) {
-          ps = ps * exp((double)pm - (double)mx) + s2 * exp((double)m2 - (double)mx);
+          ps = ps * (round ? exp((double)pm - (double)mx) : (double)tc::ex2((pm - mx) * kLog2e)) +
+               s2 * (round ? exp((double)m2 - (double)mx) : (double)tc::ex2((m2 - mx) * kLog2e));
           pm = mx;
         }
       }
       float top = pm;
 #pragma unroll
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      ps = pm == -INFINITY ? 0. : ps * exp((double)pm - (double)top);
+      ps = pm == -INFINITY ? 0. : ps * (round ? exp((double)pm - (double)top) : (double)tc::ex2((pm - top) * kLog2e));
 #pragma unroll
       for (int o = 16; o; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-      const float score = p.scores[g * W + b];
-      const bool fin = p.eos >= 0 && p.finished[g * W + b];
-      const double lse = (double)top + log(ps);
-      const int have = (int)min((int64_t)W, p.V);
-      double value = -INFINITY;
-      int token = lane;
-      if (isfinite(score) && fin) {
-        // the end token alone, then the others from the lowest
-        value = lane == 0 ? (double)score : -INFINITY;
-        token = lane == 0 ? p.eos : lane - 1 + (lane - 1 >= p.eos);
-      } else if (isfinite(score) && isfinite(lse)) {
-        token = (int)~(uint32_t)best;
-        value = (double)score + ((double)unordered((uint32_t)(best >> 32)) - lse);
+      if (lane == 0) sh.lse[q] = (double)top + log(ps);
+    }
+    __syncthreads();
+    if (round == 0) {
+      // the W best of a beam's keys: each key counts those above it, four lanes a key
+      for (int i0 = 0; i0 < 4 * joins * keys; i0 += kSelThreads) {
+        const int i = i0 + tid, k = min(i >> 2, joins * keys - 1), q = k / keys;
+        const u64 key = sh.pool[k], *pool = sh.pool + q * keys;
+        int ahead = 0;
+#pragma unroll 8
+        for (int j = tid & 3; j < keys; j += 4) ahead += pool[j] > key;
+        ahead += __shfl_xor_sync(0xffffffffu, ahead, 1);
+        ahead += __shfl_xor_sync(0xffffffffu, ahead, 2);
+        if (key && ahead < W && !(i & 3) && i < 4 * joins * keys) sh.top[q][ahead] = key;
       }
-      if (lane < W) {
-        if (lane >= have) value = -INFINITY, token = -1;  // no such candidate
-        for (uint32_t c = 0; c < C; ++c) {
-          st_remote64(&sh.cand[b][lane], c, (u64)__double_as_longlong(value));
-          st_remote32(&sh.token[b][lane], c, (uint32_t)token);
-          if (lane == 0) st_remote32(&sh.done[b], c, fin ? 1u : 0u);
+      __syncthreads();
+      // other values of those lanes: the 16-byte loads of the lane that holds the j-th key, 32 at a time
+      for (int e = warp; e < joins * W; e += kSelWarps) {
+        const int q = e / W;
+        const u64 key = sh.top[q][e - q * W], bar = sh.top[q][W - 1];
+        if (!key) continue;
+        const Row r = row_of<BF>(p, g * W + (int)crank + q * (int)C);
+        const int64_t where = r.base - r.first + (uint32_t)~(uint32_t)key, piece = where / kPiece;
+        const int sub2 = (int)(piece % per), lane2 = (int)(where - piece * kPiece) / N % 32;
+        const int64_t loads = ((r.pieces - sub2 + per - 1) / per) * (EPC / N);
+        u64 list = 0;  // lane j < W: the j-th best, for a beam with more than W of them in this lane
+        for (int64_t v0 = 0; v0 < loads; v0 += 32) {
+          const int64_t v = v0 + lane;
+          const int64_t at = r.first + (sub2 + v / (EPC / N) * per) * kPiece + (v % (EPC / N) * 32 + lane2) * N;
+          float z[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) z[k] = -INFINITY;
+          if (v < loads)
+            load_piece<BF>(p.logits, at >= r.base && at + N <= r.base + p.V, at, r.base, p.V, p.total, z);
+          u64 k2[N];
+          bool any = false;
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const int64_t idx = at + k - r.base;
+            k2[k] = v < loads && idx >= 0 && idx < p.V ? key_of(fmaxf(z[k], -INFINITY), idx) : 0;
+            if (k2[k] == key || k2[k] <= bar) k2[k] = 0;
+            any |= k2[k] != 0;
+          }
+          if (!__any_sync(0xffffffffu, any)) continue;
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            for (uint32_t hit = __ballot_sync(0xffffffffu, k2[k] != 0); hit; hit &= hit - 1) {
+              const u64 in = shfl64(k2[k], __ffs(hit) - 1);
+              const int place = __popc(__ballot_sync(0xffffffffu, lane < W && list > in));
+              const u64 up = __shfl_up_sync(0xffffffffu, list, 1);
+              if (lane < W && lane >= place) list = lane == place ? in : up;
+            }
         }
+        if (lane < W && list) sh.more[q][atomicAdd(&sh.more_count[q], 1)] = list;
+      }
+    }
+    __syncthreads();
+    // the W best of both, as candidates, to every CTA
+    const int per_beam = W + W * W;
+    for (int i = tid; i < joins * per_beam; i += kSelThreads) {
+      const int q = i / per_beam, k = i - q * per_beam, b = (int)crank + q * (int)C, n = sh.more_count[q];
+      if (k >= W + n) continue;
+      const float score = p.scores[g * W + b];
+      const bool fin = p.eos >= 0 && p.finished[g * W + b], exists = k < p.V;
+      double value = -INFINITY;
+      int token = exists ? k : -1, place = k;
+      if (!isfinite(score) || (!fin && !isfinite(sh.lse[q]))) {
+        // no candidate is better than another: the lowest tokens
+        if (k >= W) continue;
+      } else if (fin) {
+        // the end token alone, then the others from the lowest
+        if (k >= W) continue;
+        if (k == 0) value = score;
+        if (exists) token = k == 0 ? p.eos : k - 1 + (k - 1 >= p.eos);
+      } else {
+        const u64 key = k < W ? sh.top[q][k] : sh.more[q][k - W];
+        place = 0;
+        for (int j = 0; j < W; ++j) place += sh.top[q][j] > key;
+        for (int j = 0; j < n; ++j) place += sh.more[q][j] > key;
+        if (!key) {  // fewer than W values: the places behind the last
+          if (k < W && exists) continue;
+          place = k;
+          token = -1;
+        } else {
+          token = (int)~(uint32_t)key;
+          value = (double)score + ((double)unordered((uint32_t)(key >> 32)) - sh.lse[q]);
+        }
+      }
+      if (place >= W) continue;
+      for (uint32_t c = 0; c < C; ++c) {
+        st_remote64(&sh.cand[b][place], c, (u64)__double_as_longlong(value));
+        st_remote32(&sh.token[b][place], c, (uint32_t)token);
+        if (place == 0) st_remote32(&sh.done[b], c, fin ? 1u : 0u);
       }
     }
     if (tid <= W) sh.beam[tid] = -1;
+    for (int i = tid; i < W * W; i += kSelThreads) sh.rank[i] = i % W;  // a survivor's place in its own list
     tc::cluster_sync();
-    // rank of each survivor: its place in its own list, and in every other by
-    // bisection (among equals the lower beam comes first)
-    for (int i = tid; i < W * W; i += kSelThreads) {
-      const int b = i / W, j = i % W, tok = sh.token[b][j];
-      if (tok < 0) continue;
+    // plus those ahead of it in every other list (among equals the lower beam comes first)
+    for (int i = tid; i < W * W * W; i += kSelThreads) {
+      const int s = i / W, b2 = i - s * W, b = s / W, j = s - b * W;
+      if (b2 == b || sh.token[b][j] < 0) continue;
       const double v = sh.cand[b][j];
-      int rank = j;
-      for (int b2 = 0; b2 < W; ++b2) {
-        if (b2 == b) continue;
-        int n = 0;
-#pragma unroll
-        for (int step = W_MAX; step; step >>= 1)
-          if (n + step <= W && sh.token[b2][n + step - 1] >= 0 &&
-              (sh.cand[b2][n + step - 1] > v || (sh.cand[b2][n + step - 1] == v && b2 < b)))
-            n += step;
-        rank += n;
+      int n = 0;
+#pragma unroll 8
+      for (int k = 0; k < W; ++k) {
+        const double v2 = sh.cand[b2][k];
+        n += sh.token[b2][k] >= 0 && (v2 > v || (v2 == v && b2 < b));
       }
-      if (rank <= W) sh.best[rank] = v, sh.beam[rank] = b;
-      if (rank < W) sh.pick[rank] = tok;
+      if (n) atomicAdd(&sh.rank[s], n);
+    }
+    __syncthreads();
+    for (int i = tid; i < W * W; i += kSelThreads) {
+      const int b = i / W, j = i - b * W, rank = sh.rank[i];
+      if (sh.token[b][j] < 0 || rank > W) continue;
+      sh.best[rank] = sh.cand[b][j], sh.beam[rank] = b;
+      if (rank < W) sh.pick[rank] = sh.token[b][j];
     }
     __syncthreads();
     bool close = false;
@@ -465,11 +523,11 @@ cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
   if (a.G == 0) return cudaSuccess;
   SelectParams p = {a.logits, a.scores, a.finished, a.out_scores, a.out_parents, a.out_tokens, a.out_finished,
                     a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos};
-  // split while the CTAs (two per SM) stay one wave and every warp has two pieces
+  // one CTA fits an SM: split while the CTAs stay one wave and a warp has a piece
   const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);
   int dev = 0, sms = 148, C = 1;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  while (C < 8 && a.G * 2 * C <= 2 * sms && pieces > 2 * C * kSelWarps) C *= 2;
+  while (C < 8 && a.G * 2 * C <= sms && pieces > C * kSelWarps) C *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.G * C));
   cfg.blockDim = dim3(kSelThreads);

@@ -415,12 +415,12 @@ def check_select(sess, logits, scores, fin, eos, kind="f32"):
     assert np.array_equal(tok.to_host(), ref[2])
     # The sums of f32 exponentials: a term 2^-t is off by 2^-22 (exp2) + 2^-23.4 t
     # of itself (its argument's two roundings); t weighted by 2^-t averages at
-    # most log2(V) < 17 here; a term passes at most 5 f32 additions:
-    # 2^-22 + 17 * 2^-23.4 + 5 * 2^-24 < 2.1e-6, and the value is rounded once.
+    # most log2(V) < 17 here; a term passes at most 9 f32 additions:
+    # 2^-22 + 17 * 2^-23.4 + 9 * 2^-24 < 2.4e-6, and the value is rounded once.
     got = sc.to_host().astype(np.float64)
     same = got == ref[0]
     with np.errstate(invalid="ignore"):
-        assert (same | (np.abs(got - ref[0]) <= U32 * np.abs(ref[0]) + 2.1e-6)).all()
+        assert (same | (np.abs(got - ref[0]) <= U32 * np.abs(ref[0]) + 2.4e-6)).all()
 
 
 @pytest.mark.gpu
