@@ -30,8 +30,6 @@
 //
 // int8 codes become f16 exactly (see codes below), and Q and P are f16 there
 // too; key scales multiply S, value scales P.
-#include <cuda_fp16.h>
-
 #include "cache_attn.h"
 
 namespace sb {
@@ -56,37 +54,6 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two f32 rounded to packed bf16 or f16, and what the rounding left of them.
-template <bool F16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t d;
-  if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-template <bool F16>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-  if (F16) return __half22float2(*(const __half2*)&w);
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <bool F16>
-__device__ __forceinline__ uint32_t take2(float& lo, float& hi) {
-  const uint32_t w = pack2<F16>(lo, hi);
-  const float2 f = unpack2<F16>(w);
-  lo -= f.x;
-  hi -= f.y;
-  return w;
-}
-
-// Codes c in bytes 0 and 2 of t (bytes 1 and 3: anything) to two f16 values.
-// 0x6400 + (c + 128) is 1024 + c + 128 as f16 (steps of 1 there): c exactly,
-// after a subtraction.  (bf16 has no steps of 1 beyond 8 bits and would need
-// twice the instructions, which bound the int8 kernel.)
-__device__ __forceinline__ uint32_t codes(uint32_t t) {
-  const uint32_t a = (t & 0x00ff00ffu) ^ 0x64806480u;
-  __half2 x = __hsub2(*(const __half2*)&a, __half2half2(__ushort_as_half(0x6480)));
-  return *(uint32_t*)&x;
-}
 // (c + 128) 2^-24, a subnormal f16, in one instruction: for the first product,
 // where sum q (c + 128) - 128 sum q costs one or two of 24 bits.
 __device__ __forceinline__ uint32_t codes_plus_128(uint32_t t) { return (t & 0x00ff00ffu) ^ 0x00800080u; }
@@ -246,8 +213,7 @@ uint8_t* dst = ring + st * F::STAGE;
 
   // Q: k-step s takes values d .. d + 3 of the lane's EK, as the pairs of an
   // int8 word (bytes 0 and 2, bytes 1 and 3) or of consecutive bf16 values.
-  // For f16 a row is scaled by a power of two to a largest value in [2^14,
-  // 2^15), which keeps what is 2^-38 of it; S is multiplied back by `fs`.
+  // For f16 a row is scaled (f16_row_scale); S is multiplied back by `fs`.
   uint32_t q[DP / 16][4];
   float fs[NR], sum_q[NR];
 #pragma unroll
@@ -263,10 +229,9 @@ uint8_t* dst = ring + st * F::STAGE;
         for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(y[r][s][i]));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // 2^(14 - e) for a largest value of exponent e, within f32's normal range
-      const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -110), 127);
-      up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-      fs[r] = p.scale2 * __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+      float down;
+      up = f16_row_scale(big, down);
+      fs[r] = p.scale2 * down;
     }
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
@@ -310,7 +275,7 @@ uint8_t* dst = ring + st * F::STAGE;
   for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.f;
 
   const int kg = key_of<RB>(g), kc[2] = {key_of<RB>(2 * c), key_of<RB>(2 * c + 1)};
-  int st = 0, vref = -100;
+  int st = 0, vref = kVrefFirst;
   uint32_t phase = 0;
   float vdown = 0.f;
   for (; t0 < hi; t0 += STRIDE) {
@@ -398,15 +363,10 @@ uint8_t* dst = ring + st * F::STAGE;
       }
     }
     if (I8) {
-      // P times the value scales goes into f16 relative to 2^vref, above the
-      // largest scale so far: at most 2^(8 + 6), with steps of 2^-30 below 1
-      int e = -125;
+      int e = kVrefFirst;
 #pragma unroll
-      for (int i = 0; i < KB / 32; ++i) {
-        const float mine = fabsf(sc[KB + i * 32 + lane]);
-        if (mine < INFINITY) e = max(e, (int)(__float_as_uint(mine) >> 23) - 126);
-      }
-      const int top = max(__reduce_max_sync(0xffffffffu, e), -100);
+      for (int i = 0; i < KB / 32; ++i) e = max(e, scale_exponent(sc[KB + i * 32 + lane]));
+      const int top = __reduce_max_sync(0xffffffffu, e);
       if (top > vref) {
         const float f = tc::ex2((float)(vref - top));
 #pragma unroll
@@ -414,7 +374,7 @@ uint8_t* dst = ring + st * F::STAGE;
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[j][i] *= f;
         vref = top;
-        vdown = __uint_as_float((uint32_t)(127 + 6 - vref) << 23);
+        vdown = vref_down(vref);
       }
     }
     uint32_t a[KG][4];
@@ -497,7 +457,7 @@ uint8_t* dst = ring + st * F::STAGE;
   __syncthreads();  // every warp has read its last stage: the memory takes the partial outputs
 
   // the warp's parts: row, and columns 2c, 2c + 1 of block (j, e) = value (2c) EV + e of load j
-  const float vup = __uint_as_float((uint32_t)(127 - 6 + vref) << 23);
+  const float vup = vref_up(vref);
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -551,17 +511,19 @@ cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
 
 bool cache_attention_mma_takes(const CacheAttnArgs& a) {
   return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 &&
-         a.S * (a.Hq / a.cache.H) <= (a.bf16 ? 16 : 4);
+         a.S * (a.Hq / a.cache.H) <= (!a.bf16 ? 4 : a.cache.type == KvType::I8 ? 16 : 8);
 }
 
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream) {
-  const bool i8 = a.cache.type == KvType::I8, wide = a.cache.D > 64, few = a.S * (a.Hq / a.cache.H) <= 8;
-#define SB_BY_TYPE(MODE)                                                                            \
-  (wide ? i8 ? by_items<128, true, MODE>(a, stream) : by_items<128, false, MODE>(a, stream)          \
-   : i8 ? by_items<64, true, MODE>(a, stream)                                                        \
-        : by_items<64, false, MODE>(a, stream))
-  return !a.bf16 ? SB_BY_TYPE(kF32) : few ? SB_BY_TYPE(kRows8) : SB_BY_TYPE(kRows16);
-#undef SB_BY_TYPE
+  const bool i8 = a.cache.type == KvType::I8, wide = a.cache.D > 64;
+  if (!a.bf16) {
+    if (i8) return wide ? by_items<128, true, kF32>(a, stream) : by_items<64, true, kF32>(a, stream);
+    return wide ? by_items<128, false, kF32>(a, stream) : by_items<64, false, kF32>(a, stream);
+  }
+  if (a.S * (a.Hq / a.cache.H) > 8)  // int8 only
+    return wide ? by_items<128, true, kRows16>(a, stream) : by_items<64, true, kRows16>(a, stream);
+  if (i8) return wide ? by_items<128, true, kRows8>(a, stream) : by_items<64, true, kRows8>(a, stream);
+  return wide ? by_items<128, false, kRows8>(a, stream) : by_items<64, false, kRows8>(a, stream);
 }
 
 }  // namespace sb

@@ -15,20 +15,21 @@
 // roles: 8 softmax, 4 loading, 2 issuing the MMAs (one thread needs about 80
 // cycles per tcgen05.mma, more than the 64 that one takes), 2 helpers.
 //
-//   S = Q K^T   bf16 operands.  f32 queries are split exactly into three bf16
-//               parts (8 mantissa bits each) whose products accumulate into
-//               the same f32 S, so S has f32 accuracy; cache values are bf16
-//               or int8 codes, which bf16 holds exactly.
+//   S = Q K^T   f32 queries are split exactly into three bf16 (f16) parts whose
+//               products accumulate into the same f32 S, so S has f32 accuracy.
+//               For int8 caches all operands are f16, which holds codes exactly
+//               and takes half the instructions to make from them.  S has two
+//               buffers: the tensor cores form the next one during the softmax.
 //   P           exp2(S - m) times the value row's int8 scale, written back over
-//               S in TMEM as bf16 (bf16 output: one rounding, as large as the
-//               output's own) or as three bf16 parts (f32 output: f32 accuracy;
-//               two parts would leave 2^-16 of each probability).
+//               S in TMEM as bf16 or f16 (bf16 output: one rounding, as large as
+//               the output's own) or as three parts (f32 output: f32 accuracy;
+//               two bf16 parts would leave 2^-16 of each probability).
 //   O += P V    the maximum m a row refers to moves only when it would grow by
 //               more than 2^8, so O is rescaled in the first tiles and then
 //               hardly ever; exact since P, O and the sum l share m.
 //
-// bf16 tiles arrive by TMA, int8 tiles through registers (codes to bf16 on the
-// way to swizzled shared memory).  Rows of V behind the last token are zeroed
+// bf16 tiles arrive by TMA, int8 tiles by bulk copies and a conversion in shared
+// memory.  Rows of V behind the last token are zeroed
 // (0 x NaN would reach every row); a value of a drafted token that is not
 // finite is taken out of the tile and added to the rows that attend to it when
 // the outputs are joined.
@@ -49,26 +50,37 @@ using namespace tc;
 // and the softmax warps stage the queries
 constexpr int kSoftWarps = 8, kLoadWarps = 4, kMmaWarp = 12, kWarps = 16, kThreads = kWarps * 32;
 constexpr int kStageWarps = kWarps - kLoadWarps - 2;
-// Registers per thread of the four warpgroups: 2 softmax, loading, the rest.
-// They add up to the launch's 4 x 128.
-constexpr int kRegsSoft = 168, kRegsLoad = 104, kRegsRest = 72, kRegsLaunch = 128;
-static_assert(2 * kRegsSoft + kRegsLoad + kRegsRest == 4 * kRegsLaunch, "register shares");
-template <int N>
-__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr int kLoadThreads = kLoadWarps * 32;
-constexpr int NS = 2;   // K and V tiles in flight
-constexpr int NSC = 4;  // rows of scales in flight (see the loader)
+constexpr int BN = 64;  // keys of a tile
 constexpr float kLazy = 8.f;  // a row's maximum moves when it would grow by more than this (log2)
 
-// D (TMEM) (+)= A (TMEM, bf16 pairs: lane = row, column = two k) * B.
-__device__ __forceinline__ void mma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+// MMAs and commits issued by one elected lane of a converged warp: the operands
+// stay in uniform registers.  (Issued from a branch that one lane takes, each
+// MMA cost about 95 cycles.)
+__device__ __forceinline__ void mma_ss(uint32_t tmem_d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// A in TMEM: 16-bit pairs, lane = row, column = two k.
+__device__ __forceinline__ void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
       "r"(tmem_a), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
       : "memory");
 }
 
@@ -120,30 +132,17 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
-// (lo, hi) f32 to packed bf16, rounded to nearest even
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
+// 16 codes to 16 f16 values; of four codes in a row the middle two change places.
+__device__ __forceinline__ void codes_to_f16(const uint4& c, uint4* out) {
+  out[0] = make_uint4(codes(c.x), codes(c.x >> 8), codes(c.y), codes(c.y >> 8));
+  out[1] = make_uint4(codes(c.z), codes(c.z >> 8), codes(c.w), codes(c.w >> 8));
 }
-__device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// 16 codes to 16 bf16 values.  A code's low 7 bits and its sign bit, each put
-// under the exponent of 128 (bf16 steps of 1 from 128 to 256), differ by the
-// code: (128 + low) - (128 or 256) = code, exactly.
-__device__ __forceinline__ void codes_to_bf16(const uint4& c, uint4* out) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  uint32_t o[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t t = __byte_perm(w[i / 2], 0, i & 1 ? 0x4342 : 0x4140);
-    const uint32_t a = (t & 0x007f007fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
-    __nv_bfloat162 x = __hsub2(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
-    o[i] = *(uint32_t*)&x;
-  }
-  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+// kind::f16 instruction descriptor: D f32, A and B both bf16 or both f16,
+// transpose bits, N>>3, M>>4.
+__host__ __device__ constexpr uint32_t idesc_16(bool f16, int M, int N, int a_mn, int b_mn) {
+  return (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
 // 16-byte unit u (of 8 per 128-byte row and 64-value chunk) of row r in a
@@ -154,39 +153,56 @@ __device__ __forceinline__ uint32_t unit_at(int rows, int r, int unit) {
 
 __device__ __forceinline__ void loaders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kLoadThreads) : "memory"); }
 
-template <int DP, int BN, int QP>
+// One contiguous piece of global memory to shared memory; both addresses and
+// the size are multiples of 16.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int DP, int QP, bool I8>
 struct Cfg {
   static constexpr int MAXR = QP == 3 && DP == 128 ? 128 : 256;  // query rows of a CTA
+  static constexpr int SB = QP == 3 && DP == 128 ? 1 : 2;        // buffers of S per stream
   static constexpr int QTILE = 128 * DP * 2;                     // one part of 128 rows
   static constexpr int Q_BYTES = (MAXR / 128) * QP * QTILE;
   static constexpr int TILE = BN * DP * 2;
-  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NS * TILE, END = V_OFF + NS * TILE;
+  static constexpr int NS = QP == 3 && DP == 128 ? 2 : I8 ? 3 : 4;  // K and V tiles in flight
+  static constexpr int NSC = 2 * NS;                       // rows of scales in flight (see the loader)
+  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NS * TILE, RAW_OFF = V_OFF + NS * TILE;
+  static constexpr int NR = 3, RAW = 2 * BN * DP, END = RAW_OFF + (I8 ? NR * RAW : 0);  // int8 tiles as they arrive
   static constexpr int LDO = DP + 4;  // padded row of the joined outputs, f32
   static constexpr int JOIN = 256 * LDO * 4;
   static constexpr int SMEM = END > JOIN ? END : JOIN;
   static constexpr uint32_t COLS = 512;
   // S (P's first two parts in place), O, P's third part; two streams each
-  static constexpr uint32_t S_COL = 0, O_COL = 2 * BN, T_COL = O_COL + 2 * DP;
-  static_assert(2 * BN + 2 * DP + (QP == 3 ? BN : 0) <= 512, "TMEM columns");
+  static constexpr uint32_t S_COL = 0, O_COL = 2 * SB * BN, T_COL = O_COL + 2 * DP;
+  static_assert(T_COL + (QP == 3 ? SB * BN : 0) <= 512, "TMEM columns");
 };
 
 struct Shared {
-  uint64_t k_full[NS], k_free[NS], v_full[NS], v_free[NS], sc_full[NSC], s_bar[2], p_bar[2], o_bar[2], raw, q_bar;
+  uint64_t k_full[4], k_free[4], v_full[4], v_free[4], sc_full[8], s_bar[2][2], p_bar[2][2], o_bar[2], raw, q_bar, raw_full[3], raw_free[3];
   uint32_t tslot;
   volatile int abort_flag;
   int bad;  // a drafted value that is not finite was taken out of a tile
+  int sc_ref[8];  // exponent that a tile's value scales are relative to
   unsigned long long mask[kKvMaxTokens];
   int jump[kKvMaxTokens];
-  float m[256], l[256];
+  float qs[256];                // what undoes the scaling of a query row (f16)
+  float m[256], l[256], up[256];  // a row's maximum, sum, and factor of its O
   float wgt[256 * 2];  // rows of a rank x parts: at most 256 / C x C, or 128 / C x 2 C
 };
 
 // I8: int8 cache, else bf16.  QP: parts of a query (1: bf16, 3: f32).
-template <int DP, int BN, int QP, bool I8>
+template <int DP, int QP, bool I8>
 __global__ void __launch_bounds__(kThreads, 1)
     cache_attn_tc(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const Params p,
                   int* err) {
-  using F = Cfg<DP, BN, QP>;
+  using F = Cfg<DP, QP, I8>;
+  constexpr bool F16 = I8;
+  constexpr int SB = F::SB, NS = F::NS, NSC = F::NSC;
   pdl_prologue();
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Shared sh;
@@ -210,14 +226,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.k_free[i], split ? 2 : 1);  // the streams that read the tile
       mbar_init(&sh.v_free[i], split ? 2 : 1);
     }
-    for (int i = 0; i < NSC; ++i) mbar_init(&sh.sc_full[i], kLoadWarps);
+    for (int i = 0; i < NSC; ++i) mbar_init(&sh.sc_full[i], 1);
     for (int a = 0; a < 2; ++a) {
       const int mine = split ? min(128, rows - 128 * a) : rows;
-      mbar_init(&sh.s_bar[a], 1);
-      mbar_init(&sh.p_bar[a], (uint32_t)((mine + 31) / 32));
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sh.s_bar[a][i], 1);
+        mbar_init(&sh.p_bar[a][i], (uint32_t)((mine + 31) / 32));
+      }
       mbar_init(&sh.o_bar[a], 1);
     }
     mbar_init(&sh.raw, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&sh.raw_full[i], 1);
+      mbar_init(&sh.raw_free[i], kLoadWarps);
+    }
     mbar_init(&sh.q_bar, kStageWarps);
     sh.abort_flag = aligned ? 0 : 1;
     sh.bad = 0;
@@ -229,7 +251,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = sh.tslot;
+  constexpr uint32_t tmem = 0;  // all 512 columns: the address is column 0
+  if (tid == 0 && sh.tslot != 0) {
+    atomicExch(err, 67);
+    sh.abort_flag = 1;
+  }
   volatile int* abort_flag = &sh.abort_flag;
   // tiles of stream a, and the i-th of them (relative to `first`)
   auto count = [&](int a) { return split ? nt : (nt - a + 1) / 2; };
@@ -243,11 +269,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // a thread keeps its 8-value column `u` and walks the rows
     constexpr int UNITS = DP / 8, RSTEP = kStageWarps * 32 / UNITS, LOADS = QP == 1 ? 1 : 2, BATCH = QP == 1 ? 8 : 4;
     static_assert(kStageWarps * 32 % UNITS == 0, "whole rows per step");
-    const int u = (sw * 32 + lane) % UNITS, total = nt > 0 && aligned ? (split ? 256 : 128) : 0;
+    const int u = lane % UNITS, total = nt > 0 && aligned ? (split ? 256 : 128) : 0;
     const int64_t q0 = (n * p.S * p.H + h) * p.G * p.D + u * 8;
     const int64_t token = (int64_t)p.H * p.G * p.D;
 #pragma unroll 1
-    for (int k0 = (sw * 32 + lane) / UNITS; k0 < total; k0 += BATCH * RSTEP) {
+    for (int kw = sw * 32 / UNITS; kw < total; kw += BATCH * RSTEP) {  // the warp's first row of the batch
+      const int k0 = kw + lane / UNITS;
       uint4 raw[BATCH][LOADS];
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
@@ -265,29 +292,51 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
         const int i = k0 + k * RSTEP;
-        if (i >= total) continue;
         uint8_t* dst = smem + (i >> 7) * QP * F::QTILE + unit_at(128, i & 127, u);
-        if (QP == 1) {
+        if (QP == 1 && !F16) {
           const uint32_t flip = p.scale2 < 0.f ? 0x80008000u : 0u;
           const uint4 x = raw[k][0];
-          *(uint4*)dst = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+          if (i < total) *(uint4*)dst = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
         } else {
-          // x = part 0 + part 1 + part 2, each a bf16 rounding of what is left
           float x[8];
-          *(uint4*)x = raw[k][0];
-          *(uint4*)(x + 4) = raw[k][LOADS - 1];
+          if (QP == 1) {
+            const uint32_t y[4] = {raw[k][0].x, raw[k][0].y, raw[k][0].z, raw[k][0].w};
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] *= p.scale2;
+            for (int j = 0; j < 4; ++j) {
+              const float2 f = unpack2<false>(y[j]);
+              x[2 * j] = f.x, x[2 * j + 1] = f.y;
+            }
+          } else {
+            *(uint4*)x = raw[k][0];
+            *(uint4*)(x + 4) = raw[k][LOADS - 1];
+          }
+          float f = QP == 1 ? (p.scale2 < 0.f ? -1.f : 1.f) : p.scale2;
+          if (F16) {
+            float big = 0.f, down;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) big = fmaxf(big, fabsf(x[j] * f));
+#pragma unroll
+            for (int o = UNITS / 2; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const float rise = f16_row_scale(big, down);
+            if (u == 0 && i < total) sh.qs[i] = QP == 1 ? down * fabsf(p.scale2) : down;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = x[j] * f * rise;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {  // the order of the codes
+              const float y = x[j + 1];
+              x[j + 1] = x[j + 2], x[j + 2] = y;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= f;
+          }
+          // x = part 0 + part 1 + part 2, each a rounding of what is left
 #pragma unroll
           for (int part = 0; part < QP; ++part) {
             uint32_t y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              y[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
-              x[2 * j] -= bf_lo(y[j]);
-              x[2 * j + 1] -= bf_hi(y[j]);
-            }
-            *(uint4*)(dst + part * F::QTILE) = make_uint4(y[0], y[1], y[2], y[3]);
+            for (int j = 0; j < 4; ++j) y[j] = take2<F16>(x[2 * j], x[2 * j + 1]);
+            if (i < total) *(uint4*)(dst + part * F::QTILE) = make_uint4(y[0], y[1], y[2], y[3]);
           }
         }
       }
@@ -299,7 +348,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kSoftWarps) {
     // ------------------------------------------------------------ softmax
-    regs_inc<kRegsSoft>();
     stage_q(warp);
     const int a = warp >> 2, quad = warp & 3;
     const int lo_lane = split ? 0 : a * up;  // the stream's first TMEM lane
@@ -309,49 +357,60 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int local = q0 + lane;  // row within the stream
       const int row = r0 + (split ? 128 * a : 0) + min(local, mine - 1);
       const uint32_t tl = (uint32_t)(quad * 32) << 16;
-      const uint32_t tS = tmem + tl + F::S_COL + (uint32_t)(a * BN), tO = tmem + tl + F::O_COL + (uint32_t)(a * DP);
-      const uint32_t tT = tmem + tl + F::T_COL + (uint32_t)(a * BN / 2);
-      const float f0 = fabsf(p.scale2);  // bf16 queries over a bf16 cache: scaled here
+      const uint32_t tO = tmem + tl + F::O_COL + (uint32_t)(a * DP);
       float m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
+      int vref = kVrefFirst;
       const int cnt = count(a);
       // the drafted tokens' masks and every warp's part of the queries are there
       bool ok = mbar_wait(&sh.q_bar, 0, abort_flag, err, 61);
       const unsigned long long seen = sh.mask[row / p.G];
+      // S times the key's scale times f0: the scores in units of log2
+      const float f0 = F16 ? sh.qs[(split ? 128 * a : 0) + quad * 32 + lane] : QP == 1 ? fabsf(p.scale2) : 1.f;
       for (int i = 0; i < cnt; ++i) {
         const int t = tile(a, i);
         const int64_t t0 = (int64_t)(first + t) * BN;
         if (I8) ok = ok && mbar_wait(&sh.sc_full[t % NSC], (uint32_t)(t / NSC) & 1u, abort_flag, err, 51);
-        ok = ok && mbar_wait(&sh.s_bar[a], (uint32_t)i & 1u, abort_flag, err, 52);
+        ok = ok && mbar_wait(&sh.s_bar[a][i % SB], (uint32_t)(i / SB) & 1u, abort_flag, err, 52);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
         const float* fk = I8 ? sc_k[t % NSC] : nullptr;
         const float* fv = I8 ? sc_v[t % NSC] : nullptr;
-        // the row's maximum moves to mn: O and l are rescaled
+        const uint32_t tS = tmem + tl + F::S_COL + (uint32_t)((a * SB + i % SB) * BN);
+        const uint32_t tT = tmem + tl + F::T_COL + (uint32_t)((a * SB + i % SB) * BN / 2);
+        auto scale_o = [&](float f) {
+          if (i == 0) return;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_bar[a], (uint32_t)(i - 1) & 1u, abort_flag, err, 53));
+          if (!ok) return;
+          fence_after();
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t r[32];
+            tmem_ld32_async(tO + (uint32_t)c, r);
+            tmem_wait_ld();
+            reg_fence32(r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
+            tmem_st16u(tO + (uint32_t)c, r);
+            tmem_st16u(tO + (uint32_t)c + 16, r + 16);
+          }
+          tmem_wait_st();
+        };
+        // the row's maximum moves: O and l are rescaled
         auto rescale = [&](float mx) {
           const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 0.f : ex2(m - mn);
-          if (i > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_bar[a], (uint32_t)(i - 1) & 1u, abort_flag, err, 53));
-            if (!ok) return;
-            fence_after();
-#pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-              uint32_t r[32];
-              tmem_ld32_async(tO + (uint32_t)c, r);
-              tmem_wait_ld();
-              reg_fence32(r);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
-              tmem_st16u(tO + (uint32_t)c, r);
-              tmem_st16u(tO + (uint32_t)c + 16, r + 16);
-            }
-            tmem_wait_st();
-          }
+          scale_o(f);
           l2.x *= f;
           l2.y *= f;
           m = mn;
         };
+        if (I8 && sh.sc_ref[t % NSC] > vref) {
+          const int top = sh.sc_ref[t % NSC];
+          scale_o(ex2((float)(vref - top)));
+          if (!ok) break;
+          vref = top;
+        }
         auto moves = [&](float mx) { return __any_sync(0xffffffffu, mx > m + kLazy); };
         // P of the tile from S; `vis`: the columns the row sees
         auto softmax = [&](auto mask_tag, const uint32_t* vis) {
@@ -376,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (c + 32 < BN) tmem_ld32_async(tS + (uint32_t)(c + 32), r[(c / 32 + 1) & 1]);
 #pragma unroll
                 for (int j = 0; j < 32; j += 4) {
-                  float4 f = make_float4(f0, f0, f0, f0), e = f;
+                  float4 f = make_float4(1.f, 1.f, 1.f, 1.f), e = f;
                   if (I8) f = *(const float4*)(fk + c + j), e = *(const float4*)(fv + c + j);
                   const float2 g[2] = {make_float2(f.x, f.y), make_float2(f.z, f.w)};
                   const float2 h2[2] = {make_float2(e.x, e.y), make_float2(e.z, e.w)};
@@ -388,19 +447,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (I8) s = mul2(s, g[k]);
                     if (MASK) s.x = v0 ? s.x : -INFINITY, s.y = v1 ? s.y : -INFINITY;
                     mx = fmaxf(mx, fmaxf(s.x, s.y));
-                    s = I8 ? add2(s, nb) : fma2(s, g[k], nb);
+                    s = fma2(s, make_float2(f0, f0), nb);
                     float2 y = make_float2(ex2(s.x), ex2(s.y));
-                    if (MASK && !I8) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;  // f0 may be 0
+                    if (MASK) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;  // f0 may be 0
                     s2 = add2(s2, y);
                     if (I8) {
                       y = mul2(y, h2[k]);
                       if (MASK) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;
                     }
-                    w[(c + j) / 2 + k] = pack_bf16(y.x, y.y);
+                    w[(c + j) / 2 + k] = pack2<F16>(y.x, y.y);
                   }
                 }
               }
-              if (!I8 && mx != -INFINITY) mx *= f0;
+              if (mx != -INFINITY) mx *= f0;
               if (moves(mx)) {
                 rescale(mx);
                 if (!ok) return;
@@ -433,6 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
             }
+            if (mx != -INFINITY) mx *= f0;
             if (moves(mx)) {
               rescale(mx);
               if (!ok) return;
@@ -457,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   for (int k = 0; k < 4; ++k) {
                     const bool see = !MASK || (vis[c / 32] >> (half + j + k) & 1u);
                     const float s = __uint_as_float(r[half + j + k]);
-                    y[k] = ex2(I8 ? fmaf(s, g[k], -base) : s - base);
+                    y[k] = ex2(I8 ? fmaf(s * g[k], f0, -base) : s - base);
                     if (MASK) y[k] = see ? y[k] : 0.f;
                     x[j + k] = y[k];
                     if (I8 && see) x[j + k] *= h4[k];
@@ -468,10 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int part = 0; part < QP; ++part) {
                   uint32_t w[8];
 #pragma unroll
-                  for (int j = 0; j < 8; ++j) {
-                    w[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
-                    if (part + 1 < QP) x[2 * j] -= bf_lo(w[j]), x[2 * j + 1] -= bf_hi(w[j]);
-                  }
+                  for (int j = 0; j < 8; ++j) w[j] = take2<F16>(x[2 * j], x[2 * j + 1]);
                   tmem_st8u((part < 2 ? tS + (uint32_t)(c + 16 * part) : tT + (uint32_t)(c / 2)) + half / 2, w);
                 }
               }
@@ -500,17 +557,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_bar[a]);
+        if (lane == 0) mbar_arrive(&sh.p_bar[a][i % SB]);
       }
       const float l = l2.x + l2.y;
       const int at = (split ? 128 * a : a * 128) + local;
-      if (local < mine) sh.m[at] = m, sh.l[at] = l;
+      if (local < mine) sh.m[at] = m, sh.l[at] = l, sh.up[at] = I8 ? vref_up(vref) : 1.f;
     }
-    __syncwarp();
-    regs_dec<kRegsLaunch>();
   } else if (warp < kSoftWarps + kLoadWarps) {
     // ------------------------------------------------------------ loading
-    regs_dec<kRegsLoad>();
     const int lt = tid - kSoftWarps * 32;
     auto slot_free = [&](uint64_t* bars, int t, int code) {
       return t < NS || mbar_wait(&bars[t % NS], (uint32_t)(t / NS - 1) & 1u, abort_flag, err, code);
@@ -522,60 +576,94 @@ __global__ void __launch_bounds__(kThreads, 1)
       static_assert(RSTEP % 8 == 0, "a thread's pieces share a swizzle phase");
       const int u = lt % UNITS, row0 = lt / UNITS;
       const bool has = u * 16 < p.D;
-      const int64_t at0 = (nh * p.T + (int64_t)first * BN + row0) * p.D + u * 16;
       const uint32_t put0 = unit_at(BN, row0, 2 * u), put1 = unit_at(BN, row0, 2 * u + 1);
-      uint4 rk[PER], rv[PER];
-      float nk = 0.f, nv = 0.f;
-      auto fetch = [&](const void* base, int t, uint4* r) {
-        const int8_t* src = (const int8_t*)base + at0 + (int64_t)t * BN * p.D;
-        const int left = t < nt ? (int)min((int64_t)BN, end - (int64_t)(first + t) * BN) : 0;  // rows of the tile
+      // Codes arrive by bulk copies (a row range of one head is contiguous) and
+      // are converted on their way to the swizzled tiles.  (Loads into registers
+      // ahead of time do not work: the proxy fence that publishes a tile waits
+      // for a thread's outstanding loads.)
+      auto request = [&](int t) {  // one thread
+        const int64_t t0 = (int64_t)(first + t) * BN;
+        const uint32_t bytes = (uint32_t)min((int64_t)BN, end - t0) * p.D;
+        uint8_t* dst = smem + F::RAW_OFF + t % F::NR * F::RAW;
+        mbar_expect_tx(&sh.raw_full[t % F::NR], 2 * bytes);
+        bulk_load(dst, (const int8_t*)p.k + (nh * p.T + t0) * p.D, bytes, &sh.raw_full[t % F::NR]);
+        bulk_load(dst + BN * DP, (const int8_t*)p.v + (nh * p.T + t0) * p.D, bytes, &sh.raw_full[t % F::NR]);
+      };
+      int sent = 0;
+      if (lt == 0 && aligned)
+        for (; sent < F::NR && sent < nt; ++sent) request(sent);
+      // The first warp keeps the scales: keys lane and lane + 32, one tile ahead.
+      // Value scales are stored relative to 2^vref, above the largest so far.
+      float ck[2], cv[2];
+      int vref = kVrefFirst;
+      auto fetch_scales = [&](int t) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          r[j] = make_uint4(0, 0, 0, 0);
-          if (has && row0 + j * RSTEP < left) r[j] = *(const uint4*)(src + (int64_t)(j * RSTEP) * p.D);
+        for (int i = 0; i < 2; ++i) {
+          const int64_t at = (int64_t)(first + t) * BN + i * 32 + lane;
+          ck[i] = cv[i] = 0.f;
+          if (t < nt && at < end) ck[i] = p.ks[nh * p.T + at], cv[i] = p.vs[nh * p.T + at];
         }
       };
-      auto fetch_scales = [&](int t) {
-        const int64_t at = (int64_t)(first + t) * BN + lt;
-        nk = nv = 0.f;
-        if (lt < BN && t < nt && at < end) nk = p.ks[nh * p.T + at], nv = p.vs[nh * p.T + at];
+      auto take = [&](const uint8_t* src, uint4* r) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          r[j] = has ? *(const uint4*)(src + (row0 + j * RSTEP) * p.D + u * 16) : make_uint4(0, 0, 0, 0);
       };
+      // rows behind the last token hold what was there before: any byte is a
+      // finite code, and P is 0 there.  Columns behind the head are code 0.
       auto put = [&](uint8_t* dst, const uint4* r) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
           uint4 o[2];
-          codes_to_bf16(r[j], o);
-          *(uint4*)(dst + put0 + j * RSTEP * 128) = o[0];
-          *(uint4*)(dst + put1 + j * RSTEP * 128) = o[1];
+          codes_to_f16(r[j], o);
+          // the two halves of the head go to the same banks: one starts with the odd piece
+          const bool odd = u >= 4;
+          *(uint4*)(dst + (odd ? put1 : put0) + j * RSTEP * 128) = odd ? o[1] : o[0];
+          *(uint4*)(dst + (odd ? put0 : put1) + j * RSTEP * 128) = odd ? o[0] : o[1];
         }
       };
-      fetch(p.k, 0, rk);
-      fetch(p.v, 0, rv);
-      fetch_scales(0);
+      if (lt < 32) fetch_scales(0);
       for (int t = 0; t < nt; ++t) {
-        if (!__all_sync(0xffffffffu, slot_free(sh.k_free, t, 54))) break;
+        const uint8_t* raw = smem + F::RAW_OFF + t % F::NR * F::RAW;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.raw_full[t % F::NR], (uint32_t)(t / F::NR) & 1u, abort_flag, err, 65))) break;
+        uint4 rk[PER], rv[PER];
+        take(raw, rk);
+        take(raw + BN * DP, rv);
+        if (!__all_sync(0xffffffffu, slot_free(sh.k_free, t, 54) && slot_free(sh.v_free, t, 55))) break;
         put(smem + F::K_OFF + (t % NS) * F::TILE, rk);
-        // The slot of these scales was last used by tile t - NSC.  Its softmax
-        // is over: V of tile t - 1 went into a slot that PV of tile t - 1 - NS
-        // had left, and V of tile t - 2 into that of tile t - 2 - NS = t - NSC.
-        if (lt < BN) {
-          sc_k[t % NSC][lt] = QP == 1 ? nk * fabsf(p.scale2) : nk;
-          sc_v[t % NSC][lt] = nv;
+        put(smem + F::V_OFF + (t % NS) * F::TILE, rv);
+        // The slot of these scales was last used by tile t - NSC, whose softmax is
+        // over: V of tile t takes the slot that PV of tile t - NS has left.
+        if (lt < 32) {
+          const int top = __reduce_max_sync(0xffffffffu, max(scale_exponent(cv[0]), scale_exponent(cv[1])));
+          vref = max(vref, top);
+          const float down = vref_down(vref);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            sc_k[t % NSC][i * 32 + lane] = ck[i];
+            sc_v[t % NSC][i * 32 + lane] = cv[i] * down;
+          }
+          if (lane == 0) sh.sc_ref[t % NSC] = vref;
         }
-        fetch(p.k, t + 1, rk);
-        fetch_scales(t + 1);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&sh.k_full[t % NS]);
-          mbar_arrive(&sh.sc_full[t % NSC]);
+          if (lt == 0) mbar_arrive(&sh.sc_full[t % NSC]);
+          mbar_arrive(&sh.v_full[t % NS]);
+          mbar_arrive(&sh.raw_free[t % F::NR]);
         }
-        if (!__all_sync(0xffffffffu, slot_free(sh.v_free, t, 55))) break;
-        put(smem + F::V_OFF + (t % NS) * F::TILE, rv);
-        fetch(p.v, t + 1, rv);
-        fence_proxy_async();
+        if (lt < 32) fetch_scales(t + 1);
+        // this tile's place takes the tile NR further on
+        if (lt == 0 && sent < nt && mbar_wait(&sh.raw_free[t % F::NR], (uint32_t)(t / F::NR) & 1u, abort_flag, err, 66))
+          request(sent++);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.v_full[t % NS]);
+      }
+      // After an abort: no copy of this CTA may still be in flight when it leaves.
+      if (lt == 0 && *abort_flag) {
+        const unsigned long long t1 = now_ns() + kTimeoutNs;
+        for (int s = max(0, sent - F::NR); s < sent; ++s)
+          while (!mbar_try_wait(&sh.raw_full[s % F::NR], (uint32_t)(s / F::NR) & 1u) && now_ns() < t1) {}
       }
     } else {
       // Every loading thread passes every mended tile's barrier, whatever was
@@ -645,71 +733,68 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    regs_dec<kRegsRest>();
     const int a = warp - kMmaWarp;
     if (a > 1) {
       if (a == 2) tree_masks(p.parents ? p.parents + n * p.S : nullptr, p.S, lane, sh.mask, sh.jump);
       stage_q(warp - kLoadWarps - 2);
-    } else if (lane == 0) {
+    } else {
       // ---------------------------------------------------------- MMA issue of stream a
-      const uint32_t id_s = idesc_bf16(128, BN, 0, 0), id_o = idesc_bf16(128, DP, 0, 1);
+      const uint32_t id_s = idesc_16(F16, 128, BN, 0, 0), id_o = idesc_16(F16, 128, DP, 0, 1);
       const uint32_t sq = smem_u32(smem) + (split ? (uint32_t)(a * QP * F::QTILE) : 0u);
       const uint32_t sk = smem_u32(smem) + F::K_OFF, sv = smem_u32(smem) + F::V_OFF;
-      const uint32_t ts = tmem + F::S_COL + (uint32_t)(a * BN), to = tmem + F::O_COL + (uint32_t)(a * DP);
-      const uint32_t tt = tmem + F::T_COL + (uint32_t)(a * BN / 2);
+      const uint32_t to = tmem + F::O_COL + (uint32_t)(a * DP);
       const int cnt = count(a);
-      bool ok = mbar_wait(&sh.q_bar, 0, abort_flag, err, 62);
-      // S of tile i, then O of it: tcgen05 MMAs of one thread run in issue
-      // order, so S of tile i + 1 overwrites P of tile i after O has read it
-      for (int i = 0; i <= cnt && ok; ++i) {
-        if (i > 0) {
-          const int t = tile(a, i - 1);
-          ok = mbar_wait(&sh.p_bar[a], (uint32_t)(i - 1) & 1u, abort_flag, err, 58) &&
-               mbar_wait(&sh.v_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 59);
-          if (!ok) break;
-          fence_after();
-          const uint64_t bd = smem_desc(sv + (uint32_t)((t % NS) * F::TILE), BN * 128, 1024, 2);
+      bool ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_bar, 0, abort_flag, err, 62));
+      auto issue_s = [&](int i) {
+        const int t = tile(a, i);
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.k_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 57)))
+          return false;
+        fence_after();
+        const uint32_t ts = tmem + F::S_COL + (uint32_t)((a * SB + i % SB) * BN);
+        const uint64_t qd = smem_desc(sq, 16, 1024, 2);
+        const uint64_t kd = smem_desc(sk + (uint32_t)((t % NS) * F::TILE), 16, 1024, 2);
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk) {
-            const uint32_t pc = ts + (uint32_t)((kk / 2) * 32 + (kk % 2) * 8);
-            mma_bf16_ts(to, pc, bd + kk * (2048 >> 4), id_o, i > 1 || kk > 0 ? 1u : 0u);
-            if (QP == 3) {
-              mma_bf16_ts(to, pc + 16, bd + kk * (2048 >> 4), id_o, 1u);
-              mma_bf16_ts(to, tt + (uint32_t)(kk * 8), bd + kk * (2048 >> 4), id_o, 1u);
-            }
+        for (int part = QP - 1; part >= 0; --part)  // the accumulator truncates: small products first
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            mma_ss(ts, qd + ((part * F::QTILE + (kk / 4) * 128 * 128 + (kk % 4) * 32) >> 4),
+                     kd + (((kk / 4) * BN * 128 + (kk % 4) * 32) >> 4), id_s, part < QP - 1 || kk > 0 ? 1u : 0u);
+        commit(&sh.s_bar[a][i % SB]);
+        commit(&sh.k_free[t % NS]);
+        return true;
+      };
+      for (int i = 0; i < SB && i < cnt && ok; ++i) ok = issue_s(i);
+      // O of tile i, then S of tile i + SB: tcgen05 MMAs of one thread run in issue
+      // order, so that S overwrites P of tile i after O has read it
+      for (int i = 0; i < cnt && ok; ++i) {
+        const int t = tile(a, i);
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_bar[a][i % SB], (uint32_t)(i / SB) & 1u, abort_flag, err, 58) &&
+                                         mbar_wait(&sh.v_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 59));
+        if (!ok) break;
+        fence_after();
+        const uint32_t ts = tmem + F::S_COL + (uint32_t)((a * SB + i % SB) * BN);
+        const uint32_t tt = tmem + F::T_COL + (uint32_t)((a * SB + i % SB) * BN / 2);
+        const uint64_t bd = smem_desc(sv + (uint32_t)((t % NS) * F::TILE), BN * 128, 1024, 2);
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk) {
+          const uint32_t pc = ts + (uint32_t)((kk / 2) * 32 + (kk % 2) * 8);
+          mma_ts(to, pc, bd + kk * (2048 >> 4), id_o, i > 0 || kk > 0 ? 1u : 0u);
+          if (QP == 3) {
+            mma_ts(to, pc + 16, bd + kk * (2048 >> 4), id_o, 1u);
+            mma_ts(to, tt + (uint32_t)(kk * 8), bd + kk * (2048 >> 4), id_o, 1u);
           }
-          mma_commit(&sh.o_bar[a]);
-          mma_commit(&sh.v_free[t % NS]);
         }
-        if (i < cnt) {
-          const int t = tile(a, i);
-          ok = mbar_wait(&sh.k_full[t % NS], (uint32_t)(t / NS) & 1u, abort_flag, err, 57);
-          if (!ok) break;
-          fence_after();
-          const uint64_t qd = smem_desc(sq, 16, 1024, 2);
-          const uint64_t kd = smem_desc(sk + (uint32_t)((t % NS) * F::TILE), 16, 1024, 2);
-#pragma unroll
-          for (int part = QP - 1; part >= 0; --part)  // the accumulator truncates: small products first
-#pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk)
-              mma_bf16(ts, qd + ((part * F::QTILE + (kk / 4) * 128 * 128 + (kk % 4) * 32) >> 4),
-                       kd + (((kk / 4) * BN * 128 + (kk % 4) * 32) >> 4), id_s, part < QP - 1 || kk > 0 ? 1u : 0u);
-          mma_commit(&sh.s_bar[a]);
-          mma_commit(&sh.k_free[t % NS]);
-        }
+        commit(&sh.o_bar[a]);
+        commit(&sh.v_free[t % NS]);
+        if (i + SB < cnt) ok = issue_s(i + SB);
       }
       // the accumulator is final, and no MMA of the stream reads shared memory, once this passes
       if (ok && cnt > 0) mbar_wait(&sh.o_bar[a], (uint32_t)(cnt - 1) & 1u, abort_flag, err, 60);
     }
   }
-  // Registers go back to the launch's share: the loading and MMA warpgroups take
-  // theirs only once every softmax warp has had and returned its own (before
-  // that, a warpgroup that is done early could take what a softmax warp still
-  // waits for, and neither would go on).
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (warp >= kSoftWarps) regs_inc<kRegsLaunch>();
   fence_after();
   const bool failed = sh.abort_flag != 0;
 
@@ -731,7 +816,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; j += 4)
             *(uint4*)(so + (a * 128 + local) * F::LDO + c + j) =
-                count(a) > 0 ? make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]) : make_uint4(0, 0, 0, 0);
+                count(a) == 0 ? make_uint4(0, 0, 0, 0)
+                : I8          ? make_uint4(r[j], r[j + 2], r[j + 1], r[j + 3])  // the order of the codes
+                              : make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
       }
     }
   }
@@ -739,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == 0) {
     fence_after();
-    tmem_dealloc(tmem, F::COLS);
+    tmem_dealloc(sh.tslot, F::COLS);
   }
   __syncthreads();
   cluster_sync();
@@ -752,15 +839,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* wgt = sh.wgt;
     for (int k = tid; k < mine; k += kThreads) {
       const int i = k * (int)C + (int)rank;
-      float pm[16], pl[16], mx = -INFINITY, l = 0.f;
+      float pm[16], pl[16], pu[16], mx = -INFINITY, l = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        pm[j] = -INFINITY, pl[j] = 0.f;
+        pm[j] = -INFINITY, pl[j] = 0.f, pu[j] = 1.f;
         if (j < np) {
           const uint32_t c = (uint32_t)(split ? j : j / 2);
           const int at = split ? i : (j & 1) * 128 + i;
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm[j]) : "r"(cluster_addr(&sh.m[at], c)));
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pl[j]) : "r"(cluster_addr(&sh.l[at], c)));
+          if (I8) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pu[j]) : "r"(cluster_addr(&sh.up[at], c)));
         }
       }
 #pragma unroll
@@ -773,7 +861,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (j < np) wgt[k * np + j] = pm[j] / l;
+        if (j < np) wgt[k * np + j] = pm[j] == 0.f ? 0.f : pm[j] / l * pu[j];
     }
     int bad = 0;
     if (!I8)
@@ -817,9 +905,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync();
 }
 
-template <int DP, int BN, int QP, bool I8>
+template <int DP, int QP, bool I8>
 cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
-  using F = Cfg<DP, BN, QP>;
+  using F = Cfg<DP, QP, I8>;
   const KvCacheView& c = a.cache;
   const Params p = make_params(a, F::MAXR);
   CUtensorMap mk{}, mv{};
@@ -832,26 +920,26 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   int* err = tc_error_word();
   if (!err) return cudaErrorMemoryAllocation;
   const int64_t items = c.N * c.H * p.chunks;
-  // one CTA fits an SM: split until the CTAs fill the SMs once, or a CTA has two tiles
+  // one CTA fits an SM: split until the CTAs fill the SMs once, or a CTA has four tiles
   int C = 1;
-  while (C < kMaxCluster && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 2 * BN) ++C;
-  return launch_cluster(cache_attn_tc<DP, BN, QP, I8>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);
+  while (C < kMaxCluster && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 4 * BN) ++C;
+  return launch_cluster(cache_attn_tc<DP, QP, I8>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);
 }
 
 }  // namespace
 
 bool cache_attention_tc_takes(const CacheAttnArgs& a) {
-  return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 && a.S * (a.Hq / a.cache.H) > (a.bf16 ? 16 : 4);
+  return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 && !cache_attention_mma_takes(a);
 }
 
 cudaError_t cache_attention_tc(const CacheAttnArgs& a, cudaStream_t stream) {
   const bool i8 = a.cache.type == KvType::I8;
   if (a.cache.D <= 64) {
-    if (a.bf16) return i8 ? launch<64, 128, 1, true>(a, stream) : launch<64, 128, 1, false>(a, stream);
-    return i8 ? launch<64, 128, 3, true>(a, stream) : launch<64, 128, 3, false>(a, stream);
+    if (a.bf16) return i8 ? launch<64, 1, true>(a, stream) : launch<64, 1, false>(a, stream);
+    return i8 ? launch<64, 3, true>(a, stream) : launch<64, 3, false>(a, stream);
   }
-  if (a.bf16) return i8 ? launch<128, 128, 1, true>(a, stream) : launch<128, 128, 1, false>(a, stream);
-  return i8 ? launch<128, 64, 3, true>(a, stream) : launch<128, 64, 3, false>(a, stream);
+  if (a.bf16) return i8 ? launch<128, 1, true>(a, stream) : launch<128, 1, false>(a, stream);
+  return i8 ? launch<128, 3, true>(a, stream) : launch<128, 3, false>(a, stream);
 }
 
 }  // namespace sb

@@ -3,6 +3,7 @@
 // Included by .cu files only.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 
 #include <cmath>
 
@@ -14,6 +15,38 @@ namespace sb {
 namespace cattn {
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+// Two f32 rounded to packed bf16 or f16, and what the rounding left of them.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t d;
+  if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+template <bool F16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (F16) return __half22float2(*(const __half2*)&w);
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t take2(float& lo, float& hi) {
+  const uint32_t w = pack2<F16>(lo, hi);
+  const float2 f = unpack2<F16>(w);
+  lo -= f.x;
+  hi -= f.y;
+  return w;
+}
+
+// Codes c in bytes 0 and 2 of t (bytes 1 and 3: anything) to two f16 values.
+// 0x6400 + (c + 128) is 1024 + c + 128 as f16 (steps of 1 there): c exactly,
+// after a subtraction.  (bf16 has no steps of 1 beyond 8 bits and would need
+// twice the instructions, which bound the int8 kernel.)
+__device__ __forceinline__ uint32_t codes(uint32_t t) {
+  const uint32_t a = (t & 0x00ff00ffu) ^ 0x64806480u;
+  __half2 x = __hsub2(*(const __half2*)&a, __half2half2(__ushort_as_half(0x6480)));
+  return *(uint32_t*)&x;
+}
 
 struct Params {
   const void *k, *v;
@@ -162,6 +195,24 @@ __device__ __forceinline__ void store4(const Params& p, int64_t at, float4 y) {
 }
 
 constexpr int kMaxCluster = 8;
+
+// f16 operands for int8 caches.  A row of queries is scaled by a power of two to
+// a largest value in [2^14, 2^15), which keeps what is 2^-38 of it: 2^(14 - e)
+// for a largest value of exponent e, within f32's normal range; down = 1 / up.
+__device__ __forceinline__ float f16_row_scale(float largest, float& down) {
+  const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -110), 127);
+  down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+  return __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+}
+// P times the value scales goes into f16 relative to 2^vref, which is above the
+// largest scale so far: at most 2^(8 + 6), with steps of 2^-30 below 1.
+constexpr int kVrefFirst = -100;
+__device__ __forceinline__ int scale_exponent(float s) {  // 2^e > |s|; low for one that is not finite
+  s = fabsf(s);
+  return s < INFINITY ? (int)(__float_as_uint(s) >> 23) - 126 : -125;
+}
+__device__ __forceinline__ float vref_down(int vref) { return __uint_as_float((uint32_t)(127 + 6 - vref) << 23); }
+__device__ __forceinline__ float vref_up(int vref) { return __uint_as_float((uint32_t)(127 - 6 + vref) << 23); }
 
 // The weights of N partial results with base-2 maxima m: f = 2^(m - max).
 template <int N>

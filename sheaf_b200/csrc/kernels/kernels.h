@@ -280,11 +280,11 @@ struct CacheAttnArgs {
 };
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
 // The kernels for bf16 and int8 caches of head size 64 to 128 and the calls
-// they take (cache_attention dispatches): up to 16 bf16 or 4 f32 query rows
-// (tokens x query heads per cache head) multiply with warp instructions
-// (kernels/cache_attention_mma.cu), more rows with tcgen05
-// (kernels/cache_attention_tc.cu, which reports failed waits through the
-// tensor-core error word, codes 50..64).
+// they take (cache_attention dispatches): few query rows (tokens x query heads
+// per cache head: up to 4 in f32, 8 in bf16, 16 over an int8 cache) multiply
+// with warp instructions (kernels/cache_attention_mma.cu), more rows with
+// tcgen05 (kernels/cache_attention_tc.cu).  Failed waits are reported through
+// the tensor-core error word, codes 50..67.
 bool cache_attention_mma_takes(const CacheAttnArgs& a);
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream);
 bool cache_attention_tc_takes(const CacheAttnArgs& a);
