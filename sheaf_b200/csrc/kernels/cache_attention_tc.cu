@@ -12,8 +12,7 @@
 //                       at most 64 rows stream 1 uses the upper half of the
 //                       TMEM lanes, so the two use different SM quarters.
 // While one stream turns S into P the tensor cores work for the other.  Warp
-// roles: 8 softmax, 4 loading, 2 issuing the MMAs (one thread needs about 80
-// cycles per tcgen05.mma, more than the 64 that one takes), 2 helpers.
+// roles: 8 softmax, 4 loading, 2 issuing the MMAs, 1 for copies and scales.
 //
 //   S = Q K^T   f32 queries are split exactly into three bf16 (f16) parts whose
 //               products accumulate into the same f32 S, so S has f32 accuracy.
@@ -28,8 +27,8 @@
 //               more than 2^8, so O is rescaled in the first tiles and then
 //               hardly ever; exact since P, O and the sum l share m.
 //
-// bf16 tiles arrive by TMA, int8 tiles by bulk copies and a conversion in shared
-// memory.  Rows of V behind the last token are zeroed
+// bf16 tiles arrive by TMA, int8 tiles through registers (codes to f16 on the way
+// to swizzled shared memory).  Rows of V behind the last token are zeroed
 // (0 x NaN would reach every row); a value of a drafted token that is not
 // finite is taken out of the tile and added to the rows that attend to it when
 // the outputs are joined.
@@ -46,10 +45,11 @@ namespace {
 using namespace cattn;
 using namespace tc;
 
-// warps 0-7 softmax, 8-11 loading, 12 and 13 MMA issue (one per stream), 14, 15
-// and the softmax warps stage the queries
-constexpr int kSoftWarps = 8, kLoadWarps = 4, kMmaWarp = 12, kWarps = 16, kThreads = kWarps * 32;
-constexpr int kStageWarps = kWarps - kLoadWarps - 2;
+// warps 0-7 softmax, 8-11 loading (int8: conversion), 12 and 13 MMA issue (one
+// per stream), 14 copies and scales; all but 12-14 stage the queries first, 15
+// also builds the drafted tokens' masks
+constexpr int kSoftWarps = 8, kLoadWarps = 4, kMmaWarp = 12, kFeedWarp = 14, kWarps = 16, kThreads = kWarps * 32;
+constexpr int kStageWarps = kSoftWarps + kLoadWarps;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int BN = 64;  // keys of a tile
 constexpr float kLazy = 8.f;  // a row's maximum moves when it would grow by more than this (log2)
@@ -153,15 +153,6 @@ __device__ __forceinline__ uint32_t unit_at(int rows, int r, int unit) {
 
 __device__ __forceinline__ void loaders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kLoadThreads) : "memory"); }
 
-// One contiguous piece of global memory to shared memory; both addresses and
-// the size are multiples of 16.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 template <int DP, int QP, bool I8>
 struct Cfg {
   static constexpr int MAXR = QP == 3 && DP == 128 ? 128 : 256;  // query rows of a CTA
@@ -169,10 +160,14 @@ struct Cfg {
   static constexpr int QTILE = 128 * DP * 2;                     // one part of 128 rows
   static constexpr int Q_BYTES = (MAXR / 128) * QP * QTILE;
   static constexpr int TILE = BN * DP * 2;
-  static constexpr int NS = QP == 3 && DP == 128 ? 2 : I8 ? 3 : 4;  // K and V tiles in flight
+  static constexpr int NS = QP == 3 && DP == 128 ? 2 : 4;  // K and V tiles in flight
+  // Groups of loading warps that take int8 tiles in turn.  Two, with four places: one
+  // group converts while the other's loads are on their way (8 x 16K keys, 256
+  // bf16 rows of 128: 119 us, against 126 with all four warps on each tile).  With
+  // two places a group would wait for its place longer (f32: 339 us against 288).
+  static constexpr int GROUPS = NS > 2 ? 2 : 1;
   static constexpr int NSC = 2 * NS;                       // rows of scales in flight (see the loader)
-  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NS * TILE, RAW_OFF = V_OFF + NS * TILE;
-  static constexpr int NR = 3, RAW = 2 * BN * DP, END = RAW_OFF + (I8 ? NR * RAW : 0);  // int8 tiles as they arrive
+  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NS * TILE, END = V_OFF + NS * TILE;
   static constexpr int LDO = DP + 4;  // padded row of the joined outputs, f32
   static constexpr int JOIN = 256 * LDO * 4;
   static constexpr int SMEM = END > JOIN ? END : JOIN;
@@ -183,10 +178,11 @@ struct Cfg {
 };
 
 struct Shared {
-  uint64_t k_full[4], k_free[4], v_full[4], v_free[4], sc_full[8], s_bar[2][2], p_bar[2][2], o_bar[2], raw, q_bar, raw_full[3], raw_free[3];
+  uint64_t k_full[4], k_free[4], v_full[4], v_free[4], sc_full[8], s_bar[2][2], p_bar[2][2], o_bar[2], raw, mended, q_bar;
   uint32_t tslot;
   volatile int abort_flag;
   int bad;  // a drafted value that is not finite was taken out of a tile
+  int q_row[256];  // query row of a staged row, in units of D values from the slot and head's first; -1: none
   int sc_ref[8];  // exponent that a tile's value scales are relative to
   unsigned long long mask[kKvMaxTokens];
   int jump[kKvMaxTokens];
@@ -221,8 +217,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&sh.k_full[i], I8 ? kLoadWarps : 1);
-      mbar_init(&sh.v_full[i], I8 ? kLoadWarps : 1);
+      mbar_init(&sh.k_full[i], I8 ? kLoadWarps / F::GROUPS : 1);
+      mbar_init(&sh.v_full[i], I8 ? kLoadWarps / F::GROUPS : 1);
       mbar_init(&sh.k_free[i], split ? 2 : 1);  // the streams that read the tile
       mbar_init(&sh.v_free[i], split ? 2 : 1);
     }
@@ -236,11 +232,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.o_bar[a], 1);
     }
     mbar_init(&sh.raw, 1);
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(&sh.raw_full[i], 1);
-      mbar_init(&sh.raw_free[i], kLoadWarps);
-    }
-    mbar_init(&sh.q_bar, kStageWarps);
+    mbar_init(&sh.mended, 1);
+    mbar_init(&sh.q_bar, kStageWarps + 1);
     sh.abort_flag = aligned ? 0 : 1;
     sh.bad = 0;
     if (!aligned) atomicExch(err, 50);
@@ -248,6 +241,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_proxy_async();
   }
   if (warp == 0) tmem_alloc(&sh.tslot, F::COLS);
+  if (tid < 256) {
+    const int local = up ? tid & 63 : tid, row = r0 + local, s = row / p.G;
+    sh.q_row[tid] = local < rows && tid < (split ? 256 : 128) ? s * p.H * p.G + row - s * p.G : -1;
+  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -267,26 +264,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   // signs, so that the softmax can take maxima before it scales.
   auto stage_q = [&](int sw) {
     // a thread keeps its 8-value column `u` and walks the rows
-    constexpr int UNITS = DP / 8, RSTEP = kStageWarps * 32 / UNITS, LOADS = QP == 1 ? 1 : 2, BATCH = QP == 1 ? 8 : 4;
+    constexpr int UNITS = DP / 8, RSTEP = kStageWarps * 32 / UNITS, LOADS = QP == 1 ? 1 : 2, BATCH = QP == 1 ? 4 : 2;
     static_assert(kStageWarps * 32 % UNITS == 0, "whole rows per step");
     const int u = lane % UNITS, total = nt > 0 && aligned ? (split ? 256 : 128) : 0;
-    const int64_t q0 = (n * p.S * p.H + h) * p.G * p.D + u * 8;
-    const int64_t token = (int64_t)p.H * p.G * p.D;
+    const uint8_t* q0 = (const uint8_t*)p.q + ((n * p.S * p.H + h) * p.G * p.D + u * 8) * (QP == 1 ? 2 : 4);
+    const int row_bytes = p.D * (QP == 1 ? 2 : 4);
 #pragma unroll 1
     for (int kw = sw * 32 / UNITS; kw < total; kw += BATCH * RSTEP) {  // the warp's first row of the batch
       const int k0 = kw + lane / UNITS;
       uint4 raw[BATCH][LOADS];
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
-        const int i = k0 + k * RSTEP, local = up ? i & 63 : i;
+        const int at = k0 + k * RSTEP < total && u * 8 < p.D ? sh.q_row[k0 + k * RSTEP] : -1;
 #pragma unroll
-        for (int c = 0; c < LOADS; ++c) raw[k][c] = make_uint4(0, 0, 0, 0);
-        if (i < total && local < rows && u * 8 < p.D) {
-          const int row = r0 + local, s = row / p.G, g = row - s * p.G;
-          const int64_t at = q0 + s * token + g * p.D;
-#pragma unroll
-          for (int c = 0; c < LOADS; ++c)
-            raw[k][c] = *(const uint4*)((const uint8_t*)p.q + (at + 4 * c) * (QP == 1 ? 2 : 4));
+        for (int c = 0; c < LOADS; ++c) {
+          raw[k][c] = make_uint4(0, 0, 0, 0);
+          if (at >= 0) raw[k][c] = *(const uint4*)(q0 + (int64_t)at * row_bytes + 16 * c);
         }
       }
 #pragma unroll
@@ -565,34 +558,108 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < kSoftWarps + kLoadWarps) {
     // ------------------------------------------------------------ loading
+    stage_q(warp);
     const int lt = tid - kSoftWarps * 32;
     auto slot_free = [&](uint64_t* bars, int t, int code) {
       return t < NS || mbar_wait(&bars[t % NS], (uint32_t)(t / NS - 1) & 1u, abort_flag, err, code);
     };
     if constexpr (I8) {
+      constexpr int THREADS = kLoadThreads / F::GROUPS;
       constexpr int UNITS = DP / 16;                  // 16-code pieces of a row
-      constexpr int PER = BN * UNITS / kLoadThreads;  // per thread and tile
-      constexpr int RSTEP = kLoadThreads / UNITS;     // rows between a thread's pieces (a multiple of 8)
+      constexpr int PER = BN * UNITS / THREADS;  // per thread and tile
+      constexpr int RSTEP = THREADS / UNITS;     // rows between a thread's pieces (a multiple of 8)
       static_assert(RSTEP % 8 == 0, "a thread's pieces share a swizzle phase");
-      const int u = lt % UNITS, row0 = lt / UNITS;
+      // Eight lanes that store together take four pieces of two rows, whose
+      // swizzles put them into different banks.
+      const int group = lt / THREADS, gt = lt % THREADS;
+      const int u = UNITS == 8 ? (lane & 3) | (lane >> 1 & 4) : gt % UNITS;
+      const int row0 = UNITS == 8 ? (gt >> 5) * 4 + (lane >> 2 & 1) + (lane >> 3 & 2) : gt / UNITS;
       const bool has = u * 16 < p.D;
+      const int64_t at0 = (nh * p.T + (int64_t)first * BN + row0) * p.D + u * 16;
       const uint32_t put0 = unit_at(BN, row0, 2 * u), put1 = unit_at(BN, row0, 2 * u + 1);
-      // Codes arrive by bulk copies (a row range of one head is contiguous) and
-      // are converted on their way to the swizzled tiles.  (Loads into registers
-      // ahead of time do not work: the proxy fence that publishes a tile waits
-      // for a thread's outstanding loads.)
-      auto request = [&](int t) {  // one thread
-        const int64_t t0 = (int64_t)(first + t) * BN;
-        const uint32_t bytes = (uint32_t)min((int64_t)BN, end - t0) * p.D;
-        uint8_t* dst = smem + F::RAW_OFF + t % F::NR * F::RAW;
-        mbar_expect_tx(&sh.raw_full[t % F::NR], 2 * bytes);
-        bulk_load(dst, (const int8_t*)p.k + (nh * p.T + t0) * p.D, bytes, &sh.raw_full[t % F::NR]);
-        bulk_load(dst + BN * DP, (const int8_t*)p.v + (nh * p.T + t0) * p.D, bytes, &sh.raw_full[t % F::NR]);
+      uint4 rk[PER], rv[PER];
+      // Loads of the group's next tile.  They go out right behind the fence that
+      // publishes a tile: a fence waits for the thread's outstanding loads.
+      auto fetch = [&](const void* base, int t, uint4* r) {
+        const int8_t* src = (const int8_t*)base + at0 + (int64_t)t * BN * p.D;
+        const int left = t < nt ? (int)min((int64_t)BN, end - (int64_t)(first + t) * BN) : 0;  // rows of the tile
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          r[j] = make_uint4(0, 0, 0, 0);
+          if (has && row0 + j * RSTEP < left) r[j] = *(const uint4*)(src + (int64_t)(j * RSTEP) * p.D);
+        }
       };
-      int sent = 0;
-      if (lt == 0 && aligned)
-        for (; sent < F::NR && sent < nt; ++sent) request(sent);
-      // The first warp keeps the scales: keys lane and lane + 32, one tile ahead.
+      auto put = [&](uint8_t* dst, const uint4* r) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          uint4 o[2];
+          codes_to_f16(r[j], o);
+          *(uint4*)(dst + put0 + j * RSTEP * 128) = o[0];
+          *(uint4*)(dst + put1 + j * RSTEP * 128) = o[1];
+        }
+      };
+      fetch(p.k, group, rk);
+      fetch(p.v, group, rv);
+      for (int t = group; t < nt; t += F::GROUPS) {
+        if (!__all_sync(0xffffffffu, slot_free(sh.k_free, t, 54))) break;
+        put(smem + F::K_OFF + (t % NS) * F::TILE, rk);
+        if (!__all_sync(0xffffffffu, slot_free(sh.v_free, t, 55))) break;
+        put(smem + F::V_OFF + (t % NS) * F::TILE, rv);
+        fence_proxy_async();
+        fetch(p.k, t + F::GROUPS, rk);
+        fetch(p.v, t + F::GROUPS, rv);
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sh.k_full[t % NS]);
+          mbar_arrive(&sh.v_full[t % NS]);
+        }
+      }
+    } else {
+      // Tiles with drafted tokens or the end of the sequence are mended before
+      // the MMAs may read them.  Every loading thread passes every such tile's
+      // barrier, whatever was aborted (an aborted wait returns at once), so none
+      // is left waiting.
+      int mended = 0;
+      for (int t = (int)max((int64_t)0, pre / BN - first); t < nt; ++t) {
+        const int64_t t0 = (int64_t)(first + t) * BN;
+        if (t0 + BN <= pre) continue;
+        uint8_t* dv = smem + F::V_OFF + t % NS * F::TILE;
+        mbar_wait(&sh.raw, (uint32_t)mended & 1u, abort_flag, err, 56);
+        ++mended;
+        for (int i = lt; i < BN * (DP / 8); i += kLoadThreads) {
+          const int row = i / (DP / 8);
+          uint4* x = (uint4*)(dv + unit_at(BN, row, i % (DP / 8)));
+          if (t0 + row >= end) {
+            *x = make_uint4(0, 0, 0, 0);
+          } else if (t0 + row >= pre) {
+            uint32_t w[4] = {x->x, x->y, x->z, x->w};
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, bad = true;
+              if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, bad = true;
+            }
+            if (bad) {
+              *x = make_uint4(w[0], w[1], w[2], w[3]);
+              sh.bad = 1;
+            }
+          }
+        }
+        fence_proxy_async();
+        loaders_sync();
+        if (lt == 0) {
+          mbar_arrive(&sh.mended);
+          mbar_arrive(&sh.v_full[t % NS]);
+        }
+      }
+    }
+  } else if (warp == kFeedWarp) {
+    // ------------------------------------------------------------ copies and scales
+    auto slot_free = [&](uint64_t* bars, int t, int code) {
+      return t < NS || mbar_wait(&bars[t % NS], (uint32_t)(t / NS - 1) & 1u, abort_flag, err, code);
+    };
+    if constexpr (I8) {
+      // Scales of keys lane and lane + 32, one tile ahead.
       // Value scales are stored relative to 2^vref, above the largest so far.
       float ck[2], cv[2];
       int vref = kVrefFirst;
@@ -604,139 +671,69 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (t < nt && at < end) ck[i] = p.ks[nh * p.T + at], cv[i] = p.vs[nh * p.T + at];
         }
       };
-      auto take = [&](const uint8_t* src, uint4* r) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-          r[j] = has ? *(const uint4*)(src + (row0 + j * RSTEP) * p.D + u * 16) : make_uint4(0, 0, 0, 0);
-      };
-      // rows behind the last token hold what was there before: any byte is a
-      // finite code, and P is 0 there.  Columns behind the head are code 0.
-      auto put = [&](uint8_t* dst, const uint4* r) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          uint4 o[2];
-          codes_to_f16(r[j], o);
-          // the two halves of the head go to the same banks: one starts with the odd piece
-          const bool odd = u >= 4;
-          *(uint4*)(dst + (odd ? put1 : put0) + j * RSTEP * 128) = odd ? o[1] : o[0];
-          *(uint4*)(dst + (odd ? put0 : put1) + j * RSTEP * 128) = odd ? o[0] : o[1];
-        }
-      };
-      if (lt < 32) fetch_scales(0);
+      fetch_scales(0);
       for (int t = 0; t < nt; ++t) {
-        const uint8_t* raw = smem + F::RAW_OFF + t % F::NR * F::RAW;
-        if (!__all_sync(0xffffffffu, mbar_wait(&sh.raw_full[t % F::NR], (uint32_t)(t / F::NR) & 1u, abort_flag, err, 65))) break;
-        uint4 rk[PER], rv[PER];
-        take(raw, rk);
-        take(raw + BN * DP, rv);
-        if (!__all_sync(0xffffffffu, slot_free(sh.k_free, t, 54) && slot_free(sh.v_free, t, 55))) break;
-        put(smem + F::K_OFF + (t % NS) * F::TILE, rk);
-        put(smem + F::V_OFF + (t % NS) * F::TILE, rv);
         // The slot of these scales was last used by tile t - NSC, whose softmax is
-        // over: V of tile t takes the slot that PV of tile t - NS has left.
-        if (lt < 32) {
-          const int top = __reduce_max_sync(0xffffffffu, max(scale_exponent(cv[0]), scale_exponent(cv[1])));
-          vref = max(vref, top);
-          const float down = vref_down(vref);
+        // over once PV of tile t - NS has left its place.
+        if (!__all_sync(0xffffffffu, slot_free(sh.v_free, t, 68))) break;
+        const int top = __reduce_max_sync(0xffffffffu, max(scale_exponent(cv[0]), scale_exponent(cv[1])));
+        vref = max(vref, top);
+        const float down = vref_down(vref);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            sc_k[t % NSC][i * 32 + lane] = ck[i];
-            sc_v[t % NSC][i * 32 + lane] = cv[i] * down;
-          }
-          if (lane == 0) sh.sc_ref[t % NSC] = vref;
+        for (int i = 0; i < 2; ++i) {
+          sc_k[t % NSC][i * 32 + lane] = ck[i];
+          sc_v[t % NSC][i * 32 + lane] = cv[i] * down;
         }
-        fence_proxy_async();
+        if (lane == 0) sh.sc_ref[t % NSC] = vref;
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sh.k_full[t % NS]);
-          if (lt == 0) mbar_arrive(&sh.sc_full[t % NSC]);
-          mbar_arrive(&sh.v_full[t % NS]);
-          mbar_arrive(&sh.raw_free[t % F::NR]);
-        }
-        if (lt < 32) fetch_scales(t + 1);
-        // this tile's place takes the tile NR further on
-        if (lt == 0 && sent < nt && mbar_wait(&sh.raw_free[t % F::NR], (uint32_t)(t / F::NR) & 1u, abort_flag, err, 66))
-          request(sent++);
-        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.sc_full[t % NSC]);
+        fetch_scales(t + 1);
       }
-      // After an abort: no copy of this CTA may still be in flight when it leaves.
-      if (lt == 0 && *abort_flag) {
-        const unsigned long long t1 = now_ns() + kTimeoutNs;
-        for (int s = max(0, sent - F::NR); s < sent; ++s)
-          while (!mbar_try_wait(&sh.raw_full[s % F::NR], (uint32_t)(s / F::NR) & 1u) && now_ns() < t1) {}
-      }
-    } else {
-      // Every loading thread passes every mended tile's barrier, whatever was
-      // aborted (an aborted wait returns at once), so none is left waiting.
-      int mended = 0, sent_k = 0, sent_v = 0, sent_raw = 0;
-      for (int t = 0; t < nt; ++t) {
+    } else if (lane == 0 && aligned) {
+      int mend_sent = 0, sent_k = 0, sent_v = 0;
+      bool ok = true;
+      for (int t = 0; t < nt && ok; ++t) {
         const int64_t t0 = (int64_t)(first + t) * BN;
         const int s = t % NS;
         uint8_t *dk = smem + F::K_OFF + s * F::TILE, *dv = smem + F::V_OFF + s * F::TILE;
         const bool mend = t0 + BN > pre;  // drafted tokens or the end of the sequence
-        bool ok = true;
-        if (lt == 0) {
-          ok = slot_free(sh.k_free, t, 54);
-          if (ok) {
-            mbar_expect_tx(&sh.k_full[s], F::TILE);
+        // the queries' loads are not to queue behind more tiles than the streams start with
+        if (t == 2) ok = mbar_wait(&sh.q_bar, 0, abort_flag, err, 70);
+        ok = ok && slot_free(sh.k_free, t, 54);
+        if (!ok) break;
+        mbar_expect_tx(&sh.k_full[s], F::TILE);
 #pragma unroll
-            for (int c = 0; c < DP / 64; ++c)
-              tma_load_3d(dk + c * BN * 128, &mK, &sh.k_full[s], c * 64, (int)t0, (int)nh);
-            sent_k = t + 1;
-            ok = slot_free(sh.v_free, t, 55);
-          }
-          if (ok) {
-            uint64_t* bar = mend ? &sh.raw : &sh.v_full[s];
-            mbar_expect_tx(bar, F::TILE);
+        for (int c = 0; c < DP / 64; ++c)
+          tma_load_3d(dk + c * BN * 128, &mK, &sh.k_full[s], c * 64, (int)t0, (int)nh);
+        sent_k = t + 1;
+        ok = slot_free(sh.v_free, t, 55);
+        // one tile at a time is on its way to the mending warps
+        if (ok && mend && mend_sent > 0) ok = mbar_wait(&sh.mended, (uint32_t)(mend_sent - 1) & 1u, abort_flag, err, 69);
+        if (!ok) break;
+        uint64_t* bar = mend ? &sh.raw : &sh.v_full[s];
+        mbar_expect_tx(bar, F::TILE);
 #pragma unroll
-            for (int c = 0; c < DP / 64; ++c) tma_load_3d(dv + c * BN * 128, &mV, bar, c * 64, (int)t0, (int)nh);
-            if (mend) ++sent_raw;
-            else sent_v = t + 1;
-          }
-        }
-        if (mend) {
-          ok = mbar_wait(&sh.raw, (uint32_t)mended & 1u, abort_flag, err, 56) && ok;
-          ++mended;
-          for (int i = lt; i < BN * (DP / 8); i += kLoadThreads) {
-            const int row = i / (DP / 8);
-            uint4* x = (uint4*)(dv + unit_at(BN, row, i % (DP / 8)));
-            if (t0 + row >= end) {
-              *x = make_uint4(0, 0, 0, 0);
-            } else if (t0 + row >= pre) {
-              uint32_t w[4] = {x->x, x->y, x->z, x->w};
-              bool bad = false;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if ((w[j] & 0x7f80u) == 0x7f80u) w[j] &= 0xffff0000u, bad = true;
-                if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] &= 0xffffu, bad = true;
-              }
-              if (bad) {
-                *x = make_uint4(w[0], w[1], w[2], w[3]);
-                sh.bad = 1;
-              }
-            }
-          }
-          fence_proxy_async();
-          loaders_sync();
-          if (lt == 0) mbar_arrive(&sh.v_full[s]);
-        }
+        for (int c = 0; c < DP / 64; ++c) tma_load_3d(dv + c * BN * 128, &mV, bar, c * 64, (int)t0, (int)nh);
+        if (mend) ++mend_sent;
+        else sent_v = t + 1;
       }
       // After an abort: no copy of this CTA may still be in flight when it
-      // leaves.  The MMA warp may not have waited for the last ones.
-      if (lt == 0 && *abort_flag) {
+      // leaves.  The MMA warps may not have waited for the last ones.
+      if (*abort_flag) {
         const unsigned long long t1 = now_ns() + kTimeoutNs;
         for (int s = max(0, sent_k - NS); s < sent_k; ++s)
           while (!mbar_try_wait(&sh.k_full[s % NS], (uint32_t)(s / NS) & 1u) && now_ns() < t1) {}
         for (int s = max(0, sent_v - NS); s < sent_v; ++s)
           while (!mbar_try_wait(&sh.v_full[s % NS], (uint32_t)(s / NS) & 1u) && now_ns() < t1) {}
-        while (sent_raw && !mbar_try_wait(&sh.raw, (uint32_t)(sent_raw - 1) & 1u) && now_ns() < t1) {}
+        while (mend_sent && !mbar_try_wait(&sh.raw, (uint32_t)(mend_sent - 1) & 1u) && now_ns() < t1) {}
       }
     }
   } else {
     const int a = warp - kMmaWarp;
     if (a > 1) {
-      if (a == 2) tree_masks(p.parents ? p.parents + n * p.S : nullptr, p.S, lane, sh.mask, sh.jump);
-      stage_q(warp - kLoadWarps - 2);
+      tree_masks(p.parents ? p.parents + n * p.S : nullptr, p.S, lane, sh.mask, sh.jump);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_bar);
     } else {
       // ---------------------------------------------------------- MMA issue of stream a
       const uint32_t id_s = idesc_16(F16, 128, BN, 0, 0), id_o = idesc_16(F16, 128, DP, 0, 1);
@@ -864,42 +861,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j < np) wgt[k * np + j] = pm[j] == 0.f ? 0.f : pm[j] / l * pu[j];
     }
     int bad = 0;
-    if (!I8)
-      for (uint32_t c = 0; c < C; ++c) {
-        int x;
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(cluster_addr(&sh.bad, c)));
-        bad |= x;
-      }
+    if (!I8 && lane < (int)C)
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(bad) : "r"(cluster_addr(&sh.bad, (uint32_t)lane)));
+    bad = __any_sync(0xffffffffu, bad);
     __syncthreads();
     constexpr int LPR = DP / 4;
     const int gl = tid % LPR;
-    for (int k = tid / LPR; k < mine; k += kThreads / LPR) {
-      const int i = k * (int)C + (int)rank;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int j0 = 0; j0 < np; j0 += 8) {
-        float4 x[8];
+    constexpr int ROWS = kThreads / LPR;
+    for (int k0 = tid / LPR; k0 < mine; k0 += 2 * ROWS) {
+      float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+      for (int j0 = 0; j0 < np; j0 += 4) {
+        float4 x[2][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j0 + j < np) {
-            const uint32_t c = (uint32_t)(split ? j0 + j : (j0 + j) / 2);
-            const int at = split ? i : (j & 1) * 128 + i;
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(x[j].x), "=f"(x[j].y), "=f"(x[j].z), "=f"(x[j].w)
-                         : "r"(cluster_addr(so + at * F::LDO + gl * 4, c)));
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[r][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int k = k0 + r * ROWS;
+            if (j0 + j < np && k < mine) {
+              const int i = k * (int)C + (int)rank, part = j0 + j;
+              x[r][j] = ld_remote4(so + (split ? i : (part & 1) * 128 + i) * F::LDO + gl * 4,
+                                   (uint32_t)(split ? part : part / 2));
+            }
           }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j0 + j < np) {
-            const float w = wgt[k * np + j0 + j];
-            if (w != 0.f) {  // a part without keys has no meaning for its row
-              acc.x = fmaf(x[j].x, w, acc.x);
-              acc.y = fmaf(x[j].y, w, acc.y);
-              acc.z = fmaf(x[j].z, w, acc.z);
-              acc.w = fmaf(x[j].w, w, acc.w);
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = k0 + r * ROWS;
+            if (j0 + j < np && k < mine) {
+              const float f = wgt[k * np + j0 + j];
+              if (f != 0.f) add_scaled(acc[r], x[r][j], f);  // a part without keys has no meaning for its row
             }
           }
       }
-      finish4(p, w, r0 + i, gl * 4, acc, 1.f, sh.mask, bad);
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        if (k0 + r * ROWS < mine)
+          finish4(p, w, r0 + (k0 + r * ROWS) * (int)C + (int)rank, gl * 4, acc[r], 1.f, sh.mask, bad);
     }
   }
   cluster_sync();

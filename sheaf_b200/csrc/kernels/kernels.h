@@ -284,7 +284,7 @@ cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
 // per cache head: up to 4 in f32, 8 in bf16, 16 over an int8 cache) multiply
 // with warp instructions (kernels/cache_attention_mma.cu), more rows with
 // tcgen05 (kernels/cache_attention_tc.cu).  Failed waits are reported through
-// the tensor-core error word, codes 50..67.
+// the tensor-core error word, codes 50..70.
 bool cache_attention_mma_takes(const CacheAttnArgs& a);
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream);
 bool cache_attention_tc_takes(const CacheAttnArgs& a);
