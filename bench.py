@@ -58,6 +58,9 @@ def parse():
                             "ref-vag", "ref-forward", "sweep", "nanogpt-decode"])
     p.add_argument("--op", default="softmax", choices=["softmax", "layer-norm", "gelu"],
                    help="sweep workload: the op (on [65536, --dim], gelu on 2^28 elements)")
+    p.add_argument("--cache", default="", choices=["", "f32", "bf16", "int8"],
+                   help="nanogpt-decode workload: key/value caches of this type, written and read by the decoding "
+                        "operators (default: f32 caches that the decoding program takes and returns)")
     p.add_argument("--dim", type=int, default=768, help="sweep workload: D of [65536, D]")
     p.add_argument("--dtype", default="f32", choices=["f32", "bf16"], help="sweep workload: tensor type")
     p.add_argument("--vjp", action="store_true", help="sweep workload: the VJP (value-and-grad) instead of the op")
@@ -632,6 +635,7 @@ def run_decode(args):
     adds the read-back of each step's token id to the host."""
     import torch
     from sheaf_b200 import build
+    from sheaf_b200.decode import CachedDecoder
     from sheaf_b200.session import B200Session, library
     from sheaf_lowering import generate as G
     from sheaf_lowering import models as M
@@ -668,6 +672,18 @@ def run_decode(args):
         for b in [tok, key] + caches:
             b.release()
         return nt, outs[2:], outs[1]
+
+    if args.cache:
+        # the same step with the caches outside the program
+        dec = CachedDecoder(sess, c, {n: inp[n] for n, _ in M.gpt_param_leaves(c)}, 1, args.cache)
+        sampler = G.sample_program(c, 200, 0.8)
+        sess.load_stablehlo(sampler.text)
+
+        def advance(p, tok, caches, key, read_back=False):
+            tok, key = sess.call_device(sampler.qualified, [dec.forward(tok, [p]), key])
+            if read_back:
+                float(tok.to_host()[0, 0])
+            return tok, caches, key
 
     for p in range(args.warmup):
         tok, caches, key = advance(p, tok, caches, key)
@@ -707,7 +723,9 @@ def run_decode(args):
                       "steps": args.steps, "warmup": args.warmup, "ms_per_step": ms, "higher_is_better": True,
                       "scaling": "none", "vs_baseline": None, "dtype": "f32", "contraction": args.precision,
                       "data": "synthetic: seeded N(0,0.02) weights, random prompt",
-                      "config": {"workload": f"nanogpt decode with key/value cache (top-k 200, temperature 0.8), "
+                      "config": {"workload": f"nanogpt decode with {args.cache and args.cache + ' '}key/value cache "
+                                             f"{'and the decoding operators ' if args.cache else ''}"
+                                             f"(top-k 200, temperature 0.8), "
                                              f"positions {args.warmup}..{args.warmup + args.steps - 1} of {c.T}",
                                  "model": f"L{c.n_layer} D{c.n_embd} H{c.n_head} T{c.T} V{c.vocab_size}",
                                  "l2": "weights and caches (48 MB) fit in L2: latency-bound by design"},

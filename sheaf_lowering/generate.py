@@ -185,3 +185,86 @@ def gpt_decode_program(c, top_k: int = 200, temp: float = 0.8) -> Lowered:
     out += body + rng.lines + e.body
     out += [f"    return {', '.join([nid, new_key] + cache_vals)} : {res_types}", " }", "}"]
     return Lowered("\n".join(out) + "\n", fwd.module + "_dec", "decode_token", fwd.arg_names + ["key"], [], [])
+
+
+# ---------------------------------------------------------------------------
+# Decoding over caches that live outside the programs: the same model cut at
+# the attention of each layer, so that the cache and the attention over it are
+# the runtime's operators (sb_kv_cache_write, sb_kv_cache_attention).  N
+# sequences ("slots") of S tokens per call; the token at wpe row `place`.
+#   start  (wte, wpe, next.*, token [N, S], place [N, S])  -> x [N, S, D], q, k, v
+#   layer  (done.*, next.*, x, y)                          -> x, q, k, v
+#   logits (done.*, ln_f, lm_head, x, y)                   -> [N S, V]
+# q, k, v and the attention's result y are [N, S, H, D / H]; `done.*` are the
+# weights behind the attention of the layer that y belongs to, `next.*` those
+# before the next layer's attention.
+# ---------------------------------------------------------------------------
+
+DONE_WEIGHTS = ("attn.c_proj.weight", "ln_2.weight", "mlp.c_fc.weight", "mlp.c_proj.weight")
+NEXT_WEIGHTS = ("attn.c_attn.weight", "ln_1.weight")
+
+
+def gpt_cached_programs(c, slots: int, tokens: int):
+    """{"start", "layer", "logits": Lowered} for `tokens` tokens of `slots` slots per call."""
+    from .lower import Vec, lower_forward
+    D, H, V, N, S = c.n_embd, c.n_head, c.vocab_size, slots, tokens
+    Hd = D // H
+    shapes = dict(M.gpt_param_leaves(c))
+    done = [("done." + w, shapes["transformer.h.0." + w]) for w in DONE_WEIGHTS]
+    nxt = [("next." + w, shapes["transformer.h.0." + w]) for w in NEXT_WEIGHTS]
+    wte, wpe, head, ln_f = ("transformer.wte.weight", "transformer.wpe.weight", "lm_head.weight",
+                            "transformer.ln_f.weight")
+    x = ("x", (N, S, D))
+    y = ("y", (N, S, H, Hd))
+
+    def into(t, s, x):
+        h = M.layer_norm_nb(t, x, s["next.ln_1.weight"])
+        W = s["next.attn.c_attn.weight"]
+        return [x] + [t("reshape", t("@", h, t("tr", t("slice", W, i * D, (i + 1) * D))), Vec([N, S, H, Hd]))
+                      for i in range(3)]
+
+    def out_of(t, s):
+        x = t("+", s["x"], t("@", t("reshape", s["y"], Vec([N, S, D])), t("tr", s["done.attn.c_proj.weight"])))
+        return t("+", x, M.mlp_block(t, M.layer_norm_nb(t, x, s["done.ln_2.weight"]), s, "done."))
+
+    def start(t, s):
+        return into(t, s, t("+", t("get", s[wte], s["token"]), t("get", s[wpe], s["place"])))
+
+    def logits(t, s):
+        h = M.layer_norm_nb(t, out_of(t, s), s[ln_f])
+        return t("reshape", t("@", h, t("tr", s[head])), Vec([N * S, V]))
+
+    key = f"{c}-{N}x{S}"
+    return {"start": lower_forward(start, [(wte, shapes[wte]), (wpe, shapes[wpe])] + nxt +
+                                   [("token", (N, S)), ("place", (N, S))], "decode_start", key=f"gpt-start-{key}"),
+            "layer": lower_forward(lambda t, s: into(t, s, out_of(t, s)), done + nxt + [x, y], "decode_layer",
+                                   key=f"gpt-layer-{key}"),
+            "logits": lower_forward(logits, done + [(ln_f, shapes[ln_f]), (head, shapes[head]), x, y],
+                                    "decode_logits", key=f"gpt-logits-{key}")}
+
+
+def token_program(groups: int, beams: int) -> Lowered:
+    """Selected tokens (i32 [groups, beams]) as the next step's f32 token argument [groups * beams, 1]."""
+    a, b = f"tensor<{groups}x{beams}x", f"tensor<{groups * beams}x1x"
+    mod = f"tokens_{groups}x{beams}"
+    text = (f"module @{mod} {{\n func.func @f(%arg0: {a}i32>) -> {b}f32> {{\n"
+            f"    %0 = stablehlo.convert %arg0 : ({a}i32>) -> {a}f32>\n"
+            f"    %1 = stablehlo.reshape %0 : ({a}f32>) -> {b}f32>\n"
+            f"    return %1 : {b}f32>\n }}\n}}\n")
+    return Lowered(text, mod, "f", ["tokens"], [], [])
+
+
+def sample_program(c, top_k: int = 200, temp: float = 0.8) -> Lowered:
+    """(logits [1, V], key) -> (next token [1, 1], new_key), sampling as generate-token does."""
+    V = c.vocab_size
+    e, lt = Emitter(), f"tensor<1x{V}xf32>"
+    logits = e.fresh()
+    e.line(f"    {logits} = stablehlo.reshape %arg0 : ({lt}) -> tensor<1x1x{V}xf32>")
+    rng = RandomEmitter()
+    nid, new_key = _tail(e, rng, logits, 1, V, top_k, temp, "%arg1")
+    tok = e.fresh()
+    e.line(f"    {tok} = stablehlo.reshape {nid} : (tensor<f32>) -> tensor<1x1xf32>")
+    mod, res = f"sample_{V}_{top_k}", "tensor<1x1xf32>, tensor<2xf32>"
+    text = "\n".join([f"module @{mod} {{", f" func.func @sample(%arg0: {lt}, %arg1: tensor<2xf32>) -> ({res}) {{"] +
+                     rng.lines + e.body + [f"    return {tok}, {new_key} : {res}", " }", "}"]) + "\n"
+    return Lowered(text, mod, "sample", ["logits", "key"], [], [])
