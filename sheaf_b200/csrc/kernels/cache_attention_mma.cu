@@ -37,6 +37,7 @@ namespace {
 
 using namespace cattn;
 
+constexpr int NW = 4;        // warps of a CTA
 constexpr float kLazy = 8.f;  // a row's maximum moves when it would grow by more than this (log2)
 
 // D += A B, 16 x 8 x 16, of bf16 or f16 values.
@@ -77,7 +78,7 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w, bool& bad) {
 // (kRows16) or 8 (kRows8: rows 8-15 of the second product hold what bf16 left of
 // P, so P has 16 bits), f32 queries of at most 4 rows (kF32).
 enum Mode { kRows16, kRows8, kF32 };
-template <int DP, bool I8, int MODE, int NW>
+template <int DP, bool I8, int MODE, int ST>
 struct MmaCfg {
   static constexpr int RMAX = MODE == kF32 ? 4 : MODE == kRows8 ? 8 : 16;  // rows of the CTA
   static constexpr int NR = MODE == kRows16 ? 2 : 1;                       // of a lane
@@ -89,7 +90,7 @@ struct MmaCfg {
   static constexpr int RB = DP * (I8 ? 1 : 2) < 128 ? 64 : 128;  // bytes of a row in a TMA box
   static constexpr int BOXES = DP * (I8 ? 1 : 2) / RB, BOX = KB * RB;
   // a warp's stage: K boxes, V boxes; its scales stand behind all stages
-  static constexpr int STAGE = 2 * BOXES * BOX, STAGES = 3;
+  static constexpr int STAGE = 2 * BOXES * BOX, STAGES = ST;
   static constexpr int SC_OFF = NW * STAGES * STAGE, END = SC_OFF + (I8 ? NW * STAGES * KB * 8 : 0);
   static constexpr int THREADS = NW * 32;
   static constexpr int JOIN = (NW + 1) * RMAX * DP * 4;
@@ -112,11 +113,11 @@ __device__ __forceinline__ int piece_at(int key, int u) {
   return key * RB + ((RB == 128 ? u ^ (key & 7) : u ^ (key >> 1 & 3)) << 4);
 }
 
-template <int DP, bool I8, int MODE, int NW>
+template <int DP, bool I8, int MODE, int ST>
 __global__ void __launch_bounds__(NW * 32)
     cache_attn_mma(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV, const Params p,
                    int* err) {
-  using F = MmaCfg<DP, I8, MODE, NW>;
+  using F = MmaCfg<DP, I8, MODE, ST>;
   constexpr bool Q32 = MODE == kF32;
   constexpr bool F16 = I8;  // operands: f16 for int8 caches, bf16 for bf16 ones
   constexpr int KB = F::KB, NB = KB / 8, KG = KB / 16, EK = F::EK, KL = F::KL, VL = F::VL, NR = F::NR, RMAX = F::RMAX;
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(NW * 32)
   auto fetch = [&](int64_t t, int st) {
     if (lane == 0 && !s_abort) {
       tc::mbar_expect_tx(&full[st], F::STAGE);
-uint8_t* dst = ring + st * F::STAGE;
+      uint8_t* dst = ring + st * F::STAGE;
       if (F::BOXES == 1 || p.D == DP) {
         tc::tma_load_4d(dst, &mK, &full[st], 0, (int)t, 0, (int)w.nh);
         tc::tma_load_4d(dst + F::BOXES * BOX, &mV, &full[st], 0, (int)t, 0, (int)w.nh);
@@ -479,9 +480,9 @@ uint8_t* dst = ring + st * F::STAGE;
   join_and_store<NW, RMAX, DP>(p, w, r0, rows, sm, s_m, s_l, sm + NW * RMAX * DP, s_ml, s_mask, I8 ? nullptr : &s_bad);
 }
 
-template <int DP, bool I8, int MODE, int NW>
+template <int DP, bool I8, int MODE, int ST>
 cudaError_t launch(const CacheAttnArgs& a, int C, cudaStream_t stream) {
-  using F = MmaCfg<DP, I8, MODE, NW>;
+  using F = MmaCfg<DP, I8, MODE, ST>;
   const Params p = make_params(a, F::RMAX);
   const KvCacheView& c = a.cache;
   CUtensorMap mk, mv;
@@ -491,20 +492,28 @@ cudaError_t launch(const CacheAttnArgs& a, int C, cudaStream_t stream) {
     return cudaErrorNotSupported;
   int* err = tc_error_word();
   if (!err) return cudaErrorMemoryAllocation;
-  return launch_cluster(cache_attn_mma<DP, I8, MODE, NW>, c.N * c.H * p.chunks * C, C, F::THREADS, F::SMEM, stream, mk,
+  return launch_cluster(cache_attn_mma<DP, I8, MODE, ST>, c.N * c.H * p.chunks * C, C, F::THREADS, F::SMEM, stream, mk,
                         mv, p, err);
 }
 
 template <int DP, bool I8, int MODE>
 cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
   const int64_t items = a.cache.N * a.cache.H;
-  // Many items: CTAs of two warps, of which an SM holds enough for one wave.
-  // Few: four warps, split until the SMs hold their CTAs or a warp would have
-  // one step.
-  if (items >= 3 * sm_count()) return launch<DP, I8, MODE, 2>(a, 1, stream);
+  constexpr int KB = MmaCfg<DP, I8, MODE, 3>::KB;
+  const int64_t row = a.cache.D * (I8 ? 1 : 2);  // bytes
+  // Items are split while the CTAs are one wave of three per SM and a warp keeps
+  // two steps; and, for batches of uneven lengths, which would end with their longest
+  // items alone, until no CTA has more than 256 KB of K (64 x 8 items of up to 4K
+  // bf16 keys of 128: 90 us, unsplit 114).
   int C = 1;
-  while (C < kMaxCluster && items * C < 3 * sm_count() && a.cache.T / (2 * C) >= 4 * MmaCfg<DP, I8, MODE, 4>::KB) C *= 2;
-  return launch<DP, I8, MODE, 4>(a, C, stream);
+  while (C < kMaxCluster && a.cache.T / (2 * C) >= 4 * KB &&
+         (items * 2 * C <= 3 * sm_count() || a.cache.T * row > C * (256 << 10)))
+    C *= 2;
+  // An SM holds two CTAs of three stages, or three of two (64 x 12 items of up to
+  // 1K int8 keys of 64: 24.5 us, 26.8 with three stages; 128 x 4 CTAs of 2K bf16 keys
+  // of 128 each: 90 / 97; one wave of two per SM, 32 x 8 of 3.8K int8 keys: 78 / 59).
+  if (items * C > 2 * sm_count()) return launch<DP, I8, MODE, 2>(a, C, stream);
+  return launch<DP, I8, MODE, 3>(a, C, stream);
 }
 
 }  // namespace
