@@ -261,6 +261,7 @@ cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t stream) {
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream) {
   if (cache_attention_mma_takes(a)) return cache_attention_mma(a, stream);
   if (cache_attention_tc_takes(a)) return cache_attention_tc(a, stream);
+  if (cache_attention_tile_takes(a)) return cache_attention_tile(a, stream);
   switch (a.cache.type) {
     case KvType::F32: return by_dim<float>(a, stream);
     case KvType::BF16: return by_dim<__nv_bfloat16>(a, stream);

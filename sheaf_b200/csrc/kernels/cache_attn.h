@@ -1,5 +1,6 @@
 // Parts shared by the kernels of attention over a key/value cache
-// (cache_attention.cu, cache_attention_mma.cu, cache_attention_tc.cu).
+// (cache_attention.cu, cache_attention_tile.cu, cache_attention_mma.cu,
+// cache_attention_tc.cu).
 // Included by .cu files only.
 #pragma once
 #include <cuda_bf16.h>
@@ -251,13 +252,13 @@ __device__ __forceinline__ void finish4(const Params& p, const Place& w, int row
   store4(p, row_at(p, w, row) + d, make_float4(y[0], y[1], y[2], y[3]));
 }
 
-// The partial results of up to R rows, joined and written: first the NW warps'
-// of a CTA, then the CTAs' of the cluster (rank c finishes every C-th piece of
-// 4 values).  part_o [NW][R][DP], part_m, part_l [NW][R] in shared memory (m:
-// base-2 maximum, l: sum); every thread of the CTA calls once it has written
-// its parts.  cta_o [R][DP] and cta_ml [2 R] are shared too; s_bad (may be
-// null): see finish4.
-template <int NW, int R, int DP>
+// The partial results of up to R rows, joined and written: first the PARTS of a
+// CTA of NW warps, then the CTAs' of the cluster (rank c finishes every C-th piece
+// of 4 values).  part_o [PARTS][R][DP], part_m, part_l [PARTS][R] in shared memory
+// (m: base-2 maximum, l: sum); every thread of the CTA calls once it has written
+// its parts.  cta_o [R][DP] (with one part, may be part_o) and cta_ml [2 R] are
+// shared too; s_bad (may be null): see finish4.
+template <int NW, int R, int DP, int PARTS = NW>
 __device__ __forceinline__ void join_and_store(const Params& p, const Place& w, int r0, int rows,
                                                const float* part_o, const float* part_m, const float* part_l,
                                                float* cta_o, float* cta_ml, const unsigned long long* mask,
@@ -267,16 +268,16 @@ __device__ __forceinline__ void join_and_store(const Params& p, const Place& w, 
   __syncthreads();
   for (int i = tid; i < rows * V; i += NW * 32) {
     const int r = i / V, d = (i % V) * 4;
-    float m[NW], f[NW], l = 0.f;
-    float4 x[NW], a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m[PARTS], f[PARTS], l = 0.f;
+    float4 x[PARTS], a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < NW; ++j) {
+    for (int j = 0; j < PARTS; ++j) {
       m[j] = part_m[j * R + r];
       x[j] = *(const float4*)(part_o + (j * R + r) * DP + d);
     }
-    const float mx = join_weights<NW>(m, f);
+    const float mx = join_weights<PARTS>(m, f);
 #pragma unroll
-    for (int j = 0; j < NW; ++j) {
+    for (int j = 0; j < PARTS; ++j) {
       add_scaled(a, x[j], f[j]);
       l = fmaf(part_l[j * R + r], f[j], l);
     }

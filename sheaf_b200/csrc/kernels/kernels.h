@@ -287,6 +287,8 @@ cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
 // the tensor-core error word, codes 50..70.
 bool cache_attention_mma_takes(const CacheAttnArgs& a);
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream);
+bool cache_attention_tile_takes(const CacheAttnArgs& a);  // of what the other two leave
+cudaError_t cache_attention_tile(const CacheAttnArgs& a, cudaStream_t stream);
 bool cache_attention_tc_takes(const CacheAttnArgs& a);
 cudaError_t cache_attention_tc(const CacheAttnArgs& a, cudaStream_t stream);
 
