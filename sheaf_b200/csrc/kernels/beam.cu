@@ -25,6 +25,15 @@
 // neighbours of the result from different beams are closer than twice that (or
 // tie), the group's sums are taken again in f64, whose exponentials would
 // otherwise bound the kernel.  So the order is that of f64 sums in every case.
+//
+// 32 x 8 beams over 50304 f32 logits (52 MB, 7.9 us of reading): 18.3 us (172 us
+// with every sum in f64).  About 10 us of that are not the pass but what 4 beams
+// over 65 values take as well (10.5 us): the launch, two cluster barriers, the
+// join and the second look at the W best lanes.
+//
+// The reordering moves bytes: 64 beams' caches of 12 layers, 12 heads, 1K positions
+// of 64 bf16 values (a third to nine tenths of them live): 395 us, 5.4 TB/s
+// written and read; a thread reads its 16 bytes of all beams before it writes any.
 #include <cuda_bf16.h>
 
 #include <cmath>
@@ -87,8 +96,9 @@ __device__ __forceinline__ void load_vec(const void* buf, int64_t at, float* x) 
 }
 
 // Values at .. at + N - 1 of the logits buffer (at: a multiple of N) where they
-// belong to the row [base, base + V), -inf elsewhere.  `inside`: all of them do.  The buffer's last values are loaded one by one where the 16
-// bytes would pass its end.
+// belong to the row [base, base + V), -inf elsewhere.  `inside`: all of them do.
+// The buffer's last values are loaded one by one where the 16 bytes would pass its
+// end.
 template <bool BF>
 __device__ __forceinline__ void load_piece(const void* buf, bool inside, int64_t at, int64_t base, int64_t V,
                                            int64_t total, float* x) {
@@ -523,7 +533,8 @@ cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
   if (a.G == 0) return cudaSuccess;
   SelectParams p = {a.logits, a.scores, a.finished, a.out_scores, a.out_parents, a.out_tokens, a.out_finished,
                     a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos};
-  // one CTA fits an SM: split while the CTAs stay one wave and a warp has a piece
+  // One CTA fits an SM: split while the CTAs stay one wave and a warp has a piece (32
+  // groups of 8 beams over 50304 values: 1 CTA each 50 us, 2: 28, 4: 18, 8: 38).
   const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);
   int dev = 0, sms = 148, C = 1;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

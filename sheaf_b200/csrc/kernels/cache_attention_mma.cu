@@ -216,11 +216,12 @@ __global__ void __launch_bounds__(NW * 32)
   // int8 word (bytes 0 and 2, bytes 1 and 3) or of consecutive bf16 values.
   // For f16 a row is scaled (f16_row_scale); S is multiplied back by `fs`.
   uint32_t q[DP / 16][4];
-  float fs[NR], sum_q[NR];
+  float fs[NR], pre[NR], sum_q[NR];
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     float up = 1.f;
     fs[r] = p.scale2;
+    pre[r] = 1.f;
     sum_q[r] = 0.f;
     if (F16) {
       float big = 0.f;
@@ -233,6 +234,9 @@ __global__ void __launch_bounds__(NW * 32)
       float down;
       up = f16_row_scale(big, down);
       fs[r] = p.scale2 * down;
+      // A row's factor up to 1 goes before the key's scale, a larger one after it:
+      // neither product passes f32's range unless the score does.
+      if (fabsf(fs[r]) <= 1.f) pre[r] = fs[r], fs[r] = 1.f;
     }
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
@@ -259,9 +263,7 @@ __global__ void __launch_bounds__(NW * 32)
     if (F16 && !Q32) {
       sum_q[r] += __shfl_xor_sync(0xffffffffu, sum_q[r], 1);
       sum_q[r] += __shfl_xor_sync(0xffffffffu, sum_q[r], 2);
-      // acc = 2^-24 sum q (c + 128):  S = acc 2^24 fs - 128 fs sum q
-      sum_q[r] *= 128.f * fs[r];
-      fs[r] *= 16777216.f;
+      sum_q[r] *= 128.f * pre[r];  // acc = 2^-24 sum q (c + 128):  S = (acc 2^24 - 128 sum q) pre fs
     }
   }
   __syncthreads();
@@ -314,15 +316,14 @@ __global__ void __launch_bounds__(NW * 32)
       for (int i = 0; i < 2; ++i) {
         if (Q32) {
           const float y = s[b][i] + s[b][2 + i];
-          x[b][0][i] = (y + __shfl_xor_sync(0xffffffffu, y, 16)) * fs[0];
+          x[b][0][i] = (y + __shfl_xor_sync(0xffffffffu, y, 16)) * (I8 ? pre[0] : 1.f);
         } else {
 #pragma unroll
           for (int r = 0; r < NR; ++r)
-            x[b][r][i] = I8 ? fmaf(s[b][2 * r + i], fs[r], -sum_q[r]) : s[b][2 * r + i] * fs[r];
+            x[b][r][i] = I8 ? fmaf(s[b][2 * r + i], 16777216.f * pre[r], -sum_q[r]) : s[b][2 * r + i];
         }
-        if (I8)
 #pragma unroll
-          for (int r = 0; r < NR; ++r) x[b][r][i] *= i ? f.y : f.x;
+        for (int r = 0; r < NR; ++r) x[b][r][i] = (I8 ? x[b][r][i] * (i ? f.y : f.x) : x[b][r][i]) * fs[r];
       }
     }
     const bool masked = t0 + KB > w.pre || t0 + KB > hi;
@@ -518,9 +519,17 @@ cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
+// As many rows as the instruction has.  There it is the faster one: 16 bf16 rows of
+// 4 x 8 caches of 30K keys of 128 take 86 us from bf16 and 67 from int8, on tcgen05
+// 97 and 128; of 8 x 12 caches of 465 keys of 64, 8.6 and 9.5, 12.4 and 14.8; 4 f32
+// rows of 16 x 8 caches of 4K keys of 128, 57 and 37, 90 and 137 (on the CUDA cores
+// 125 and 241).  Reading the cache bounds the long bf16 calls (one bf16 row of 4 x 8
+// x 30K keys of 128: 79 us, 6.2 TB/s); int8 ones (59 us, 4.3 TB/s) the conversion of
+// codes and of P, some five half-rate instructions per word of four codes; short ones
+// their set-up and joining, some 5 us.
 bool cache_attention_mma_takes(const CacheAttnArgs& a) {
   return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 &&
-         a.S * (a.Hq / a.cache.H) <= (!a.bf16 ? 4 : a.cache.type == KvType::I8 ? 16 : 8);
+         a.S * (a.Hq / a.cache.H) <= (a.bf16 ? 16 : 4);
 }
 
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream) {
@@ -529,8 +538,10 @@ cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream) {
     if (i8) return wide ? by_items<128, true, kF32>(a, stream) : by_items<64, true, kF32>(a, stream);
     return wide ? by_items<128, false, kF32>(a, stream) : by_items<64, false, kF32>(a, stream);
   }
-  if (a.S * (a.Hq / a.cache.H) > 8)  // int8 only
-    return wide ? by_items<128, true, kRows16>(a, stream) : by_items<64, true, kRows16>(a, stream);
+  if (a.S * (a.Hq / a.cache.H) > 8) {
+    if (i8) return wide ? by_items<128, true, kRows16>(a, stream) : by_items<64, true, kRows16>(a, stream);
+    return wide ? by_items<128, false, kRows16>(a, stream) : by_items<64, false, kRows16>(a, stream);
+  }
   if (i8) return wide ? by_items<128, true, kRows8>(a, stream) : by_items<64, true, kRows8>(a, stream);
   return wide ? by_items<128, false, kRows8>(a, stream) : by_items<64, false, kRows8>(a, stream);
 }

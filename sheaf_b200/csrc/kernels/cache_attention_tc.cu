@@ -33,6 +33,14 @@
 // finite is taken out of the tile and added to the rows that attend to it when
 // the outputs are joined.
 //
+// 8 x 4 caches of 16K keys of 128, 256 bf16 rows (69 GFLOP, 41 us of tensor time,
+// bf16 cache 22 us of reading): 80 us from bf16, 0.86 PFLOP/s, 1.9K cycles per
+// tile of which the MMAs take three quarters; 119 us from int8, whose softmax
+// (two more multiplications per score) and conversion take 2.9K.  f32 queries
+// have three times the products: 194 and 277 us.  63 f32 rows over 8 x 12 caches
+// of 1K keys of 64: 22 and 30 us, of which 12 are there without a cache: the
+// launch, the staging of the queries, the cluster's join.
+//
 // Every mbarrier wait is bounded.  TMEM is freed before the cluster barrier: a
 // CTA that holds TMEM never waits for another CTA.
 #include <type_traits>
@@ -52,6 +60,8 @@ constexpr int kSoftWarps = 8, kLoadWarps = 4, kMmaWarp = 12, kFeedWarp = 14, kWa
 constexpr int kStageWarps = kSoftWarps + kLoadWarps;
 constexpr int kLoadThreads = kLoadWarps * 32;
 constexpr int BN = 64;  // keys of a tile
+// Sums of query x code stay below 2^30: times a key scale below this they are finite.
+constexpr float kBigScale = 1.2379400392853803e27f;  // 2^90
 constexpr float kLazy = 8.f;  // a row's maximum moves when it would grow by more than this (log2)
 
 // MMAs and commits issued by one elected lane of a converged warp: the operands
@@ -183,6 +193,7 @@ struct Shared {
   volatile int abort_flag;
   int bad;  // a drafted value that is not finite was taken out of a tile
   int q_row[256];  // query row of a staged row, in units of D values from the slot and head's first; -1: none
+  int sc_big[8];  // a key scale of the tile is 2^90 or more
   int sc_ref[8];  // exponent that a tile's value scales are relative to
   unsigned long long mask[kKvMaxTokens];
   int jump[kKvMaxTokens];
@@ -405,9 +416,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           vref = top;
         }
         auto moves = [&](float mx) { return __any_sync(0xffffffffu, mx > m + kLazy); };
-        // P of the tile from S; `vis`: the columns the row sees
+        // P of the tile from S; `vis`: the columns the row sees.  The masked way also
+        // takes any scale: a row's factor f0 up to 1 goes before the key's, a larger
+        // one after it, so that neither product passes f32's range unless the score does.
         auto softmax = [&](auto mask_tag, const uint32_t* vis) {
           constexpr bool MASK = decltype(mask_tag)::value;
+          const float pre = MASK && I8 ? fminf(f0, 1.f) : 1.f, f1 = MASK && I8 ? fmaxf(f0, 1.f) : f0;
           if constexpr (QP == 1) {
             // One pass with the maximum as it stands: P is kept in registers
             // until the tile's own maximum is known.  If that moved too far
@@ -437,12 +451,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float2 s = make_float2(__uint_as_float(x[j + 2 * k]), __uint_as_float(x[j + 2 * k + 1]));
                     const bool v0 = !MASK || (vis[c / 32] >> (j + 2 * k) & 1u);
                     const bool v1 = !MASK || (vis[c / 32] >> (j + 2 * k + 1) & 1u);
+                    if (I8 && MASK) s = mul2(s, make_float2(pre, pre));
                     if (I8) s = mul2(s, g[k]);
                     if (MASK) s.x = v0 ? s.x : -INFINITY, s.y = v1 ? s.y : -INFINITY;
                     mx = fmaxf(mx, fmaxf(s.x, s.y));
-                    s = fma2(s, make_float2(f0, f0), nb);
+                    s = fma2(s, make_float2(f1, f1), nb);
                     float2 y = make_float2(ex2(s.x), ex2(s.y));
-                    if (MASK) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;  // f0 may be 0
+                    if (MASK) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;  // f1 may be 0
                     s2 = add2(s2, y);
                     if (I8) {
                       y = mul2(y, h2[k]);
@@ -452,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   }
                 }
               }
-              if (mx != -INFINITY) mx *= f0;
+              if (mx != -INFINITY) mx *= f1;
               if (moves(mx)) {
                 rescale(mx);
                 if (!ok) return;
@@ -479,13 +494,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                   float s = __uint_as_float(r[j + k]);
-                  if (I8) s *= g[k];
+                  if (I8) s = s * pre * g[k];
                   if (MASK && !(vis[c / 32] >> (j + k) & 1u)) s = -INFINITY;
                   mx = fmaxf(mx, s);
                 }
               }
             }
-            if (mx != -INFINITY) mx *= f0;
+            if (mx != -INFINITY) mx *= f1;
             if (moves(mx)) {
               rescale(mx);
               if (!ok) return;
@@ -510,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   for (int k = 0; k < 4; ++k) {
                     const bool see = !MASK || (vis[c / 32] >> (half + j + k) & 1u);
                     const float s = __uint_as_float(r[half + j + k]);
-                    y[k] = ex2(I8 ? fmaf(s * g[k], f0, -base) : s - base);
+                    y[k] = ex2(I8 ? fmaf(s * pre * g[k], f1, -base) : s - base);
                     if (MASK) y[k] = see ? y[k] : 0.f;
                     x[j + k] = y[k];
                     if (I8 && see) x[j + k] *= h4[k];
@@ -528,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         };
-        if (t0 + BN > pre) {
+        if (t0 + BN > pre || (I8 && sh.sc_big[t % NSC])) {
           uint32_t vis[BN / 32];
           const int64_t off = pos - t0;  // column of drafted token 0
 #pragma unroll
@@ -684,7 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           sc_k[t % NSC][i * 32 + lane] = ck[i];
           sc_v[t % NSC][i * 32 + lane] = cv[i] * down;
         }
-        if (lane == 0) sh.sc_ref[t % NSC] = vref;
+        const bool big = __any_sync(0xffffffffu, !(ck[0] < kBigScale && ck[1] < kBigScale));
+        if (lane == 0) sh.sc_ref[t % NSC] = vref, sh.sc_big[t % NSC] = big;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.sc_full[t % NSC]);
         fetch_scales(t + 1);
@@ -919,7 +935,9 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   int* err = tc_error_word();
   if (!err) return cudaErrorMemoryAllocation;
   const int64_t items = c.N * c.H * p.chunks;
-  // one CTA fits an SM: split until the CTAs fill the SMs once, or a CTA has four tiles
+  // One CTA fits an SM (shared memory, and all of its TMEM): split until the CTAs
+  // fill the SMs once, or a CTA has four tiles, since a second wave would repeat the
+  // 10 us that a CTA takes without keys.
   int C = 1;
   while (C < kMaxCluster && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 4 * BN) ++C;
   return launch_cluster(cache_attn_tc<DP, QP, I8>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);

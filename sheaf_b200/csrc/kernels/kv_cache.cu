@@ -10,6 +10,11 @@
 // and attention can apply it to a score or a probability instead of a row.
 // A NaN is written as 0 and an infinity as the largest finite f32, so that one
 // bad value leaves the row's other codes usable.
+//
+// Bytes bound both.  8 x 1024 tokens of 12 heads of 64, f32 to int8, and the read
+// back to f32 (128 MB): 27.4 us, 4.7 TB/s (much of it stays in L2 between the two);
+// a ragged read of 24 slots of 4K positions, int8 to f32 (430 MB): 72 us, 6.0
+// TB/s, 0.92 of a copy; one token of one sequence: 4 us, the latency of a launch.
 #include <cuda_bf16.h>
 
 #include <cfloat>
@@ -108,58 +113,50 @@ struct WriteParams {
 };
 
 // A group of LPR lanes carries one row: with 8 values a lane the row's largest
-// magnitude is a butterfly of log2(LPR) shuffles.  A block takes RPT rows per
-// group of one slot's keys, then values; all their loads come first.
-template <typename TI, typename TC, int LPR, int RPT>
+// magnitude is a butterfly of log2(LPR) shuffles.  The groups of a block take rows
+// of one slot's keys, then values.  (Four rows per group, their loads first, were no
+// faster for a prompt, 13.1 us against 13.0, and slower for less: 8 x 64 tokens 3.3
+// and 2.4.)
+template <typename TI, typename TC, int LPR>
 __global__ void __launch_bounds__(kThreads) write_kernel(const WriteParams p) {
   pdl_prologue();
-  constexpr int GROUPS = kThreads / LPR;
   const int lane = threadIdx.x % LPR;
-  const unsigned n = blockIdx.x / p.blocks, r0 = blockIdx.x % p.blocks * (GROUPS * RPT) + threadIdx.x / LPR;
-  const int64_t first = p.pos[n];
-  float x[RPT][EPL];
-  int64_t at[RPT];
-  unsigned which[RPT];
+  const unsigned n = blockIdx.x / p.blocks;
+  unsigned r = blockIdx.x % p.blocks * (kThreads / LPR) + threadIdx.x / LPR;
+  const unsigned which = r >= p.rows;
+  if (which) r -= p.rows;
+  const unsigned s = r / p.H, h = r - s * p.H;
+  const int64_t first = p.pos[n], t = first + s;
+  const bool in = r < p.rows && first >= 0 && t < p.T && lane * EPL < p.D;
+  const int64_t at = ((int64_t)n * p.H + h) * p.T + t;
+  float x[EPL];
 #pragma unroll
-  for (int k = 0; k < RPT; ++k) {
-    unsigned r = r0 + k * GROUPS;
-    which[k] = r >= p.rows;
-    if (which[k]) r -= p.rows;
-    const unsigned s = r / p.H, h = r - s * p.H;
-    const int64_t t = first + s;
-    const bool in = r < p.rows && first >= 0 && t < p.T && lane * EPL < p.D;
-    at[k] = in ? ((int64_t)n * p.H + h) * p.T + t : -1;
+  for (int i = 0; i < EPL; ++i) x[i] = 0.f;
+  if (in) load8((const TI*)(which ? p.src[1] : p.src[0]) + ((int64_t)n * p.rows + r) * p.D + lane * EPL, x);
+  if constexpr (sizeof(TC) == 1) {
+    float m = 0.f, odd = 0.f;  // odd: NaN unless all values are finite
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) x[k][i] = 0.f;
-    if (in) load8((const TI*)(which[k] ? p.src[1] : p.src[0]) + ((int64_t)n * p.rows + r) * p.D + lane * EPL, x[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < RPT; ++k) {
-    if constexpr (sizeof(TC) == 1) {
-      float m = 0.f, odd = 0.f;  // odd: NaN unless all values are finite
+    for (int i = 0; i < EPL; ++i) {
+      odd = fmaf(x[i], 0.f, odd);
+      m = fmaxf(m, fabsf(x[i]));
+    }
+    if (odd != 0.f) {
+      m = 0.f;
 #pragma unroll
       for (int i = 0; i < EPL; ++i) {
-        odd = fmaf(x[k][i], 0.f, odd);
-        m = fmaxf(m, fabsf(x[k][i]));
+        x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -FLT_MAX), FLT_MAX);
+        m = fmaxf(m, fabsf(x[i]));
       }
-      if (odd != 0.f) {
-        m = 0.f;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i) {
-          x[k][i] = x[k][i] != x[k][i] ? 0.f : fminf(fmaxf(x[k][i], -FLT_MAX), FLT_MAX);
-          m = fmaxf(m, fabsf(x[k][i]));
-        }
-      }
-#pragma unroll
-      for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float sc = __fdiv_rn(m, 127.f);
-      if (at[k] >= 0) {
-        *(uint2*)((int8_t*)(which[k] ? p.dst[1] : p.dst[0]) + at[k] * p.D + lane * EPL) = codes8(x[k], sc);
-        if (lane == 0) (which[k] ? p.scale[1] : p.scale[0])[at[k]] = sc;
-      }
-    } else {
-      if (at[k] >= 0) store8((TC*)(which[k] ? p.dst[1] : p.dst[0]) + at[k] * p.D + lane * EPL, x[k]);
     }
+#pragma unroll
+    for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float sc = __fdiv_rn(m, 127.f);
+    if (in) {
+      *(uint2*)((int8_t*)(which ? p.dst[1] : p.dst[0]) + at * p.D + lane * EPL) = codes8(x, sc);
+      if (lane == 0) (which ? p.scale[1] : p.scale[0])[at] = sc;
+    }
+  } else {
+    if (in) store8((TC*)(which ? p.dst[1] : p.dst[0]) + at * p.D + lane * EPL, x);
   }
 }
 
@@ -242,31 +239,22 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ReadParams p) {
   }
 }
 
-template <typename TI, typename TC, int LPR, int RPT>
+template <typename TI, typename TC, int LPR>
 cudaError_t launch_write(WriteParams p, int64_t N, cudaStream_t stream) {
-  const int64_t per = kThreads / LPR * RPT;
+  constexpr int64_t per = kThreads / LPR;
   const int64_t blocks = (2 * (int64_t)p.rows + per - 1) / per;
   if (blocks * N > INT32_MAX) return cudaErrorInvalidValue;
   p.blocks = (unsigned)blocks;
-  return launch_pdl(write_kernel<TI, TC, LPR, RPT>, dim3((unsigned)(blocks * N)), dim3(kThreads), 0, stream, p);
-}
-
-template <typename TI, typename TC, int LPR>
-cudaError_t by_rows(const WriteParams& p, int64_t N, cudaStream_t stream) {
-  // several rows per group once there are blocks for every SM all the same
-  constexpr int64_t groups = kThreads / LPR;
-  if (2 * (int64_t)p.rows >= 4 * groups && N * 2 * p.rows / (4 * groups) >= 296)
-    return launch_write<TI, TC, LPR, 4>(p, N, stream);
-  return launch_write<TI, TC, LPR, 1>(p, N, stream);
+  return launch_pdl(write_kernel<TI, TC, LPR>, dim3((unsigned)(blocks * N)), dim3(kThreads), 0, stream, p);
 }
 
 template <typename TI, typename TC>
 cudaError_t write_rows(const WriteParams& p, int64_t N, cudaStream_t stream) {
-  if (p.D <= 16) return by_rows<TI, TC, 2>(p, N, stream);
-  if (p.D <= 32) return by_rows<TI, TC, 4>(p, N, stream);
-  if (p.D <= 64) return by_rows<TI, TC, 8>(p, N, stream);
-  if (p.D <= 128) return by_rows<TI, TC, 16>(p, N, stream);
-  return by_rows<TI, TC, 32>(p, N, stream);
+  if (p.D <= 16) return launch_write<TI, TC, 2>(p, N, stream);
+  if (p.D <= 32) return launch_write<TI, TC, 4>(p, N, stream);
+  if (p.D <= 64) return launch_write<TI, TC, 8>(p, N, stream);
+  if (p.D <= 128) return launch_write<TI, TC, 16>(p, N, stream);
+  return launch_write<TI, TC, 32>(p, N, stream);
 }
 
 template <typename TC, typename TO>

@@ -48,6 +48,16 @@ sb_status* cuda_status(cudaError_t e, const char* what) {
                                cudaGetErrorString(e) + ")");
 }
 
+// No exception leaves an entry point (an allocation of the host may fail).
+template <typename F>
+sb_status* op_guarded(F f) {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    return make_status(SB_STATUS_RESOURCE_EXHAUSTED, e.what());
+  }
+}
+
 #define SB_CUDA(expr)                                   \
   do {                                                  \
     cudaError_t e_ = (expr);                            \
@@ -1829,12 +1839,20 @@ sb_status* op_rank4(const sb_buffer* b, const char* what) {
   return nullptr;
 }
 
+sb_status* op_launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return nullptr;
+  if (e == cudaErrorInvalidValue)
+    return make_status(SB_STATUS_INVALID_ARGUMENT, std::string(what) + ": too large for one launch");
+  return cuda_status(e, what);
+}
+
 const int* ints(const sb_buffer* b) { return b ? (const int*)b->ptr : nullptr; }
 
 }  // namespace
 
 sb_status* sb_kv_cache_write(sb_session* s, const sb_kv_cache* cache, sb_buffer* positions, sb_buffer* k,
                              sb_buffer* v) {
+  return op_guarded([&]() -> sb_status* {
   if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
   KvCacheView c;
   SB_OP(op_cache(s, cache, &c));
@@ -1850,11 +1868,13 @@ sb_status* sb_kv_cache_write(sb_session* s, const sb_kv_cache* cache, sb_buffer*
   SB_CUDA(cudaSetDevice(s->dev->ordinal));
   if (!k->bytes || !c.T) return nullptr;
   cudaError_t e = kv_cache_write(c, ints(positions), k->ptr, v->ptr, k->type.dtype == DType::BF16, S, s->dev->stream);
-  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_write");
+  return op_launched(e, "sb_kv_cache_write");
+  });
 }
 
 sb_status* sb_kv_cache_read(sb_session* s, const sb_kv_cache* cache, sb_buffer* starts, sb_buffer* counts,
                             sb_buffer* k_out, sb_buffer* v_out) {
+  return op_guarded([&]() -> sb_status* {
   if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
   KvCacheView c;
   SB_OP(op_cache(s, cache, &c));
@@ -1872,11 +1892,13 @@ sb_status* sb_kv_cache_read(sb_session* s, const sb_kv_cache* cache, sb_buffer* 
   if (!k_out->bytes || !c.T) return nullptr;
   cudaError_t e = kv_cache_read(c, ints(starts), ints(counts), k_out->ptr, v_out->ptr,
                                 k_out->type.dtype == DType::BF16, S, s->dev->stream);
-  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_read");
+  return op_launched(e, "sb_kv_cache_read");
+  });
 }
 
 sb_status* sb_kv_cache_attention(sb_session* s, const sb_kv_cache* cache, sb_buffer* positions, sb_buffer* parents,
                                  sb_buffer* q, float scale, sb_buffer* out) {
+  return op_guarded([&]() -> sb_status* {
   if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
   KvCacheView c;
   SB_OP(op_cache(s, cache, &c));
@@ -1914,12 +1936,14 @@ sb_status* sb_kv_cache_attention(sb_session* s, const sb_kv_cache* cache, sb_buf
   a.scale = scale;
   if (cache_attention_tc_takes(a) || cache_attention_mma_takes(a)) s->used_tc = true;
   cudaError_t e = cache_attention(a, s->dev->stream);
-  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_kv_cache_attention");
+  return op_launched(e, "sb_kv_cache_attention");
+  });
 }
 
 sb_status* sb_beam_select(sb_session* s, sb_buffer* logits, sb_buffer* scores, sb_buffer* finished, int64_t eos,
                           sb_buffer* out_scores, sb_buffer* out_parents, sb_buffer* out_tokens,
                           sb_buffer* out_finished) {
+  return op_guarded([&]() -> sb_status* {
   if (!s) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL session");
   if (!scores || !logits) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL buffer");
   if (scores->type.shape.size() != 2 || logits->type.shape.size() != 2)
@@ -1966,11 +1990,13 @@ sb_status* sb_beam_select(sb_session* s, sb_buffer* logits, sb_buffer* scores, s
   a.out_finished = out_finished ? (int*)out_finished->ptr : nullptr;
   a.eos = eos < 0 ? -1 : eos;
   cudaError_t e = beam_select(a, s->dev->stream);
-  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_beam_select");
+  return op_launched(e, "sb_beam_select");
+  });
 }
 
 sb_status* sb_beam_reorder(sb_session* s, size_t count, sb_buffer* const* states, const int32_t* time_axes,
                            sb_buffer* parents, sb_buffer* lengths) {
+  return op_guarded([&]() -> sb_status* {
   if (!s || (count && (!states || !time_axes))) return make_status(SB_STATUS_INVALID_ARGUMENT, "NULL argument");
   if (!parents || parents->type.shape.size() != 2)
     return make_status(SB_STATUS_INVALID_ARGUMENT, "parents has two dimensions: groups and beams");
@@ -2008,7 +2034,8 @@ sb_status* sb_beam_reorder(sb_session* s, size_t count, sb_buffer* const* states
   SB_CUDA(cudaSetDevice(s->dev->ordinal));
   if (W == 1) return nullptr;  // nothing can move
   cudaError_t e = beam_reorder(st.data(), (int64_t)count, ints(parents), ints(lengths), G, W, s->dev->stream);
-  return e == cudaSuccess ? nullptr : cuda_status(e, "sb_beam_reorder");
+  return op_launched(e, "sb_beam_reorder");
+  });
 }
 
 sb_status* sb_buffer_d2h(sb_session* s, sb_buffer* b, void* host, size_t bytes, int64_t timeout_ms) {

@@ -289,6 +289,26 @@ def test_attention_scales(sess, kind, src, scale, n_tok, G, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D", [(1, 1, 64), (1, 4, 128), (6, 2, 64), (20, 2, 64), (12, 1, 32)])
+@pytest.mark.parametrize("e", [-110, 115])
+def test_attention_of_ordinary_scores_from_extreme_factors(sess, src, n_tok, G, D, e):
+    """Queries near an end of f32's range over int8 keys whose scales undo it (both by powers of two)."""
+    rng = np.random.default_rng(n_tok + D)
+    N, H, T = 2, 2, 90
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), "int8")
+    scales[0] = np.ldexp(scales[0], -e)
+    cache.k_scale = put(sess, scales[0])
+    q = np.ldexp(rand(rng, (N, n_tok, G * H, D), src), e)
+    pos = [T - n_tok, 17]
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, 1 / math.sqrt(D))
+    out = put(sess, np.zeros(q.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
+    assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("src", ["f32", "bf16"])
 @pytest.mark.parametrize("n_tok,G,D", [(1, 1, 64), (1, 4, 128), (6, 2, 64), (40, 2, 64), (40, 4, 128)])
