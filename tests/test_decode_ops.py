@@ -226,6 +226,10 @@ ATT_CASES = [  # slots, tokens, q heads, heads, capacity, head size, positions
     (1, 33, 8, 1, 777, 64, [700]),
     (1, 9, 4, 2, 70, 256, [50]),
     (2, 12, 2, 1, 33, 16, [20, 30]),
+    (2, 10, 6, 3, 75, 48, [20, 70]),
+    (1, 20, 4, 2, 140, 96, [100]),
+    (2, 8, 4, 2, 150, 112, [9, 140]),
+    (1, 64, 3, 1, 200, 64, [130]),                    # 192 rows
 ]
 
 
@@ -241,14 +245,12 @@ def tree_of(rng, N, n_tok):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("case", ATT_CASES, ids=lambda c: "x".join(map(str, c[:6])))
+@pytest.mark.parametrize("case,tree", [(c, t) for c in ATT_CASES for t in (False, True) if c[1] > 1 or not t],
+                         ids=lambda c: "x".join(map(str, c[:6])) if isinstance(c, tuple) else "tree" if c else "chain")
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("src", ["f32", "bf16"])
-@pytest.mark.parametrize("tree", [False, True])
 def test_attention(sess, case, kind, src, tree):
     N, n_tok, Hq, H, T, D, pos = case
-    if tree and n_tok == 1:
-        pytest.skip("one token has no tree")
     rng = np.random.default_rng(n_tok * 1000 + T + D)
     cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
     q = rand(rng, (N, n_tok, Hq, D), src)
