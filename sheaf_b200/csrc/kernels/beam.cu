@@ -26,7 +26,7 @@
 // tie), the group's sums are taken again in f64, whose exponentials would
 // otherwise bound the kernel.  So the order is that of f64 sums in every case.
 //
-// 32 x 8 beams over 50304 f32 logits (52 MB, 7.9 us of reading): 18.3 us (172 us
+// 32 x 8 beams over 50304 f32 logits (52 MB, 7.9 us of reading): 17.3 us (172 us
 // with every sum in f64).  About 10 us of that are not the pass but what 4 beams
 // over 65 values take as well (10.5 us): the launch, two cluster barriers, the
 // join and the second look at the W best lanes.
@@ -175,10 +175,27 @@ __device__ __forceinline__ Row row_of(const SelectParams& p, int64_t row) {
 template <bool BF>
 __device__ __forceinline__ void load_row(const SelectParams& p, const Row& r, int64_t c, int lane, float* x) {
   constexpr int N = BF ? 8 : 4;
-  const bool inside = r.first + c * kPiece >= r.base && r.first + (c + 1) * kPiece <= r.base + p.V;
+  const int64_t at0 = r.first + c * kPiece + lane * N;
+  if (r.first + c * kPiece >= r.base && r.first + (c + 1) * kPiece <= r.base + p.V) {
 #pragma unroll
-  for (int i = 0; i < EPC / N; ++i)
-    load_piece<BF>(p.logits, inside, r.first + c * kPiece + (i * 32 + lane) * N, r.base, p.V, p.total, x + i * N);
+    for (int i = 0; i < EPC / N; ++i) load_vec<BF>(p.logits, at0 + i * 32 * N, x + i * N);
+  } else {  // the row begins or ends in this piece: all loads first, then what does not belong to it
+#pragma unroll
+    for (int i = 0; i < EPC / N; ++i) {
+      const int64_t at = at0 + i * 32 * N;
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[i * N + k] = -INFINITY;
+      if (at < r.base + p.V && at + N <= p.total) load_vec<BF>(p.logits, at, x + i * N);
+    }
+#pragma unroll
+    for (int i = 0; i < EPC / N; ++i) {
+      const int64_t at = at0 + i * 32 * N;
+      if (at < r.base + p.V && at + N > p.total) load_piece<BF>(p.logits, false, at, r.base, p.V, p.total, x + i * N);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (at + k < r.base || at + k >= r.base + p.V) x[i * N + k] = -INFINITY;
+    }
+  }
 }
 __device__ __forceinline__ u64 key_of(float x, int64_t idx) {
   return (u64)ordered(x) << 32 | (uint32_t)~(uint32_t)idx;
@@ -534,7 +551,7 @@ cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
   SelectParams p = {a.logits, a.scores, a.finished, a.out_scores, a.out_parents, a.out_tokens, a.out_finished,
                     a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos};
   // One CTA fits an SM: split while the CTAs stay one wave and a warp has a piece (32
-  // groups of 8 beams over 50304 values: 1 CTA each 50 us, 2: 28, 4: 18, 8: 38).
+  // groups of 8 beams over 50304 values: 1 CTA each 50 us, 2: 28, 4: 17, 8: 38).
   const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);
   int dev = 0, sms = 148, C = 1;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

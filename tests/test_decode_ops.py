@@ -269,6 +269,26 @@ def test_attention(sess, case, kind, src, tree):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("N,H,n_tok", [(71, 8, 1), (128, 4, 2), (131, 4, 1)])
+def test_attention_of_many_uneven_slots(sess, kind, src, N, H, n_tok):
+    """More (slot, head) pairs than run at once; idle, empty, equal and full slots among them."""
+    T, D = 150, 64
+    rng = np.random.default_rng(N)
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    pos = rng.integers(0, T, N)
+    pos[[0, 5, 9, 30]] = -1, 0, 2 ** 31 - 1, -7
+    pos[40:50] = 77
+    q = rand(rng, (N, n_tok, H, D), src)
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, 1 / math.sqrt(D))
+    out = put(sess, np.full(q.shape, 7.0, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
+    assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
 @pytest.mark.parametrize("scale", [0.0, -0.2, 40.0])
 @pytest.mark.parametrize("n_tok,G,D", [(1, 2, 64), (20, 2, 64), (40, 4, 128)])
 def test_attention_scales(sess, kind, src, scale, n_tok, G, D):
