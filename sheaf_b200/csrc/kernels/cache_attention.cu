@@ -51,7 +51,9 @@ __device__ __forceinline__ void load_raw(const float* p, Raw<float>& r) {
                : "l"(p));
 }
 __device__ __forceinline__ void load_raw(const __nv_bfloat16* p, Raw<__nv_bfloat16>& r) {
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w)
+               : "l"(p));
 }
 __device__ __forceinline__ void load_raw(const int8_t* p, Raw<int8_t>& r) {
   asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.a.x), "=r"(r.a.y) : "l"(p));

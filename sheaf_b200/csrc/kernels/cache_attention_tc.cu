@@ -188,7 +188,8 @@ struct Cfg {
 };
 
 struct Shared {
-  uint64_t k_full[4], k_free[4], v_full[4], v_free[4], sc_full[8], s_bar[2][2], p_bar[2][2], o_bar[2], raw, mended, q_bar;
+  uint64_t k_full[4], k_free[4], v_full[4], v_free[4], sc_full[8], s_bar[2][2], p_bar[2][2], o_bar[2];
+  uint64_t raw, mended, q_bar;
   uint32_t tslot;
   volatile int abort_flag;
   int bad;  // a drafted value that is not finite was taken out of a tile
@@ -771,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < DP / 16; ++kk)
             mma_ss(ts, qd + ((part * F::QTILE + (kk / 4) * 128 * 128 + (kk % 4) * 32) >> 4),
-                     kd + (((kk / 4) * BN * 128 + (kk % 4) * 32) >> 4), id_s, part < QP - 1 || kk > 0 ? 1u : 0u);
+                   kd + (((kk / 4) * BN * 128 + (kk % 4) * 32) >> 4), id_s, part < QP - 1 || kk > 0 ? 1u : 0u);
         commit(&sh.s_bar[a][i % SB]);
         commit(&sh.k_free[t % NS]);
         return true;

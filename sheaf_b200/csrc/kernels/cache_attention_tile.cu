@@ -191,8 +191,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
             if (!(t < hi && (t < w.pre || (seen >> (t - w.pos) & 1ull)))) s[r][j] = -INFINITY;
           }
         }
-        float mx = s[r][0];
-        mx = warp_max(fmaxf(mx, s[r][1]));
+        const float mx = warp_max(fmaxf(s[r][0], s[r][1]));
         if (mx > m[r]) {
           const float f = tc::ex2(m[r] - mx);
           l[r] *= f;

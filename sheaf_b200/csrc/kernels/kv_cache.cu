@@ -259,7 +259,8 @@ cudaError_t write_rows(const WriteParams& p, int64_t N, cudaStream_t stream) {
 
 template <typename TC, typename TO>
 cudaError_t read_rows(ReadParams p, int64_t N, cudaStream_t stream) {
-  const int64_t units = p.S * (p.D * (int64_t)sizeof(TC) / 16), blocks = (units + kThreads * kReadUnits - 1) / (kThreads * kReadUnits);
+  constexpr int64_t per = kThreads * kReadUnits;
+  const int64_t units = p.S * (p.D * (int64_t)sizeof(TC) / 16), blocks = (units + per - 1) / per;
   if (blocks * 2 * N * p.H > INT32_MAX) return cudaErrorInvalidValue;
   p.blocks = (unsigned)blocks;
   return launch_pdl(read_kernel<TC, TO>, dim3((unsigned)(blocks * 2 * N * p.H)), dim3(kThreads), 0, stream, p);
