@@ -21,7 +21,8 @@
 // split needs no workspace in memory and no atomics: results do not depend on
 // timing, and graphs that run at the same time share nothing.
 //
-// It takes f32 caches and heads outside 64 .. 128, up to 8 rows or over 128 values.
+// It takes up to 8 rows over f32 caches, up to 3 over others of heads of 32 or less,
+// and every call of heads over 128.
 // One row of 4 x 8 f32 caches of 30K keys of 128: 148 us, 6.6 TB/s, as fast as a
 // copy; of 64 x 12 caches of 512 keys of 64: 38 us, 5.4 TB/s; of one sequence of
 // 200 keys, 6 heads: 4.1 us, launch and latency.  From 4 rows on the FMAs and the
@@ -244,7 +245,7 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   // which the cluster's places do not allow at once, 10.7; 128 of 4K keys of 128, 81
   // and 84; 32 of 30K keys, 148, unsplit 615.)
   int C = 1;
-  while (C < kMaxCluster && items * 2 * C <= 2 * sm_count() && a.cache.T / (2 * C) >= 32) C *= 2;
+  while (may_double(C, items) && items * 2 * C <= 2 * sm_count() && a.cache.T / (2 * C) >= 32) C *= 2;
   const size_t smem = (size_t)((kWarps + 1) * R * LPK * EPL) * sizeof(float);
   return launch_cluster(cache_attn_kernel<CT, LPK, R, U>, items * C, C, kThreads, smem, stream, p);
 }
@@ -254,16 +255,19 @@ cudaError_t by_rows(const CacheAttnArgs& a, cudaStream_t stream) {
   const int64_t rows = a.S * (a.Hq / a.cache.H);
   if (rows <= 1) return launch<CT, LPK, 1, 4>(a, stream);
   if (rows <= 2) return launch<CT, LPK, 2, 4>(a, stream);
-  if (rows <= 4) return launch<CT, LPK, 4, 4>(a, stream);
-  return launch<CT, LPK, 8, 2>(a, stream);
+  if constexpr (sizeof(CT) == 4 || LPK > 16)
+    if (rows > 4) return launch<CT, LPK, 8, 2>(a, stream);
+  return launch<CT, LPK, 4, 4>(a, stream);
 }
 
 template <typename CT>
 cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t stream) {
   if (a.cache.D <= 16) return by_rows<CT, 2>(a, stream);
   if (a.cache.D <= 32) return by_rows<CT, 4>(a, stream);
-  if (a.cache.D <= 64) return by_rows<CT, 8>(a, stream);
-  if (a.cache.D <= 128) return by_rows<CT, 16>(a, stream);
+  if constexpr (sizeof(CT) == 4) {
+    if (a.cache.D <= 64) return by_rows<CT, 8>(a, stream);
+    if (a.cache.D <= 128) return by_rows<CT, 16>(a, stream);
+  }
   return by_rows<CT, 32>(a, stream);
 }
 

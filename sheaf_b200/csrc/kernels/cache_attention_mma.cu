@@ -507,7 +507,7 @@ cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
   // items alone, until no CTA has more than 256 KB of K (64 x 8 items of up to 4K
   // bf16 keys of 128: 90 us, unsplit 114).
   int C = 1;
-  while (C < kMaxCluster && a.cache.T / (2 * C) >= 4 * KB &&
+  while (may_double(C, items) && a.cache.T / (2 * C) >= 4 * KB &&
          (items * 2 * C <= 3 * sm_count() || a.cache.T * row > C * (256 << 10)))
     C *= 2;
   // An SM holds two CTAs of three stages, or three of two (64 x 12 items of up to
@@ -528,8 +528,7 @@ cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
 // codes and of P, some five half-rate instructions per word of four codes; short ones
 // their set-up and joining, some 5 us.
 bool cache_attention_mma_takes(const CacheAttnArgs& a) {
-  return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 &&
-         a.S * (a.Hq / a.cache.H) <= (a.bf16 ? 16 : 4);
+  return on_tensor_cores(a) && a.S * (a.Hq / a.cache.H) <= (a.bf16 ? 16 : 4);
 }
 
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream) {

@@ -942,14 +942,14 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   // 27 us, unsplit 84; 32 of 256 rows over 16K: 80 and 265; 24 of 63 rows over 1K of
   // 64: 14 and 20.)
   int C = 1;
-  while (C < kMaxCluster && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 4 * BN) ++C;
+  while (C < kPortable && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 4 * BN) ++C;
   return launch_cluster(cache_attn_tc<DP, QP, I8>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);
 }
 
 }  // namespace
 
 bool cache_attention_tc_takes(const CacheAttnArgs& a) {
-  return a.cache.type != KvType::F32 && a.cache.D >= 64 && a.cache.D <= 128 && !cache_attention_mma_takes(a);
+  return on_tensor_cores(a) && !cache_attention_mma_takes(a);
 }
 
 cudaError_t cache_attention_tc(const CacheAttnArgs& a, cudaStream_t stream) {

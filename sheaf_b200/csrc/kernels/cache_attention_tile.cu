@@ -1,6 +1,5 @@
-// Attention of many query rows over a cache on the CUDA cores: f32 caches, whose
-// products take all 24 bits, and heads that the tensor-core kernels do not take.
-// Same definition as cache_attention.cu.
+// Attention of many query rows over an f32 cache, whose products take all 24 bits,
+// on the CUDA cores.  Same definition as cache_attention.cu.
 //
 // That kernel holds 8 query rows in registers and reads the cache once per 8
 // rows.  Here a CTA of W warps takes 8 W rows, and tiles of 64 keys pass through two
@@ -25,27 +24,23 @@ using namespace cattn;
 constexpr int RW = 8;                  // rows of a warp
 constexpr int KPL = 2, BN = 32 * KPL;  // keys of a lane and of a tile
 
-template <typename CT, int DP, int W>
+template <int DP, int W>
 struct TileCfg {
   static constexpr int DPL = DP / 32, R = W * RW;         // output columns of a lane, rows of the CTA
-  static constexpr int ROW = DP * (int)sizeof(CT) + 16;   // bytes; lanes' rows start in different banks
+  static constexpr int ROW = DP * 4 + 16;   // bytes; lanes' rows start in different banks
   static constexpr int TILE = BN * ROW, STAGE = 2 * TILE;  // K and V
   static constexpr int KV_OFF = R * DP * 4, P_OFF = KV_OFF + 2 * STAGE, SMEM = P_OFF + W * BN * RW * 4;
 };
 
-__device__ __forceinline__ float widen1(float x) { return x; }
-__device__ __forceinline__ float widen1(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float widen1(int8_t x) { return (float)x; }
-
 // N consecutive values from shared memory.
-template <int N, typename CT>
+template <int N>
 __device__ __forceinline__ void take(const void* p, float* x) {
-  struct alignas(N * sizeof(CT) < 16 ? N * sizeof(CT) : 16) Vec {
-    CT v[N];
+  struct alignas(N * 4) Vec {
+    float v[N];
   };
   const Vec y = *(const Vec*)p;
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = widen1(y.v[i]);
+  for (int i = 0; i < N; ++i) x[i] = y.v[i];
 }
 
 __device__ __forceinline__ float warp_max(float x) {
@@ -54,11 +49,10 @@ __device__ __forceinline__ float warp_max(float x) {
   return y;
 }
 
-template <typename CT, int DP, int W>
+template <int DP, int W>
 __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
-  using F = TileCfg<CT, DP, W>;
+  using F = TileCfg<DP, W>;
   constexpr int DPL = F::DPL, R = F::R, ROW = F::ROW;
-  constexpr bool I8 = sizeof(CT) == 1;
   pdl_prologue();
   extern __shared__ __align__(16) uint8_t sm[];
   __shared__ unsigned long long s_mask[kKvMaxTokens];
@@ -74,23 +68,23 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
   // this CTA's positions, in whole tiles
   const int64_t per = ((w.end + w.C - 1) / w.C + BN - 1) / BN * BN;
   const int64_t lo = min((int64_t)w.rank * per, w.end), hi = min(lo + per, w.end);
-  const uint8_t* const kb = (const uint8_t*)p.k + w.nh * p.T * p.D * (int64_t)sizeof(CT);
-  const uint8_t* const vb = (const uint8_t*)p.v + w.nh * p.T * p.D * (int64_t)sizeof(CT);
-  constexpr int PIECES = DP * (int)sizeof(CT) / 16;  // 16-byte pieces of a row, padded
+  const uint8_t* const kb = (const uint8_t*)p.k + w.nh * p.T * p.D * (int64_t)4;
+  const uint8_t* const vb = (const uint8_t*)p.v + w.nh * p.T * p.D * (int64_t)4;
+  constexpr int PIECES = DP * 4 / 16;  // 16-byte pieces of a row, padded
   const int u = tid % PIECES, key0 = tid / PIECES;
   constexpr int KSTEP = W * 32 / PIECES;
   static_assert(W * 32 % PIECES == 0, "whole rows per step");
-  const bool has = u * 16 < p.D * (int)sizeof(CT);
+  const bool has = u * 16 < p.D * 4;
   // Keys t .. t + BN into stage `st`, zeros behind the last one.
   auto fetch = [&](int64_t t, int st) {
     const uint32_t dst = tc::smem_u32(sm + F::KV_OFF + st * F::STAGE) + key0 * ROW + u * 16;
-    const int64_t at = (t + key0) * p.D * (int64_t)sizeof(CT) + u * 16;
+    const int64_t at = (t + key0) * p.D * (int64_t)4 + u * 16;
     if (!has) return;
 #pragma unroll
     for (int k = 0; k < BN; k += KSTEP) {
       if (KSTEP > BN && key0 >= BN) break;
       const bool in = t + key0 + k < hi;
-      const int64_t from = in ? at + (int64_t)k * p.D * (int)sizeof(CT) : 0;
+      const int64_t from = in ? at + (int64_t)k * p.D * 4 : 0;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + k * ROW), "l"(kb + from), "r"(in ? 16 : 0)
                    : "memory");
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + F::TILE + k * ROW), "l"(vb + from),
@@ -99,22 +93,12 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
     }
   };
   auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
-  float ks[KPL], vs[KPL];  // the next tile's scales of the lane's keys
-  auto fetch_scales = [&](int64_t t) {
-#pragma unroll
-    for (int j = 0; j < KPL; ++j) {
-      const int64_t at = t + 32 * j + lane;
-      ks[j] = vs[j] = 0.f;
-      if (I8 && at < hi) ks[j] = p.ks[w.nh * p.T + at], vs[j] = p.vs[w.nh * p.T + at];
-    }
-  };
   if (tid < R) {
     s_tok[tid] = min(r0 + tid, p.S * p.G - 1) / p.G;
     s_at[tid] = row_at(p, w, r0 + min(tid, rows - 1));
   }
   if (lo < hi) fetch(lo, 0);
   commit();
-  fetch_scales(lo);
   __syncthreads();
   // queries times scale log2(e)
 #pragma unroll 4
@@ -152,7 +136,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
     __syncthreads();
     if (warp * RW < rows) {
       const uint8_t* const tk = sm + F::KV_OFF + st * F::STAGE;
-      const uint8_t* const tv = tk + F::TILE + lane * DPL * sizeof(CT);
+      const uint8_t* const tv = tk + F::TILE + lane * DPL * 4;
       float s[RW][KPL];
 #pragma unroll
       for (int r = 0; r < RW; ++r)
@@ -164,7 +148,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
         for (int d = d0; d < d0 + 16; d += 4) {
           float k[KPL][4];
 #pragma unroll
-          for (int j = 0; j < KPL; ++j) take<4, CT>(tk + (32 * j + lane) * ROW + d * sizeof(CT), k[j]);
+          for (int j = 0; j < KPL; ++j) take<4>(tk + (32 * j + lane) * ROW + d * 4, k[j]);
 #pragma unroll
           for (int r = 0; r < RW; ++r) {
             const float4 q = *(const float4*)(wq + r * DP + d);
@@ -180,9 +164,6 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
       const bool masked = t0 + BN > w.pre || t0 + BN > hi;
 #pragma unroll
       for (int r = 0; r < RW; ++r) {
-        if (I8)
-#pragma unroll
-          for (int j = 0; j < KPL; ++j) s[r][j] *= ks[j];
         if (masked) {
           const unsigned long long seen = s_mask[s_tok[row0 + r]];
 #pragma unroll
@@ -202,10 +183,8 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
         const float base = m[r] == -INFINITY ? 0.f : m[r];
 #pragma unroll
         for (int j = 0; j < KPL; ++j) {
-          const float e = tc::ex2(s[r][j] - base);
-          l[r] += e;
-          // a masked key's scale may be anything
-          s[r][j] = I8 ? (masked && s[r][j] == -INFINITY ? 0.f : e * vs[j]) : e;
+          s[r][j] = tc::ex2(s[r][j] - base);
+          l[r] += s[r][j];
         }
       }
 #pragma unroll
@@ -219,9 +198,9 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
 #pragma unroll 4
         for (int key = 0; key < BN; ++key) {
           float v[DPL], y[RW];
-          take<DPL, CT>(tv + key * ROW, v);
-          take<4, float>(sp + key * RW, y);
-          take<4, float>(sp + key * RW + 4, y + 4);
+          take<DPL>(tv + key * ROW, v);
+          take<4>(sp + key * RW, y);
+          take<4>(sp + key * RW + 4, y + 4);
 #pragma unroll
           for (int r = 0; r < RW; ++r)
             if (!MASK || y[r] != 0.f)  // what a masked position holds does not matter, NaN included
@@ -232,7 +211,6 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
       if (masked) add(std::true_type{});
       else add(std::false_type{});
     }
-    fetch_scales(t0 + BN);
     __syncthreads();  // the stage has been read
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -248,9 +226,9 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
   join_and_store<W, R, DP, 1>(p, w, r0, rows, sq, s_m, s_l, sq, s_ml, s_mask, nullptr);
 }
 
-template <typename CT, int DP, int W>
+template <int DP, int W>
 cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
-  using F = TileCfg<CT, DP, W>;
+  using F = TileCfg<DP, W>;
   const Params p = make_params(a, F::R);
   const int64_t items = a.cache.N * a.cache.H * p.chunks;
   // Split until the CTAs fill the SMs (228 KB of shared memory each) or have one
@@ -258,33 +236,26 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   // them taken a second wave followed (96 items of 3 CTAs, 2 per SM: 77 us, of 2: 64).
   const int per_sm = (228 << 10) / (F::SMEM + (4 << 10));
   int C = 1;
-  while (C < kMaxCluster && items * (C + 1) * 4 <= (per_sm > 1 ? 3 * per_sm : 4) * sm_count() &&
+  while (C < kPortable && items * (C + 1) * 4 <= (per_sm > 1 ? 3 * per_sm : 4) * sm_count() &&
          a.cache.T / (C + 1) >= BN)
     ++C;
-  return launch_cluster(cache_attn_tile<CT, DP, W>, items * C, C, W * 32, F::SMEM, stream, p);
-}
-
-template <typename CT>
-cudaError_t by_dim(const CacheAttnArgs& a, cudaStream_t stream) {
-  const bool few = a.S * (a.Hq / a.cache.H) <= 32;
-  if (a.cache.D <= 32) return few ? launch<CT, 32, 4>(a, stream) : launch<CT, 32, 8>(a, stream);
-  if (a.cache.D <= 64) return few ? launch<CT, 64, 4>(a, stream) : launch<CT, 64, 8>(a, stream);
-  return few ? launch<CT, 128, 4>(a, stream) : launch<CT, 128, 8>(a, stream);
+  if (C == kPortable && may_double(C, items) && a.cache.T / (2 * C) >= BN) C *= 2;
+  return launch_cluster(cache_attn_tile<DP, W>, items * C, C, W * 32, F::SMEM, stream, p);
 }
 
 }  // namespace
 
 // 9 rows: 30 us against 37 (8 x 12 caches of 609 keys of 64), 9.0 against 8.0 for
 // the smallest calls.
-bool cache_attention_tile_takes(const CacheAttnArgs& a) { return a.cache.D <= 128 && a.S * (a.Hq / a.cache.H) > 8; }
+bool cache_attention_tile_takes(const CacheAttnArgs& a) {
+  return a.cache.type == KvType::F32 && a.cache.D <= 128 && a.S * (a.Hq / a.cache.H) > 8;
+}
 
 cudaError_t cache_attention_tile(const CacheAttnArgs& a, cudaStream_t stream) {
-  switch (a.cache.type) {
-    case KvType::F32: return by_dim<float>(a, stream);
-    case KvType::BF16: return by_dim<__nv_bfloat16>(a, stream);
-    case KvType::I8: return by_dim<int8_t>(a, stream);
-  }
-  return cudaErrorInvalidValue;
+  const bool few = a.S * (a.Hq / a.cache.H) <= 32;
+  if (a.cache.D <= 32) return few ? launch<32, 4>(a, stream) : launch<32, 8>(a, stream);
+  if (a.cache.D <= 64) return few ? launch<64, 4>(a, stream) : launch<64, 8>(a, stream);
+  return few ? launch<128, 4>(a, stream) : launch<128, 8>(a, stream);
 }
 
 }  // namespace sb

@@ -62,6 +62,15 @@ struct Params {
   float scale2;         // scale * log2(e)
 };
 
+// The calls that go to the tensor cores (cache_attention_mma.cu and _tc.cu, heads
+// padded to 64 or 128).  Heads up to 32 only from 4 rows on: one row of 64 x 12
+// int8 caches of 512 keys of 32 takes 21.5 us there and 15.1 on the CUDA cores, 4
+// rows of 19 x 4 of 6K keys 22 and 63, 160 rows of 15 x 4 of 1.5K bf16 keys 22 and
+// 137; one row with heads of 48, 23.6 and 28.0.
+inline bool on_tensor_cores(const CacheAttnArgs& a) {
+  return a.cache.type != KvType::F32 && a.cache.D <= 128 && (a.cache.D > 32 || a.S * (a.Hq / a.cache.H) >= 4);
+}
+
 inline Params make_params(const CacheAttnArgs& a, int chunk_rows) {
   const KvCacheView& c = a.cache;
   const int G = (int)(a.Hq / c.H), rows = (int)a.S * G;
@@ -73,6 +82,15 @@ inline int sm_count() {
   int dev = 0, n = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
   return n;
+}
+
+// CTAs of a cluster: 8 is what every GPU takes.  Twice that goes where a few
+// long items would leave SMs idle, at most one CTA per SM: one sequence's 8 heads of
+// 30K bf16 keys of 128, 34 us against 53, f32 keys 47 and 89; with 16 items, which
+// 8 CTAs each spread over most SMs, it was slower (26 us, 21.5).
+constexpr int kPortable = 8, kMaxCluster = 16;
+inline bool may_double(int C, int64_t items) {
+  return C < kPortable || (C < kMaxCluster && items * 2 * C <= sm_count());
 }
 
 template <typename... K, typename... A>
@@ -95,6 +113,17 @@ cudaError_t launch_cluster(void (*kern)(K...), int64_t blocks, int cluster, int 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
+  if (cluster > kPortable) {  // where the GPU has room for one
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    int fit = 0;
+    e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
+    if (e != cudaSuccess || fit < 1) {
+      cudaGetLastError();
+      cfg.gridDim.x = (unsigned)(blocks / cluster * kPortable);
+      at[1].val.clusterDim.x = kPortable;
+    }
+  }
   launch_counter().fetch_add(1, std::memory_order_relaxed);
   return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
 }
@@ -195,7 +224,6 @@ __device__ __forceinline__ void store4(const Params& p, int64_t at, float4 y) {
   }
 }
 
-constexpr int kMaxCluster = 8;
 
 // f16 operands for int8 caches.  A row of queries is scaled by a power of two to
 // a largest value in [2^14, 2^15), which keeps what is 2^-38 of it: 2^(14 - e)

@@ -279,13 +279,13 @@ struct CacheAttnArgs {
   float scale = 1.f;  // multiplier of q.k before the softmax
 };
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
-// The kernels for bf16 and int8 caches of head size 64 to 128 and the calls
-// they take (cache_attention dispatches): few query rows (tokens x query heads
-// per cache head: up to 4 in f32, 16 in bf16) multiply with warp instructions
+// The kernels for bf16 and int8 caches of head size up to 128 and the calls they
+// take (cache_attention dispatches): few query rows (tokens x query heads per
+// cache head: up to 4 in f32, 16 in bf16) multiply with warp instructions
 // (kernels/cache_attention_mma.cu), more rows with tcgen05
 // (kernels/cache_attention_tc.cu).  Failed waits are reported through the
-// tensor-core error word, codes 50..70.  Of the other calls, more than 8 rows of
-// heads up to 128 go through tiles in shared memory (cache_attention_tile.cu).
+// tensor-core error word, codes 50..70.  More than 8 rows over f32 caches of such
+// heads go through tiles in shared memory (cache_attention_tile.cu).
 bool cache_attention_mma_takes(const CacheAttnArgs& a);
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream);
 bool cache_attention_tile_takes(const CacheAttnArgs& a);

@@ -269,6 +269,25 @@ def test_attention(sess, case, kind, src, tree):
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D,T", [(1, 1, 64, 9000), (1, 4, 128, 5000), (3, 4, 64, 6000), (1, 1, 256, 3000),
+                                         (1, 2, 32, 4000)])
+def test_attention_of_one_long_sequence(sess, kind, src, n_tok, G, D, T):
+    """Few (slot, head) pairs over many keys: the widest splits; the second slot leaves most of them empty."""
+    N, H = 2, 2
+    rng = np.random.default_rng(T + D)
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    q = rand(rng, (N, n_tok, G * H, D), src)
+    pos = [T - n_tok - 1, 70]
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, 1 / math.sqrt(D))
+    out = put(sess, np.zeros(q.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
+    assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
 @pytest.mark.parametrize("N,H,n_tok", [(71, 8, 1), (128, 4, 2), (131, 4, 1)])
 def test_attention_of_many_uneven_slots(sess, kind, src, N, H, n_tok):
     """More (slot, head) pairs than run at once; idle, empty, equal and full slots among them."""
