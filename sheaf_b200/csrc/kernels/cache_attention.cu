@@ -253,11 +253,16 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
 template <typename CT, int LPK>
 cudaError_t by_rows(const CacheAttnArgs& a, cudaStream_t stream) {
   const int64_t rows = a.S * (a.Hq / a.cache.H);
-  if (rows <= 1) return launch<CT, LPK, 1, 4>(a, stream);
-  if (rows <= 2) return launch<CT, LPK, 2, 4>(a, stream);
-  if constexpr (sizeof(CT) == 4 || LPK > 16)
+  // Rows of the cache under way per group: four; eight for heads over 128, of which a
+  // warp holds one at a time, in 8 or 16 bits (16 x 8 caches of 3K bf16 keys of 256: 62
+  // us, 82 with four; f32, twice the bytes and registers, 125 and 117).  With four
+  // query rows int8 codes leave no registers for eight (32 and 38 us).
+  constexpr bool NARROW = LPK == 32 && sizeof(CT) < 4;
+  if (rows <= 1) return launch<CT, LPK, 1, NARROW ? 8 : 4>(a, stream);
+  if (rows <= 2) return launch<CT, LPK, 2, NARROW ? 8 : 4>(a, stream);
+  if constexpr (sizeof(CT) == 4 || LPK == 32)
     if (rows > 4) return launch<CT, LPK, 8, 2>(a, stream);
-  return launch<CT, LPK, 4, 4>(a, stream);
+  return launch<CT, LPK, 4, NARROW && sizeof(CT) == 2 ? 8 : 4>(a, stream);
 }
 
 template <typename CT>
