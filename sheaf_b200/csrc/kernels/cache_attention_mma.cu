@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w, bool& bad) {
 
 // DP: head size padded to 64 or 128.  MODE: bf16 queries of at most 16 rows
 // (kRows16) or 8 (kRows8: rows 8-15 of the second product hold what bf16 left of
-// P, so P has 16 bits), f32 queries of at most 4 rows (kF32).
+// P, so P has 16 bits), f32 queries in blocks of 4 rows (kF32).
 enum Mode { kRows16, kRows8, kF32 };
 template <int DP, bool I8, int MODE, int ST>
 struct MmaCfg {
@@ -519,16 +519,21 @@ cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-// As many rows as the instruction has.  There it is the faster one: 16 bf16 rows of
-// 4 x 8 caches of 30K keys of 128 take 86 us from bf16 and 67 from int8, on tcgen05
-// 97 and 128; of 8 x 12 caches of 465 keys of 64, 8.6 and 9.5, 12.4 and 14.8; 4 f32
-// rows of 16 x 8 caches of 4K keys of 128, 57 and 37, 90 and 137 (on the CUDA cores
-// 125 and 241).  Reading the cache bounds the long bf16 calls (one bf16 row of 4 x 8
-// x 30K keys of 128: 79 us, 6.2 TB/s); int8 ones (59 us, 4.3 TB/s) the conversion of
-// codes and of P, some five half-rate instructions per word of four codes; short ones
-// their set-up and joining, some 5 us.
+// As many bf16 rows as the instruction has, and f32 rows in two blocks of 4, whose
+// second reading of the cache is from L2.  There it is the faster one: 16 bf16 rows
+// of 4 x 8 caches of 30K keys of 128 take 86 us from bf16 and 67 from int8, on
+// tcgen05 97 and 128; of 8 x 12 caches of 465 keys of 64, 8.6 and 9.5, 12.4 and 14.8;
+// 8 f32 rows of 8 x 12 caches of 6K keys of 128, 83 and 80, 129 and 193 (three blocks,
+// 12 rows: 123 and 116, but of 300 keys 29 and 34, 17 and 22).  Two blocks of bf16
+// rows lose it: 32 rows of 6K keys, 95 us from bf16, 77 on tcgen05.  4 f32 rows of 16
+// x 8 caches of 4K keys of 128, 57 and 37 us, on the CUDA cores 125 and 241.
+//
+// Reading the cache bounds the long bf16 calls (one bf16 row of 4 x 8 x 30K keys of
+// 128: 79 us, 6.2 TB/s); int8 ones (59 us, 4.3 TB/s) the conversion of codes and of P,
+// some five half-rate instructions per word of four codes; short ones their set-up
+// and joining, some 5 us.
 bool cache_attention_mma_takes(const CacheAttnArgs& a) {
-  return on_tensor_cores(a) && a.S * (a.Hq / a.cache.H) <= (a.bf16 ? 16 : 4);
+  return on_tensor_cores(a) && a.S * (a.Hq / a.cache.H) <= (a.bf16 ? 16 : 8);
 }
 
 cudaError_t cache_attention_mma(const CacheAttnArgs& a, cudaStream_t stream) {

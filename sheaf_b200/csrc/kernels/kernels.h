@@ -281,7 +281,7 @@ struct CacheAttnArgs {
 cudaError_t cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
 // The kernels for bf16 and int8 caches of head size up to 128 and the calls they
 // take (cache_attention dispatches): few query rows (tokens x query heads per
-// cache head: up to 4 in f32, 16 in bf16) multiply with warp instructions
+// cache head: up to 8 in f32, 16 in bf16) multiply with warp instructions
 // (kernels/cache_attention_mma.cu), more rows with tcgen05
 // (kernels/cache_attention_tc.cu).  Failed waits are reported through the
 // tensor-core error word, codes 50..70.  More than 8 rows over f32 caches of such

@@ -230,6 +230,9 @@ ATT_CASES = [  # slots, tokens, q heads, heads, capacity, head size, positions
     (1, 20, 4, 2, 140, 96, [100]),
     (2, 8, 4, 2, 150, 112, [9, 140]),
     (1, 64, 3, 1, 200, 64, [130]),                    # 192 rows
+    (2, 3, 4, 2, 300, 64, [250, 30]),
+    (1, 8, 2, 2, 500, 128, [450]),
+    (2, 5, 2, 2, 90, 32, [80, 87]),
 ]
 
 
