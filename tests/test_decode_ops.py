@@ -708,3 +708,31 @@ def test_captured_and_replayed(sess):
         for a, c in zip(results(), want[seed]):
             assert np.array_equal(a, c)
     del g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,n_tok", [("f32", 1), ("f32", 12), ("bf16", 1), ("int8", 5), ("int8", 20)])
+def test_each_attention_kernel_captured(sess, kind, n_tok):
+    """The widest splits of every kernel inside a graph, with positions that change between replays."""
+    import torch
+    N, H, T, D = 1, 2, 5000, 64
+    rng = np.random.default_rng(n_tok)
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    k, v = values(arrays, scales)
+    q = rand(rng, (N, n_tok, H, D))
+    pos = torch.zeros(N, dtype=torch.int32, device="cuda")
+    hq, hp, out = put(sess, q), sess.wrap_torch(pos), sess.zeros(q.shape)
+    sess.synchronize()
+    stream = torch.cuda.ExternalStream(sess.cuda_stream)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        sess.kv_cache_attention(cache, hp, hq, out)
+    for at in (0, 4000, 31):
+        pos.fill_(at)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            g.replay()
+        torch.cuda.synchronize()
+        ref, dots, vmax, live = R.attention(k, v, [at], q, 1 / math.sqrt(D))
+        assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, "f32")).all()
+    del g
