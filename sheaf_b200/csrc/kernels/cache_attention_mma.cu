@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(NW * 32)
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) {
     if (t0 + i * STRIDE < hi) fetch(t0 + i * STRIDE, i);
-    copies_commit();
+    if (I8) copies_commit();
   }
   if (warp == 0) tree_masks(p.parents ? p.parents + w.n * p.S : nullptr, p.S, lane, s_mask, s_jump);
 
@@ -282,7 +282,10 @@ __global__ void __launch_bounds__(NW * 32)
   uint32_t phase = 0;
   float vdown = 0.f;
   for (; t0 < hi; t0 += STRIDE) {
-    copies_wait<STAGES - 1>();
+    if (I8) {  // a lane's copies of scales are there for the others once the warp has met
+      copies_wait<STAGES - 1>();
+      __syncwarp();
+    }
     if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[st], phase, &s_abort, err, 64))) break;
     const uint8_t *const stage = ring + st * F::STAGE, *const stage_v = stage + F::BOXES * BOX;
     const float* const sc = scales + st * KB * 2;
@@ -445,10 +448,10 @@ __global__ void __launch_bounds__(NW * 32)
       }
     __syncwarp();  // the stage has been read
     if (t0 + STAGES * STRIDE < hi) fetch(t0 + STAGES * STRIDE, st);
-    copies_commit();
+    if (I8) copies_commit();
     if (++st == STAGES) st = 0, phase ^= 1u;
   }
-  copies_wait<0>();
+  if (I8) copies_wait<0>();
   if (s_abort && lane == 0 && t0 < hi) {  // the boxes of the steps that were not taken may still be on their way
     const unsigned long long give_up = tc::now_ns() + tc::kTimeoutNs;
     for (int i = 0; i < STAGES && t0 < hi; ++i, t0 += STRIDE) {

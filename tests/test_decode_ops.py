@@ -736,3 +736,27 @@ def test_each_attention_kernel_captured(sess, kind, n_tok):
         ref, dots, vmax, live = R.attention(k, v, [at], q, 1 / math.sqrt(D))
         assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, "f32")).all()
     del g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("src,group", [("f32", 1), ("bf16", 4), ("bf16", 16)])
+def test_int8_scales_copied_by_other_lanes(sess, src, group):
+    """Few rows over int8 caches of many steps: every lane reads scales that other lanes of its warp copied.  Equal
+    bits from call to call, and the definition's values."""
+    rng = np.random.default_rng(group)
+    N, H, T, D = 6, 4, 1500, 64
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), "int8")
+    for s in scales:  # a scale taken from another place would show
+        s *= np.exp2(rng.integers(-3, 4, s.shape)).astype(np.float32)
+    cache = S.KVCache(cache.k, cache.v, *[put(sess, s) for s in scales])
+    pos = rng.integers(0, T, N)
+    q = rand(rng, (N, 1, group * H, D), src)
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, 1 / math.sqrt(D))
+    hq, hp = put(sess, q, src), put(sess, np.int32(pos))
+    outs = [put(sess, np.zeros(q.shape, np.float32), src) for _ in range(20)]
+    for out in outs:
+        sess.kv_cache_attention(cache, hp, hq, out)
+    got = [out.to_host() for out in outs]
+    assert (np.abs(got[0] - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
+    assert all(np.array_equal(g, got[0]) for g in got)
