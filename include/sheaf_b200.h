@@ -263,7 +263,10 @@ SB_API sb_status* sb_kv_cache_read(sb_session* session, const sb_kv_cache* cache
  * reads cache head h / (query heads / heads).  Positions beyond the capacity
  * hold nothing; a slot with a negative position is idle.  A token without keys
  * gets zeros.  What stands at positions that a token does not attend to does
- * not matter, NaN included.  Scores, softmax and sums are f32. */
+ * not matter, NaN included.  Scores, softmax and sums are f32.  bf16 calls may
+ * leave out 2^-16 of each probability before its product with a value, and over
+ * int8 caches, with more than 8 rows (tokens x query heads per cache head),
+ * 2^-11; f32 calls take all of it. */
 SB_API sb_status* sb_kv_cache_attention(sb_session* session, const sb_kv_cache* cache, sb_buffer* positions,
                                         sb_buffer* parents, sb_buffer* q, float scale, sb_buffer* out);
 

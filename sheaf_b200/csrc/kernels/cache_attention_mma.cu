@@ -120,6 +120,12 @@ __global__ void __launch_bounds__(NW * 32)
   using F = MmaCfg<DP, I8, MODE, ST>;
   constexpr bool Q32 = MODE == kF32;
   constexpr bool F16 = I8;  // operands: f16 for int8 caches, bf16 for bf16 ones
+  // 9 to 16 bf16 rows fill A, so the second part of P takes products of its own: over
+  // bf16 caches, which reading bounds (8 x 12 caches of 465 keys 9.2 us, 9.0 with one
+  // part, that is with 2^-8 of each probability left out in place of 2^-16).  f16 leaves
+  // 2^-11 out, an eighth of the output's rounding, and keeps one (4 x 8 int8 caches of
+  // 30K keys of 128: 68 us, 76 with two).
+  constexpr bool P2 = MODE == kRows16 && !I8;
   constexpr int KB = F::KB, NB = KB / 8, KG = KB / 16, EK = F::EK, KL = F::KL, VL = F::VL, NR = F::NR, RMAX = F::RMAX;
   constexpr int RB = F::RB, BOX = F::BOX, STAGES = F::STAGES;
   extern __shared__ __align__(1024) float sm[];  // the warps' stages, later their partial outputs
@@ -382,7 +388,7 @@ __global__ void __launch_bounds__(NW * 32)
         vdown = vref_down(vref);
       }
     }
-    uint32_t a[KG][4];
+    uint32_t a[KG][4], a2[KG][4];  // P, and with P2 what its rounding left
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -406,7 +412,8 @@ __global__ void __launch_bounds__(NW * 32)
           dst[0] = take2<F16>(y[0], y[1]);
           dst[1] = pack2<F16>(y[0], y[1]);
         } else {
-          dst[r] = pack2<F16>(y[0], y[1]);
+          dst[r] = take2<F16>(y[0], y[1]);
+          if (P2) a2[b / 2][(b & 1) * 2 + r] = pack2<F16>(y[0], y[1]);
         }
       }
 #pragma unroll
@@ -444,6 +451,7 @@ __global__ void __launch_bounds__(NW * 32)
             }
           }
           mma16816<F16>(o[j * F::EV + e], a[k], b[0], b[1]);
+          if (P2) mma16816<F16>(o[j * F::EV + e], a2[k], b[0], b[1]);
         }
       }
     __syncwarp();  // the stage has been read

@@ -20,9 +20,12 @@
 //               and takes half the instructions to make from them.  S has two
 //               buffers: the tensor cores form the next one during the softmax.
 //   P           exp2(S - m) times the value row's int8 scale, written back over
-//               S in TMEM as bf16 or f16 (bf16 output: one rounding, as large as
-//               the output's own) or as three parts (f32 output: f32 accuracy;
-//               two bf16 parts would leave 2^-16 of each probability).
+//               S in TMEM as parts: three for f32 output (f32 accuracy), two of
+//               bf16 for bf16 output (2^-16 of each probability is left out; one
+//               part, 2^-8, would be as far off as the output's own rounding, with
+//               80 us for the 8 x 4 caches of 16K below in place of 94), one of f16
+//               for bf16 output of int8 caches (2^-11 is left out, an eighth of the
+//               output's rounding; a second part took 142 us in place of 122).
 //   O += P V    the maximum m a row refers to moves only when it would grow by
 //               more than 2^8, so O is rescaled in the first tiles and then
 //               hardly ever; exact since P, O and the sum l share m.
@@ -167,6 +170,7 @@ template <int DP, int QP, bool I8>
 struct Cfg {
   static constexpr int MAXR = QP == 3 && DP == 128 ? 128 : 256;  // query rows of a CTA
   static constexpr int SB = QP == 3 && DP == 128 ? 1 : 2;        // buffers of S per stream
+  static constexpr int PP = QP == 3 ? 3 : I8 ? 1 : 2;            // parts of P
   static constexpr int QTILE = 128 * DP * 2;                     // one part of 128 rows
   static constexpr int Q_BYTES = (MAXR / 128) * QP * QTILE;
   static constexpr int TILE = BN * DP * 2;
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   int* err) {
   using F = Cfg<DP, QP, I8>;
   constexpr bool F16 = I8;
-  constexpr int SB = F::SB, NS = F::NS, NSC = F::NSC;
+  constexpr int SB = F::SB, NS = F::NS, NSC = F::NSC, PP = F::PP;
   pdl_prologue();
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Shared sh;
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float2 nb = make_float2(-base, -base);
               float mx = -INFINITY;
               float2 s2 = make_float2(0.f, 0.f);
-              uint32_t w[BN / 2];
+              uint32_t w[BN / 2], w2[PP == 2 ? BN / 2 : 1];  // P, and what its rounding left
               uint32_t r[2][32];
               tmem_ld32_async(tS, r[0]);
 #pragma unroll
@@ -464,7 +468,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                       y = mul2(y, h2[k]);
                       if (MASK) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;
                     }
-                    w[(c + j) / 2 + k] = pack2<F16>(y.x, y.y);
+                    w[(c + j) / 2 + k] = take2<F16>(y.x, y.y);
+                    if (PP == 2) w2[(c + j) / 2 + k] = pack2<F16>(y.x, y.y);
                   }
                 }
               }
@@ -476,7 +481,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               l2 = add2(l2, s2);
 #pragma unroll
-              for (int c = 0; c < BN / 32; ++c) tmem_st16u(tS + (uint32_t)(32 * c), w + 16 * c);
+              for (int c = 0; c < BN / 32; ++c) {
+                tmem_st16u(tS + (uint32_t)(32 * c), w + 16 * c);
+                if (PP == 2) tmem_st16u(tS + (uint32_t)(32 * c + 16), w2 + 16 * c);
+              }
               return;
             }
           } else {
@@ -793,10 +801,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int kk = 0; kk < BN / 16; ++kk) {
           const uint32_t pc = ts + (uint32_t)((kk / 2) * 32 + (kk % 2) * 8);
           mma_ts(to, pc, bd + kk * (2048 >> 4), id_o, i > 0 || kk > 0 ? 1u : 0u);
-          if (QP == 3) {
-            mma_ts(to, pc + 16, bd + kk * (2048 >> 4), id_o, 1u);
-            mma_ts(to, tt + (uint32_t)(kk * 8), bd + kk * (2048 >> 4), id_o, 1u);
-          }
+          if (PP > 1) mma_ts(to, pc + 16, bd + kk * (2048 >> 4), id_o, 1u);
+          if (PP > 2) mma_ts(to, tt + (uint32_t)(kk * 8), bd + kk * (2048 >> 4), id_o, 1u);
         }
         commit(&sh.o_bar[a]);
         commit(&sh.v_free[t % NS]);

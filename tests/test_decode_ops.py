@@ -760,3 +760,30 @@ def test_int8_scales_copied_by_other_lanes(sess, src, group):
     got = [out.to_host() for out in outs]
     assert (np.abs(got[0] - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
     assert all(np.array_equal(g, got[0]) for g in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n_tok,G,D", [(1, 8, 64), (9, 1, 64), (16, 1, 128), (4, 4, 48), (20, 1, 64), (33, 4, 128),
+                                       (64, 3, 64), (10, 1, 256)])
+def test_bf16_probabilities_keep_their_bits(sess, kind, n_tok, G, D):
+    """Values that cancel: what the probabilities' rounding leaves out stands beside an output near zero.  The bound
+    is elementwise: the output's own rounding (half a bf16 step of the element), the evaluation in f32 (see
+    attention_bound), and what a bf16 call may leave out of each probability: 2^-16, or 2^-11 over int8 caches,
+    times at most the largest value."""
+    rng = np.random.default_rng(n_tok + D)
+    N, H, T = 3, 2, 90
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    arrays[1] = np.where(np.arange(T)[:, None] % 2, 100, -100).astype(arrays[1].dtype) * np.ones_like(arrays[1])
+    if scales:
+        scales[1][:] = 0.01
+    cache = S.KVCache(*([put(sess, a, kind) for a in arrays] + [put(sess, s) for s in scales]))
+    q = rand(rng, (N, n_tok, G * H, D), "bf16")
+    pos, scale = [6, 0, 23], 0.01 if not scales else 0.001
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, scale)
+    out = put(sess, np.zeros(q.shape, np.float32), "bf16")
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, "bf16"), out, scale=scale)
+    left = (2.0 ** -11 if kind == "int8" else 2.0 ** -16) * vmax[..., None]
+    bound = attention_bound(dots, vmax, live, D, ref, "f32") + left
+    assert (np.abs(out.to_host() - ref) <= bound * (1 + UBF) + UBF * np.abs(ref)).all()
