@@ -69,9 +69,9 @@ struct SelectParams {
   int W, eos;
 };
 
-// Order-preserving image of an f32 that is not NaN.
+// Order-preserving image of an f32 that is not NaN; one image for both zeros, which are equal.
 __device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t u = __float_as_uint(x);
+  const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) {

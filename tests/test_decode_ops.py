@@ -787,3 +787,24 @@ def test_bf16_probabilities_keep_their_bits(sess, kind, n_tok, G, D):
     left = (2.0 ** -11 if kind == "int8" else 2.0 ** -16) * vmax[..., None]
     bound = attention_bound(dots, vmax, live, D, ref, "f32") + left
     assert (np.abs(out.to_host() - ref) <= bound * (1 + UBF) + UBF * np.abs(ref)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [65, 5000])
+@pytest.mark.parametrize("W", [1, 3, 8])
+def test_beam_select_zeros_of_both_signs_are_equal(sess, kind, V, W):
+    """-0 and +0 among the best logits, side by side (one lane has both) and far apart, in both orders: each token
+    once, the lower token first."""
+    rng = np.random.default_rng(V + W)
+    for zeros in ([-0.0, 0.0], [0.0, -0.0], [-0.0, 0.0, -0.0, 0.0, 0.0, -0.0]):
+        for step in (1, 9):
+            x = -1 - rng.random((W, V)).astype(np.float32)
+            x[:, 3:3 + step * len(zeros):step] = zeros
+            x[0, 1] = -0.0
+            x[0, V - 1] = 0.0
+            x = R.bf16_round(x) if kind == "bf16" else x
+            for scores in (np.zeros((1, W)), -np.arange(W)[None]):
+                check_select(sess, x, np.float32(scores), np.zeros((1, W), np.int32), -1, kind)
+    check_select(sess, np.where(rng.random((W, V)) < 0.5, np.float32(-0.0), np.float32(0)), np.zeros((1, W), np.float32),
+                 np.zeros((1, W), np.int32), -1, kind)
