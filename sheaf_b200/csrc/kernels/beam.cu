@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectPara
       int at = -1;
       if (mine) {
         auto piece = [&](const float* x, int64_t c) {
-          float top = x[0];
+          float top = fmaxf(x[0], -INFINITY);  // NaN counts as -inf, in every one of the values too
 #pragma unroll
           for (int i = 1; i < EPC; ++i) top = fmaxf(top, x[i]);
           if (top > best || at < 0) {

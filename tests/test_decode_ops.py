@@ -808,3 +808,18 @@ def test_beam_select_zeros_of_both_signs_are_equal(sess, kind, V, W):
                 check_select(sess, x, np.float32(scores), np.zeros((1, W), np.int32), -1, kind)
     check_select(sess, np.where(rng.random((W, V)) < 0.5, np.float32(-0.0), np.float32(0)), np.zeros((1, W), np.float32),
                  np.zeros((1, W), np.int32), -1, kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("W,V,runs", [(1, 9000, [(0, 2048)]), (2, 40000, [(0, 33000)]), (4, 70000, [(0, 69990)]),
+                                      (16, 5000, [(0, 1024), (3000, 4100)]), (16, 2100, [(0, 2099)]),
+                                      (3, 6001, [(5, 5990)])])
+def test_beam_select_runs_of_nan(sess, kind, W, V, runs):
+    """A run of NaN logits long enough that a lane's first values are NaN altogether, before, between and behind
+    finite ones: each counts as -inf, the other tokens as ever."""
+    x = (np.random.default_rng(V).standard_normal((2 * W, V)) * 2).astype(np.float32)
+    x = R.bf16_round(x) if kind == "bf16" else x
+    for a, b in runs:
+        x[::2, a:b] = np.nan
+    check_select(sess, x, -np.arange(2 * W, dtype=np.float32).reshape(2, W) / 8, np.zeros((2, W), np.int32), -1, kind)
