@@ -22,9 +22,10 @@
 //
 // Within a beam the order is the logits' own.  Between beams it needs lse.  The
 // first round sums f32 exponentials, off by less than kFastError; if two
-// neighbours of the result from different beams are closer than twice that (or
-// tie), the group's sums are taken again in f64, whose exponentials would
-// otherwise bound the kernel.  So the order is that of f64 sums in every case.
+// neighbours of the result from different beams, or its last candidate and any
+// that was not selected from another beam, are closer than twice that (or tie),
+// the group's sums are taken again in f64, whose exponentials would otherwise
+// bound the kernel.  So the order is that of f64 sums in every case.
 //
 // 32 x 8 beams over 50304 f32 logits (52 MB, 7.9 us of reading): 17.3 us (172 us
 // with every sum in f64).  About 10 us of that are not the pass but what 4 beams
@@ -196,6 +197,10 @@ __device__ __forceinline__ void load_row(const SelectParams& p, const Row& r, in
         if (at + k < r.base || at + k >= r.base + p.V) x[i * N + k] = -INFINITY;
     }
   }
+}
+// Whether the order of two candidates of different beams may be other than that of exact sums.
+__device__ __forceinline__ bool too_close(double ahead, double behind) {
+  return behind != -INFINITY && ahead - behind < 2 * kFastError + 1e-15 * fabs(ahead);
 }
 __device__ __forceinline__ u64 key_of(float x, int64_t idx) {
   return (u64)ordered(x) << 32 | (uint32_t)~(uint32_t)idx;
@@ -456,9 +461,15 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectPara
     if (round == 0 && tid < W) {
       const int b1 = sh.beam[tid], b2 = sh.beam[tid + 1];
       // finished beams' candidates and -inf are exact
-      close = b1 >= 0 && b2 >= 0 && b1 != b2 && sh.best[tid + 1] != -INFINITY &&
-              sh.best[tid] - sh.best[tid + 1] < 2 * kFastError + 1e-15 * fabs(sh.best[tid]);
+      close = b1 >= 0 && b2 >= 0 && b1 != b2 && too_close(sh.best[tid], sh.best[tid + 1]);
     }
+    // behind the last place another beam's candidates may stand after several of its own beam's
+    if (round == 0)
+      for (int i = tid; i < W * W; i += kSelThreads) {
+        const int b = i / W, j = i - b * W;
+        close |= sh.rank[i] >= W && sh.token[b][j] >= 0 && b != sh.beam[W - 1] &&
+                 too_close(sh.best[W - 1], sh.cand[b][j]);
+      }
     if (__syncthreads_or(close)) {
       tc::cluster_sync();  // every CTA has read the candidates before they are written again
       continue;

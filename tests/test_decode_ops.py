@@ -823,3 +823,34 @@ def test_beam_select_runs_of_nan(sess, kind, W, V, runs):
     for a, b in runs:
         x[::2, a:b] = np.nan
     check_select(sess, x, -np.arange(2 * W, dtype=np.float32).reshape(2, W) / 8, np.zeros((2, W), np.int32), -1, kind)
+
+
+def near_values(rng, G, W, V, gap):
+    """Groups whose last place is between beam 0's two best, which are equal, and the second best of the last beam,
+    `gap` of the value away (up to the scores' rounding, 2^-24): logits [G, W, V] and scores [G, W].  The other
+    beams' best are clearly ahead of both, all else is clearly behind."""
+    x = rng.standard_normal((G, W, V)).astype(np.float32)
+    s = np.zeros((G, W), np.float32)
+    for g in range(G):
+        a, b = rng.choice(V, 2, replace=False)
+        x[g, 0, [a, b]] = 8.5
+        for w in range(1, W):
+            t = rng.choice(V, 2, replace=False)
+            x[g, w, t] = 12.0, 8.25
+        lse = np.log(np.exp(x[g].astype(np.float64)).sum(1))
+        s[g, W - 1] = 8.5 - lse[0] + gap[g] - (8.25 - lse[W - 1])
+        s[g, 1:W - 1] = 0.5 - np.arange(W - 2) / 16
+    return x, s
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("W,V", [(2, 3000), (2, 50304), (4, 4097), (8, 1500)])
+def test_beam_select_order_at_the_last_place(sess, W, V):
+    """Two equal candidates of one beam at the cut, and another beam's behind them that f64 sums put before or after
+    them by less than f32 sums can tell."""
+    rng = np.random.default_rng(W + V)
+    G = 48 if V < 9000 else 12
+    x, s = near_values(rng, G, W, V, rng.uniform(-6e-7, 6e-7, G))
+    ref = R.beam_select(x.reshape(G * W, V), s)
+    assert len(set(ref[1][:, -1])) == 2  # either beam has the last place somewhere
+    check_select(sess, x.reshape(G * W, V), s, np.zeros((G, W), np.int32), -1)
