@@ -48,12 +48,15 @@ namespace {
 
 constexpr int kSelWarps = 16, kSelThreads = kSelWarps * 32;
 // Bound on the error of an lse from f32 exponentials of V <= 2^31 values.  A
-// term 2^-t has a relative error of at most 2^-22 (ex2) + 2^-23.4 t (its
-// argument, two roundings), and terms with t > 32 + log2 of the sum of the
-// others' number are below it; the mean t of the sum's weight is at most
-// log2(V) < 32; 32 terms are added in f32 (at most 9 additions each), the rest
-// in f64: 2^-22 + 32 * 2^-23.4 + 9 * 2^-24 < 4e-6.
-constexpr double kFastError = 4e-6;
+// term 2^-t (t: what the value is below its warp's base, in units of log2) has a
+// relative error of at most 2^-22 (ex2) + 2^-23.4 |t| (its argument, two
+// roundings), and terms with t > 32 + log2 of the sum of the others' number are
+// below it.  A base is at most the row's maximum, so the mean of t by the sum's
+// weight is at most log2(V); and at least the warp's less kBaseRoom - log2(V), so
+// the mean of |t| is at most kBaseRoom.  32 terms are added in f32 (at most 9
+// additions each), the rest in f64, in which sums also pass from one base to
+// another: 2^-22 + kBaseRoom * 2^-23.4 + 9 * 2^-24 < 4e-6.
+constexpr double kFastError = 4e-6, kBaseRoom = 35;
 constexpr int EPC = 32;              // values per lane and piece
 constexpr int kPiece = EPC * 32;     // values per warp and piece
 constexpr int W_MAX = (int)kBeamMax;
@@ -68,6 +71,7 @@ struct SelectParams {
   int *out_parents, *out_tokens, *out_finished;
   int64_t V, total;  // total: values of the whole logits buffer
   int W, eos;
+  float step;  // a value this far above its warp's base moves the base
 };
 
 // Order-preserving image of an f32 that is not NaN; one image for both zeros, which are equal.
@@ -226,7 +230,7 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectPara
   float x[EPC], y[EPC];
   if (beam < W && sub < row.pieces) load_row<BF>(p, row, sub, lane, x);
   const bool mine = beam < W && !(p.eos >= 0 && p.finished[g * W + beam]);
-  float wm = -INFINITY;  // the warp's maximum
+  float wm = -INFINITY;  // what the warp's sums are relative to (base)
 
   for (int round = 0;; ++round) {
     double sum = 0.;
@@ -238,8 +242,14 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectPara
           float top = fmaxf(x[0], -INFINITY);  // NaN counts as -inf, in every one of the values too
 #pragma unroll
           for (int i = 1; i < EPC; ++i) top = fmaxf(top, x[i]);
+          if (__any_sync(0xffffffffu, top > wm + p.step)) {  // the first piece, and hardly ever again
+            float up = top;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, o));
+            if (wm != -INFINITY) sum *= exp((double)wm - (double)up);
+            wm = up;
+          }
           if (top > best || at < 0) {
-            if (top > best) sum *= (double)tc::ex2((best - top) * kLog2e);
             const int64_t at0 = row.first + c * kPiece + lane * N - row.base;
             int found = -1;
             if (top > -INFINITY) {
@@ -254,12 +264,12 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectPara
             }
             if (found >= 0) best = top, at = (int)(at0 + found);
           }
-          const float base = best == -INFINITY ? 0.f : best;
+          const float b = wm == -INFINITY ? 0.f : wm;
           auto sum_up = [&](bool clean) {
             float e[4];
 #pragma unroll
             for (int i = 0; i < EPC; ++i) {
-              const float v = tc::ex2(((clean ? fmaxf(x[i], -INFINITY) : x[i]) - base) * kLog2e);
+              const float v = tc::ex2(((clean ? fmaxf(x[i], -INFINITY) : x[i]) - b) * kLog2e);
               e[i % 4] = i < 4 ? v : e[i % 4] + v;
             }
             return (e[0] + e[1]) + (e[2] + e[3]);
@@ -276,10 +286,6 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectPara
           piece(y, c + per);
         }
       }
-      wm = best;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-      if (best != -INFINITY) sum *= (double)tc::ex2((best - wm) * kLog2e);
       // the W best of the lanes' keys, in order
       const u64 key = at < 0 ? 0 : key_of(best, at);
       sh.pool[tid] = key;
@@ -319,23 +325,23 @@ __global__ void __launch_bounds__(kSelThreads, 1) select_kernel(const SelectPara
     }
     for (int q = kSelWarps - 1 - warp; q < joins; q += kSelWarps) {  // the sums, by the last warps
       const int b = (int)crank + q * (int)C;
-      float pm = -INFINITY;  // lane k (and k + 32, ..): the parts of the sum
-      double ps = 0.;
-      for (int k = lane; k < per; k += 32) {
-        const int id = b * per + k;
-        const float m2 = ld_remote_f(&sh.m[id % kSelWarps], id / kSelWarps);
-        const double s2 = __longlong_as_double((long long)ld_remote64(&sh.s[id % kSelWarps], id / kSelWarps));
-        const float mx = fmaxf(pm, m2);
-        if (mx != -INFINITY) {
-          ps = ps * (round ? exp((double)pm - (double)mx) : (double)tc::ex2((pm - mx) * kLog2e)) +
-               s2 * (round ? exp((double)m2 - (double)mx) : (double)tc::ex2((m2 - mx) * kLog2e));
-          pm = mx;
-        }
+      constexpr int PARTS = 8 * kSelWarps / 32;  // of a lane: k, k + 32, ..
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) {
+        const int k = lane + 32 * i, id = b * per + k;
+        if (k < per) top = fmaxf(top, ld_remote_f(&sh.m[id % kSelWarps], id / kSelWarps));
       }
-      float top = pm;
 #pragma unroll
       for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      ps = pm == -INFINITY ? 0. : ps * (round ? exp((double)pm - (double)top) : (double)tc::ex2((pm - top) * kLog2e));
+      double ps = 0.;
+#pragma unroll 1
+      for (int i = 0; i < PARTS && lane + 32 * i < per; ++i) {
+        const int id = b * per + lane + 32 * i;
+        const double s2 = __longlong_as_double((long long)ld_remote64(&sh.s[id % kSelWarps], id / kSelWarps));
+        const float m2 = ld_remote_f(&sh.m[id % kSelWarps], id / kSelWarps);
+        if (m2 != -INFINITY) ps += s2 * exp((double)m2 - (double)top);
+      }
 #pragma unroll
       for (int o = 16; o; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
       if (lane == 0) sh.lse[q] = (double)top + log(ps);
@@ -560,7 +566,8 @@ __global__ void __launch_bounds__(kReThreads) reorder_kernel(const __grid_consta
 cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
   if (a.G == 0) return cudaSuccess;
   SelectParams p = {a.logits, a.scores, a.finished, a.out_scores, a.out_parents, a.out_tokens, a.out_finished,
-                    a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos};
+                    a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos,
+                    (float)((kBaseRoom - std::log2((double)a.V)) * std::log(2.))};
   // One CTA fits an SM: split while the CTAs stay one wave and a warp has a piece (32
   // groups of 8 beams over 50304 values: 1 CTA each 50 us, 2: 28, 4: 17, 8: 38).
   const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);

@@ -854,3 +854,22 @@ def test_beam_select_order_at_the_last_place(sess, W, V):
     ref = R.beam_select(x.reshape(G * W, V), s)
     assert len(set(ref[1][:, -1])) == 2  # either beam has the last place somewhere
     check_select(sess, x.reshape(G * W, V), s, np.zeros((G, W), np.int32), -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,rise", [("f32", 30.0), ("bf16", 8.0), ("f32", 2.0)])
+def test_beam_select_scores_of_rising_logits(sess, kind, rise):
+    """4M logits that rise along the vocabulary: a lane's maximum moves with each of its pieces, and the scores stay
+    within the 4e-6 that is said of them (before their own rounding), the order that of 64-bit sums."""
+    W, V = 16, 1 << 22
+    rng = np.random.default_rng(5)
+    x = (np.linspace(0, rise, V) + rng.random((W, 1))).astype(np.float32)
+    if kind == "bf16":
+        x = R.bf16_round(x)
+    s = -np.sort(rng.random((1, W))).astype(np.float32) / 64
+    ref = R.beam_select(x, s)
+    osc, par, tok = sess.zeros((1, W)), sess.zeros((1, W), "i32"), sess.zeros((1, W), "i32")
+    sess.beam_select(put(sess, x, kind), put(sess, s), osc, par, tok)
+    assert np.array_equal(par.to_host(), ref[1])
+    assert np.array_equal(tok.to_host(), ref[2])
+    assert (np.abs(osc.to_host() - ref[0]) <= U32 * np.abs(ref[0]) + 4e-6).all()
