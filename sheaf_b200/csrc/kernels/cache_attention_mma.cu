@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(NW * 32)
   const int kg = key_of<RB>(g), kc[2] = {key_of<RB>(2 * c), key_of<RB>(2 * c + 1)};
   int st = 0, vref = kVrefFirst;
   uint32_t phase = 0;
-  float vdown = 0.f;
+  float vdown = vref_down(kVrefFirst);
   for (; t0 < hi; t0 += STRIDE) {
     if (I8) {  // a lane's copies of scales are there for the others once the warp has met
       copies_wait<STAGES - 1>();

@@ -235,7 +235,7 @@ __device__ __forceinline__ float f16_row_scale(float largest, float& down) {
 }
 // P times the value scales goes into f16 relative to 2^vref, which is above the
 // largest scale so far: at most 2^(8 + 6), with steps of 2^-30 below 1.
-constexpr int kVrefFirst = -100;
+constexpr int kVrefFirst = -120;  // low enough for every normal scale; its factors are normal f32
 __device__ __forceinline__ int scale_exponent(float s) {  // 2^e > |s|; low for one that is not finite
   s = fabsf(s);
   return s < INFINITY ? (int)(__float_as_uint(s) >> 23) - 126 : -125;

@@ -873,3 +873,24 @@ def test_beam_select_scores_of_rising_logits(sess, kind, rise):
     assert np.array_equal(par.to_host(), ref[1])
     assert np.array_equal(tok.to_host(), ref[2])
     assert (np.abs(osc.to_host() - ref[0]) <= U32 * np.abs(ref[0]) + 4e-6).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D", [(1, 1, 32), (1, 1, 64), (1, 4, 128), (6, 2, 64), (12, 1, 48), (20, 2, 64),
+                                       (33, 4, 128), (2, 1, 256)])
+@pytest.mark.parametrize("e", [-112, 100])
+def test_attention_of_extreme_values(sess, src, n_tok, G, D, e):
+    """Value scales near the ends of f32's range: outputs of that size, by every kernel."""
+    rng = np.random.default_rng(n_tok + D)
+    N, H, T = 2, 2, 170
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), "int8")
+    scales[1] = np.ldexp(scales[1], e)
+    cache.v_scale = put(sess, scales[1])
+    q = rand(rng, (N, n_tok, G * H, D), src)
+    pos = [T - n_tok, 17]
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, 1 / math.sqrt(D))
+    out = put(sess, np.zeros(q.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
+    assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
