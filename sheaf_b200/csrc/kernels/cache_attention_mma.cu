@@ -30,6 +30,8 @@
 //
 // int8 codes become f16 exactly (see codes below), and Q and P are f16 there
 // too; key scales multiply S, value scales P.
+#include <type_traits>
+
 #include "cache_attn.h"
 
 namespace sb {
@@ -284,15 +286,24 @@ __global__ void __launch_bounds__(NW * 32)
   for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.f;
 
   const int kg = key_of<RB>(g), kc[2] = {key_of<RB>(2 * c), key_of<RB>(2 * c + 1)};
-  int st = 0, vref = kVrefFirst;
+  int st = 0, vref[NR];
   uint32_t phase = 0;
-  float vdown = vref_down(kVrefFirst);
-  for (; t0 < hi; t0 += STRIDE) {
+  float vdown[NR], top[NR];  // top: a row's largest P times scale, once they are wide
+  ScaleRange range;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) vref[r] = kVrefFirst, vdown[r] = vref_down(kVrefFirst), top[r] = 0.f;
+  auto ready = [&] {  // the keys at t0, and the range of their scales
     if (I8) {  // a lane's copies of scales are there for the others once the warp has met
       copies_wait<STAGES - 1>();
       __syncwarp();
+#pragma unroll
+      for (int i = 0; i < KB / 32; ++i) range.lane_adds(scales[(st * 2 + 1) * KB + i * 32 + lane]);
+      range.join_lanes();
     }
-    if (!__all_sync(0xffffffffu, tc::mbar_wait(&full[st], phase, &s_abort, err, 64))) break;
+    return __all_sync(0xffffffffu, tc::mbar_wait(&full[st], phase, &s_abort, err, 64)) != 0;
+  };
+  auto turn = [&](auto wide_tag) {
+    constexpr bool WIDE = decltype(wide_tag)::value;
     const uint8_t *const stage = ring + st * F::STAGE, *const stage_v = stage + F::BOXES * BOX;
     const float* const sc = scales + st * KB * 2;
     float s[NB][4];
@@ -349,6 +360,7 @@ __global__ void __launch_bounds__(NW * 32)
           }
         }
     }
+    const float lazy = WIDE && range.big() ? 0.f : kLazy;
     float mx[NR];
     bool move = false;
 #pragma unroll
@@ -358,13 +370,14 @@ __global__ void __launch_bounds__(NW * 32)
       for (int b = 0; b < NB; ++b) mx[r] = fmaxf(mx[r], fmaxf(x[b][r][0], x[b][r][1]));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      move |= mx[r] > m[r] + kLazy;
+      move |= mx[r] > m[r] + lazy;
     }
     if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const float mn = fmaxf(m[r], mx[r]), f = mn == -INFINITY ? 0.f : tc::ex2(m[r] - mn);
         l[r] *= f;
+        if (WIDE) top[r] *= f;
         m[r] = mn;
 #pragma unroll
         for (int j = 0; j < DP / 8; ++j) {
@@ -373,19 +386,39 @@ __global__ void __launch_bounds__(NW * 32)
         }
       }
     }
-    if (I8) {
-      int e = kVrefFirst;
+    if (I8 && (WIDE || range.hi > vref[0])) {
+      int next[NR];
+      bool change = !WIDE;
 #pragma unroll
-      for (int i = 0; i < KB / 32; ++i) e = max(e, scale_exponent(sc[KB + i * 32 + lane]));
-      const int top = __reduce_max_sync(0xffffffffu, e);
-      if (top > vref) {
-        const float f = tc::ex2((float)(vref - top));
+      for (int r = 0; r < NR; ++r) {
+        next[r] = range.hi;
+        if (WIDE) {
+          const float base = m[r] == -INFINITY ? 0.f : m[r];
+          float big = 0.f;
 #pragma unroll
-        for (int j = 0; j < DP / 8; ++j)
+          for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[j][i] *= f;
-        vref = top;
-        vdown = vref_down(vref);
+            for (int i = 0; i < 2; ++i)
+              if (x[b][r][i] != -INFINITY) big = fmaxf(big, tc::ex2(x[b][r][i] - base) * fabsf(sc[KB + b * 8 + kc[i]]));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+          big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+          top[r] = fmaxf(top[r], big);
+          next[r] = wide_vref(vref[r], top[r]);
+          change |= next[r] != vref[r];
+        }
+      }
+      if (__any_sync(0xffffffffu, change)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float f = pow2(vref[r] - next[r]);
+#pragma unroll
+          for (int j = 0; j < DP / 8; ++j) {
+            o[j][2 * r] *= f, o[j][2 * r + 1] *= f;
+            if (MODE != kRows16) o[j][2] *= f, o[j][3] *= f;
+          }
+          vref[r] = next[r];
+          vdown[r] = vref_down(vref[r]);
+        }
       }
     }
     uint32_t a[KG][4], a2[KG][4];  // P, and with P2 what its rounding left
@@ -395,13 +428,13 @@ __global__ void __launch_bounds__(NW * 32)
       for (int r = 0; r < NR; ++r) {
         const float base = m[r] == -INFINITY ? 0.f : m[r];
         float2 f = make_float2(1.f, 1.f);
-        if (I8) f = make_float2(sc[KB + b * 8 + kc[0]] * vdown, sc[KB + b * 8 + kc[1]] * vdown);
+        if (I8) f = make_float2(sc[KB + b * 8 + kc[0]], sc[KB + b * 8 + kc[1]]);
         float y[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float e = tc::ex2(x[b][r][i] - base);
           l[r] += e;
-          y[i] = I8 ? (masked && x[b][r][i] == -INFINITY ? 0.f : e * (i ? f.y : f.x)) : e;
+          y[i] = I8 ? (masked && x[b][r][i] == -INFINITY ? 0.f : e * (i ? f.y : f.x) * vdown[r]) : e;
         }
         uint32_t* dst = &a[b / 2][(b & 1) * 2];
         if (Q32) {
@@ -458,6 +491,13 @@ __global__ void __launch_bounds__(NW * 32)
     if (t0 + STAGES * STRIDE < hi) fetch(t0 + STAGES * STRIDE, st);
     if (I8) copies_commit();
     if (++st == STAGES) st = 0, phase ^= 1u;
+    t0 += STRIDE;
+  };
+  while (t0 < hi && ready() && !range.wide) turn(std::false_type{});
+  if constexpr (I8) {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) top[r] = m[r] == -INFINITY ? 0.f : pow2(vref[r]);
+    while (t0 < hi && ready()) turn(std::true_type{});
   }
   if (I8) copies_wait<0>();
   if (s_abort && lane == 0 && t0 < hi) {  // the boxes of the steps that were not taken may still be on their way
@@ -470,9 +510,9 @@ __global__ void __launch_bounds__(NW * 32)
   __syncthreads();  // every warp has read its last stage: the memory takes the partial outputs
 
   // the warp's parts: row, and columns 2c, 2c + 1 of block (j, e) = value (2c) EV + e of load j
-  const float vup = vref_up(vref);
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
+    const float vup = vref_up(vref[r]);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     const int row = Q32 ? g & 3 : g + 8 * r;

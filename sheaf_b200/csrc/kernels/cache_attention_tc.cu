@@ -191,6 +191,10 @@ struct Cfg {
   static_assert(T_COL + (QP == 3 ? SB * BN : 0) <= 512, "TMEM columns");
 };
 
+// Flags of a tile's scales.  A key scale is 2^90 or more; from this tile on rows have exponents of their own and the
+// value scales stand as they are (see kEven); and rows' maxima are not lazy.
+enum { kBigKey = 1, kWide = 2, kEager = 4 };
+
 struct Shared {
   uint64_t k_full[4], k_free[4], v_full[4], v_free[4], sc_full[8], s_bar[2][2], p_bar[2][2], o_bar[2];
   uint64_t raw, mended, q_bar;
@@ -198,8 +202,8 @@ struct Shared {
   volatile int abort_flag;
   int bad;  // a drafted value that is not finite was taken out of a tile
   int q_row[256];  // query row of a staged row, in units of D values from the slot and head's first; -1: none
-  int sc_big[8];  // a key scale of the tile is 2^90 or more
-  int sc_ref[8];  // exponent that a tile's value scales are relative to
+  // of a tile's scales: exponent that the value scales are relative to, times 8, and flags
+  int sc_info[8];
   unsigned long long mask[kKvMaxTokens];
   int jump[kKvMaxTokens];
   float qs[256];                // what undoes the scaling of a query row (f16)
@@ -370,20 +374,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
       int vref = kVrefFirst;
+      float big = 0.f;  // the row's largest P times scale, once they are wide
       const int cnt = count(a);
       // the drafted tokens' masks and every warp's part of the queries are there
       bool ok = mbar_wait(&sh.q_bar, 0, abort_flag, err, 61);
-      const unsigned long long seen = sh.mask[row / p.G];
+      const unsigned long long* const seen_at = &sh.mask[row / p.G];
+      const int pos32 = (int)pos, pre32 = (int)pre, end32 = (int)end;  // a cache's positions are ints
       // S times the key's scale times f0: the scores in units of log2
       const float f0 = F16 ? sh.qs[(split ? 128 * a : 0) + quad * 32 + lane] : QP == 1 ? fabsf(p.scale2) : 1.f;
-      for (int i = 0; i < cnt; ++i) {
+      auto ready = [&](int i) {  // S and the scales of the i-th tile
         const int t = tile(a, i);
-        const int64_t t0 = (int64_t)(first + t) * BN;
         if (I8) ok = ok && mbar_wait(&sh.sc_full[t % NSC], (uint32_t)(t / NSC) & 1u, abort_flag, err, 51);
         ok = ok && mbar_wait(&sh.s_bar[a][i % SB], (uint32_t)(i / SB) & 1u, abort_flag, err, 52);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         fence_after();
+        return ok;
+      };
+      auto turn = [&](int i, auto wide_tag) {  // S of the i-th tile into P
+        constexpr bool WIDE = decltype(wide_tag)::value;
+        const int t = tile(a, i), info = I8 ? sh.sc_info[t % NSC] : 0;
+        const float lazy = WIDE && info & kEager ? 0.f : kLazy;
+        const int t0 = (first + t) * BN;  // below `end`, which is an int's
         const float* fk = I8 ? sc_k[t % NSC] : nullptr;
         const float* fv = I8 ? sc_v[t % NSC] : nullptr;
         const uint32_t tS = tmem + tl + F::S_COL + (uint32_t)((a * SB + i % SB) * BN);
@@ -412,20 +423,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           scale_o(f);
           l2.x *= f;
           l2.y *= f;
+          if (WIDE) big *= f;
           m = mn;
         };
-        if (I8 && sh.sc_ref[t % NSC] > vref) {
-          const int top = sh.sc_ref[t % NSC];
-          scale_o(ex2((float)(vref - top)));
-          if (!ok) break;
-          vref = top;
+        // wide scales: the row's exponent for P times scale of at most `largest`; whether any row's moved
+        auto reref = [&](float largest) {
+          big = fmaxf(big, largest);
+          const int next = wide_vref(vref, big);
+          if (!__any_sync(0xffffffffu, next != vref)) return false;
+          scale_o(pow2(vref - next));
+          vref = next;
+          return true;
+        };
+        if (I8 && !WIDE && info >> 3 > vref) {
+          scale_o(ex2((float)(vref - (info >> 3))));
+          if (!ok) return;
+          vref = info >> 3;
         }
-        auto moves = [&](float mx) { return __any_sync(0xffffffffu, mx > m + kLazy); };
+        auto moves = [&](float mx) { return __any_sync(0xffffffffu, mx > m + lazy); };
         // P of the tile from S; `vis`: the columns the row sees.  The masked way also
         // takes any scale: a row's factor f0 up to 1 goes before the key's, a larger
-        // one after it, so that neither product passes f32's range unless the score does.
+        // one after it, so that neither product passes f32's range unless the score does;
+        // and wide scales.
         auto softmax = [&](auto mask_tag, const uint32_t* vis) {
-          constexpr bool MASK = decltype(mask_tag)::value;
+          constexpr bool MASK = WIDE || decltype(mask_tag)::value;
           const float pre = MASK && I8 ? fminf(f0, 1.f) : 1.f, f1 = MASK && I8 ? fmaxf(f0, 1.f) : f0;
           if constexpr (QP == 1) {
             // One pass with the maximum as it stands: P is kept in registers
@@ -434,7 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (;;) {
               const float base = m == -INFINITY ? 0.f : m;
               const float2 nb = make_float2(-base, -base);
-              float mx = -INFINITY;
+              float mx = -INFINITY, largest = 0.f;
+              const float down = WIDE ? vref_down(vref) : 1.f;
               float2 s2 = make_float2(0.f, 0.f);
               uint32_t w[BN / 2], w2[PP == 2 ? BN / 2 : 1];  // P, and what its rounding left
               uint32_t r[2][32];
@@ -467,6 +489,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (I8) {
                       y = mul2(y, h2[k]);
                       if (MASK) y.x = v0 ? y.x : 0.f, y.y = v1 ? y.y : 0.f;
+                      if (WIDE) {
+                        largest = fmaxf(largest, fmaxf(fabsf(y.x), fabsf(y.y)));
+                        y = mul2(y, make_float2(down, down));
+                      }
                     }
                     w[(c + j) / 2 + k] = take2<F16>(y.x, y.y);
                     if (PP == 2) w2[(c + j) / 2 + k] = pack2<F16>(y.x, y.y);
@@ -476,6 +502,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (mx != -INFINITY) mx *= f1;
               if (moves(mx)) {
                 rescale(mx);
+                if (!ok) return;
+                continue;
+              }
+              if (WIDE && reref(largest)) {
                 if (!ok) return;
                 continue;
               }
@@ -515,6 +545,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) return;
             }
             const float base = m == -INFINITY ? 0.f : m;
+            if (WIDE) {
+              float largest = 0.f;
+#pragma unroll 1
+              for (int c = 0; c < BN; c += 32) {
+                uint32_t r[32];
+                tmem_ld32_async(tS + (uint32_t)c, r);
+                tmem_wait_ld();
+                reg_fence32(r);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (vis[c / 32] >> j & 1u)
+                    largest = fmaxf(largest, ex2(fmaf(__uint_as_float(r[j]) * pre * fk[c + j], f1, -base)) * fabsf(fv[c + j]));
+              }
+              do {
+                reref(largest);
+                if (!ok) return;
+              } while (__any_sync(0xffffffffu, wide_vref(vref, big) != vref));
+            }
+            const float down = WIDE ? vref_down(vref) : 1.f;
 #pragma unroll
             for (int c = 0; c < BN; c += 32) {
               uint32_t r[32];
@@ -537,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     y[k] = ex2(I8 ? fmaf(s * pre * g[k], f1, -base) : s - base);
                     if (MASK) y[k] = see ? y[k] : 0.f;
                     x[j + k] = y[k];
-                    if (I8 && see) x[j + k] *= h4[k];
+                    if (I8 && see) x[j + k] = WIDE ? x[j + k] * h4[k] * down : x[j + k] * h4[k];
                   }
                   l2 = add2(l2, add2(make_float2(y[0], y[1]), make_float2(y[2], y[3])));
                 }
@@ -552,29 +601,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         };
-        if (t0 + BN > pre || (I8 && sh.sc_big[t % NSC])) {
+        if (WIDE || pre32 - t0 < BN || (I8 && info & kBigKey)) {
           uint32_t vis[BN / 32];
-          const int64_t off = pos - t0;  // column of drafted token 0
+          const int before = pre32 - t0, fit = end32 - t0;  // columns in front of the drafted tokens, and in all
+          const unsigned long long seen = pos < p.T ? *seen_at : 0ull;
 #pragma unroll
           for (int vw = 0; vw < BN / 32; ++vw) {
-            const int64_t c0 = vw * 32;
-            const uint32_t before = pre - t0 >= c0 + 32 ? ~0u : pre - t0 <= c0 ? 0u : (1u << (pre - t0 - c0)) - 1u;
-            const int64_t j0 = c0 - off;  // drafted token at the word's first column
-            uint32_t d = 0;
-            if (j0 >= 0) d = j0 < 64 ? (uint32_t)(seen >> j0) : 0u;
-            else if (j0 > -32) d = (uint32_t)(seen << -j0);
-            const uint32_t fit = end - t0 >= c0 + 32 ? ~0u : end - t0 <= c0 ? 0u : (1u << (end - t0 - c0)) - 1u;
-            vis[vw] = (before | (pos < p.T ? d : 0u)) & fit;
+            const int c0 = vw * 32, j0 = c0 - (pos32 - t0);  // drafted token at the word's first column
+            const uint32_t b = before >= c0 + 32 ? ~0u : before <= c0 ? 0u : (1u << (before - c0)) - 1u;
+            const uint32_t d = j0 >= 64 || j0 <= -32 ? 0u : (uint32_t)(j0 >= 0 ? seen >> j0 : seen << -j0);
+            vis[vw] = (b | d) & (fit >= c0 + 32 ? ~0u : fit <= c0 ? 0u : (1u << (fit - c0)) - 1u);
           }
           softmax(std::true_type{}, vis);
         } else {
           softmax(std::false_type{}, nullptr);
         }
-        if (!ok) break;
+        if (!ok) return;
         tmem_wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_bar[a][i % SB]);
+      };
+      int i = 0;
+      for (; i < cnt && ready(i); ++i) {
+        if (I8 && sh.sc_info[tile(a, i) % NSC] & kWide) break;
+        turn(i, std::false_type{});
+        if (!ok) break;
+      }
+      if constexpr (I8) {
+        big = m == -INFINITY ? 0.f : pow2(vref);
+        for (; i < cnt && ok && ready(i); ++i) turn(i, std::true_type{});
       }
       const float l = l2.x + l2.y;
       const int at = (split ? 128 * a : a * 128) + local;
@@ -684,9 +740,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     if constexpr (I8) {
       // Scales of keys lane and lane + 32, one tile ahead.
-      // Value scales are stored relative to 2^vref, above the largest so far.
+      // Value scales are stored relative to 2^range.hi, above the largest so far, until they are wide.
       float ck[2], cv[2];
-      int vref = kVrefFirst;
+      ScaleRange range;
       auto fetch_scales = [&](int t) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -700,16 +756,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The slot of these scales was last used by tile t - NSC, whose softmax is
         // over once PV of tile t - NS has left its place.
         if (!__all_sync(0xffffffffu, slot_free(sh.v_free, t, 68))) break;
-        const int top = __reduce_max_sync(0xffffffffu, max(scale_exponent(cv[0]), scale_exponent(cv[1])));
-        vref = max(vref, top);
-        const float down = vref_down(vref);
+        range.lane_adds(cv[0]);
+        range.lane_adds(cv[1]);
+        range.join_lanes();
+        const float down = range.wide ? 1.f : vref_down(range.hi);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           sc_k[t % NSC][i * 32 + lane] = ck[i];
           sc_v[t % NSC][i * 32 + lane] = cv[i] * down;
         }
         const bool big = __any_sync(0xffffffffu, !(ck[0] < kBigScale && ck[1] < kBigScale));
-        if (lane == 0) sh.sc_ref[t % NSC] = vref, sh.sc_big[t % NSC] = big;
+        if (lane == 0)
+          sh.sc_info[t % NSC] = range.hi * 8 + (big ? kBigKey : 0) + (range.wide ? kWide : 0) + (range.big() ? kEager : 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.sc_full[t % NSC]);
         fetch_scales(t + 1);

@@ -233,15 +233,47 @@ __device__ __forceinline__ float f16_row_scale(float largest, float& down) {
   down = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
   return __uint_as_float((uint32_t)(127 + 14 - e) << 23);
 }
-// P times the value scales goes into f16 relative to 2^vref, which is above the
-// largest scale so far: at most 2^(8 + 6), with steps of 2^-30 below 1.
+// P times the value scales goes into f16 relative to a power of two, 2^vref, with
+// steps of 2^-30 of it: at most 2^(8 + 6).  As long as the scales met so far lie
+// within 2^kEven of one another, 2^vref is above the largest of them, for all rows
+// alike.  Past that the scales are "wide", from that tile on: vref is a row's own,
+// by the largest P times scale of the keys that the row sees, so that neither a key
+// that it does not see nor one of little weight takes bits from the others.  (8 x 4
+// caches of 16K keys of 128, 256 bf16 rows: 126 us, wide 312; 4 x 8 of 30K, 4 rows:
+// 61 and 68.  So the limit is far above what the values of a text differ by, and
+// leaves the smallest scale 22 bits.)
 constexpr int kVrefFirst = -120;  // low enough for every normal scale; its factors are normal f32
-__device__ __forceinline__ int scale_exponent(float s) {  // 2^e > |s|; low for one that is not finite
-  s = fabsf(s);
-  return s < INFINITY ? (int)(__float_as_uint(s) >> 23) - 126 : -125;
-}
+constexpr int kVrefLast = 127;
+constexpr int kEven = 8;
+constexpr int kBigExponent = 100;  // wide too, and rows' maxima are not lazy: 2^8 times such a scale may pass f32's range
 __device__ __forceinline__ float vref_down(int vref) { return __uint_as_float((uint32_t)(127 + 6 - vref) << 23); }
 __device__ __forceinline__ float vref_up(int vref) { return __uint_as_float((uint32_t)(127 - 6 + vref) << 23); }
+__device__ __forceinline__ float pow2(int e) {  // 0 below f32's normal range
+  return e < -126 ? 0.f : __uint_as_float((uint32_t)(127 + min(e, 127)) << 23);
+}
+// The exponents of the scales met so far by a warp: 2^hi is above the largest, 2^(lo - 1) at most the smallest of the
+// lane's.  Zeros (which need no bits) and scales that are not finite (which leave none) do not count.
+struct ScaleRange {
+  int hi = kVrefFirst, lane_hi = kVrefFirst, lo = kVrefLast + 1;
+  bool wide = false;
+  __device__ __forceinline__ void lane_adds(float s) {
+    const uint32_t u = __float_as_uint(s) & 0x7fffffffu;
+    const int e = max((int)(u >> 23) - 126, kVrefFirst);
+    if (u - 1u < 0x7f800000u - 1u) lane_hi = max(lane_hi, e), lo = min(lo, e);
+  }
+  __device__ __forceinline__ bool big() const { return hi > kBigExponent; }
+  __device__ __forceinline__ void join_lanes() {  // one vote as long as nothing changes
+    if (!__any_sync(0xffffffffu, lane_hi > hi || lo < hi - kEven)) return;
+    hi = __reduce_max_sync(0xffffffffu, lane_hi);
+    wide = wide || big() || __any_sync(0xffffffffu, lo < hi - kEven);
+  }
+};
+// A row's vref among wide scales; `largest`: of P times scale so far, relative to the row's present maximum.  It
+// comes down at once, where the row's other keys need the bits, and goes up when f16 would not hold the next.
+__device__ __forceinline__ int wide_vref(int vref, float largest) {
+  const int e = min(max((int)(__float_as_uint(largest) >> 23) - 126, kVrefFirst), kVrefLast);
+  return largest > 0.f && (e > vref + 8 || e < vref) ? max(e, vref - 120) : vref;
+}
 
 // The weights of N partial results with base-2 maxima m: f = 2^(m - max).
 template <int N>

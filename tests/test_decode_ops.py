@@ -894,3 +894,75 @@ def test_attention_of_extreme_values(sess, src, n_tok, G, D, e):
     out = put(sess, np.zeros(q.shape, np.float32), src)
     sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
     assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, src)).all()
+
+
+FAR_SHAPES = [(1, 1, 64), (1, 1, 32), (1, 4, 128), (6, 1, 64), (7, 2, 48), (12, 1, 64), (4, 3, 128), (20, 2, 64),
+              (33, 4, 128), (64, 3, 64), (2, 1, 256)]
+
+
+def weighted_bound(k, v, pos, q, scale, parents, src, kind):
+    """The 64-bit result, and how far an evaluation may be from it where value rows differ by orders of magnitude: a
+    relative error of e in each probability (see attention_bound) moves an element by at most 2 e sum p |v|, the sum
+    over the keys that the token sees; what a bf16 call may leave out of a probability, and its output's rounding.
+    f16 products keep 2^-30 of the row's largest p |v|, which is within e of the row's largest sum."""
+    ref, dots, _, live = R.attention(k, v, pos, q, scale, parents)
+    total = R.attention(k, np.abs(v), pos, q, scale, parents)[0].max(-1)
+    e = 2 * (q.shape[-1] + 4) * U32 * dots + (live + 64) * U32
+    b = 2 * e * total
+    if src == "bf16":
+        b = b + (2.0 ** -11 if kind == "int8" else 2.0 ** -16) * total
+    b = b[..., None] * np.ones_like(ref)
+    return ref, b * (1 + UBF) + UBF * np.abs(ref) if src == "bf16" else b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D", [c for c in FAR_SHAPES if c[0] > 1])
+@pytest.mark.parametrize("ratio", [1e3, 1e6, 1e30, 1e38, 1e-30])
+def test_attention_value_scales_of_unseen_tokens(sess, src, n_tok, G, D, ratio):
+    """Drafted tokens whose int8 value rows are larger or smaller than all others by orders of magnitude (1e38: as an
+    infinity is stored), early and late in a tree: the tokens that do not attend to them give what they gave."""
+    rng = np.random.default_rng(n_tok + D)
+    N, H, T, pos = 3, 2, 230, [150, 0, 61]
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), "int8")
+    far = {n_tok // 2, n_tok - 1}
+    for n in range(N):
+        for t in far:
+            scales[1][n, :, pos[n] + t] *= np.float32(ratio)
+            arrays[1][n, :, pos[n] + t] //= 2
+    cache.v_scale, cache.v = put(sess, scales[1]), put(sess, arrays[1])
+    q = rand(rng, (N, n_tok, G * H, D), src)
+    parents = np.full((N, n_tok), -1, np.int32)
+    parents[:, n_tok // 2 + 1:n_tok - 1] = 0
+    k, v = values(arrays, scales)
+    ref, bound = weighted_bound(k, v, pos, q, 1 / math.sqrt(D), parents, src, "int8")
+    out = put(sess, np.zeros(q.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out, parents=put(sess, parents))
+    assert (np.abs(out.to_host() - ref) <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D", FAR_SHAPES)
+@pytest.mark.parametrize("ratio", [1e3, 1e6, 1e9, 1e20])
+@pytest.mark.parametrize("at", [0, 100, 399])
+def test_attention_value_scales_of_little_weight(sess, src, n_tok, G, D, ratio, at):
+    """One int8 value row larger than the others by orders of magnitude at a probability that undoes it, before,
+    between and behind the others: all of them count."""
+    rng = np.random.default_rng(n_tok + D + at)
+    N, H, T, pos = 2, 2, 480, [400, 400]
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), "int8")
+    scales[0] *= 0.1
+    scale = 1 / math.sqrt(D)
+    q = np.repeat(np.repeat(rand(rng, (N, 1, H, D)), n_tok, 1), G, 2)
+    q = R.bf16_round(q + 0.01 * rand(rng, q.shape))
+    u = q[:, 0, ::G]
+    arrays[0][:, :, at] = -np.rint(u * 127 / np.abs(u).max(-1, keepdims=True))
+    scales[0][:, :, at] = -np.log(ratio) / (scale * (u * arrays[0][:, :, at]).sum(-1))
+    scales[1][:, :, at] *= np.float32(ratio)
+    cache = S.KVCache(*([put(sess, a) for a in arrays] + [put(sess, s) for s in scales]))
+    k, v = values(arrays, scales)
+    ref, bound = weighted_bound(k, v, pos, q, scale, None, src, "int8")
+    out = put(sess, np.zeros(q.shape, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
+    assert (np.abs(out.to_host() - ref) <= bound).all()
