@@ -937,9 +937,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         pm[j] = ex2(pm[j] - base);
         l = fmaf(pl[j], pm[j], l);
       }
+      // A part without keys has no meaning for its row.  No part has one where the scores are -inf or NaN
+      // throughout, which gives NaN as in the formula, or where there are no keys (see finish4).
+      const float none = mx == -INFINITY ? NAN : 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j)
-        if (j < np) wgt[k * np + j] = pm[j] == 0.f ? 0.f : pm[j] / l * pu[j];
+        if (j < np) wgt[k * np + j] = pm[j] == 0.f ? none : pm[j] / l * pu[j];
     }
     int bad = 0;
     if (!I8 && lane < (int)C)
@@ -972,7 +975,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int k = k0 + r * ROWS;
             if (j0 + j < np && k < mine) {
               const float f = wgt[k * np + j0 + j];
-              if (f != 0.f) add_scaled(acc[r], x[r][j], f);  // a part without keys has no meaning for its row
+              if (f != 0.f) add_scaled(acc[r], x[r][j], f);
             }
           }
       }

@@ -966,3 +966,33 @@ def test_attention_value_scales_of_little_weight(sess, src, n_tok, G, D, ratio, 
     out = put(sess, np.zeros(q.shape, np.float32), src)
     sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
     assert (np.abs(out.to_host() - ref) <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D", [(1, 1, 32), (2, 2, 64), (12, 1, 64), (20, 2, 64), (33, 4, 128), (2, 1, 256)])
+def test_attention_of_scores_that_are_nan_or_all_lowest(sess, kind, src, n_tok, G, D):
+    """A query with a NaN gives NaN, and so do scores of -inf throughout (their softmax is 0 / 0); the other rows
+    their values; a row without keys stays zero."""
+    rng = np.random.default_rng(n_tok + D)
+    N, H, T, pos = 3, 2, 120, [90, 0, -1]
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    q = rand(rng, (N, n_tok, G * H, D), src)
+    k, v = values(arrays, scales)
+    ref, dots, vmax, live = R.attention(k, v, pos, q, 1 / math.sqrt(D))
+    bad = np.zeros(q.shape[:3], bool)
+    bad[:, n_tok // 2, 0] = True
+    q[:, n_tok // 2, 0, 5] = np.nan
+    if not scales:
+        arrays[0][0, 1] = -np.inf
+        q[0, :, G:] = np.abs(q[0, :, G:]) + 1
+        bad[0, :, G:] = True
+        cache.k = put(sess, arrays[0], kind)
+    out = put(sess, np.full(q.shape, 7.0, np.float32), src)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
+    got = out.to_host()
+    assert np.isnan(got[bad & (live > 0)]).all()
+    assert not got[live == 0].any()
+    ok = ~bad
+    assert (np.abs(got - ref) <= attention_bound(dots, vmax, live, D, ref, src))[ok].all()
