@@ -168,6 +168,8 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
       }
     }
     const bool masked = t0 + TK > w.pre || t0 + TK > hi;
+    uint32_t hidden = 0;  // bit u R + r: row r does not see the position
+    static_assert(U * R <= 32, "a bit each");
     if (masked) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           const bool see = t < hi && (t < w.pre || (s_mask[tok[r]] >> (t - w.pos) & 1ull));
-          if (!see) s[u][r] = -INFINITY;
+          if (!see) s[u][r] = -INFINITY, hidden |= 1u << (u * R + r);
         }
       }
     }
@@ -204,8 +206,8 @@ __global__ void __launch_bounds__(kThreads) cache_attn_kernel(const Params p) {
       for (int r = 0; r < R; ++r) {
         float y = s[u][r];
         if constexpr (sizeof(CT) == 1) y *= vsc[u];
-        // a masked position may hold anything, NaN included: it adds nothing
-        if (!masked || s[u][r] != 0.f) {
+        // what a row does not see may hold anything, NaN included: it adds nothing
+        if (!masked || !(hidden >> (u * R + r) & 1u)) {
 #pragma unroll
           for (int i = 0; i < EPL; ++i) o[r][i] = fmaf(y, x[i], o[r][i]);
         }

@@ -164,12 +164,14 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
       const bool masked = t0 + BN > w.pre || t0 + BN > hi;
 #pragma unroll
       for (int r = 0; r < RW; ++r) {
+        bool hidden[KPL] = {};
         if (masked) {
           const unsigned long long seen = s_mask[s_tok[row0 + r]];
 #pragma unroll
           for (int j = 0; j < KPL; ++j) {
             const int64_t t = t0 + 32 * j + lane;
-            if (!(t < hi && (t < w.pre || (seen >> (t - w.pos) & 1ull)))) s[r][j] = -INFINITY;
+            hidden[j] = !(t < hi && (t < w.pre || (seen >> (t - w.pos) & 1ull)));
+            if (hidden[j]) s[r][j] = -INFINITY;
           }
         }
         const float mx = warp_max(fmaxf(s[r][0], s[r][1]));
@@ -185,6 +187,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
         for (int j = 0; j < KPL; ++j) {
           s[r][j] = tc::ex2(s[r][j] - base);
           l[r] += s[r][j];
+          if (masked && hidden[j]) s[r][j] = -0.f;  // no probability: what the position holds does not matter, NaN included
         }
       }
 #pragma unroll
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_tile(const Params p) {
           take<4>(sp + key * RW + 4, y + 4);
 #pragma unroll
           for (int r = 0; r < RW; ++r)
-            if (!MASK || y[r] != 0.f)  // what a masked position holds does not matter, NaN included
+            if (!MASK || __float_as_uint(y[r]) != 0x80000000u)
 #pragma unroll
               for (int i = 0; i < DPL; ++i) o[r][i] = fmaf(y[r], v[i], o[r][i]);
         }

@@ -996,3 +996,28 @@ def test_attention_of_scores_that_are_nan_or_all_lowest(sess, kind, src, n_tok, 
     assert not got[live == 0].any()
     ok = ~bad
     assert (np.abs(got - ref) <= attention_bound(dots, vmax, live, D, ref, src))[ok].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("n_tok,G,D", [(1, 1, 32), (1, 2, 64), (7, 1, 64), (12, 1, 64), (20, 2, 64), (33, 4, 128),
+                                       (2, 1, 256)])
+def test_attention_of_nan_at_no_weight(sess, kind, src, n_tok, G, D):
+    """A NaN value row that a token attends to reaches it whatever its probability, one that rounds to 0 too, in
+    full steps of keys as in the last."""
+    rng = np.random.default_rng(n_tok + D)
+    N, H, T, pos = 2, 1, 400, [370, 20]
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    q = np.abs(rand(rng, (N, n_tok, G * H, D), src)) + 1
+    q = R.bf16_round(q)
+    for n in range(N):  # scores of some -1000 for the first key and the last before the drafted ones
+        at = [0, pos[n] - 1][n]
+        arrays[0][n, :, at] = -100
+        if scales:
+            scales[0][n, :, at] = 1
+            scales[1][n, :, at] = np.nan
+        else:
+            arrays[1][n, :, at] = np.nan
+    got = _attend(sess, arrays, scales, kind, pos, q, src, np.full((N, n_tok), -1, np.int32))
+    assert np.isnan(got).all()
