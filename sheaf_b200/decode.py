@@ -67,9 +67,10 @@ class CachedDecoder:
         if tuple(tokens.shape) != (N, S):
             raise B200Error(3, f"tokens are [{N}, S], not {tuple(tokens.shape)}")
         progs = self._load(S)
-        pos = np.asarray(positions, np.int32)
+        pos = np.asarray(positions, np.int64)
         if pos.shape != (N,) or (pos + S > self.c.block_size).any():
             raise B200Error(3, f"positions are [{N}] and end within the {self.c.block_size} of the model")
+        pos = np.maximum(pos, -1).astype(np.int32)
         depth = np.tile(np.arange(S, dtype=np.int32), (N, 1))
         tree = None
         if parents is not None:

@@ -263,3 +263,14 @@ def test_device_idle_slots_and_refusals(fp32_session):
         assert np.array_equal(a, b)
     with pytest.raises(S.B200Error):
         dec.forward(np.zeros((2, 65)), [0, 0])
+
+
+def test_positions_near_the_ends_of_their_type():
+    """Positions whose end passes 32 bits are refused; far negative ones are idle slots."""
+    dec = CachedDecoder(OracleSession(), C, params_of(C, 1), 2)
+    for far in (2 ** 31 - 1, 2 ** 31, 2 ** 40):
+        with pytest.raises(S.B200Error) as e:
+            dec.forward(np.zeros((2, 1)), [0, far])
+        assert e.value.code == 3
+    idle = [dec.forward(np.zeros((2, 1)), [0, far]).to_host() for far in (-1, -2 ** 31, -2 ** 40)]
+    assert np.array_equal(idle[0][0], idle[1][0]) and np.array_equal(idle[0][0], idle[2][0])
