@@ -260,7 +260,8 @@ SB_API sb_status* sb_kv_cache_read(sb_session* session, const sb_kv_cache* cache
  * ones (a chain), else those on the path parents[n][t], parents[n][parents[n]
  * [t]], .. (a tree of drafted tokens); a parent outside [0, t) ends the path.
  * q, out [slots, tokens, query heads, head size], f32 or bf16; query head h
- * reads cache head h / (query heads / heads).  Positions beyond the capacity
+ * reads cache head h / (query heads / heads).  scale is finite, and so is its
+ * product with log2(e) in f32.  Positions beyond the capacity
  * hold nothing; a slot with a negative position is idle.  A token without keys
  * gets zeros.  What stands at positions that a token does not attend to does
  * not matter, NaN included.  Scores, softmax and sums are f32.  bf16 calls may

@@ -1915,7 +1915,9 @@ sb_status* sb_kv_cache_attention(sb_session* s, const sb_kv_cache* cache, sb_buf
   if (S > kKvMaxTokens)
     return make_status(SB_STATUS_INVALID_ARGUMENT, "at most " + std::to_string(kKvMaxTokens) +
                                                        " tokens per slot, got " + std::to_string(S));
-  if (!std::isfinite(scale)) return make_status(SB_STATUS_INVALID_ARGUMENT, "scale is not finite");
+  // the kernels take scores in units of log2
+  if (!std::isfinite(scale * 1.4426950408889634f))
+    return make_status(SB_STATUS_INVALID_ARGUMENT, "scale times log2(e) is not finite in f32");
   SB_OP(op_aliases({out}, {cache->k, cache->v, cache->k_scale, cache->v_scale, positions, parents, q}));
   std::lock_guard<std::mutex> g(s->mu);
   SB_CUDA(cudaSetDevice(s->dev->ordinal));

@@ -1021,3 +1021,26 @@ def test_attention_of_nan_at_no_weight(sess, kind, src, n_tok, G, D):
             arrays[1][n, :, at] = np.nan
     got = _attend(sess, arrays, scales, kind, pos, q, src, np.full((N, n_tok), -1, np.int32))
     assert np.isnan(got).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n_tok,D", [(1, 64), (20, 64), (1, 256)])
+def test_attention_at_the_largest_scales(sess, lib, kind, n_tok, D):
+    """A scale whose product with log2(e) passes f32's range is refused; the largest that fits gives queries of zero
+    the mean of the values."""
+    rng = np.random.default_rng(D)
+    cache, arrays, scales = make_cache(sess, rng, (1, 2, 50, D), kind)
+    k, v = values(arrays, scales)
+    q = np.zeros((1, n_tok, 2, D), np.float32)
+    out, pos = sess.zeros(q.shape), put(sess, np.int32([20]))
+    n0 = lib.sb_kernel_launch_count()
+    for scale in (2.4e38, 3.4e38, -2.4e38, float("inf")):
+        with pytest.raises(S.B200Error) as e:
+            sess.kv_cache_attention(cache, pos, put(sess, q), out, scale=scale)
+        assert e.value.code == 3
+    assert lib.sb_kernel_launch_count() == n0
+    ref, dots, vmax, live = R.attention(k, v, [20], q, 1.0)
+    for scale in (2.3e38, -2.3e38):
+        sess.kv_cache_attention(cache, pos, put(sess, q), out, scale=scale)
+        assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, "f32")).all()
