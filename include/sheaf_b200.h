@@ -267,7 +267,9 @@ SB_API sb_status* sb_kv_cache_read(sb_session* session, const sb_kv_cache* cache
  * not matter, NaN included.  Scores, softmax and sums are f32.  bf16 calls may
  * leave out 2^-16 of each probability before its product with a value, and over
  * int8 caches, with more than 8 rows (tokens x query heads per cache head),
- * 2^-11; f32 calls take all of it. */
+ * 2^-11; f32 calls take all of it.  Over bf16 and int8 caches the tensor cores'
+ * f32 sums truncate: f32 outputs fall short by up to some 6e-6 of themselves, and
+ * by 1.5e-10 per position beyond 32K positions. */
 SB_API sb_status* sb_kv_cache_attention(sb_session* session, const sb_kv_cache* cache, sb_buffer* positions,
                                         sb_buffer* parents, sb_buffer* q, float scale, sb_buffer* out);
 

@@ -1010,6 +1010,13 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   // 64: 14 and 20.)
   int C = 1;
   while (C < kPortable && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 4 * BN) ++C;
+  // The accumulators truncate, so an output falls short by a little with every MMA added
+  // to it: of f32 calls, with three parts of P, some 1.5e-7 of itself per tile of a
+  // stream.  So a stream takes at most 32 of their tiles, whatever that costs in waves
+  // (12 x 8 caches of 12K keys of 64, 20 rows: off by 5e-6 at 3 CTAs each, 1.4e-5 at 1),
+  // up to the 8 CTAs of 32K keys.
+  const int64_t streams = a.S * (a.Hq / c.H) > 128 && F::MAXR > 128 ? 1 : 2;
+  while (QP == 3 && C < kPortable && (c.T + BN - 1) / BN > 32 * streams * C) ++C;
   return launch_cluster(cache_attn_tc<DP, QP, I8>, items * C, C, kThreads, F::SMEM, stream, mk, mv, p, err);
 }
 

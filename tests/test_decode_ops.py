@@ -1044,3 +1044,24 @@ def test_attention_at_the_largest_scales(sess, lib, kind, n_tok, D):
     for scale in (2.3e38, -2.3e38):
         sess.kv_cache_attention(cache, pos, put(sess, q), out, scale=scale)
         assert (np.abs(out.to_host() - ref) <= attention_bound(dots, vmax, live, D, ref, "f32")).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "int8"])
+@pytest.mark.parametrize("src", ["f32"])
+def test_attention_sums_over_long_caches(sess, kind, src):
+    """f32 rows on the tensor cores over many long caches, which are split no further to fill the SMs: the sums, which
+    truncate, stay short.  32 tiles of 64 keys take 12 additions each, which fall short by half a step of f32 on the
+    average, 2^-24 of the sum at most: 384 of them 2.3e-5 of the outputs."""
+    rng = np.random.default_rng(3)
+    N, H, T, D, n_tok = 10, 8, 24000, 64, 9
+    cache, arrays, scales = make_cache(sess, rng, (N, H, T, D), kind)
+    q = rand(rng, (N, n_tok, H, D), src)
+    pos = [T - n_tok] * N
+    out = sess.zeros(q.shape)
+    sess.kv_cache_attention(cache, put(sess, np.int32(pos)), put(sess, q, src), out)
+    some = slice(0, None, 4)
+    k, v = values([a[some] for a in arrays], [s[some] for s in scales])
+    ref = R.attention(k, v, pos[some], q[some], 1 / math.sqrt(D))[0]
+    got = out.to_host()[some].astype(np.float64)
+    assert np.linalg.norm(got - ref) <= 384 * U32 * np.linalg.norm(ref)
