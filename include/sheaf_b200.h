@@ -234,7 +234,8 @@ SB_API sb_status* sb_optimizer_adamw_step(sb_session* session, size_t leaf_count
  *   scale = max|x| / 127 rounded to f32,
  *   code  = x / scale rounded to the nearest integer, ties to even, exactly
  * (all zero when the scale is 0).  A NaN is written as 0, an infinity as the
- * largest finite f32 of its sign. */
+ * largest finite f32 of its sign (whose 127 * scale an f32 read gives back as an
+ * infinity, since that scale rounds up). */
 typedef struct sb_kv_cache {
   sb_buffer *k, *v, *k_scale, *v_scale;
 } sb_kv_cache;

@@ -27,10 +27,10 @@
 // the group's sums are taken again in f64, whose exponentials would otherwise
 // bound the kernel.  So the order is that of f64 sums in every case.
 //
-// 32 x 8 beams over 50304 f32 logits (52 MB, 7.9 us of reading): 17.3 us (172 us
-// with every sum in f64).  About 10 us of that are not the pass but what 4 beams
-// over 65 values take as well (10.5 us): the launch, two cluster barriers, the
-// join and the second look at the W best lanes.
+// 32 x 8 beams over 50304 f32 logits (52 MB, 7.9 us of reading): 19.3 us, 17.3 in a
+// replayed graph (172 us with every sum in f64).  About 10 us of that are not the
+// pass but what 4 beams over 65 values take as well (10.7 us): the launch, two
+// cluster barriers, the join and the second look at the W best lanes.
 //
 // The reordering moves bytes: 64 beams' caches of 12 layers, 12 heads, 1K positions
 // of 64 bf16 values (a third to nine tenths of them live): 395 us, 5.4 TB/s
@@ -569,7 +569,7 @@ cudaError_t beam_select(const BeamSelectArgs& a, cudaStream_t stream) {
                     a.V, a.G * a.W * a.V, (int)a.W, (int)a.eos,
                     (float)((kBaseRoom - std::log2((double)a.V)) * std::log(2.))};
   // One CTA fits an SM: split while the CTAs stay one wave and a warp has a piece (32
-  // groups of 8 beams over 50304 values: 1 CTA each 50 us, 2: 28, 4: 17, 8: 38).
+  // groups of 8 beams over 50304 values: 1 CTA each 47 us, 2: 26, 4: 17, 8: 37).
   const int64_t pieces = a.W * ((a.V + kPiece - 1) / kPiece);
   int dev = 0, sms = 148, C = 1;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

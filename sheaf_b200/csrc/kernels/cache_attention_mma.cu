@@ -556,14 +556,15 @@ cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
   // Items are split while the CTAs are one wave of three per SM and a warp keeps
   // two steps; and, for batches of uneven lengths, which would end with their longest
   // items alone, until no CTA has more than 256 KB of K (64 x 8 items of up to 4K
-  // bf16 keys of 128: 90 us, unsplit 114).
+  // bf16 keys of 128: 91 us, unsplit 96).
   int C = 1;
   while (may_double(C, items) && a.cache.T / (2 * C) >= 4 * KB &&
          (items * 2 * C <= 3 * sm_count() || a.cache.T * row > C * (256 << 10)))
     C *= 2;
-  // An SM holds two CTAs of three stages, or three of two (64 x 12 items of up to
-  // 1K int8 keys of 64: 24.5 us, 26.8 with three stages; 128 x 4 CTAs of 2K bf16 keys
-  // of 128 each: 90 / 97; one wave of two per SM, 32 x 8 of 3.8K int8 keys: 78 / 59).
+  // An SM holds two CTAs of three stages, or three of two (replayed graphs: 64 x 12
+  // items of up to 1K int8 keys of 64, 25.6 us, 28.7 with three stages; 128 x 4 of up to
+  // 2K bf16 keys of 128, 53 and 58; but 32 x 8 of 3.8K int8 keys of 128 as one wave of two
+  // per SM, 87 and 64).
   if (items * C > 2 * sm_count()) return launch<DP, I8, MODE, 2>(a, C, stream);
   return launch<DP, I8, MODE, 3>(a, C, stream);
 }
@@ -571,16 +572,17 @@ cudaError_t by_items(const CacheAttnArgs& a, cudaStream_t stream) {
 }  // namespace
 
 // As many bf16 rows as the instruction has, and f32 rows in two blocks of 4, whose
-// second reading of the cache is from L2.  There it is the faster one: 16 bf16 rows
-// of 4 x 8 caches of 30K keys of 128 take 86 us from bf16 and 67 from int8, on
-// tcgen05 97 and 128; of 8 x 12 caches of 465 keys of 64, 8.6 and 9.5, 12.4 and 14.8;
-// 8 f32 rows of 8 x 12 caches of 6K keys of 128, 83 and 80, 129 and 193 (three blocks,
-// 12 rows: 123 and 116, but of 300 keys 29 and 34, 17 and 22).  Two blocks of bf16
-// rows lose it: 32 rows of 6K keys, 95 us from bf16, 77 on tcgen05.  4 f32 rows of 16
-// x 8 caches of 4K keys of 128, 57 and 37 us, on the CUDA cores 125 and 241.
+// second reading of the cache is from L2.  There it is the faster one (in replayed
+// graphs): 16 bf16 rows of 4 x 8 caches of 30K keys of 128 take 86 us from bf16 and 69
+// from int8, on tcgen05 101 and 130; of 8 x 12 caches of 465 keys of 64, 9.1 and 9.8,
+// 13.2 and 15.3; 8 f32 rows of 8 x 12 caches of 6K keys of 128, 83 and 83, 136 and 200
+// (three blocks, 12 rows: 123 and 120, but of 300 keys 29 and 34, 17 and 23).  Two
+// blocks of bf16 rows lose it: 32 rows of 6K keys, 104 us from bf16, 81 on tcgen05
+// (from int8 88 and 114, but of 632 keys of 64 19 and 17).  4 f32 rows of 16 x 8 caches
+// of 4K keys of 128, 57 and 39 us, on the CUDA cores 125 and 241.
 //
 // Reading the cache bounds the long bf16 calls (one bf16 row of 4 x 8 x 30K keys of
-// 128: 79 us, 6.2 TB/s); int8 ones (59 us, 4.3 TB/s) the conversion of codes and of P,
+// 128: 83 us, 6.0 TB/s); int8 ones (60 us, 4.2 TB/s) the conversion of codes and of P,
 // some five half-rate instructions per word of four codes; short ones their set-up
 // and joining, some 5 us.
 bool cache_attention_mma_takes(const CacheAttnArgs& a) {

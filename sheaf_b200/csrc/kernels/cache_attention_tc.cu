@@ -23,7 +23,7 @@
 //               S in TMEM as parts: three for f32 output (f32 accuracy), two of
 //               bf16 for bf16 output (2^-16 of each probability is left out; one
 //               part, 2^-8, would be as far off as the output's own rounding, with
-//               80 us for the 8 x 4 caches of 16K below in place of 94), one of f16
+//               80 us for the 8 x 4 caches of 16K below in place of 95), one of f16
 //               for bf16 output of int8 caches (2^-11 is left out, an eighth of the
 //               output's rounding; a second part took 142 us in place of 122).
 //   O += P V    the maximum m a row refers to moves only when it would grow by
@@ -37,12 +37,11 @@
 // the outputs are joined.
 //
 // 8 x 4 caches of 16K keys of 128, 256 bf16 rows (69 GFLOP, 41 us of tensor time,
-// bf16 cache 22 us of reading): 80 us from bf16, 0.86 PFLOP/s, 1.9K cycles per
-// tile of which the MMAs take three quarters; 119 us from int8, whose softmax
-// (two more multiplications per score) and conversion take 2.9K.  f32 queries
-// have three times the products: 194 and 277 us.  63 f32 rows over 8 x 12 caches
-// of 1K keys of 64: 22 and 30 us, of which 12 are there without a cache: the
-// launch, the staging of the queries, the cluster's join.
+// 61 with both parts of P; bf16 cache 22 us of reading): 95 us from bf16; 124 us
+// from int8, held by the softmax (two more multiplications per score) and the
+// conversion.  f32 queries have three times the products: 198 and 294 us.  63 f32
+// rows over 8 x 12 caches of 1K keys of 64: 22 and 30 us, of which 12 are there
+// without a cache: the launch, the staging of the queries, the cluster's join.
 //
 // Every mbarrier wait is bounded.  TMEM is freed before the cluster barrier: a
 // CTA that holds TMEM never waits for another CTA.
@@ -177,8 +176,9 @@ struct Cfg {
   static constexpr int NS = QP == 3 && DP == 128 ? 2 : 4;  // K and V tiles in flight
   // Groups of loading warps that take int8 tiles in turn.  Two, with four places: one
   // group converts while the other's loads are on their way (8 x 16K keys, 256
-  // bf16 rows of 128: 119 us, against 126 with all four warps on each tile).  With
-  // two places a group would wait for its place longer (f32: 339 us against 288).
+  // bf16 rows of 128: 124 us, against 134 with all four warps on each tile; short f32
+  // calls lose, 63 rows over 1K keys of 64: 30 against 28).  With two places a group
+  // would wait for its place longer.
   static constexpr int GROUPS = NS > 2 ? 2 : 1;
   static constexpr int NSC = 2 * NS;                       // rows of scales in flight (see the loader)
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + NS * TILE, END = V_OFF + NS * TILE;
@@ -1006,7 +1006,7 @@ cudaError_t launch(const CacheAttnArgs& a, cudaStream_t stream) {
   // One CTA fits an SM (shared memory, and all of its TMEM): split until the CTAs
   // fill the SMs once, or a CTA has four tiles, since a second wave would repeat the
   // 10 us that a CTA takes without keys.  (8 items of 128 rows over 8K keys of 128:
-  // 27 us, unsplit 84; 32 of 256 rows over 16K: 80 and 265; 24 of 63 rows over 1K of
+  // 28 us, unsplit 94; 32 of 256 rows over 16K: 95 and 289; 24 of 63 rows over 1K of
   // 64: 14 and 20.)
   int C = 1;
   while (C < kPortable && items * (C + 1) <= sm_count() && c.T / (C + 1) >= 4 * BN) ++C;

@@ -9,7 +9,8 @@
 // One scale per row keeps a row's error below s / 2 whatever other rows hold,
 // and attention can apply it to a score or a probability instead of a row.
 // A NaN is written as 0 and an infinity as the largest finite f32, so that one
-// bad value leaves the row's other codes usable.
+// bad value leaves the row's other codes usable (the scale of such a row rounds up,
+// so that f32 reads the code 127 back as an infinity).
 //
 // Bytes bound both.  8 x 1024 tokens of 12 heads of 64, f32 to int8, and the read
 // back to f32 (128 MB): 27.4 us, 4.7 TB/s (much of it stays in L2 between the two);
